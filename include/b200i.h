@@ -39,6 +39,10 @@ extern "C" {
 #define B200I_W_INT8_EXP 2   /* int8 codes + int32 power-of-two exponent per row */
 #define B200I_W_INT8_SCALE 3 /* int8 codes + float32 scale per row (extension) */
 
+/* types of the paged cache and of the rows that meet it */
+#define B200I_T_F32 0
+#define B200I_T_BF16 1
+
 /* --- identity of the loaded binary ---------------------------------------------------
  * Replace linalg_numeric_mode / linalg_profile_version / linalg_numerical_profile /
  * lowbit_profile_version / linalg_vendor (bindings/_mojolearn_linalg.mojo:143-157)
@@ -413,6 +417,45 @@ int64_t b200i_ffma_probe(int64_t device, void *stream, float *scratch, int64_t b
 /* Kernels launched by this library since load (all devices); the benchmark
  * reports the difference over its timed region. */
 int64_t b200i_launch_count(void);
+
+/* --- the paged cache, device pointers, asynchronous on the caller's stream -------------------------
+ * No counterpart in the reference, whose decode state is one contiguous cache per batch, and not part of its numerical
+ * contract: sums run in 32 bits in an order of the kernel's own choice (the same words for the same call).
+ *
+ * k_cache and v_cache are [pages, n_kv, page, head_dim]; page a power of two from 16 to 256, head_dim a multiple of 8 up to
+ * 128. page_table [batch, max_pages] int32 names each sequence's pages in the order of its positions. The rows of all
+ * sequences stand one after another: sequence b's are cu[b] .. cu[b + 1] (cu int32, batch + 1 of them, ascending), and
+ * lengths[b] (int32) counts what its cache holds with them: its row i is at position lengths[b] - (cu[b + 1] - cu[b]) + i.
+ * Rows past cu[batch] belong to no sequence: nothing is read for them and nothing written. The three arrays are read on
+ * the device; a page number outside the pool counts as a page of zeros, is not written, and sets the status word
+ * (b200i_decode_status) to 11. Row and cache types: float32 and float32, float32 and bfloat16, bfloat16 and bfloat16. */
+
+/* Rows q [rows, n_heads * head_dim], k and v [rows, n_kv * head_dim] with row pitches ldq, ldk, ldv in elements (column blocks
+ * of a fused product), starting on 16-byte boundaries. q_out [rows, n_heads * head_dim] receives the rotated queries in the row
+ * type, the caches the rotated keys and the values in theirs. q_norm, k_norm (float32 [head_dim], may be NULL): an RMSNorm
+ * over each head's vector before the rotation, norm_kind 0 with weight w, 2 with 1 + w. cosv, sinv (float32
+ * [positions, rope_dim / 2], both NULL = no rotation): row p is position p's; rope_dim as in b200i_qkv_rope_cache (0 = head_dim). */
+int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_cache, void *v_cache, const void *q, const void *k,
+                           const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int64_t row_type, int64_t cache_type,
+                           const float *cosv, const float *sinv, int64_t rope_dim, int64_t positions, const float *q_norm,
+                           const float *k_norm, double eps, int64_t norm_kind, const int32_t *page_table, const int32_t *cu,
+                           const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                           int64_t pages, int64_t page, int64_t max_pages, char *err, int64_t err_cap);
+
+/* out [rows, n_heads, head_dim] in the row type: softmax over the keys a row sees of scale * q.k (capped to
+ * softcap * tanh(z / softcap) where softcap > 0), times the values. A row at position p sees the positions up to p and, where
+ * window > 0, after p - window; one that sees none is zero. What stands in positions that a row does not see, or past a
+ * sequence's length, has no influence on it. max_new and max_length bound the sequences' new tokens and lengths as the host knows
+ * them (max_new is held to: a sequence with more rows sets the status word to 12 and its further rows are not written; max_length
+ * only chooses how the work is cut). `ws`: the scratch that b200i_paged_attention_workspace_bytes asks for, 256-byte aligned. */
+int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache,
+                              const void *v_cache, int64_t row_type, int64_t cache_type, const int32_t *page_table,
+                              const int32_t *cu, const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv,
+                              int64_t head_dim, int64_t pages, int64_t page, int64_t max_pages, int64_t max_new,
+                              int64_t max_length, double scale, int64_t window, double softcap, void *ws, int64_t ws_bytes,
+                              char *err, int64_t err_cap);
+int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch,
+                                              int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length);
 
 #ifdef __cplusplus
 }

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "../../include/b200i.h"
+#include "library.h"
 #include "comm.cuh"
 #include "decode.cuh"
 #include "decode_pair.cuh"
@@ -778,6 +779,37 @@ size_t wkind_elem_bytes(int wkind) { return wkind == W_F32 ? 4 : (wkind == W_BF1
 
 } // namespace
 
+
+// ---- for the library's other translation units (library.h) ----
+namespace b200i_library {
+
+int64_t refuse(char *err, int64_t cap, const char *fmt, ...) {
+    if (err && cap > 0) {
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(err, (size_t)cap, fmt, ap);
+        va_end(ap);
+    }
+    return 1;
+}
+void accept(char *err, int64_t cap) { clear(err, cap); }
+int64_t enter_device(int64_t device, char *err, int64_t cap, int *out) { return select_device(device, err, cap, out); }
+int device_sms(int device) { return sm_count(device); }
+int *status_word(int device) {
+    static std::atomic<int *> known[MAX_DEVICES];
+    int *p = known[device].load();
+    if (p) return p;
+    void *at = nullptr;
+    if (cudaGetSymbolAddress(&at, g_decode_status) != cudaSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    known[device].store(static_cast<int *>(at));
+    return static_cast<int *>(at);
+}
+void count_launches(int n) { g_launches += n; }
+
+} // namespace b200i_library
 
 extern "C" {
 

@@ -15,31 +15,49 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libb200i.so")
 #: the negative-control build: every window admitted (-DB200I_SABOTAGE_ADMIT_ALWAYS); loaded only by the tests
 SABOTAGE_LIB = os.path.join(HERE, "libb200i_sabotage_admit.so")
-SOURCES = ["b200i.cu"]
-HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".cuh")) + [os.path.join("..", "..", "include", "b200i.h")]
+SOURCES = ["b200i.cu", "paged.cu"]
+HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".cuh")) + ["library.h", os.path.join("..", "..", "include", "b200i.h")]
+#: which headers a source includes: an object is compiled again where one of its own is newer (the paged cache's kernels stand apart)
+OWN_HEADERS = {"paged.cu": [f for f in HEADERS if f.startswith("paged") or not f.endswith(".cuh")],
+               "b200i.cu": [f for f in HEADERS if not f.startswith("paged")]}
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-fmad=false", "-ftz=false", "-prec-div=true", "-prec-sqrt=true",
-    "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default", "-cudart", "shared",
+    "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default", "-cudart", "shared",
 ]
 
 
+def _older(made, deps):
+    """Whether `made` is missing or older than one of the files it is made of."""
+    return not os.path.exists(made) or any(os.path.exists(d) and os.path.getmtime(d) > os.path.getmtime(made) for d in deps)
+
+
+def _sources(source):
+    return [os.path.join(HERE, f) for f in [source] + OWN_HEADERS[source]] + [os.path.abspath(__file__)]
+
+
 def stale(lib=LIB):
-    if not os.path.exists(lib):
-        return True
-    t = os.path.getmtime(lib)
-    deps = [os.path.join(HERE, s) for s in SOURCES + HEADERS] + [os.path.abspath(__file__)]
-    return any(os.path.exists(d) and os.path.getmtime(d) > t for d in deps)
+    return _older(lib, [d for s in SOURCES for d in _sources(s)])
 
 
 def build(force=False, verbose=False, sabotage=False):
+    """Every source compiled to an object of its own, those that are out of date at the same time, then linked."""
     lib = SABOTAGE_LIB if sabotage else LIB
     if not force and not stale(lib):
         return lib
-    nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [nvcc] + NVCC_FLAGS + (["-DB200I_SABOTAGE_ADMIT_ALWAYS"] if sabotage else []) + (["-Xptxas", "-v"] if verbose else []) \
-        + [os.path.join(HERE, s) for s in SOURCES] + ["-o", lib]
-    subprocess.run(cmd, check=True)
+    nvcc = [os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")] + NVCC_FLAGS
+    objects, running = [], []
+    for source in SOURCES:
+        admit = sabotage and source == "b200i.cu"  # the only source that the negative control changes
+        objects.append(os.path.join(HERE, source[:-3] + ("_sabotage_admit.o" if admit else ".o")))
+        if force or verbose or _older(objects[-1], _sources(source)):
+            cmd = nvcc + (["-DB200I_SABOTAGE_ADMIT_ALWAYS"] if admit else []) + (["-Xptxas", "-v"] if verbose else []) + \
+                ["-c", os.path.join(HERE, source), "-o", objects[-1]]
+            running.append((cmd, subprocess.Popen(cmd)))
+    failed = [cmd for cmd, p in running if p.wait() != 0]
+    if failed:
+        raise subprocess.CalledProcessError(1, failed[0])
+    subprocess.run(nvcc + ["-shared"] + objects + ["-o", lib], check=True)
     return lib
 
 

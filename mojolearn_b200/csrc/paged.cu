@@ -1,0 +1,123 @@
+// The paged cache's entry points of the C ABI: argument checks, choice of kernel, launches. Declared in include/b200i.h.
+#include <algorithm>
+
+#include "../../include/b200i.h"
+#include "library.h"
+#include "paged.cuh"
+#include "paged_append.cuh"
+
+using namespace b200i;
+using b200i_library::refuse;
+
+namespace {
+
+constexpr int64_t MOST = 0x7FFFFFFF;
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// What both calls check, and the part of the arguments that they share. `who` names the call in messages.
+int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cache_type, const void *page_table, const void *cu, const void *lengths, int64_t rows,
+                    int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t pages, int64_t page, int64_t max_pages, char *err, int64_t err_cap) {
+    if (rows <= 0 || batch <= 0 || n_heads <= 0 || n_kv <= 0 || head_dim <= 0 || pages <= 0 || page <= 0 || max_pages <= 0)
+        return refuse(err, err_cap, "%s: extents must be positive", who);
+    if (rows > MOST / 2 || batch > MOST / 2 || pages > MOST || max_pages > MOST || max_pages * page > MOST)
+        return refuse(err, err_cap, "%s: rows, sequences, pages and positions are counted in 31 bits", who);
+    if (n_heads % n_kv != 0 || n_heads > 65535) return refuse(err, err_cap, "%s: n_heads must be a multiple of n_kv and below 65536", who);
+    if (head_dim % 8 != 0 || head_dim > PAGED_MAX_HD) return refuse(err, err_cap, "%s: head_dim must be a multiple of 8 up to %d", who, PAGED_MAX_HD);
+    if (page < 16 || page > 256 || (page & (page - 1)) != 0) return refuse(err, err_cap, "%s: a page holds a power of two from 16 to 256 positions", who);
+    if ((row_type != B200I_T_F32 && row_type != B200I_T_BF16) || (cache_type != B200I_T_F32 && cache_type != B200I_T_BF16) ||
+        (row_type == B200I_T_BF16 && cache_type == B200I_T_F32))
+        return refuse(err, err_cap, "%s: rows and cache are float32 and float32, float32 and bfloat16, or bfloat16 and bfloat16", who);
+    if (pages * n_kv * page > MOST) return refuse(err, err_cap, "%s: a pool of more than 2^31 - 1 rows of head_dim", who);
+    if (!page_table || !cu || !lengths) return refuse(err, err_cap, "%s: null page table, row offsets or lengths", who);
+    int shift = 0;
+    while ((1 << shift) < page) shift++;
+    c->table = static_cast<const int *>(page_table), c->cu = static_cast<const int *>(cu), c->lengths = static_cast<const int *>(lengths);
+    c->rows = rows, c->batch = (int)batch, c->heads = (int)n_heads, c->kv = (int)n_kv, c->group = (int)(n_heads / n_kv), c->hd = (int)head_dim;
+    c->pages = (int)pages, c->page_shift = shift, c->max_pages = (int)max_pages;
+    return 0;
+}
+
+// After the arguments: the device and its status word.
+int64_t enter(PagedCall *c, const char *who, int64_t device, char *err, int64_t err_cap) {
+    int dev;
+    if (b200i_library::enter_device(device, err, err_cap, &dev)) return 1;
+    c->status = b200i_library::status_word(dev);
+    return c->status ? 0 : refuse(err, err_cap, "%s: the device has no status word", who);
+}
+
+bool rows_fit(int64_t ld, int64_t width, int64_t type) { return ld >= width && (ld * (type == B200I_T_F32 ? 4 : 2)) % 16 == 0; }
+
+} // namespace
+
+extern "C" {
+
+int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_cache, void *v_cache, const void *q, const void *k, const void *v, int64_t ldq, int64_t ldk,
+                           int64_t ldv, int64_t row_type, int64_t cache_type, const float *cosv, const float *sinv, int64_t rope_dim, int64_t positions, const float *q_norm,
+                           const float *k_norm, double eps, int64_t norm_kind, const int32_t *page_table, const int32_t *cu, const int32_t *lengths, int64_t rows, int64_t batch,
+                           int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t pages, int64_t page, int64_t max_pages, char *err, int64_t err_cap) {
+    AppendCall a;
+    if (shared_part(&a.c, "paged_append", row_type, cache_type, page_table, cu, lengths, rows, batch, n_heads, n_kv, head_dim, pages, page, max_pages, err, err_cap)) return 1;
+    if (!q_out || !k_cache || !v_cache || !q || !k || !v) return refuse(err, err_cap, "paged_append: null storage");
+    if (!aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
+        !rows_fit(ldq, n_heads * head_dim, row_type) || !rows_fit(ldk, n_kv * head_dim, row_type) || !rows_fit(ldv, n_kv * head_dim, row_type))
+        return refuse(err, err_cap, "paged_append: rows must start on 16-byte boundaries and hold their heads side by side");
+    if ((cosv == nullptr) != (sinv == nullptr)) return refuse(err, err_cap, "paged_append: cos without sin, or sin without cos");
+    if (rope_dim == 0 || !cosv) rope_dim = head_dim;
+    if (rope_dim < 0 || rope_dim > head_dim || rope_dim % 2 != 0) return refuse(err, err_cap, "paged_append: rope_dim %lld does not fit head_dim %lld", (long long)rope_dim, (long long)head_dim);
+    if (cosv && (positions <= 0 || positions > MOST)) return refuse(err, err_cap, "paged_append: the rotation table holds no position");
+    if (norm_kind != 0 && norm_kind != 2) return refuse(err, err_cap, "paged_append: norm kind %lld is not 0 (weight w) or 2 (weight 1 + w)", (long long)norm_kind);
+    a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.k_cache = k_cache, a.v_cache = v_cache, a.ldq = ldq, a.ldk = ldk, a.ldv = ldv;
+    a.cosv = cosv, a.sinv = sinv, a.q_norm = q_norm, a.k_norm = k_norm, a.rope_dim = (int)rope_dim, a.positions = (int)positions;
+    a.eps = (float)eps, a.norm_shift = norm_kind == 2 ? 1.0f : 0.0f;
+    if (enter(&a.c, "paged_append", device, err, err_cap)) return 1;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (row_type == B200I_T_BF16)
+        LIBRARY_CUDA_TRY((launch_append<__nv_bfloat16, __nv_bfloat16>(a, st)));
+    else if (cache_type == B200I_T_BF16)
+        LIBRARY_CUDA_TRY((launch_append<float, __nv_bfloat16>(a, st)));
+    else
+        LIBRARY_CUDA_TRY((launch_append<float, float>(a, st)));
+    b200i_library::count_launches(1);
+    b200i_library::accept(err, err_cap);
+    return 0;
+}
+
+int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                                              int64_t max_new, int64_t max_length) {
+    (void)device, (void)row_type, (void)cache_type, (void)rows, (void)batch, (void)n_heads, (void)n_kv, (void)head_dim, (void)max_new, (void)max_length;
+    return 0;
+}
+
+int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, int64_t row_type, int64_t cache_type,
+                              const int32_t *page_table, const int32_t *cu, const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                              int64_t pages, int64_t page, int64_t max_pages, int64_t max_new, int64_t max_length, double scale, int64_t window, double softcap, void *ws,
+                              int64_t ws_bytes, char *err, int64_t err_cap) {
+    AttendCall a;
+    if (shared_part(&a.c, "paged_attention", row_type, cache_type, page_table, cu, lengths, rows, batch, n_heads, n_kv, head_dim, pages, page, max_pages, err, err_cap)) return 1;
+    if (!out || !q || !k_cache || !v_cache) return refuse(err, err_cap, "paged_attention: null storage");
+    if (!aligned16(out) || !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !rows_fit(ldq, n_heads * head_dim, row_type))
+        return refuse(err, err_cap, "paged_attention: rows must start on 16-byte boundaries and hold their heads side by side");
+    if (max_new <= 0 || max_length <= 0) return refuse(err, err_cap, "paged_attention: the bounds on new tokens and lengths must be positive");
+    if (window < 0 || !(softcap >= 0.0) || softcap > 1e30 || !(scale > -1e30 && scale < 1e30)) return refuse(err, err_cap, "paged_attention: window, softcap or scale is out of range");
+    if (ws_bytes < 0 || (ws_bytes > 0 && !ws)) return refuse(err, err_cap, "paged_attention: a workspace size without a workspace");
+    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.scale = (float)scale, a.softcap = (float)softcap;
+    a.window = (int)std::min(window, MOST), a.max_new = (int)std::min(max_new, MOST);
+    if (enter(&a.c, "paged_attention", device, err, err_cap)) return 1;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long units = rows * n_heads;
+    if ((units + 3) / 4 > MOST) return refuse(err, err_cap, "paged_attention: too many rows for one call");
+    const unsigned grid = (unsigned)((units + 3) / 4);
+    if (row_type == B200I_T_BF16)
+        attend_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
+    else if (cache_type == B200I_T_BF16)
+        attend_plain_kernel<float, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
+    else
+        attend_plain_kernel<float, float><<<grid, 128, 0, st>>>(a);
+    LIBRARY_CUDA_TRY(cudaGetLastError());
+    b200i_library::count_launches(1);
+    b200i_library::accept(err, err_cap);
+    return 0;
+}
+
+} // extern "C"

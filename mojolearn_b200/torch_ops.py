@@ -91,6 +91,10 @@ def check_status(device=None):
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     index = dev.index if dev.index is not None else torch.cuda.current_device()
     v = int(_native.lib().b200i_decode_status(index))
+    if v == 11:
+        raise _native.NativeError("mojolearn_b200: a page table names a page outside the pool (status 11); nothing was written there and zeros were read")
+    if v == 12:
+        raise _native.NativeError("mojolearn_b200: a sequence has more new tokens than the call's max_new (status 12); the further rows were not written")
     if v != 0:
         raise _native.NativeError("mojolearn_b200: a bounded device-side wait ran out (status %d); results computed "
                                   "since the last check are incomplete" % v)
