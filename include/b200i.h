@@ -455,7 +455,8 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
                               int64_t max_length, double scale, int64_t window, double softcap, void *ws, int64_t ws_bytes,
                               char *err, int64_t err_cap);
 int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch,
-                                              int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length);
+                                              int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length,
+                                              int64_t window);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,7 @@
 #include "library.h"
 #include "paged.cuh"
 #include "paged_append.cuh"
+#include "paged_few.cuh"
 
 using namespace b200i;
 using b200i_library::refuse;
@@ -39,11 +40,29 @@ int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cac
 }
 
 // After the arguments: the device and its status word.
-int64_t enter(PagedCall *c, const char *who, int64_t device, char *err, int64_t err_cap) {
-    int dev;
-    if (b200i_library::enter_device(device, err, err_cap, &dev)) return 1;
-    c->status = b200i_library::status_word(dev);
+int64_t enter(PagedCall *c, const char *who, int64_t device, int *dev, char *err, int64_t err_cap) {
+    if (b200i_library::enter_device(device, err, err_cap, dev)) return 1;
+    c->status = b200i_library::status_word(*dev);
     return c->status ? 0 : refuse(err, err_cap, "%s: the device has no status word", who);
+}
+
+// The kernel of a call and how its work is cut.
+struct AttendPlan {
+    int few;      // rows of a sequence and key head, where they are few (else 0)
+    int hdp, nt;  // head_dim as it is laid out in shared memory; sets of eight rows
+    FewPlan cut;
+};
+constexpr int FEW_ROWS = 16;
+
+AttendPlan attend_plan(int device, int64_t cache_type, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
+    AttendPlan p = {};
+    p.hdp = head_dim <= 64 ? 64 : 128;
+    const int64_t group = n_heads / n_kv;
+    if (max_new <= FEW_ROWS && max_new * group <= FEW_ROWS) {
+        p.few = (int)(max_new * group), p.nt = p.few <= 8 ? 1 : 2;
+        p.cut = few_plan(b200i_library::device_sms(device), (int)batch, (int)n_kv, p.hdp, p.nt, cache_type == B200I_T_F32 ? 32 : 64, max_new, max_length, (int)std::min(window, MOST));
+    }
+    return p;
 }
 
 bool rows_fit(int64_t ld, int64_t width, int64_t type) { return ld >= width && (ld * (type == B200I_T_F32 ? 4 : 2)) % 16 == 0; }
@@ -70,7 +89,8 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
     a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.k_cache = k_cache, a.v_cache = v_cache, a.ldq = ldq, a.ldk = ldk, a.ldv = ldv;
     a.cosv = cosv, a.sinv = sinv, a.q_norm = q_norm, a.k_norm = k_norm, a.rope_dim = (int)rope_dim, a.positions = (int)positions;
     a.eps = (float)eps, a.norm_shift = norm_kind == 2 ? 1.0f : 0.0f;
-    if (enter(&a.c, "paged_append", device, err, err_cap)) return 1;
+    int dev;
+    if (enter(&a.c, "paged_append", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (row_type == B200I_T_BF16)
         LIBRARY_CUDA_TRY((launch_append<__nv_bfloat16, __nv_bfloat16>(a, st)));
@@ -84,9 +104,12 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
 }
 
 int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
-                                              int64_t max_new, int64_t max_length) {
-    (void)device, (void)row_type, (void)cache_type, (void)rows, (void)batch, (void)n_heads, (void)n_kv, (void)head_dim, (void)max_new, (void)max_length;
-    return 0;
+                                              int64_t max_new, int64_t max_length, int64_t window) {
+    if (rows <= 0 || batch <= 0 || n_kv <= 0 || n_heads < n_kv || head_dim <= 0 || max_new <= 0 || max_length <= 0 || window < 0) return 0;
+    (void)row_type;
+    int dev = (int)device;
+    if (device < 0 && cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); dev = -1; }
+    return attend_plan(dev, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window).cut.bytes;
 }
 
 int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, int64_t row_type, int64_t cache_type,
@@ -103,19 +126,32 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (ws_bytes < 0 || (ws_bytes > 0 && !ws)) return refuse(err, err_cap, "paged_attention: a workspace size without a workspace");
     a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.scale = (float)scale, a.softcap = (float)softcap;
     a.window = (int)std::min(window, MOST), a.max_new = (int)std::min(max_new, MOST);
-    if (enter(&a.c, "paged_attention", device, err, err_cap)) return 1;
+    int dev, launches = 0;
+    if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const long long units = rows * n_heads;
-    if ((units + 3) / 4 > MOST) return refuse(err, err_cap, "paged_attention: too many rows for one call");
-    const unsigned grid = (unsigned)((units + 3) / 4);
-    if (row_type == B200I_T_BF16)
-        attend_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
-    else if (cache_type == B200I_T_BF16)
-        attend_plain_kernel<float, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
-    else
-        attend_plain_kernel<float, float><<<grid, 128, 0, st>>>(a);
-    LIBRARY_CUDA_TRY(cudaGetLastError());
-    b200i_library::count_launches(1);
+    const AttendPlan p = attend_plan(dev, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
+    if (ws_bytes < p.cut.bytes) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.cut.bytes);
+    if (p.few) {
+        if (row_type == B200I_T_BF16)
+            LIBRARY_CUDA_TRY((launch_few<__nv_bfloat16, __nv_bfloat16>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
+        else if (cache_type == B200I_T_BF16)
+            LIBRARY_CUDA_TRY((launch_few<float, __nv_bfloat16>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
+        else
+            LIBRARY_CUDA_TRY((launch_few<float, float>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
+    } else {
+        const long long units = rows * n_heads;
+        if ((units + 3) / 4 > MOST) return refuse(err, err_cap, "paged_attention: too many rows for one call");
+        const unsigned grid = (unsigned)((units + 3) / 4);
+        if (row_type == B200I_T_BF16)
+            attend_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
+        else if (cache_type == B200I_T_BF16)
+            attend_plain_kernel<float, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
+        else
+            attend_plain_kernel<float, float><<<grid, 128, 0, st>>>(a);
+        LIBRARY_CUDA_TRY(cudaGetLastError());
+        launches = 1;
+    }
+    b200i_library::count_launches(launches);
     b200i_library::accept(err, err_cap);
     return 0;
 }

@@ -145,7 +145,7 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
         return out
     with _on(q.device):
         types = _TYPES[q.dtype], _TYPES[k_cache.dtype]
-        need = int(_native.lib().b200i_paged_attention_workspace_bytes(q.device.index, *types, rows, batch, n_heads, n_kv, hd, max_new, max_length))
+        need = int(_native.lib().b200i_paged_attention_workspace_bytes(q.device.index, *types, rows, batch, n_heads, n_kv, hd, max_new, max_length, int(window)))
         ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
         _native.call("b200i_paged_attention", q.device.index, _stream(q.device), _vp(out), _vp(q), ldq, _vp(k_cache), _vp(v_cache), *types, _vp(page_table), _vp(cu),
                      _vp(lengths), rows, batch, n_heads, n_kv, hd, pages, page, max_pages, max_new, max_length, 1.0 / math.sqrt(hd) if scale is None else float(scale),
