@@ -6,6 +6,8 @@
 #include "paged.cuh"
 #include "paged_append.cuh"
 #include "paged_few.cuh"
+#include "paged_fine.cuh"
+#include "paged_many.cuh"
 
 using namespace b200i;
 using b200i_library::refuse;
@@ -23,6 +25,7 @@ int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cac
         return refuse(err, err_cap, "%s: extents must be positive", who);
     if (rows > MOST / 2 || batch > MOST / 2 || pages > MOST || max_pages > MOST || max_pages * page > MOST)
         return refuse(err, err_cap, "%s: rows, sequences, pages and positions are counted in 31 bits", who);
+    if (rows * n_heads > MOST) return refuse(err, err_cap, "%s: rows times heads are counted in 31 bits", who);
     if (n_heads % n_kv != 0 || n_heads > 65535) return refuse(err, err_cap, "%s: n_heads must be a multiple of n_kv and below 65536", who);
     if (head_dim % 8 != 0 || head_dim > PAGED_MAX_HD) return refuse(err, err_cap, "%s: head_dim must be a multiple of 8 up to %d", who, PAGED_MAX_HD);
     if (page < 16 || page > 256 || (page & (page - 1)) != 0) return refuse(err, err_cap, "%s: a page holds a power of two from 16 to 256 positions", who);
@@ -51,16 +54,20 @@ struct AttendPlan {
     int few;      // rows of a sequence and key head, where they are few (else 0)
     int hdp, nt;  // head_dim as it is laid out in shared memory; sets of eight rows
     FewPlan cut;
+    ManyPlan cut_many; // where they are many
+    int64_t bytes() const { return few ? cut.bytes : cut_many.bytes; }
 };
 constexpr int FEW_ROWS = 16;
 
-AttendPlan attend_plan(int device, int64_t cache_type, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
+AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
     AttendPlan p = {};
     p.hdp = head_dim <= 64 ? 64 : 128;
     const int64_t group = n_heads / n_kv;
     if (max_new <= FEW_ROWS && max_new * group <= FEW_ROWS) {
         p.few = (int)(max_new * group), p.nt = p.few <= 8 ? 1 : 2;
         p.cut = few_plan(b200i_library::device_sms(device), (int)batch, (int)n_kv, p.hdp, p.nt, cache_type == B200I_T_F32 ? 32 : 64, max_new, max_length, (int)std::min(window, MOST));
+    } else {
+        p.cut_many = many_plan(b200i_library::device_sms(device), row_type == B200I_T_BF16 ? ManyShape<128>::BLOCK_ROWS : FINE_ROWS, p.hdp);
     }
     return p;
 }
@@ -106,10 +113,9 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
 int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
                                               int64_t max_new, int64_t max_length, int64_t window) {
     if (rows <= 0 || batch <= 0 || n_kv <= 0 || n_heads < n_kv || head_dim <= 0 || max_new <= 0 || max_length <= 0 || window < 0) return 0;
-    (void)row_type;
     int dev = (int)device;
     if (device < 0 && cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); dev = -1; }
-    return attend_plan(dev, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window).cut.bytes;
+    return attend_plan(dev, row_type, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window).bytes();
 }
 
 int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, int64_t row_type, int64_t cache_type,
@@ -129,8 +135,8 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const AttendPlan p = attend_plan(dev, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
-    if (ws_bytes < p.cut.bytes) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.cut.bytes);
+    const AttendPlan p = attend_plan(dev, row_type, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
+    if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
     if (p.few) {
         if (row_type == B200I_T_BF16)
             LIBRARY_CUDA_TRY((launch_few<__nv_bfloat16, __nv_bfloat16>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
@@ -139,17 +145,12 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
         else
             LIBRARY_CUDA_TRY((launch_few<float, float>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
     } else {
-        const long long units = rows * n_heads;
-        if ((units + 3) / 4 > MOST) return refuse(err, err_cap, "paged_attention: too many rows for one call");
-        const unsigned grid = (unsigned)((units + 3) / 4);
         if (row_type == B200I_T_BF16)
-            attend_plain_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
+            LIBRARY_CUDA_TRY(p.hdp == 64 ? launch_many_as<64>(a, p.cut_many, ws, dev, st, &launches) : launch_many_as<128>(a, p.cut_many, ws, dev, st, &launches));
         else if (cache_type == B200I_T_BF16)
-            attend_plain_kernel<float, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
+            LIBRARY_CUDA_TRY((p.hdp == 64 ? launch_fine_as<__nv_bfloat16, 64>(a, p.cut_many, ws, dev, st, &launches) : launch_fine_as<__nv_bfloat16, 128>(a, p.cut_many, ws, dev, st, &launches)));
         else
-            attend_plain_kernel<float, float><<<grid, 128, 0, st>>>(a);
-        LIBRARY_CUDA_TRY(cudaGetLastError());
-        launches = 1;
+            LIBRARY_CUDA_TRY((p.hdp == 64 ? launch_fine_as<float, 64>(a, p.cut_many, ws, dev, st, &launches) : launch_fine_as<float, 128>(a, p.cut_many, ws, dev, st, &launches)));
     }
     b200i_library::count_launches(launches);
     b200i_library::accept(err, err_cap);

@@ -142,20 +142,4 @@ __device__ __noinline__ void attend_row_plain(const AttendCall &a, int b, int ro
         if (lane + 32 * i < hd) paged_write(out + lane + 32 * i, l == 0.0f ? 0.0f : (acc[i] + part[i]) / l);
 }
 
-// The simplest form of the operator: a warp a (row, head).
-template <typename RT, typename CT>
-__global__ void __launch_bounds__(128) attend_plain_kernel(const AttendCall a) {
-    const long long unit = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (unit >= a.c.rows * a.c.heads) return;
-    const int row = (int)(unit / a.c.heads), h = (int)(unit % a.c.heads);
-    const int b = paged_row_seq(a.c, row);
-    if (b < 0) return; // a row of no sequence is left as it is
-    const PagedSeq s = paged_seq(a.c, b);
-    if (row - s.first >= a.max_new) {
-        if ((threadIdx.x & 31) == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
-        return;
-    }
-    attend_row_plain<RT, CT>(a, b, row, s.pos0 + row - s.first, s.length, h);
-}
-
 } // namespace b200i

@@ -51,39 +51,37 @@ __device__ __forceinline__ int few_tiles(const AttendCall &a, const PagedSeq &s,
     return s.n == 0 ? 0 : max(1, (s.length + keys - 1) / keys - t0);
 }
 
-struct FewPlace {
-    int b, kvh, tile, count; // a tile of an item of `count`
-    long long left;          // tiles of the block from here
-    long long line;          // where on the line the item begins
-    long long per;           // tiles a block
+// A block's place on the line of all items' tiles.
+struct LinePlace {
+    int b, kvh;       // the sequence and key head in which it begins
+    long long in;     // tiles of that sequence and key head before it
+    long long size;   // tiles of the sequence and key head
+    long long left;   // tiles of the block
+    long long per;    // tiles a block
+    long long start;  // where the block begins
 };
 
-// Where block `block` of `blocks` begins on the line. All threads of the block call it; `sh` holds 16 words.
-__device__ __forceinline__ FewPlace few_place(const AttendCall &a, int keys, bool whole, int block, int blocks, long long *sh) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    int mine = 0, t0;
-    long long sum = 0;
-    for (int b = tid; b < a.c.batch; b += blockDim.x) {
-        mine = few_tiles(a, paged_seq(a.c, b), keys, &t0);
-        sum += whole ? (mine > 0) : mine;
-    }
-    const long long own = sum; // of one sequence where the batch is within the block
+// `size_of(b)`: the tiles of one key head of sequence b. All threads of the block call it; `sh` holds 16 words.
+template <typename F>
+__device__ __forceinline__ LinePlace line_place(const PagedCall &c, F size_of, int block, int blocks, long long *sh) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
+    long long mine = 0, sum = 0;
+    for (int b = tid; b < c.batch; b += blockDim.x) sum += mine = size_of(b);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
     if (lane == 0) sh[warp] = sum;
     __syncthreads();
     long long total = 0;
     for (int w = 0; w < warps; w++) total += sh[w];
-    total *= a.c.kv;
+    total *= c.kv;
     const long long per = (total + blocks - 1) / blocks, start = per * block;
     __syncthreads();
-    if (tid == 0) sh[8] = -1;
+    if (tid == 0) sh[12] = -1;
     long long before = 0; // of the sequences before this round's
-    for (int b0 = 0; b0 < a.c.batch && start < total; b0 += blockDim.x) {
+    for (int b0 = 0; b0 < c.batch && start < total; b0 += blockDim.x) {
         const int b = b0 + tid;
-        int n = 0;
-        if (b < a.c.batch) n = a.c.batch <= blockDim.x ? mine : few_tiles(a, paged_seq(a.c, b), keys, &t0);
-        const long long here = a.c.batch <= blockDim.x ? own : (whole ? (n > 0) : n);
+        long long here = mine; // what the first loop left, where that saw the whole batch
+        if (c.batch > (int)blockDim.x) here = b < c.batch ? size_of(b) : 0;
         long long scan = here;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -97,18 +95,36 @@ __device__ __forceinline__ FewPlace few_place(const AttendCall &a, int keys, boo
             if (w < warp) base += sh[w];
             before += sh[w];
         }
-        const long long from = (base + scan - here) * a.c.kv, to = (base + scan) * a.c.kv;
+        const long long from = (base + scan - here) * c.kv, to = (base + scan) * c.kv;
         if (start >= from && start < to) { // one thread of one round
-            const long long in = start - from, size = whole ? 1 : n;
-            sh[8] = b, sh[9] = in / size, sh[10] = whole ? 0 : in % size, sh[11] = n, sh[12] = start - (whole ? 0 : in % size);
+            const long long in = start - from;
+            sh[12] = b, sh[13] = in / here, sh[14] = in % here, sh[15] = here;
         }
         __syncthreads();
     }
     __syncthreads();
+    LinePlace p;
+    p.per = per, p.start = start;
+    p.left = sh[12] < 0 ? 0 : min(per, total - start);
+    p.b = (int)sh[12], p.kvh = (int)sh[13], p.in = sh[14], p.size = sh[15];
+    return p;
+}
+
+struct FewPlace {
+    int b, kvh, tile, count; // a tile of an item of `count`
+    long long left;          // tiles of the block from here (where items are whole: items)
+    long long line;          // where on the line the item begins
+    long long per;           // tiles a block
+};
+__device__ __forceinline__ FewPlace few_place(const AttendCall &a, int keys, bool whole, int block, int blocks, long long *sh) {
+    const auto tiles = [&](int b) {
+        int t0;
+        return few_tiles(a, paged_seq(a.c, b), keys, &t0);
+    };
+    const LinePlace l = line_place(a.c, [&](int b) -> long long { return whole ? (long long)(tiles(b) > 0) : (long long)tiles(b); }, block, blocks, sh);
     FewPlace p;
-    p.per = per;
-    p.left = sh[8] < 0 ? 0 : min(per, total - start);
-    p.b = (int)sh[8], p.kvh = (int)sh[9], p.tile = (int)sh[10], p.count = (int)sh[11], p.line = sh[12];
+    p.b = l.b, p.kvh = l.kvh, p.tile = whole ? 0 : (int)l.in, p.count = l.left > 0 ? (whole ? tiles(l.b) : (int)l.size) : 0;
+    p.left = l.left, p.line = l.start - l.in, p.per = l.per;
     return p;
 }
 
@@ -168,14 +184,21 @@ __device__ __forceinline__ void few_values(unsigned (&f)[3][4], const unsigned c
     }
 }
 
-// d += A B over pieces of both: those whose places together are below three (2^-24 of the whole and up)
-template <int PA, int PB>
+// d += A B over pieces of both: those whose places together are below three (2^-24 of the whole and up), the smallest first. The
+// tensor cores cut their sums off instead of rounding them: with EXACT the product begins at zero and is added to d in 32-bit arithmetic
+// (32 heads of 1250 float32 keys are off by 3.1e-6 without it).
+template <bool EXACT, int PA, int PB>
 __device__ __forceinline__ void few_mma(float (&d)[4], const unsigned (&a)[PA][4], const unsigned (&b0)[PB], const unsigned (&b1)[PB]) {
+    float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < PA; i++)
+    for (int places = 2; places >= 0; places--)
 #pragma unroll
-        for (int j = 0; j < PB; j++)
-            if (i + j < 3) pg_mma(d, a[i], b0[j], b1[j]);
+        for (int i = 0; i < PA; i++)
+            if (places - i >= 0 && places - i < PB) pg_mma(EXACT ? part : d, a[i], b0[places - i], b1[places - i]);
+    if (EXACT) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] += part[i];
+    }
 }
 
 template <typename RT, typename CT, int HDP, int NT>
@@ -183,6 +206,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attend_few_kernel(const __grid
     using Shape = FewShape<HDP, NT>;
     constexpr int KEYS = FewKeys<CT>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, BOX_COLS = 128 / (int)sizeof(CT), BOXES = HDP / BOX_COLS;
     constexpr int QP = sizeof(RT) == 4 ? 3 : 1, CP = sizeof(CT) == 4 ? 3 : 1, PP = sizeof(RT) == 4 ? 3 : 2; // pieces of a query, of a key or value, of a weight
+    constexpr bool EXACT = sizeof(RT) == 4;
     constexpr int GROUPS = KEYS / 16, KS = HDP / 16, ROWS = NT * 8;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *ring = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u);
@@ -327,7 +351,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attend_few_kernel(const __grid
                     unsigned k[CP][4];
                     few_keys(k, kt, key0, ks, lane, static_cast<const CT *>(nullptr));
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) few_mma<CP, QP>(z[nt], k, q0[nt][ks], q1[nt][ks]);
+                    for (int nt = 0; nt < NT; nt++) few_mma<EXACT>(z[nt], k, q0[nt][ks], q1[nt][ks]);
                 }
                 const bool edge = j0 + 16 > s.pos0 + 1 || j0 < all_lo;
                 unsigned w0[NT][PP], w1[NT][PP];
@@ -384,7 +408,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attend_few_kernel(const __grid
                     unsigned v[CP][4];
                     few_values(v, vt, key0, mt, lane, keep, static_cast<const CT *>(nullptr));
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) few_mma<CP, PP>(o[nt][mt], v, w0[nt], w1[nt]);
+                    for (int nt = 0; nt < NT; nt++) few_mma<EXACT>(o[nt][mt], v, w0[nt], w1[nt]);
                 }
             }
             __syncwarp();

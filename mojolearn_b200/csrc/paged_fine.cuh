@@ -1,0 +1,435 @@
+// Attention of many float32 rows over a paged cache on the tcgen05 tensor cores, to 32-bit accuracy.
+//
+// A 32-bit word is the sum of three bfloat16 pieces of 8 bits each, and a product of two words the sum of the products of their
+// pieces; those down to 2^-24 of the whole are taken (three of them where the cache is bfloat16, which is one piece; six where it is
+// float32), each exact, the small ones first. Weights go in as three pieces too: two leave 2.4e-6 of an output out (9000 keys).
+// The tensor pipe cuts its sums off where it adds to a large one (an output summed there over all keys was off by 2.2e-6 to 4.3e-6, by 1e-6 or less
+// this way): a tile's P V begins at zero, and the softmax threads add it to their row's 32-bit registers, rounding to nearest.
+//
+// Bound: the tensor pipe at 6 (bfloat16 cache) or 12 (float32) times head_dim x 2 operations a (row, key) against 71 TFLOP/s of fma:
+// 270 to 135 TFLOP/s of 4 head_dim operations at the measured bfloat16 rate. Rows, items, parts and the line are those of paged_many.cuh; a block
+// has 128 rows and one stream of 64-key tiles, and two S in tensor memory, so that the softmax of one tile runs under the products of its
+// neighbours; the output of a tile is read while the next score is made. The pieces of Q are in tensor memory (192 columns of 512 at head_dim 128) beside O (128) and two S that their P is
+// written over (96 each): the products read only keys and values from shared memory, whose 64 rows a product would not pay for Q's.
+// A bfloat16 cache comes in by tensor-map copies; of a float32 one four warps read the rows and write their pieces.
+#pragma once
+#include "paged_many.cuh"
+
+namespace b200i {
+
+constexpr int FINE_THREADS = 384, FINE_KEYS = 64, FINE_ROWS = 128; // four warps of softmax, four that bring keys and values, and a group of which one issues
+constexpr int FINE_REGS = 240, FINE_REGS_LOAD = 144, FINE_REGS_LESS = 120; // a thread: together 504 = 3 x 168, what the block is launched with
+
+template <typename CT, int HDP> struct FineShape {
+    static constexpr int PIECES = sizeof(CT) == 4 ? 3 : 1;
+    static constexpr int TILE = HDP * 128;               // bytes of 64 rows of bfloat16
+    static constexpr int SLOT = PIECES * TILE;
+    static constexpr int ROOM = 216 * 1024 / SLOT;
+    static constexpr int SLOTS = ROOM > 8 ? 8 : ROOM;
+    static constexpr int SMEM = 1024 + SLOTS * SLOT + 256;
+};
+
+template <typename CT, int HDP>
+__global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ManyCall f) {
+    using Shape = FineShape<CT, HDP>;
+    using Walk = ManyWalk<FINE_ROWS, FINE_KEYS, 1>;
+    constexpr int SLOTS = Shape::SLOTS, SLOT = Shape::SLOT, TILE = Shape::TILE, CP = Shape::PIECES, BOXES = HDP / 64, HALF_COLS = FINE_KEYS * 128, BR = FINE_ROWS;
+    constexpr int Q_COLS = HDP / 2, O_AT = 3 * Q_COLS, S_AT = O_AT + HDP, S_COLS = 96; // columns of tensor memory
+    static_assert(S_AT + 2 * S_COLS <= 512, "tensor memory");
+    extern __shared__ __align__(128) unsigned char smem[];
+    unsigned char *ring = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u);
+    unsigned long long *full = reinterpret_cast<unsigned long long *>(ring + SLOTS * SLOT), *empty = full + SLOTS;
+    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *o_free = o_full + 1, *q_full = o_free + 1, *tail = q_full + 1; // 2 SLOTS + 8 <= 32 words
+    __shared__ long long place[16];
+    __shared__ unsigned tmem_slot;
+    __shared__ int dead;
+    const AttendCall &a = f.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int s = 0; s < SLOTS; s++) {
+            pg_bar_init(&full[s], CP == 1 ? 1 : 128);
+            pg_bar_init(&empty[s], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            pg_bar_init(&s_full[i], 1);
+            pg_bar_init(&p_full[i], 128);
+        }
+        pg_bar_init(o_full, 1);
+        pg_bar_init(o_free, 128);
+        pg_bar_init(q_full, 128);
+        pg_bar_init(tail, 1);
+        dead = 0;
+        f.head[blockIdx.x * 8] = -1;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_smem(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    const LinePlace line = line_place(a.c, [&](int b) { return Walk::steps_of(a, b); }, blockIdx.x, gridDim.x, place);
+    pg_fence_before();
+    __syncthreads();
+    pg_fence_after();
+    const unsigned tmem = tmem_slot;
+    const int page = 1 << a.c.page_shift;
+    Walk w;
+    w.begin(a, line);
+    const ManyItem &item = w.item;
+
+    if (warp >= 4 && warp < 8) { // ---------------- keys and values ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FINE_REGS_LOAD));
+        // in the order of their first use: K0 K1 V0 K2 V1 K3 ...
+        const auto load_of = [](int u, int tiles, bool *is_v) {
+            const int lead = min(2, tiles), v = u - lead;
+            const bool mixed = v < 2 * (tiles - lead);
+            *is_v = v >= 0 && (!mixed || (v & 1) == 0);
+            return v < 0 ? u : (mixed ? (*is_v ? v / 2 : v / 2 + lead) : (tiles - lead) + (v - 2 * (tiles - lead)));
+        };
+        unsigned ld = 0;
+        bool alive = true;
+        if (CP == 1 && warp == 4) {
+            unsigned tails = 0;
+            const int box_rows = min(page, FINE_KEYS);
+            while (w.left > 0 && alive) {
+                const int tiles = w.tiles(), first = w.first(), last_page = (item.high - 1) >> a.c.page_shift;
+                const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
+                for (int u = 0; u < 2 * tiles; u++, ld++) {
+                    bool is_v;
+                    const int tile = load_of(u, tiles, &is_v), slot = (int)(ld % SLOTS), pos = (item.t0 + first + tile) * FINE_KEYS;
+                    if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u))) {
+                        alive = false;
+                        break;
+                    }
+                    const int there = min(FINE_KEYS / box_rows, max(0, (item.high - pos + box_rows - 1) / box_rows)); // pieces that hold positions that some row sees
+                    unsigned char *dst = ring + slot * SLOT;
+                    const bool clean = is_v && (pos + FINE_KEYS > item.high || pos < item.low); // rows of values that no row sees are to be zero
+                    unsigned long long *bar = clean ? tail : &full[slot];
+                    if (lane == 0) pg_bar_expect(bar, (unsigned)(there * box_rows * 128 * BOXES));
+                    __syncwarp();
+                    for (int x = lane; x < there * BOXES; x += 32) {
+                        const int piece = x / BOXES, box = x % BOXES, at = pos + piece * box_rows, index = at >> a.c.page_shift;
+                        int row = a.c.pages * a.c.kv * page; // past the pool: zeros
+                        const int id = index <= last_page ? ids[index] : -1;
+                        if ((unsigned)id < (unsigned)a.c.pages)
+                            row = ((id * a.c.kv + w.kvh) << a.c.page_shift) + (at & (page - 1));
+                        else
+                            atomicExch(a.c.status, PAGED_BAD_PAGE);
+                        pg_tma_load(dst + box * HALF_COLS + piece * (box_rows * 128), is_v ? &map_v : &map_k, bar, box * 64, row);
+                    }
+                    if (clean) {
+                        if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(tail, tails & 1u))) {
+                            alive = false;
+                            break;
+                        }
+                        tails++;
+                        for (int x = lane; x < FINE_KEYS * 8 * BOXES; x += 32) { // 16 bytes each; a row's are in one swizzle atom, so their order does not matter
+                            const int at = pos + ((x >> 3) & (FINE_KEYS - 1));
+                            if (at >= item.high || at < item.low) *reinterpret_cast<uint4 *>(dst + x * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) pg_bar_arrive(&full[slot]);
+                    }
+                }
+                if (alive) w.next(a);
+            }
+            if (!alive) { // copies in flight end before the block does
+                if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
+                for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
+            }
+        } else if (CP == 3) {
+            constexpr int CHUNKS = HDP / 8, ROWS_AT_ONCE = 128 / CHUNKS, N = FINE_KEYS / ROWS_AT_ONCE; // a thread: N pieces of 8 columns, of rows ROWS_AT_ONCE apart
+            const int mine = tid - 128, chunk = mine % CHUNKS, row0 = mine / CHUNKS;
+            while (w.left > 0) {
+                const int tiles = w.tiles(), first = w.first();
+                const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
+                const auto page_ids = [&](int (&id)[N], int u) { // the pages of a load's rows; -1: nothing to read
+                    bool is_v;
+                    const int pos = (item.t0 + first + load_of(u, tiles, &is_v)) * FINE_KEYS + row0;
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int at = pos + i * ROWS_AT_ONCE;
+                        id[i] = at >= item.low && at < item.high ? ids[at >> a.c.page_shift] : -1;
+                        if (at >= item.low && at < item.high && (unsigned)id[i] >= (unsigned)a.c.pages) {
+                            atomicExch(a.c.status, PAGED_BAD_PAGE);
+                            id[i] = -1;
+                        }
+                    }
+                };
+                int id[N];
+                page_ids(id, 0);
+                for (int u = 0; u < 2 * tiles; u++, ld++) {
+                    bool is_v;
+                    const int tile = load_of(u, tiles, &is_v), slot = (int)(ld % SLOTS), pos = (item.t0 + first + tile) * FINE_KEYS + row0;
+                    const float *from = static_cast<const float *>(is_v ? a.v : a.k);
+                    float4 x[N][2];
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        x[i][0] = x[i][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (id[i] >= 0 && chunk * 8 < a.c.hd) {
+                            const long long at = ((((long long)id[i] * a.c.kv + w.kvh) << a.c.page_shift) + ((pos + i * ROWS_AT_ONCE) & (page - 1))) * a.c.hd + chunk * 8;
+                            x[i][0] = __ldg(reinterpret_cast<const float4 *>(from + at)), x[i][1] = __ldg(reinterpret_cast<const float4 *>(from + at + 4));
+                        }
+                    }
+                    if (u + 1 < 2 * tiles) page_ids(id, u + 1);
+                    if (alive && !pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u)) {
+                        atomicExch(a.c.status, PAGED_WAIT);
+                        alive = false; // it goes on without waiting and without writing
+                    }
+                    if (!alive) continue;
+                    unsigned char *dst = ring + slot * SLOT + (chunk >> 3) * HALF_COLS;
+#pragma unroll
+                    for (int i = 0; i < N; i++) {
+                        const int row = row0 + i * ROWS_AT_ONCE;
+                        unsigned p[4][3];
+                        pg_split<3>(p[0], x[i][0].x, x[i][0].y), pg_split<3>(p[1], x[i][0].z, x[i][0].w);
+                        pg_split<3>(p[2], x[i][1].x, x[i][1].y), pg_split<3>(p[3], x[i][1].z, x[i][1].w);
+#pragma unroll
+                        for (int k = 0; k < 3; k++)
+                            *reinterpret_cast<uint4 *>(dst + k * TILE + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    pg_bar_arrive(&full[slot]);
+                }
+                w.next(a);
+            }
+        }
+    } else if (warp >= 8) { // ---------------- the products ----------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FINE_REGS_LESS));
+        if (tid == 256) {
+            unsigned ld = 0, items = 0, tile_count = 0;
+            bool alive = true;
+            const unsigned r0 = pg_smem(ring);
+            const auto here = [&](unsigned long long *bar, unsigned parity) {
+                if (alive && !pg_bar_wait(bar, parity)) alive = false;
+                pg_fence_after();
+                return alive;
+            };
+            const auto score = [&](unsigned i, unsigned buffer) { // S = Q K^T, K being load i
+                const unsigned d = tmem + S_AT + buffer * S_COLS;
+                bool add = false;
+#pragma unroll 1
+                for (int places = 2; places >= 0; places--) // of the pieces of both together: the smallest products first
+#pragma unroll 1
+                    for (int k = 0; k < CP && k <= places; k++) {
+                        const unsigned kd = pg_desc_low(r0 + (i % SLOTS) * SLOT + k * TILE), qa = tmem + (places - k) * Q_COLS;
+#pragma unroll
+                        for (int ks = 0; ks < HDP / 16; ks++) {
+                            pg_mma_ts(d, qa + ks * 8, pg_desc(kd + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_idesc(FINE_KEYS, false), add);
+                            add = true;
+                        }
+                    }
+                pg_commit(&empty[i % SLOTS]);
+                pg_commit(&s_full[buffer]);
+            };
+            const auto value = [&](unsigned i, unsigned buffer) { // O = P V, V being load i
+                bool add = false;
+#pragma unroll 1
+                for (int places = 2; places >= 0; places--)
+#pragma unroll 1
+                    for (int k = 0; k < CP && k <= places; k++) {
+                        const unsigned vd = pg_desc_low(r0 + (i % SLOTS) * SLOT + k * TILE, HALF_COLS), pa = tmem + S_AT + buffer * S_COLS + (places - k) * 32;
+#pragma unroll
+                        for (int ks = 0; ks < FINE_KEYS / 16; ks++) {
+                            pg_mma_ts(tmem + O_AT, pa + ks * 8, pg_desc(vd + ks * 2048 / 16), pg_idesc(HDP, true), add);
+                            add = true;
+                        }
+                    }
+                pg_commit(&empty[i % SLOTS]);
+                pg_commit(o_full);
+            };
+            while (w.left > 0 && alive) {
+                const int tiles = w.tiles();
+                here(q_full, items & 1u);
+                items++;
+                const unsigned t0 = tile_count; // tiles done before the item: the buffers and barriers go on from item to item
+                for (int j = 0; j < min(2, tiles) && alive; j++)
+                    if (here(&full[ld % SLOTS], (ld / SLOTS) & 1u)) score(ld++, (t0 + j) & 1u);
+                for (int j = 0; j < tiles && alive; j++) {
+                    const unsigned t = t0 + j;
+                    if (!here(&full[ld % SLOTS], (ld / SLOTS) & 1u) || !here(&p_full[t & 1u], (t >> 1) & 1u) || !here(o_free, (t & 1u) ^ 1u)) break; // O of the tile before is read
+                    value(ld++, t & 1u);
+                    if (j + 2 < tiles && here(&full[ld % SLOTS], (ld / SLOTS) & 1u)) score(ld++, t & 1u);
+                }
+                tile_count += tiles;
+                if (alive) w.next(a);
+            }
+            if (!alive) atomicExch(a.c.status, PAGED_WAIT);
+        }
+        __syncwarp();
+    } else { // ---------------- the softmax: a thread a row ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FINE_REGS));
+        const unsigned at = tmem + ((unsigned)(warp * 32) << 16);
+        const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+        const float size = unit == 0.0f ? 1.0f : fabsf(unit);
+        unsigned tile_count = 0;
+        bool alive = true, first_part = true;
+        const auto give_up = [&] {
+            if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
+            alive = false; // it goes on without waiting; nothing of the block is stored from here on
+        };
+        while (w.left > 0) {
+            const int tiles = w.tiles(), first = w.first(), row = item.row0 + tid;
+            const bool valid = tid < item.rows;
+            if (w.s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
+            const float *src = static_cast<const float *>(a.q) + (long long)(w.s.first + row / a.c.group) * a.ldq + (long long)(w.kvh * a.c.group + row % a.c.group) * a.c.hd;
+#pragma unroll 1
+            for (int c = 0; c < HDP; c += 32) { // the row's pieces into tensor memory
+                unsigned p[3][16];
+#pragma unroll
+                for (int i = 0; i < 32; i += 4) {
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (valid && c + i < a.c.hd) x = *reinterpret_cast<const float4 *>(src + c + i);
+                    unsigned lo[3], hi[3];
+                    pg_split<3>(lo, x.x, x.y);
+                    pg_split<3>(hi, x.z, x.w);
+#pragma unroll
+                    for (int k = 0; k < 3; k++) p[k][i / 2] = lo[k], p[k][i / 2 + 1] = hi[k];
+                }
+#pragma unroll
+                for (int k = 0; k < 3; k++) pg_st16(at + k * Q_COLS + c / 2, p[k]);
+            }
+            pg_wait_st();
+            pg_fence_before();
+            pg_bar_arrive(q_full);
+            const int hi = valid ? w.s.pos0 + row / a.c.group + 1 : 0, lo = a.window ? hi - a.window : 0;
+            float m = -INFINITY, l = 0.0f, o[HDP];
+#pragma unroll
+            for (int c = 0; c < HDP; c++) o[c] = 0.0f;
+            const auto take = [&](unsigned t) { // o += the output of tile t
+                if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(o_full, t & 1u))) give_up();
+                if (!alive) return;
+                pg_fence_after();
+#pragma unroll
+                for (int c = 0; c < HDP; c += 32) {
+                    unsigned v[32];
+                    pg_ld32(v, at + O_AT + c);
+                    pg_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[c + i] += __uint_as_float(v[i]);
+                }
+                pg_fence_before();
+                pg_bar_arrive(o_free);
+            };
+            for (int j = 0; j < tiles; j++) {
+                const unsigned t = tile_count + j, s_at = at + S_AT + (t & 1u) * S_COLS;
+                const int pos = (item.t0 + first + j) * FINE_KEYS;
+                if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&s_full[t & 1u], (t >> 1) & 1u))) give_up();
+                if (!alive) continue;
+                pg_fence_after();
+                unsigned z[64];
+                pg_ld32(z, s_at), pg_ld32(z + 32, s_at + 32);
+                pg_wait_ld();
+                float *x = reinterpret_cast<float *>(z);
+                if (a.softcap > 0.0f) pg_tanh<64>(x, inner);
+                if (unit <= 0.0f) { // a negative scale turns the order of the scores around, none makes them all alike
+#pragma unroll
+                    for (int c = 0; c < 64; c++) x[c] = unit < 0.0f ? -x[c] : 0.0f;
+                }
+                if (__any_sync(0xFFFFFFFFu, valid && (pos + FINE_KEYS > hi || pos < lo))) {
+#pragma unroll
+                    for (int c = 0; c < 64; c++)
+                        if (pos + c >= hi || pos + c < lo) x[c] = -INFINITY;
+                }
+                float top[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int c = 4; c < 64; c += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], x[c + e]);
+                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * size, to = most > m ? most : m;
+                const float keep = m == -INFINITY ? 0.0f : paged_exp2(m - to), base = to == -INFINITY ? 0.0f : to;
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 64; c += 16) {
+                    unsigned p[3][8];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                        const float w0 = paged_exp2(fmaf(x[c + i], size, -base)), w1 = paged_exp2(fmaf(x[c + i + 1], size, -base));
+                        sum[i & 2] += w0, sum[(i & 2) + 1] += w1;
+                        unsigned piece[3];
+                        pg_split<3>(piece, w0, w1);
+#pragma unroll
+                        for (int k = 0; k < 3; k++) p[k][i / 2] = piece[k];
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; k++) pg_st8(s_at + k * 32 + c / 2, p[k]);
+                }
+                pg_wait_st();
+                pg_fence_before();
+                pg_bar_arrive(&p_full[t & 1u]);
+                l = fmaf(l, keep, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                if (j > 0) take(t - 1);
+                if (__any_sync(0xFFFFFFFFu, to > m)) {
+#pragma unroll
+                    for (int c = 0; c < HDP; c++) o[c] *= keep;
+                }
+                m = to;
+            }
+            tile_count += tiles;
+            take(tile_count - 1);
+
+            // ---- the item's (or its part's) end ----
+            const bool is_whole = w.skip == 0 && w.steps() == item.steps;
+            const long long slot = (long long)blockIdx.x * 2 + (first_part && w.skip > 0 ? 0 : 1);
+            bool wrong = false;
+            if (valid && alive && !dead) {
+                float *out = static_cast<float *>(a.out) + ((long long)(w.s.first + row / a.c.group) * a.c.heads + w.kvh * a.c.group + row % a.c.group) * a.c.hd;
+                float4 *part = reinterpret_cast<float4 *>(f.part + (slot * BR + tid) * HDP);
+#pragma unroll
+                for (int c = 0; c < HDP; c += 4) {
+                    if (!is_whole) {
+                        part[c / 4] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                    } else if (c < a.c.hd) {
+                        const float4 y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(__fdiv_rn(o[c], l), __fdiv_rn(o[c + 1], l), __fdiv_rn(o[c + 2], l), __fdiv_rn(o[c + 3], l));
+                        *reinterpret_cast<float4 *>(out + c) = y;
+                        wrong |= !isfinite(y.x) || !isfinite(y.y) || !isfinite(y.z) || !isfinite(y.w);
+                    }
+                }
+                if (!is_whole) {
+                    float *ml = f.part + (long long)gridDim.x * 2 * BR * HDP + slot * 2 * BR;
+                    ml[tid] = m, ml[BR + tid] = l;
+                }
+            }
+            if (!is_whole && tid == 0 && w.skip == 0 && alive && !dead) {
+                int *head = f.head + blockIdx.x * 8;
+                head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = (int)(w.line - line.start), head[5] = (int)line.per;
+            }
+            unsigned rest = __ballot_sync(0xFFFFFFFFu, wrong);
+            while (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
+                const int k = __ffs(rest) - 1, bad = __shfl_sync(0xFFFFFFFFu, row, k);
+                rest &= rest - 1;
+                attend_row_plain<float, CT>(a, w.b, w.s.first + bad / a.c.group, w.s.pos0 + bad / a.c.group, w.s.length, w.kvh * a.c.group + bad % a.c.group);
+            }
+            first_part = false;
+            w.next(a);
+        }
+    }
+    pg_fence_before();
+    __syncthreads();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ---- host side ----
+template <typename CT, int HDP>
+cudaError_t launch_fine_as(const AttendCall &a, const ManyPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
+    using Shape = FineShape<CT, HDP>;
+    ManyCall f;
+    f.a = a, f.part = static_cast<float *>(ws), f.head = reinterpret_cast<int *>(static_cast<float *>(ws) + p.part_floats);
+    alignas(64) CUtensorMap map_k, map_v;
+    const long long rows = ((long long)a.c.pages * a.c.kv) << a.c.page_shift;
+    const int box = std::min(1 << a.c.page_shift, FINE_KEYS);
+    constexpr bool f32 = sizeof(CT) == 4;
+    if (!paged_map(&map_k, a.k, rows, a.c.hd, f32, box) || !paged_map(&map_v, a.v, rows, a.c.hd, f32, box)) return cudaErrorNotSupported;
+    static std::atomic<bool> known[64];
+    if (device >= 64 || !known[device].load()) {
+        const cudaError_t e = cudaFuncSetAttribute(attend_fine_kernel<CT, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+        if (e != cudaSuccess) return e;
+        if (device < 64) known[device].store(true);
+    }
+    attend_fine_kernel<CT, HDP><<<p.blocks, FINE_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
+    attend_join_rows_kernel<float, CT, HDP, FINE_ROWS><<<dim3(p.blocks, FINE_ROWS / 8), 256, 0, st>>>(f);
+    *launches += 2;
+    return cudaGetLastError();
+}
+
+} // namespace b200i
