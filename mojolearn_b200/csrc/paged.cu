@@ -1,5 +1,6 @@
 // The paged cache's entry points of the C ABI: argument checks, choice of kernel, launches. Declared in include/b200i.h.
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/b200i.h"
 #include "library.h"
@@ -26,7 +27,7 @@ int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cac
     if (rows > MOST / 2 || batch > MOST / 2 || pages > MOST || max_pages > MOST || max_pages * page > MOST)
         return refuse(err, err_cap, "%s: rows, sequences, pages and positions are counted in 31 bits", who);
     if (rows * n_heads > MOST) return refuse(err, err_cap, "%s: rows times heads are counted in 31 bits", who);
-    if (n_heads % n_kv != 0 || n_heads > 65535) return refuse(err, err_cap, "%s: n_heads must be a multiple of n_kv and below 65536", who);
+    if (n_heads % n_kv != 0 || n_heads > 32767) return refuse(err, err_cap, "%s: n_heads must be a multiple of n_kv and below 32768", who);
     if (head_dim % 8 != 0 || head_dim > PAGED_MAX_HD) return refuse(err, err_cap, "%s: head_dim must be a multiple of 8 up to %d", who, PAGED_MAX_HD);
     if (page < 16 || page > 256 || (page & (page - 1)) != 0) return refuse(err, err_cap, "%s: a page holds a power of two from 16 to 256 positions", who);
     if ((row_type != B200I_T_F32 && row_type != B200I_T_BF16) || (cache_type != B200I_T_F32 && cache_type != B200I_T_BF16) ||
@@ -38,6 +39,7 @@ int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cac
     while ((1 << shift) < page) shift++;
     c->table = static_cast<const int *>(page_table), c->cu = static_cast<const int *>(cu), c->lengths = static_cast<const int *>(lengths);
     c->rows = rows, c->batch = (int)batch, c->heads = (int)n_heads, c->kv = (int)n_kv, c->group = (int)(n_heads / n_kv), c->hd = (int)head_dim;
+    c->group_part = (unsigned)((1ull << 32) / (unsigned long long)c->group + 1);
     c->pages = (int)pages, c->page_shift = shift, c->max_pages = (int)max_pages;
     return 0;
 }
@@ -130,7 +132,11 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (max_new <= 0 || max_length <= 0) return refuse(err, err_cap, "paged_attention: the bounds on new tokens and lengths must be positive");
     if (window < 0 || !(softcap >= 0.0) || softcap > 1e30 || !(scale > -1e30 && scale < 1e30)) return refuse(err, err_cap, "paged_attention: window, softcap or scale is out of range");
     if (ws_bytes < 0 || (ws_bytes > 0 && !ws)) return refuse(err, err_cap, "paged_attention: a workspace size without a workspace");
-    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.scale = (float)scale, a.softcap = (float)softcap;
+    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.flip = scale < 0.0, a.softcap = (float)softcap;
+    a.scale = std::max(fabsf((float)scale), 1e-30f); // none makes all weights alike, as does next to none
+    a.cap_inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f, a.cap_outer = a.softcap > 0.0f ? a.softcap / a.scale : 0.0f;
+    float power = 1.0f;
+    for (int i = 0; i < 4; i++) power *= a.cap_inner * a.cap_inner, a.cap_near[i] = CAP_NEAR[i] * power;
     a.window = (int)std::min(window, MOST), a.max_new = (int)std::min(max_new, MOST);
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;

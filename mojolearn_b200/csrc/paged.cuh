@@ -25,6 +25,7 @@ struct PagedCall {
     long long rows;        // of q: the extent cu is held to
     int batch, heads, kv, group, hd;
     int pages, page_shift, max_pages;
+    unsigned group_part;   // 2^32 / group + 1, rounded down: the upper half of a product with it is a quotient
 };
 
 // One sequence's part of a call.
@@ -89,7 +90,9 @@ struct AttendCall {
     const void *q, *k, *v;
     void *out;
     long long ldq;  // elements between rows of q
-    float scale, softcap;
+    float scale, softcap;  // scale > 0: a negative one is the queries' sign (flip)
+    int flip;
+    float cap_inner, cap_outer, cap_near[4]; // of capped scores (paged_many.cuh): scale / softcap, its inverse, its even powers times the polynomial's coefficients
     int window;     // 0: none
     int max_new;    // a sequence's rows past these are not computed
 };
@@ -117,7 +120,7 @@ __device__ __noinline__ void attend_row_plain(const AttendCall &a, int b, int ro
             kx[i] = at >= 0 && lane + 32 * i < hd ? paged_read(static_cast<const CT *>(a.k) + at + lane + 32 * i) : 0.0f;
             if (lane + 32 * i < hd) dot = fmaf(qv[i], kx[i], dot);
         }
-        float z = paged_warp_sum(dot) * a.scale;
+        float z = paged_warp_sum(a.flip ? -dot : dot) * a.scale;
         if (a.softcap > 0.0f) z = a.softcap * tanhf(z / a.softcap);
         const float m2 = z > m || z != z ? z : m;
         if (m2 == -INFINITY) continue; // a weight of zero

@@ -61,7 +61,7 @@ struct LinePlace {
     long long start;  // where the block begins
 };
 
-// `size_of(b)`: the tiles of one key head of sequence b. All threads of the block call it; `sh` holds 16 words.
+// `size_of(b)`: the tiles of one key head of sequence b. All threads of the block call it; `sh` holds 32 words.
 template <typename F>
 __device__ __forceinline__ LinePlace line_place(const PagedCall &c, F size_of, int block, int blocks, long long *sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = (int)blockDim.x >> 5;
@@ -76,7 +76,7 @@ __device__ __forceinline__ LinePlace line_place(const PagedCall &c, F size_of, i
     total *= c.kv;
     const long long per = (total + blocks - 1) / blocks, start = per * block;
     __syncthreads();
-    if (tid == 0) sh[12] = -1;
+    if (tid == 0) sh[28] = -1;
     long long before = 0; // of the sequences before this round's
     for (int b0 = 0; b0 < c.batch && start < total; b0 += blockDim.x) {
         const int b = b0 + tid;
@@ -98,15 +98,15 @@ __device__ __forceinline__ LinePlace line_place(const PagedCall &c, F size_of, i
         const long long from = (base + scan - here) * c.kv, to = (base + scan) * c.kv;
         if (start >= from && start < to) { // one thread of one round
             const long long in = start - from;
-            sh[12] = b, sh[13] = in / here, sh[14] = in % here, sh[15] = here;
+            sh[28] = b, sh[29] = in / here, sh[30] = in % here, sh[31] = here;
         }
         __syncthreads();
     }
     __syncthreads();
     LinePlace p;
     p.per = per, p.start = start;
-    p.left = sh[12] < 0 ? 0 : min(per, total - start);
-    p.b = (int)sh[12], p.kvh = (int)sh[13], p.in = sh[14], p.size = sh[15];
+    p.left = sh[28] < 0 ? 0 : min(per, total - start);
+    p.b = (int)sh[28], p.kvh = (int)sh[29], p.in = sh[30], p.size = sh[31];
     return p;
 }
 
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attend_few_kernel(const __grid
     float *meet = reinterpret_cast<float *>(ring + SLOTS * Shape::SLOT);
     unsigned long long *full = reinterpret_cast<unsigned long long *>(meet + Shape::MEET / 4), *empty = full + SLOTS;
     __shared__ float ml[FEW_WARPS][2][ROWS];
-    __shared__ long long place[16];
+    __shared__ long long place[32];
     __shared__ unsigned bad_rows;
     __shared__ int dead;
     const AttendCall &a = f.a;
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attend_few_kernel(const __grid
     }
 
     // ---------------- the products ----------------
-    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+    const float unit = (a.softcap > 0.0f ? a.softcap : a.scale) * PAGED_LOG2E, inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
     unsigned it = 0;
     bool alive = true, first_part = true;
     while (p.left > 0) {
@@ -310,6 +310,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attend_few_kernel(const __grid
                     const int col = ks * 16 + h * 8 + (lane & 3) * 2;
                     if (r < rows && col < a.c.hd) x[2 * h] = paged_read(src + col), x[2 * h + 1] = paged_read(src + col + 1);
                 }
+                if (a.flip) x[0] = -x[0], x[1] = -x[1], x[2] = -x[2], x[3] = -x[3];
                 pg_split<QP>(q0[nt][ks], x[0], x[1]);
                 pg_split<QP>(q1[nt][ks], x[2], x[3]);
             }

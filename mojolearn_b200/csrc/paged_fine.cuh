@@ -18,7 +18,7 @@
 namespace b200i {
 
 constexpr int FINE_THREADS = 384, FINE_KEYS = 64, FINE_ROWS = 128; // four warps of softmax, four that bring keys and values, and a group of which one issues
-constexpr int FINE_REGS = 240, FINE_REGS_LOAD = 144, FINE_REGS_LESS = 120; // a thread: together 504 = 3 x 168, what the block is launched with
+constexpr int FINE_REGS = 232, FINE_REGS_LOAD = 144, FINE_REGS_LESS = 128; // a thread: together 504 = 3 x 168, what the block is launched with
 
 template <typename CT, int HDP> struct FineShape {
     static constexpr int PIECES = sizeof(CT) == 4 ? 3 : 1;
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
     unsigned char *ring = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u);
     unsigned long long *full = reinterpret_cast<unsigned long long *>(ring + SLOTS * SLOT), *empty = full + SLOTS;
     unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *o_free = o_full + 1, *q_full = o_free + 1, *tail = q_full + 1; // 2 SLOTS + 8 <= 32 words
-    __shared__ long long place[16];
+    __shared__ long long place[32];
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
     const AttendCall &a = f.a;
@@ -74,7 +74,6 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
     const int page = 1 << a.c.page_shift;
     Walk w;
     w.begin(a, line);
-    const ManyItem &item = w.item;
 
     if (warp >= 4 && warp < 8) { // ---------------- keys and values ----------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(FINE_REGS_LOAD));
@@ -91,7 +90,8 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             unsigned tails = 0;
             const int box_rows = min(page, FINE_KEYS);
             while (w.left > 0 && alive) {
-                const int tiles = w.tiles(), first = w.first(), last_page = (item.high - 1) >> a.c.page_shift;
+                const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                const int tiles = w.tiles(item), first = w.first(item), last_page = (item.high - 1) >> a.c.page_shift;
                 const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
                 for (int u = 0; u < 2 * tiles; u++, ld++) {
                     bool is_v;
@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             constexpr int CHUNKS = HDP / 8, ROWS_AT_ONCE = 128 / CHUNKS, N = FINE_KEYS / ROWS_AT_ONCE; // a thread: N pieces of 8 columns, of rows ROWS_AT_ONCE apart
             const int mine = tid - 128, chunk = mine % CHUNKS, row0 = mine / CHUNKS;
             while (w.left > 0) {
-                const int tiles = w.tiles(), first = w.first();
+                const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                const int tiles = w.tiles(item), first = w.first(item);
                 const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
                 const auto page_ids = [&](int (&id)[N], int u) { // the pages of a load's rows; -1: nothing to read
                     bool is_v;
@@ -228,10 +229,11 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 for (int places = 2; places >= 0; places--)
 #pragma unroll 1
                     for (int k = 0; k < CP && k <= places; k++) {
-                        const unsigned vd = pg_desc_low(r0 + (i % SLOTS) * SLOT + k * TILE, HALF_COLS), pa = tmem + S_AT + buffer * S_COLS + (places - k) * 32;
+                        const int piece = places - k, next = piece < 2 ? 32 : 16; // columns from 32 keys' piece to the next 32 keys'
+                        const unsigned vd = pg_desc_low(r0 + (i % SLOTS) * SLOT + k * TILE, HALF_COLS), pa = tmem + S_AT + buffer * S_COLS + (piece < 2 ? piece * 16 : 64);
 #pragma unroll
                         for (int ks = 0; ks < FINE_KEYS / 16; ks++) {
-                            pg_mma_ts(tmem + O_AT, pa + ks * 8, pg_desc(vd + ks * 2048 / 16), pg_idesc(HDP, true), add);
+                            pg_mma_ts(tmem + O_AT, pa + (ks >> 1) * next + (ks & 1) * 8, pg_desc(vd + ks * 2048 / 16), pg_idesc(HDP, true), add);
                             add = true;
                         }
                     }
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 pg_commit(o_full);
             };
             while (w.left > 0 && alive) {
-                const int tiles = w.tiles();
+                const int tiles = w.tiles(w.item(a, paged_seq(a.c, w.b)));
                 here(q_full, items & 1u);
                 items++;
                 const unsigned t0 = tile_count; // tiles done before the item: the buffers and barriers go on from item to item
@@ -260,8 +262,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
     } else { // ---------------- the softmax: a thread a row ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FINE_REGS));
         const unsigned at = tmem + ((unsigned)(warp * 32) << 16);
-        const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
-        const float size = unit == 0.0f ? 1.0f : fabsf(unit);
+        const float unit = a.scale * PAGED_LOG2E;
         unsigned tile_count = 0;
         bool alive = true, first_part = true;
         const auto give_up = [&] {
@@ -269,10 +270,12 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             alive = false; // it goes on without waiting; nothing of the block is stored from here on
         };
         while (w.left > 0) {
-            const int tiles = w.tiles(), first = w.first(), row = item.row0 + tid;
+            const PagedSeq s = paged_seq(a.c, w.b);
+            const ManyItem item = w.item(a, s);
+            const int tiles = w.tiles(item), first = w.first(item), row = item.row0 + tid;
             const bool valid = tid < item.rows;
-            if (w.s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
-            const float *src = static_cast<const float *>(a.q) + (long long)(w.s.first + row / a.c.group) * a.ldq + (long long)(w.kvh * a.c.group + row % a.c.group) * a.c.hd;
+            if (s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
+            const float *src = static_cast<const float *>(a.q) + (long long)(s.first + row / a.c.group) * a.ldq + (long long)(w.kvh * a.c.group + row % a.c.group) * a.c.hd;
 #pragma unroll 1
             for (int c = 0; c < HDP; c += 32) { // the row's pieces into tensor memory
                 unsigned p[3][16];
@@ -280,6 +283,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 for (int i = 0; i < 32; i += 4) {
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     if (valid && c + i < a.c.hd) x = *reinterpret_cast<const float4 *>(src + c + i);
+                    if (a.flip) x = make_float4(-x.x, -x.y, -x.z, -x.w);
                     unsigned lo[3], hi[3];
                     pg_split<3>(lo, x.x, x.y);
                     pg_split<3>(hi, x.z, x.w);
@@ -292,10 +296,11 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             pg_wait_st();
             pg_fence_before();
             pg_bar_arrive(q_full);
-            const int hi = valid ? w.s.pos0 + row / a.c.group + 1 : 0, lo = a.window ? hi - a.window : 0;
-            float m = -INFINITY, l = 0.0f, o[HDP];
+            const int hi = valid ? s.pos0 + row / a.c.group + 1 : 0, lo = a.window ? hi - a.window : 0;
+            float m = -INFINITY, l = 0.0f;
+            unsigned long long o[HDP / 2]; // two columns each
 #pragma unroll
-            for (int c = 0; c < HDP; c++) o[c] = 0.0f;
+            for (int c = 0; c < HDP / 2; c++) o[c] = 0;
             const auto take = [&](unsigned t) { // o += the output of tile t
                 if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(o_full, t & 1u))) give_up();
                 if (!alive) return;
@@ -304,9 +309,9 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 for (int c = 0; c < HDP; c += 32) {
                     unsigned v[32];
                     pg_ld32(v, at + O_AT + c);
-                    pg_wait_ld();
+                    pg_wait_ld(v);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[c + i] += __uint_as_float(v[i]);
+                    for (int i = 0; i < 32; i += 2) o[(c + i) / 2] = pg_add2(o[(c + i) / 2], pg_two(__uint_as_float(v[i]), __uint_as_float(v[i + 1])));
                 }
                 pg_fence_before();
                 pg_bar_arrive(o_free);
@@ -317,51 +322,65 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&s_full[t & 1u], (t >> 1) & 1u))) give_up();
                 if (!alive) continue;
                 pg_fence_after();
-                unsigned z[64];
-                pg_ld32(z, s_at), pg_ld32(z + 32, s_at + 32);
-                pg_wait_ld();
-                float *x = reinterpret_cast<float *>(z);
-                if (a.softcap > 0.0f) pg_tanh<64>(x, inner);
-                if (unit <= 0.0f) { // a negative scale turns the order of the scores around, none makes them all alike
+                const bool edge = __any_sync(0xFFFFFFFFu, valid && (pos + FINE_KEYS > hi || pos < lo));
+                unsigned z[32];
+                float *x = reinterpret_cast<float *>(z), top[2] = {-INFINITY, -INFINITY};
+                const auto hide = [&](int c) {
+                    if (!edge) return;
 #pragma unroll
-                    for (int c = 0; c < 64; c++) x[c] = unit < 0.0f ? -x[c] : 0.0f;
+                    for (int i = 0; i < 32; i++)
+                        if (pos + c + i >= hi || pos + c + i < lo) x[i] = -INFINITY;
+                };
+#pragma unroll
+                for (int c = 32; c >= 0; c -= 32) { // the largest score; the first columns come last and stay for their weights
+                    pg_ld32(z, s_at + c);
+                    pg_wait_ld(z);
+                    hide(c);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) top[0] = pg_max3(top[0], x[i], x[i + 1]), top[1] = pg_max3(top[1], x[i + 2], x[i + 3]);
                 }
-                if (__any_sync(0xFFFFFFFFu, valid && (pos + FINE_KEYS > hi || pos < lo))) {
+                float most = fmaxf(top[0], top[1]);
+                if (a.softcap > 0.0f) pg_cap_fine<2>(top, a), most = most == -INFINITY ? most : fmaxf(top[0], top[1]); // (-infinity: nothing is seen)
+                most *= unit;
+                const float to = most > m ? most : m, keep = m == -INFINITY ? 0.0f : paged_exp2(m - to), base = to == -INFINITY ? 0.0f : to;
+                const unsigned long long unit2 = pg_two(unit, unit), base2 = pg_two(-base, -base);
+                unsigned long long sum[2] = {0, 0};
 #pragma unroll
-                    for (int c = 0; c < 64; c++)
-                        if (pos + c >= hi || pos + c < lo) x[c] = -INFINITY;
-                }
-                float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int c = 4; c < 64; c += 4)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], x[c + e]);
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * size, to = most > m ? most : m;
-                const float keep = m == -INFINITY ? 0.0f : paged_exp2(m - to), base = to == -INFINITY ? 0.0f : to;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    unsigned p[3][8];
-#pragma unroll
-                    for (int i = 0; i < 16; i += 2) {
-                        const float w0 = paged_exp2(fmaf(x[c + i], size, -base)), w1 = paged_exp2(fmaf(x[c + i + 1], size, -base));
-                        sum[i & 2] += w0, sum[(i & 2) + 1] += w1;
-                        unsigned piece[3];
-                        pg_split<3>(piece, w0, w1);
-#pragma unroll
-                        for (int k = 0; k < 3; k++) p[k][i / 2] = piece[k];
+                for (int c = 0; c < 64; c += 32) {
+                    if (c) {
+                        pg_ld32(z, s_at + c);
+                        pg_wait_ld(z);
                     }
+                    if (a.softcap > 0.0f) pg_cap_fine<32>(x, a);
+                    if (c || a.softcap > 0.0f) hide(c);
 #pragma unroll
-                    for (int k = 0; k < 3; k++) pg_st8(s_at + k * 32 + c / 2, p[k]);
+                    for (int h = 0; h < 2; h++) {
+                        unsigned p[3][8];
+#pragma unroll
+                        for (int i = 0; i < 16; i += 2) {
+                            float w0, w1;
+                            pg_one(pg_fma2(pg_two(x[16 * h + i], x[16 * h + i + 1]), unit2, base2), w0, w1);
+                            w0 = paged_exp2(w0), w1 = paged_exp2(w1);
+                            sum[(i / 2) & 1] = pg_add2(sum[(i / 2) & 1], pg_two(w0, w1));
+                            unsigned piece[3];
+                            pg_split<3>(piece, w0, w1);
+#pragma unroll
+                            for (int k = 0; k < 3; k++) p[k][i / 2] = piece[k];
+                        }
+                        // over columns of S that have been read, and the 32 behind it: 32 keys' pieces at c, c + 16 and 64 + c / 2
+                        pg_st8(s_at + c + 8 * h, p[0]), pg_st8(s_at + c + 16 + 8 * h, p[1]), pg_st8(s_at + 64 + c / 2 + 8 * h, p[2]);
+                    }
                 }
                 pg_wait_st();
                 pg_fence_before();
                 pg_bar_arrive(&p_full[t & 1u]);
-                l = fmaf(l, keep, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                float s0, s1;
+                pg_one(pg_add2(sum[0], sum[1]), s0, s1);
+                l = fmaf(l, keep, s0 + s1);
                 if (j > 0) take(t - 1);
                 if (__any_sync(0xFFFFFFFFu, to > m)) {
 #pragma unroll
-                    for (int c = 0; c < HDP; c++) o[c] *= keep;
+                    for (int c = 0; c < HDP / 2; c++) o[c] = pg_mul2(o[c], pg_two(keep, keep));
                 }
                 m = to;
             }
@@ -369,18 +388,21 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             take(tile_count - 1);
 
             // ---- the item's (or its part's) end ----
-            const bool is_whole = w.skip == 0 && w.steps() == item.steps;
+            const bool is_whole = w.skip == 0 && w.steps(item) == item.steps;
             const long long slot = (long long)blockIdx.x * 2 + (first_part && w.skip > 0 ? 0 : 1);
             bool wrong = false;
             if (valid && alive && !dead) {
-                float *out = static_cast<float *>(a.out) + ((long long)(w.s.first + row / a.c.group) * a.c.heads + w.kvh * a.c.group + row % a.c.group) * a.c.hd;
+                float *out = static_cast<float *>(a.out) + ((long long)(s.first + row / a.c.group) * a.c.heads + w.kvh * a.c.group + row % a.c.group) * a.c.hd;
                 float4 *part = reinterpret_cast<float4 *>(f.part + (slot * BR + tid) * HDP);
 #pragma unroll
                 for (int c = 0; c < HDP; c += 4) {
+                    float4 y;
+                    pg_one(o[c / 2], y.x, y.y), pg_one(o[c / 2 + 1], y.z, y.w);
                     if (!is_whole) {
-                        part[c / 4] = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+                        part[c / 4] = y;
                     } else if (c < a.c.hd) {
-                        const float4 y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(__fdiv_rn(o[c], l), __fdiv_rn(o[c + 1], l), __fdiv_rn(o[c + 2], l), __fdiv_rn(o[c + 3], l));
+                        const float share = l == 0.0f ? 0.0f : 1.0f / l;
+                        y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(y.x * share, y.y * share, y.z * share, y.w * share);
                         *reinterpret_cast<float4 *>(out + c) = y;
                         wrong |= !isfinite(y.x) || !isfinite(y.y) || !isfinite(y.z) || !isfinite(y.w);
                     }
@@ -392,13 +414,13 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             }
             if (!is_whole && tid == 0 && w.skip == 0 && alive && !dead) {
                 int *head = f.head + blockIdx.x * 8;
-                head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = (int)(w.line - line.start), head[5] = (int)line.per;
+                head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = w.line, head[5] = (int)line.per;
             }
             unsigned rest = __ballot_sync(0xFFFFFFFFu, wrong);
             while (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
                 const int k = __ffs(rest) - 1, bad = __shfl_sync(0xFFFFFFFFu, row, k);
                 rest &= rest - 1;
-                attend_row_plain<float, CT>(a, w.b, w.s.first + bad / a.c.group, w.s.pos0 + bad / a.c.group, w.s.length, w.kvh * a.c.group + bad % a.c.group);
+                attend_row_plain<float, CT>(a, w.b, s.first + bad / a.c.group, s.pos0 + bad / a.c.group, s.length, w.kvh * a.c.group + bad % a.c.group);
             }
             first_part = false;
             w.next(a);
@@ -427,7 +449,7 @@ cudaError_t launch_fine_as(const AttendCall &a, const ManyPlan &p, void *ws, int
         if (device < 64) known[device].store(true);
     }
     attend_fine_kernel<CT, HDP><<<p.blocks, FINE_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    attend_join_rows_kernel<float, CT, HDP, FINE_ROWS><<<dim3(p.blocks, FINE_ROWS / 8), 256, 0, st>>>(f);
+    attend_join_rows_kernel<float, CT, HDP, FINE_ROWS><<<dim3(p.blocks, FINE_ROWS / 32), 256, 0, st>>>(f);
     *launches += 2;
     return cudaGetLastError();
 }

@@ -5,7 +5,7 @@
 // Bound: the tensor pipe, 4 head_dim operations a (row, key), and beside it the exponentials: 16 a clock on an SM against 8192
 // operations, so at head_dim 128 the two pipes need the same time and neither may wait for the other.
 // Rows. A row is a (token, head of the key head's group), so grouped heads share the keys that are brought in.
-// Block. Two streams, each of four softmax warps (a thread a row), an S of 128 columns and an O of head_dim columns in tensor memory: while one
+// Block. Two streams, each of eight softmax warps (two threads a row, for half of a tile's columns each), an S of 128 columns and an O of head_dim columns in tensor memory: while one
 // stream's softmax runs, the other's products do. A block of more than 128 rows gives each stream 128 of them and the same keys; one
 // of up to 128 gives both streams the rows, and every other tile of keys each, and joins the two at the end. One thread issues
 // the products: S = Q K^T from shared memory, O += P V with P (bfloat16, over the columns of S that it came from) read from tensor
@@ -19,14 +19,14 @@
 
 namespace b200i {
 
-constexpr int MANY_THREADS = 384, MANY_KEYS = 128; // two streams' softmax, and a group of warps of which one copies and one issues
-constexpr int MANY_REGS = 208, MANY_REGS_LESS = 88;  // a thread: 2 x 208 + 88 = 504 = 3 x 168, what the block is launched with
+constexpr int MANY_THREADS = 640, MANY_KEYS = 128; // two groups of four warps a stream, and one of which one warp copies and one issues
+constexpr int MANY_REGS = 96, MANY_REGS_LESS = 96;
 
 template <int HDP> struct ManyShape {
     static constexpr int TILE = HDP * 256;     // bytes of 128 rows of bfloat16
     static constexpr int QUERY = 2 * TILE;     // a stream each; the streams' meeting place too
     static constexpr int BLOCK_ROWS = 256;
-    static constexpr int ROOM = (226 * 1024 - 1024 - 4096 - QUERY) / TILE;
+    static constexpr int ROOM = (226 * 1024 - 1024 - 2560 - QUERY) / TILE;
     static constexpr int SLOTS = ROOM > 8 ? 8 : ROOM;
     static constexpr int SMEM = 1024 + QUERY + SLOTS * TILE + 256;
 };
@@ -57,11 +57,15 @@ __device__ __forceinline__ void pg_commit(unsigned long long *bar) {
 }
 __device__ __forceinline__ void pg_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void pg_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void pg_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pg_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 #define PG_R8(v, i) "r"((v)[i]), "r"((v)[i + 1]), "r"((v)[i + 2]), "r"((v)[i + 3]), "r"((v)[i + 4]), "r"((v)[i + 5]), "r"((v)[i + 6]), "r"((v)[i + 7])
 #define PG_W8(v, i) "=r"((v)[i]), "=r"((v)[i + 1]), "=r"((v)[i + 2]), "=r"((v)[i + 3]), "=r"((v)[i + 4]), "=r"((v)[i + 5]), "=r"((v)[i + 6]), "=r"((v)[i + 7])
+#define PG_RW8(v, i) "+r"((v)[i]), "+r"((v)[i + 1]), "+r"((v)[i + 2]), "+r"((v)[i + 3]), "+r"((v)[i + 4]), "+r"((v)[i + 5]), "+r"((v)[i + 6]), "+r"((v)[i + 7])
+// Waits for the loads so far; `v` are words of the last of them, which nothing may use before.
+__device__ __forceinline__ void pg_wait_ld(unsigned *v) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : PG_RW8(v, 0), PG_RW8(v, 8), PG_RW8(v, 16), PG_RW8(v, 24)::"memory");
+}
 // 32 columns of a lane's row
 __device__ __forceinline__ void pg_ld32(unsigned *v, unsigned taddr) {
     asm volatile(
@@ -71,13 +75,13 @@ __device__ __forceinline__ void pg_ld32(unsigned *v, unsigned taddr) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void pg_st32(unsigned taddr, const unsigned *v) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, "
-        "%27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-        PG_R8(v, 0), PG_R8(v, 8), PG_R8(v, 16), PG_R8(v, 24)
-        : "memory");
+__device__ __forceinline__ void pg_ld16(unsigned *v, unsigned taddr) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : PG_W8(v, 0), PG_W8(v, 8)
+                 : "r"(taddr)
+                 : "memory");
 }
+__device__ __forceinline__ void pg_wait_ld16(unsigned *v) { asm volatile("tcgen05.wait::ld.sync.aligned;" : PG_RW8(v, 0), PG_RW8(v, 8)::"memory"); }
 __device__ __forceinline__ void pg_st16(unsigned taddr, const unsigned *v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr), PG_R8(v, 0), PG_R8(v, 8)
@@ -87,30 +91,108 @@ __device__ __forceinline__ void pg_st8(unsigned taddr, const unsigned *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), PG_R8(v, 0) : "memory");
 }
 
-// x = tanh(x inner) of a row's N scores. Where all of a warp's are within 0.35, as capped scores mostly are, by the series x - x^3 / 3 + 2 x^5 / 15
-// - 17 x^7 / 315 + 62 x^9 / 2835 - 1382 x^11 / 155925, whose next term is 1.2e-8 of x there; elsewhere sign(x) (1 - 2 / (1 + e^{2 |x|})).
+// Two 32-bit words at a time.
+__device__ __forceinline__ unsigned long long pg_two(float x, float y) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void pg_one(unsigned long long v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ unsigned long long pg_fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+    return r;
+}
+__device__ __forceinline__ unsigned long long pg_add2(unsigned long long x, unsigned long long y) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ unsigned long long pg_mul2(unsigned long long x, unsigned long long y) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+    return r;
+}
+__device__ __forceinline__ float pg_max3(float x, float y, float z) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+// 2^x of two words of at most 8 without the exponential unit: x = n + f, f in [-1/2, 1/2], a cubic of f (its largest relative error, 2^-13.7, made least
+// by reweighted least squares; for weights that are rounded to 8 bits), and n added to the exponent. NaN gives a huge word or NaN, never a small one.
+constexpr float EXP_C0 = 0.99992806f, EXP_C1 = 0.69326097f, EXP_C2 = 0.24261115f, EXP_C3 = 0.05517167f;
+__device__ __forceinline__ float pg_max_nan(float x, float y) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void pg_exp2_cubic(unsigned long long v, float &x, float &y) {
+    pg_one(v, x, y);
+    const unsigned long long c = pg_two(pg_max_nan(x, -126.0f), pg_max_nan(y, -126.0f)), round = pg_two(12582912.0f, 12582912.0f), back = pg_two(-12582912.0f, -12582912.0f);
+    const unsigned long long n = pg_add2(c, round), f = pg_fma2(pg_add2(n, back), pg_two(-1.0f, -1.0f), c);
+    unsigned long long p = pg_fma2(f, pg_two(EXP_C3, EXP_C3), pg_two(EXP_C2, EXP_C2));
+    p = pg_fma2(p, f, pg_two(EXP_C1, EXP_C1)), p = pg_fma2(p, f, pg_two(EXP_C0, EXP_C0));
+    float nx, ny, px, py;
+    pg_one(n, nx, ny), pg_one(p, px, py);
+    x = __uint_as_float((__float_as_uint(nx) << 23) + __float_as_uint(px)), y = __uint_as_float((__float_as_uint(ny) << 23) + __float_as_uint(py));
+}
+
+// Capped scores before their scale: x = tanh(x inner) / inner, inner = scale / softcap, so that the scale that follows is the uncapped one's.
+// Far from zero as sign(x) (1 - 2 / (1 + e^{2 |x inner|})); both forms for every score where one of the warp's is far, and no branch between them.
+__device__ __forceinline__ float pg_cap_far(float x, float inner, float outer) {
+    const float e = paged_exp2(fabsf(x) * (inner * 2.0f * PAGED_LOG2E));
+    return copysignf((1.0f - __fdividef(2.0f, 1.0f + e)) * outer, x); // (the quotient of a huge or infinite e is zero)
+}
+// Near zero by x + x^3 P(x^2): for weights of 8 bits a polynomial over |x inner| <= 1, whose largest error, 4e-6, was made least by reweighted
+// least squares (CAP_NEAR; with inner's powers in AttendCall); a warp whose scores are all below the cap, as they mostly are, does only this.
+constexpr float CAP_NEAR[4] = {-0.33297876f, 0.13021576f, -0.04450673f, 0.00886790f};
 template <int N>
-__device__ __forceinline__ void pg_tanh(float *x, float inner) {
+__device__ __forceinline__ void pg_cap(float *x, const AttendCall &a) {
     float most = 0.0f;
 #pragma unroll
-    for (int c = 0; c < N; c++) {
-        x[c] *= inner;
-        most = fmaxf(most, fabsf(x[c]));
+    for (int c = 0; c < N; c += 2) most = pg_max3(most, fabsf(x[c]), fabsf(x[c + 1]));
+    unsigned long long k[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) k[i] = pg_two(a.cap_near[i], a.cap_near[i]);
+    const auto near = [&](int c, float &y0, float &y1) {
+        const unsigned long long v = pg_two(x[c], x[c + 1]), q = pg_mul2(v, v);
+        unsigned long long p = pg_fma2(q, k[3], k[2]);
+        p = pg_fma2(q, p, k[1]), p = pg_fma2(q, p, k[0]);
+        pg_one(pg_fma2(pg_mul2(v, q), p, v), y0, y1);
+    };
+    if (!__any_sync(0xFFFFFFFFu, most > a.cap_outer)) {
+#pragma unroll
+        for (int c = 0; c < N; c += 2) near(c, x[c], x[c + 1]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < N; c += 2) {
+            float y0, y1;
+            near(c, y0, y1);
+            const float f0 = pg_cap_far(x[c], a.cap_inner, a.cap_outer), f1 = pg_cap_far(x[c + 1], a.cap_inner, a.cap_outer);
+            x[c] = fabsf(x[c]) > a.cap_outer ? f0 : y0, x[c + 1] = fabsf(x[c + 1]) > a.cap_outer ? f1 : y1;
+        }
     }
-    const auto series = [](float v) {
-        const float q = v * v;
+}
+// To 32-bit accuracy by the series x - x^3 / 3 + 2 x^5 / 15 - 17 x^7 / 315 + 62 x^9 / 2835 - 1382 x^11 / 155925 within 0.35, whose next term is 1.2e-8 of x there.
+template <int N>
+__device__ __forceinline__ void pg_cap_fine(float *x, const AttendCall &a) {
+    float most = 0.0f;
+#pragma unroll
+    for (int c = 0; c < N; c++) most = fmaxf(most, fabsf(x[c]));
+    const auto near = [&](float y) {
+        const float v = y * a.cap_inner, q = v * v;
         float s = fmaf(q, -1382.0f / 155925.0f, 62.0f / 2835.0f);
         s = fmaf(q, s, -17.0f / 315.0f), s = fmaf(q, s, 2.0f / 15.0f), s = fmaf(q, s, -1.0f / 3.0f);
-        return fmaf(v * q, s, v);
+        return fmaf(y * q, s, y);
     };
-    if (!__any_sync(0xFFFFFFFFu, most > 0.35f)) {
+    if (!__any_sync(0xFFFFFFFFu, most * a.cap_inner > 0.35f)) {
 #pragma unroll
-        for (int c = 0; c < N; c++) x[c] = series(x[c]);
+        for (int c = 0; c < N; c++) x[c] = near(x[c]);
     } else {
 #pragma unroll
         for (int c = 0; c < N; c++) {
-            const float e = paged_exp2(fabsf(x[c]) * (2.0f * PAGED_LOG2E)), far = copysignf(1.0f - __fdividef(2.0f, 1.0f + e), x[c]);
-            x[c] = fabsf(x[c]) > 0.35f ? (e > 1e30f ? copysignf(1.0f, x[c]) : far) : series(x[c]);
+            const float y = near(x[c]), f = pg_cap_far(x[c], a.cap_inner, a.cap_outer);
+            x[c] = fabsf(x[c]) * a.cap_inner > 0.35f ? f : y;
         }
     }
 }
@@ -118,6 +200,7 @@ __device__ __forceinline__ void pg_tanh(float *x, float inner) {
 // An item: up to BR rows of one sequence and key head, over tiles of KEYS keys.
 struct ManyItem {
     int row0, rows;    // of the sequence and key head
+    int token0, head0; // of the first of them
     int t0, tiles;     // tiles that some row sees
     int low, high;     // and positions
     bool pair;         // a step is a tile; else (two streams, and rows for one) two tiles, one a stream
@@ -128,6 +211,7 @@ __device__ __forceinline__ ManyItem many_item(const AttendCall &a, const PagedSe
     ManyItem i;
     i.row0 = block * BR, i.rows = min(n * a.c.group - i.row0, BR);
     const int first = i.row0 / a.c.group, last = (i.row0 + i.rows - 1) / a.c.group;
+    i.token0 = first, i.head0 = i.row0 - first * a.c.group;
     i.high = min(s.length, max(s.pos0 + last + 1, 0));
     i.low = a.window ? min(max(s.pos0 + first + 1 - a.window, 0), i.high) : 0;
     i.t0 = i.low / KEYS;
@@ -136,58 +220,141 @@ __device__ __forceinline__ ManyItem many_item(const AttendCall &a, const PagedSe
     i.steps = i.pair ? i.tiles : (i.tiles + 1) / 2;
     return i;
 }
+// The token and the head (of the key head's group) of an item's row r.
+__device__ __forceinline__ int2 many_row(const AttendCall &a, const ManyItem &i, int r) {
+    const unsigned n = (unsigned)(i.head0 + r), t = a.c.group == 1 ? n : __umulhi(n, a.c.group_part); // n / group: n group < 2^32
+    return make_int2(i.token0 + (int)t, (int)(n - t * (unsigned)a.c.group));
+}
 __device__ __forceinline__ int many_blocks(const AttendCall &a, int n, int block_rows) { return (int)(((long long)n * a.c.group + block_rows - 1) / block_rows); }
 
-// A block's way along the line of all items' steps; every warp of the block goes it by itself.
+// A block's way along the line of all items' steps; every warp of the block goes it by itself. Only the place is kept from item
+// to item: what follows from it is read again.
 template <int BR, int KEYS, int STREAMS> struct ManyWalk {
-    int b, kvh, block, blocks, n;
-    PagedSeq s;
-    ManyItem item;
-    int skip;          // steps of the item that other blocks do before this one
-    long long left;    // steps of the block from here
-    long long line;    // where on the line the item begins
+    int b, kvh, block;
+    int skip;  // steps of the item that other blocks do before this one
+    int left;  // steps of the block from here
+    int line;  // where on the line the item begins, from where the block does
 
+    static __device__ __forceinline__ int rows_of(const AttendCall &a, const PagedSeq &s) { return min(s.n, a.max_new); } // tokens that are computed
     static __device__ __forceinline__ long long steps_of(const AttendCall &a, int b) {
         const PagedSeq s = paged_seq(a.c, b);
-        const int n = min(s.n, a.max_new), blocks = many_blocks(a, n, BR);
+        const int n = rows_of(a, s), blocks = many_blocks(a, n, BR);
         long long sum = 0;
         for (int i = 0; i < blocks; i++) sum += many_item<BR, KEYS, STREAMS>(a, s, n, i).steps;
         return sum;
     }
     __device__ __forceinline__ void begin(const AttendCall &a, const LinePlace &p) {
-        b = p.b, kvh = p.kvh, block = 0, left = p.left, line = p.start - p.in, skip = 0;
+        b = p.b, kvh = p.kvh, block = 0, left = (int)p.left, line = 0, skip = 0;
         if (left <= 0) return;
+        const PagedSeq s = paged_seq(a.c, b);
+        const int n = rows_of(a, s);
         long long in = p.in;
-        sequence(a);
-        item = many_item<BR, KEYS, STREAMS>(a, s, n, 0);
-        while (in >= item.steps) in -= item.steps, line += item.steps, item = many_item<BR, KEYS, STREAMS>(a, s, n, ++block);
-        skip = (int)in;
-    }
-    __device__ __forceinline__ void sequence(const AttendCall &a) { s = paged_seq(a.c, b), n = min(s.n, a.max_new), blocks = many_blocks(a, n, BR); }
-    __device__ __forceinline__ int steps() const { return (int)min((long long)(item.steps - skip), left); } // that the block does of the item
-    __device__ __forceinline__ int first() const { return item.pair ? skip : 2 * skip; }                    // its first tile
-    __device__ __forceinline__ int tiles() const { return min(item.pair ? skip + steps() : 2 * (skip + steps()), item.tiles) - first(); }
-    __device__ __forceinline__ void next(const AttendCall &a) {
-        left -= steps();
-        if (left <= 0) return;
-        line += item.steps, skip = 0;
-        if (++block >= blocks) {
-            block = 0;
-            if (++kvh >= a.c.kv) {
-                kvh = 0, b++;
-                while (b + 1 < a.c.batch && paged_seq(a.c, b).n == 0) b++;
-                sequence(a);
-            }
+        for (;; block++) {
+            const int steps = many_item<BR, KEYS, STREAMS>(a, s, n, block).steps;
+            if (in < steps) break;
+            in -= steps;
         }
-        item = many_item<BR, KEYS, STREAMS>(a, s, n, block);
+        skip = (int)in, line = -skip;
+    }
+    __device__ __forceinline__ ManyItem item(const AttendCall &a, const PagedSeq &s) const { return many_item<BR, KEYS, STREAMS>(a, s, rows_of(a, s), block); }
+    __device__ __forceinline__ int steps(const ManyItem &i) const { return min(i.steps - skip, left); } // that the block does of the item
+    __device__ __forceinline__ int first(const ManyItem &i) const { return i.pair ? skip : 2 * skip; }  // its first tile
+    __device__ __forceinline__ int tiles(const ManyItem &i) const { return min(i.pair ? skip + steps(i) : 2 * (skip + steps(i)), i.tiles) - first(i); }
+    __device__ __forceinline__ void next(const AttendCall &a) {
+        const PagedSeq s = paged_seq(a.c, b);
+        const ManyItem i = item(a, s);
+        left -= steps(i), line += i.steps, skip = 0;
+        if (left <= 0 || ++block < many_blocks(a, rows_of(a, s), BR)) return;
+        block = 0;
+        if (++kvh < a.c.kv) return;
+        kvh = 0, b++;
+        while (b + 1 < a.c.batch && paged_seq(a.c, b).n == 0) b++;
     }
 };
+
+// 64 scores of a row, in tensor memory at s_at: their largest, and then their weights, of which the sum is returned and the bfloat16 words put
+// at p_at. Apart by what a tile needs, so that the common one is a straight run of instructions (scores that are capped; keys that are not
+// seen: the row sees columns lo .. hi - 1), and loops of 32 columns, so that the code of a tile that comes seldom is not long: fetched from L2 it
+// took 8000 cycles where all columns were written out. A quarter of the exponentials of the common uncapped tile is made beside the unit that
+// makes the others (16 a clock).
+template <bool EDGE>
+__device__ __forceinline__ float many_largest(unsigned s_at, int lo, int hi) {
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+    for (int h = 0; h < 2; h++, lo -= 32, hi -= 32) {
+        unsigned z[32];
+        const float *x = reinterpret_cast<const float *>(z);
+        pg_ld32(z, s_at + 32 * h);
+        pg_wait_ld(z);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = EDGE && (i + e >= hi || i + e < lo) ? -INFINITY : x[i + e];
+            top[0] = pg_max3(top[0], y[0], y[1]), top[1] = pg_max3(top[1], y[2], y[3]);
+        }
+    }
+    return fmaxf(top[0], top[1]);
+}
+template <bool CAP, bool EDGE>
+__device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at, unsigned p_at, float unit, float base, int lo, int hi) {
+    const unsigned long long unit2 = pg_two(unit, unit), base2 = pg_two(-base, -base);
+    unsigned long long sum[2] = {0, 0};
+#pragma unroll 1
+    for (int h = 0; h < 2; h++, lo -= 32, hi -= 32) {
+        unsigned z[32], p[16];
+        float *x = reinterpret_cast<float *>(z);
+        pg_ld32(z, s_at + 32 * h);
+        pg_wait_ld(z);
+        if (CAP) {
+            if (EDGE) { // what is not seen may be anything
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                    if (i >= hi || i < lo) x[i] = 0.0f;
+            }
+            pg_cap<32>(x, a);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            if (EDGE) {
+                if (i >= hi || i < lo) x[i] = -INFINITY;
+                if (i + 1 >= hi || i + 1 < lo) x[i + 1] = -INFINITY;
+            }
+            const unsigned long long v = pg_fma2(pg_two(x[i], x[i + 1]), unit2, base2);
+            float w0, w1;
+            if (!EDGE && !CAP && i % 8 == 6) {
+                pg_exp2_cubic(v, w0, w1);
+            } else {
+                pg_one(v, w0, w1);
+                w0 = paged_exp2(w0), w1 = paged_exp2(w1);
+            }
+            sum[(i / 2) & 1] = pg_add2(sum[(i / 2) & 1], pg_two(w0, w1));
+            p[i / 2] = pg_pack(w0, w1);
+        }
+        // the first columns' words wait for nobody: they lie over scores that both threads of the row have read twice or keep in registers
+        pg_st16(p_at + 16 * h, p);
+    }
+    float s0, s1;
+    pg_one(pg_add2(sum[0], sum[1]), s0, s1);
+    return s0 + s1;
+}
 
 struct ManyCall {
     AttendCall a;
     float *part; // [blocks][2][BLOCK_ROWS][HDP], then [blocks][2][2][BLOCK_ROWS] of m and l
     int *head;   // [blocks][8]: sequence (or -1), key head, block of rows, steps, steps of the block before it, steps a block
 };
+
+// 16 columns of an output that is there, or zeros.
+__device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some) {
+    if (some) {
+        pg_ld16(o, at);
+        pg_wait_ld16(o);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[i] = 0;
+    }
+}
 
 template <int HDP>
 __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ManyCall f) {
@@ -198,9 +365,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *query = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u), *ring = query + Shape::QUERY;
     unsigned long long *full = reinterpret_cast<unsigned long long *>(ring + SLOTS * TILE), *empty = full + SLOTS;
-    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *q_full = o_full + 2, *tail = q_full + 1; // 2 SLOTS + 8 <= 32 words
-    __shared__ float stats[2][2][128];
-    __shared__ long long place[16];
+    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 4, *q_full = o_full + 2, *tail = q_full + 1; // 2 SLOTS + 10 <= 32 words
+    __shared__ float stats[2][2][128], half_stat[2][2][128]; // m and l of a stream's rows; what the two threads of a row tell each other
+    __shared__ long long place[32];
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
     const AttendCall &a = f.a;
@@ -212,16 +379,16 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         }
         for (int i = 0; i < 2; i++) {
             pg_bar_init(&s_full[i], 1);
-            pg_bar_init(&p_full[i], 128);
+            pg_bar_init(&p_full[2 * i], 128), pg_bar_init(&p_full[2 * i + 1], 128);
             pg_bar_init(&o_full[i], 1);
         }
-        pg_bar_init(q_full, 256);
+        pg_bar_init(q_full, 512);
         pg_bar_init(tail, 1);
         dead = 0;
         f.head[blockIdx.x * 8] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 9) {
+    if (warp == 17) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_smem(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -233,16 +400,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     const int page = 1 << a.c.page_shift, box_rows = min(page, MANY_KEYS);
     Walk w;
     w.begin(a, line);
-    const ManyItem &item = w.item;
 
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MANY_REGS_LESS));
-    if (warp == 8) { // ---------------- the copies ----------------
+    if (warp >= 16) {
+    if (warp == 16) { // ---------------- the copies ----------------
         unsigned ld = 0, tails = 0;
         bool alive = true;
         while (w.left > 0 && alive) {
-            const int tiles = w.tiles(), first = w.first();
-            const int last_page = (item.high - 1) >> a.c.page_shift;
+            const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+            const int tiles = w.tiles(item), first = w.first(item), last_page = (item.high - 1) >> a.c.page_shift;
             const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
             // in the order of their first use: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 K3 ... where the streams have tiles of their own
             const int lead = min(item.pair ? 1 : 2, tiles);
@@ -293,7 +458,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         }
         if (!alive) // copies in flight end before the block does
             for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
-    } else if (warp == 9) { // ---------------- the products ----------------
+    } else if (warp == 17) { // ---------------- the products ----------------
         if (lane == 0) {
             unsigned ld = 0, items = 0, p_count[2] = {0, 0};
             bool alive = true;
@@ -310,18 +475,22 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     pg_mma_ss(d, pg_desc(q + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_desc(k + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_idesc(128, false), ks > 0);
                 pg_commit(&s_full[stream]);
             };
-            const auto value = [&](int stream, unsigned i, bool add) { // O += P V, V being load i
+            const auto value = [&](int stream, unsigned i, bool add) { // O += P V, V being load i, as the two halves of P come; false where they do not
                 const unsigned v = pg_desc_low(r0 + (i % SLOTS) * TILE, HALF_COLS), d = tmem + 256 + stream * 128;
+                for (int half = 0; half < 2; half++) {
+                    if (alive && !pg_bar_wait(&p_full[2 * stream + half], p_count[stream] & 1u)) alive = false;
+                    if (!alive) return false;
+                    pg_fence_after();
 #pragma unroll
-                for (int ks = 0; ks < 8; ks++) pg_mma_ts(d, tmem + stream * 128 + ks * 8, pg_desc(v + ks * 2048 / 16), pg_idesc(HDP, true), add || ks > 0);
-            };
-            const auto weights = [&](int stream) { // the stream's P is there
-                if (alive && !pg_bar_wait(&p_full[stream], p_count[stream] & 1u)) alive = false;
+                    for (int ks = 0; ks < 4; ks++)
+                        pg_mma_ts(d, tmem + stream * 128 + half * 64 + ks * 8, pg_desc(v + half * (64 * 128 / 16) + ks * 2048 / 16), pg_idesc(HDP, true), add || half > 0 || ks > 0);
+                }
                 p_count[stream]++;
-                pg_fence_after();
+                return true;
             };
             while (w.left > 0 && alive) {
-                const int tiles = w.tiles(), first = w.first();
+                const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                const int tiles = w.tiles(item);
                 if (!pg_bar_wait(q_full, items & 1u)) alive = false;
                 items++;
                 pg_fence_after();
@@ -334,9 +503,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                         here(v);
                         if (j + 1 < tiles) k = ld++;
                         for (int stream = 0; stream < 2 && alive; stream++) {
-                            weights(stream);
-                            if (!alive) break;
-                            value(stream, v, j > 0);
+                            if (!value(stream, v, j > 0)) break;
                             if (stream == 1) pg_commit(&empty[v % SLOTS]);
                             if (j + 1 < tiles) {
                                 if (stream == 0) here(k);
@@ -356,9 +523,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     for (int j = 0; j < tiles && alive; j++) {
                         const int stream = j & 1;
                         here(ld);
-                        weights(stream);
-                        if (!alive) break;
-                        value(stream, ld, j > 1);
+                        if (!value(stream, ld, j > 1)) break;
                         pg_commit(&empty[ld % SLOTS]);
                         ld++;
                         if (j + 2 < tiles) {
@@ -378,103 +543,99 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         }
         __syncwarp();
     }
-    } else { // ---------------- the softmax of a stream: a thread a row ----------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MANY_REGS));
-        const int stream = warp >> 2, r = tid & 127;
-        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, s_at = tmem + lanes + stream * 128, o_at = tmem + lanes + 256 + stream * 128;
-        const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+    } else { // ---------------- the softmax of a stream: two threads a row, 64 columns of a tile each ----------------
+        const int stream = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, s_at = tmem + lanes + stream * 128 + 64 * half, o_at = tmem + lanes + 256 + stream * 128;
+        const float unit = a.scale * PAGED_LOG2E;
         unsigned s_count = 0, o_count = 0;
         bool alive = true, first_part = true;
+        const auto meet = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + stream) : "memory"); }; // of the stream's threads
         while (w.left > 0) {
-            const int tiles = w.tiles(), first = w.first();
-            if (w.s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
-            // the rows into shared memory, K-major and swizzled; a stream its own rows, or half of the columns of the shared ones
+            const PagedSeq s = paged_seq(a.c, w.b);
+            const ManyItem item = w.item(a, s);
+            const int tiles = w.tiles(item);
+            if (s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
+            // the rows into shared memory, K-major and swizzled: a stream its own, or both the shared ones
             {
-                constexpr int CHUNKS = HDP / 8; // 16 bytes of bfloat16
-                const int tile = item.pair ? stream : 0;
-                for (int u = r; u < 128 * CHUNKS; u += 128) {
-                    const int row = u / CHUNKS, chunk = u % CHUNKS, at = item.row0 + tile * 128 + row;
-                    if (!item.pair && (chunk & 1) != stream) continue;
-                    const T *src = static_cast<const T *>(a.q) + (long long)(w.s.first + at / a.c.group) * a.ldq + (long long)(w.kvh * a.c.group + at % a.c.group) * a.c.hd + chunk * 8;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (tile * 128 + row < item.rows && chunk * 8 < a.c.hd) x = *reinterpret_cast<const uint4 *>(src);
-                    *reinterpret_cast<uint4 *>(query + tile * TILE + (chunk >> 3) * HALF_COLS + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = x;
+                constexpr int CHUNKS = HDP / 8, N = CHUNKS / 2; // of 16 bytes; that a thread brings where its stream has rows of its own, all asked for at once
+                const int tile = item.pair ? stream : 0, chunk = tid % CHUNKS, row0 = (item.pair ? tid & 255 : tid) / CHUNKS, step = (item.pair ? 256 : 512) / CHUNKS;
+                const unsigned flip = a.flip ? 0x80008000u : 0u;
+                uint4 x[N];
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int row = row0 + i * step;
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (row < 128 && tile * 128 + row < item.rows && chunk * 8 < a.c.hd) {
+                        const int2 at = many_row(a, item, tile * 128 + row);
+                        x[i] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) + (long long)(s.first + at.x) * a.ldq + (w.kvh * a.c.group + at.y) * a.c.hd + chunk * 8);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    const int row = row0 + i * step;
+                    if (row < 128)
+                        *reinterpret_cast<uint4 *>(query + tile * TILE + (chunk >> 3) * HALF_COLS + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
+                            make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 pg_bar_arrive(q_full);
             }
-            const int mine = (item.pair ? stream * 128 : 0) + r, row = item.row0 + mine;
+            const int mine = (item.pair ? stream * 128 : 0) + r;
             const bool valid = mine < item.rows;
-            const int hi = valid ? w.s.pos0 + row / a.c.group + 1 : 0, lo = a.window ? hi - a.window : 0;
+            const int2 place = many_row(a, item, mine);
+            // of the first tile's columns of this thread, those that the row sees
+            int hi = valid ? s.pos0 + place.x + 1 : 0, lo = a.window ? hi - a.window : 0;
+            const int begin = (item.t0 + w.first(item) + (item.pair ? 0 : stream)) * MANY_KEYS + 64 * half, step = (item.pair ? 1 : 2) * MANY_KEYS;
+            hi -= begin, lo -= begin;
             float m = -INFINITY, l = 0.0f;
-            int taken = 0;
-            for (int j = item.pair ? 0 : stream; j < tiles; j += item.pair ? 1 : 2, taken++) {
-                const int pos = (item.t0 + first + j) * MANY_KEYS;
+            const int all = item.pair ? tiles : (tiles + 1 - stream) / 2;
+            for (int j = 0; j < all; j++, hi -= step, lo -= step) {
                 if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&s_full[stream], s_count & 1u))) {
                     if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
                     alive = false; // it goes on without waiting, so that the others meet it; nothing of the block is stored from here on
                 }
                 s_count++;
-                if (!alive) continue;
                 pg_fence_after();
-                unsigned z[128];
-#pragma unroll
-                for (int c = 0; c < 4; c++) pg_ld32(z + 32 * c, s_at + 32 * c);
-                pg_wait_ld();
-                float *x = reinterpret_cast<float *>(z);
-                if (a.softcap > 0.0f) pg_tanh<128>(x, inner);
-                if (unit <= 0.0f) { // a negative scale turns the order of the scores around, none makes them all alike
-#pragma unroll
-                    for (int c = 0; c < 128; c++) x[c] = unit < 0.0f ? -x[c] : 0.0f;
+                const bool edge = __any_sync(0xFFFFFFFFu, valid && (hi < 64 || lo > 0));
+                float most = -INFINITY;
+                if (alive) most = edge ? many_largest<true>(s_at, lo, hi) : many_largest<false>(s_at, lo, hi);
+                half_stat[stream][half][r] = most;
+                meet();
+                if (!alive) continue;
+                most = fmaxf(most, half_stat[stream][1 - half][r]); // (not written again before both have given their weights)
+                if (a.softcap > 0.0f) {
+                    float capped[2] = {most, 0.0f};
+                    pg_cap<2>(capped, a);
+                    most = most == -INFINITY ? most : capped[0]; // (nothing is seen)
                 }
-                const float size = unit == 0.0f ? 1.0f : fabsf(unit);
-                if (__any_sync(0xFFFFFFFFu, valid && (pos + MANY_KEYS > hi || pos < lo))) {
-#pragma unroll
-                    for (int c = 0; c < 128; c++)
-                        if (pos + c >= hi || pos + c < lo) x[c] = -INFINITY;
-                }
-                float top[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int c = 4; c < 128; c += 4)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = fmaxf(top[e], x[c + e]);
-                const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * size;
-                if (__any_sync(0xFFFFFFFFu, most > m + 8.0f)) {
+                most *= unit;
+                if (__any_sync(0xFFFFFFFFu, most > m + 8.0f)) { // alike in both halves
                     const float to = most > m ? most : m, keep = m == -INFINITY ? 0.0f : paged_exp2(m - to);
                     m = to, l *= keep;
-                    if (taken > 0) {
+                    if (j > 0) {
 #pragma unroll 1
-                        for (int c = 0; c < HDP; c += 32) {
-                            unsigned o[32];
-                            pg_ld32(o, o_at + c);
-                            pg_wait_ld();
+                        for (int c = half * (HDP / 2); c < (half + 1) * (HDP / 2); c += 16) {
+                            unsigned o[16];
+                            pg_ld16(o, o_at + c);
+                            pg_wait_ld16(o);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                            pg_st32(o_at + c, o);
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                            pg_st16(o_at + c, o);
                         }
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < 128; c += 32) {
-                    unsigned p[16];
-#pragma unroll
-                    for (int i = 0; i < 32; i += 2) {
-                        const float w0 = paged_exp2(fmaf(x[c + i], size, -base)), w1 = paged_exp2(fmaf(x[c + i + 1], size, -base));
-                        sum[i & 2] += w0, sum[(i & 2) + 1] += w1;
-                        p[i / 2] = pg_pack(w0, w1);
-                    }
-                    pg_st16(s_at + c / 2, p);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (a.softcap > 0.0f)
+                    l += edge ? many_weights<true, true>(a, s_at, s_at, unit, base, lo, hi) : many_weights<true, false>(a, s_at, s_at, unit, base, lo, hi);
+                else
+                    l += edge ? many_weights<false, true>(a, s_at, s_at, unit, base, lo, hi) : many_weights<false, false>(a, s_at, s_at, unit, base, lo, hi);
                 pg_wait_st();
                 pg_fence_before();
-                pg_bar_arrive(&p_full[stream]);
+                pg_bar_arrive(&p_full[2 * stream + half]);
             }
 
             // ---- the item's (or its part's) end ----
-            if (taken > 0) {
+            if (all > 0) {
                 if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&o_full[stream], o_count & 1u))) {
                     if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
                     alive = false;
@@ -482,137 +643,172 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 o_count++;
                 pg_fence_after();
             }
-            const bool is_whole = w.skip == 0 && w.steps() == item.steps;
+            meet(); // the last largest scores are read
+            half_stat[stream][half][r] = l;
+            meet();
+            l = half_stat[stream][0][r] + half_stat[stream][1][r];
+            const bool is_whole = w.skip == 0 && w.steps(item) == item.steps, some = all > 0 && alive;
             const long long slot = (long long)blockIdx.x * 2 + (first_part && w.skip > 0 ? 0 : 1);
+            // the columns that this thread finishes: half of its row's, or where the streams share rows a quarter
+            constexpr int Q4 = HDP / 4;
+            const int from = item.pair ? half * (HDP / 2) : (stream * 2 + half) * Q4, to = from + (item.pair ? HDP / 2 : Q4);
             float keep = 1.0f;
-            int from = 0, to = HDP; // the columns that this stream finishes
-            if (!item.pair) { // the streams' results meet where the queries were: each finishes half of the columns
-                stats[stream][0][r] = m, stats[stream][1][r] = l;
-                asm volatile("bar.sync 1, 256;" ::: "memory"); // both streams are done with their products, so with the queries too
+            if (!item.pair) { // the streams' results meet where the queries were
+                if (half == 0) stats[stream][0][r] = m, stats[stream][1][r] = l;
+                asm volatile("bar.sync 3, 512;" ::: "memory"); // both streams are done with their products, so with the queries too
                 const float other_m = stats[1 - stream][0][r], other_l = stats[1 - stream][1][r], top = fmaxf(m, other_m);
                 keep = m == -INFINITY ? 0.0f : paged_exp2(m - top);
                 l = l * keep + (other_m == -INFINITY ? 0.0f : other_l * paged_exp2(other_m - top));
                 m = top;
-                from = stream * (HDP / 2), to = from + HDP / 2;
+                const int theirs = ((1 - stream) * 2 + half) * Q4;
 #pragma unroll 1
-                for (int c = (1 - stream) * (HDP / 2); c < (2 - stream) * (HDP / 2); c += 32) {
-                    unsigned o[32];
-                    if (taken > 0 && alive) {
-                        pg_ld32(o, o_at + c);
-                        pg_wait_ld();
-                    } else {
+                for (int c = theirs; c < theirs + Q4; c += 16) {
+                    unsigned o[16];
+                    many_output(o, o_at + c, some);
 #pragma unroll
-                        for (int i = 0; i < 32; i++) o[i] = 0;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; i += 4)
+                    for (int i = 0; i < 16; i += 4)
                         reinterpret_cast<float4 *>(query)[((c + i) / 4) * 128 + r] = make_float4(__uint_as_float(o[i]) * keep, __uint_as_float(o[i + 1]) * keep, __uint_as_float(o[i + 2]) * keep,
                                                                                                 __uint_as_float(o[i + 3]) * keep);
                 }
-                asm volatile("bar.sync 1, 256;" ::: "memory");
+                asm volatile("bar.sync 3, 512;" ::: "memory");
             }
-            bool wrong = false;
-            const float share = l == 0.0f ? 0.0f : 1.0f / l;
-            T *out = static_cast<T *>(a.out) + ((long long)(w.s.first + row / a.c.group) * a.c.heads + w.kvh * a.c.group + row % a.c.group) * a.c.hd;
+            const float share = !is_whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l); // (where nothing is seen, O is zero, or not finite and done again)
+            const unsigned long long keep2 = pg_two(keep * share, keep * share), share2 = pg_two(share, share);
+            unsigned long long odd = 0; // zero times what is stored: NaN where that is not finite
+            T *out = static_cast<T *>(a.out) + ((long long)(s.first + place.x) * a.c.heads + w.kvh * a.c.group + place.y) * a.c.hd;
+            float *part = f.part + (slot * BR + mine) * HDP;
+            const bool store = valid && !dead;
 #pragma unroll 1
-            for (int c = from; c < to; c += 32) {
-                unsigned o[32];
-                if (taken > 0 && alive) {
-                    pg_ld32(o, o_at + c);
-                    pg_wait_ld();
+            for (int c = from; c < to; c += 16) {
+                unsigned o[16];
+                many_output(o, o_at + c, some);
+                float y[16];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    unsigned long long v = pg_mul2(pg_two(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), keep2);
+                    if (!item.pair) {
+                        const float2 z = reinterpret_cast<const float2 *>(query)[(((c + i) / 4) * 128 + r) * 2 + (i / 2) % 2];
+                        v = pg_fma2(pg_two(z.x, z.y), share2, v);
+                    }
+                    odd = pg_fma2(v, 0, odd);
+                    pg_one(v, y[i], y[i + 1]);
+                }
+                if (!store) continue;
+                if (is_whole) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 8)
+                        if (c + i < a.c.hd)
+                            *reinterpret_cast<uint4 *>(out + c + i) = make_uint4(pg_pack(y[i], y[i + 1]), pg_pack(y[i + 2], y[i + 3]), pg_pack(y[i + 4], y[i + 5]), pg_pack(y[i + 6], y[i + 7]));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = 0;
+                    for (int i = 0; i < 16; i += 4) *reinterpret_cast<float4 *>(part + c + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
                 }
-                float y[32];
-#pragma unroll
-                for (int i = 0; i < 32; i += 4) {
-                    const float4 z = item.pair ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : reinterpret_cast<const float4 *>(query)[((c + i) / 4) * 128 + r];
-                    y[i] = __uint_as_float(o[i]) * keep + z.x, y[i + 1] = __uint_as_float(o[i + 1]) * keep + z.y;
-                    y[i + 2] = __uint_as_float(o[i + 2]) * keep + z.z, y[i + 3] = __uint_as_float(o[i + 3]) * keep + z.w;
-                }
-                if (!valid) continue;
-                if (!is_whole) {
-                    float4 *dst = reinterpret_cast<float4 *>(f.part + (slot * BR + mine) * HDP + c);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) dst[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                    continue;
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    y[i] = l == 0.0f ? 0.0f : y[i] * share;
-                    wrong |= !isfinite(y[i]);
-                }
-                if (dead) continue;
-#pragma unroll
-                for (int i = 0; i < 32; i += 8)
-                    if (c + i < a.c.hd)
-                        *reinterpret_cast<uint4 *>(out + c + i) = make_uint4(pg_pack(y[i], y[i + 1]), pg_pack(y[i + 2], y[i + 3]), pg_pack(y[i + 4], y[i + 5]), pg_pack(y[i + 6], y[i + 7]));
             }
             if (!is_whole) {
                 float *ml = f.part + (long long)gridDim.x * 2 * BR * HDP + slot * 2 * BR;
                 if (valid && from == 0) ml[mine] = m, ml[BR + mine] = l;
                 if (tid == 0 && w.skip == 0 && !dead) {
                     int *head = f.head + blockIdx.x * 8;
-                    head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = (int)(w.line - line.start), head[5] = (int)line.per;
+                    head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = w.line, head[5] = (int)line.per;
                 }
             }
-            unsigned rest = __ballot_sync(0xFFFFFFFFu, wrong);
-            while (rest) { // a masked key's zero weight met a value that is not finite
-                const int k = __ffs(rest) - 1, at = __shfl_sync(0xFFFFFFFFu, row, k);
+            float odd0, odd1;
+            pg_one(odd, odd0, odd1);
+            unsigned rest = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
+            while (rest) { // a masked key's zero weight met a value that is not finite. Every thread of a row that sees it so does the whole row: the same words.
+                const int k = __ffs(rest) - 1, token = __shfl_sync(0xFFFFFFFFu, place.x, k), head = __shfl_sync(0xFFFFFFFFu, place.y, k);
                 rest &= rest - 1;
-                attend_row_plain<T, T>(a, w.b, w.s.first + at / a.c.group, w.s.pos0 + at / a.c.group, w.s.length, w.kvh * a.c.group + at % a.c.group);
+                attend_row_plain<T, T>(a, w.b, s.first + token, s.pos0 + token, s.length, w.kvh * a.c.group + head);
             }
             pg_fence_before();
-            asm volatile("bar.sync 1, 256;" ::: "memory"); // `query` and `stats` are read
+            asm volatile("bar.sync 3, 512;" ::: "memory"); // `query` and the statistics are read
             first_part = false;
             w.next(a);
         }
     }
     pg_fence_before();
     __syncthreads();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 17) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-// The parts of an item that several blocks share: a warp a row. blockIdx.x: the block that began it.
+// The parts of an item that several blocks share, in the order of its keys: a warp four rows, a lane the statistics of a part and HDP / 32 columns.
+// blockIdx.x: the block that began the item.
 template <typename RT, typename CT, int HDP, int BR>
 __global__ void __launch_bounds__(256) attend_join_rows_kernel(const ManyCall f) {
+    constexpr int ROWS = 4, N = HDP / 32;
     const AttendCall &a = f.a;
-    const int c0 = blockIdx.x, mine = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int c0 = blockIdx.x, lane = threadIdx.x & 31, mine = (blockIdx.y * 8 + (threadIdx.x >> 5)) * ROWS;
     const int *head = f.head + c0 * 8;
-    const int b = head[0];
+    const int b = head[0], kvh = head[1], block = head[2], count = head[3], from = head[4], per = head[5];
     if (b < 0) return;
-    const int kvh = head[1], block = head[2], count = head[3], from = head[4], per = head[5];
     const PagedSeq s = paged_seq(a.c, b);
-    const int row = block * BR + mine;
-    if (row >= min(s.n, a.max_new) * a.c.group) return;
+    const int rows = min(min(s.n, a.max_new) * a.c.group - block * BR, BR);
+    if (mine >= rows) return;
     const int parts = min(1 + (int)((from + (long long)count - 1) / per), (int)gridDim.x - c0);
     const float *ml = f.part + (long long)gridDim.x * 2 * BR * HDP;
-    constexpr int N = HDP / 32;
-    float top = -INFINITY;
-    for (int i = 0; i < parts; i++) top = fmaxf(top, ml[((long long)(c0 + i) * 2 + (i == 0)) * 2 * BR + mine]);
-    float l = 0.0f, o[N];
+    const auto slot = [&](int i) { return (long long)(c0 + i) * 2 + (i == 0); };
+    float top[ROWS], l[ROWS], o[ROWS][N];
 #pragma unroll
-    for (int k = 0; k < N; k++) o[k] = 0.0f;
-    for (int i = 0; i < parts; i++) {
-        const long long slot = (long long)(c0 + i) * 2 + (i == 0);
-        const float m = ml[slot * 2 * BR + mine], keep = m == -INFINITY ? 0.0f : paged_exp2(m - top);
-        l = fmaf(ml[slot * 2 * BR + BR + mine], keep, l);
+    for (int r = 0; r < ROWS; r++) {
+        top[r] = -INFINITY, l[r] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < N; k++) o[k] = fmaf(f.part[(slot * BR + mine) * HDP + lane * N + k], keep, o[k]);
+        for (int k = 0; k < N; k++) o[r][k] = 0.0f;
     }
-    const int token = row / a.c.group, h = kvh * a.c.group + row % a.c.group;
-    RT *out = static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd;
-    bool wrong = false;
+    for (int i = lane; i < parts; i += 32) {
+        const float4 m = *reinterpret_cast<const float4 *>(ml + slot(i) * 2 * BR + mine); // (rows past the item's hold anything, and are not stored)
+        top[0] = fmaxf(top[0], m.x), top[1] = fmaxf(top[1], m.y), top[2] = fmaxf(top[2], m.z), top[3] = fmaxf(top[3], m.w);
+    }
 #pragma unroll
-    for (int k = 0; k < N; k++) {
-        const float y = l == 0.0f ? 0.0f : o[k] / l;
-        if (lane * N + k < a.c.hd) {
-            paged_write(out + lane * N + k, y);
-            wrong |= !isfinite(y);
+    for (int r = 0; r < ROWS; r++)
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xFFFFFFFFu, top[r], d));
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float keep[ROWS] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (i0 + lane < parts) {
+            const float *at = ml + slot(i0 + lane) * 2 * BR + mine;
+            const float4 m = *reinterpret_cast<const float4 *>(at), sums = *reinterpret_cast<const float4 *>(at + BR);
+            const float ms[ROWS] = {m.x, m.y, m.z, m.w}, ls[ROWS] = {sums.x, sums.y, sums.z, sums.w};
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                keep[r] = ms[r] == -INFINITY ? 0.0f : paged_exp2(ms[r] - top[r]);
+                l[r] = fmaf(ls[r], keep[r], l[r]);
+            }
+        }
+        const int here = min(32, parts - i0);
+#pragma unroll 2
+        for (int i = 0; i < here; i++) {
+            const float *at = f.part + (slot(i0 + i) * BR + mine) * HDP + lane * N;
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                const float k = __shfl_sync(0xFFFFFFFFu, keep[r], i);
+                float x[N];
+                if constexpr (N == 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(at + r * HDP);
+                    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2 *>(at + r * HDP);
+                    x[0] = v.x, x[1] = v.y;
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) o[r][e] = fmaf(x[e], k, o[r][e]);
+            }
         }
     }
-    if (__any_sync(0xFFFFFFFFu, wrong)) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
+    for (int r = 0; r < ROWS && mine + r < rows; r++) {
+        const float sum = paged_warp_sum(l[r]);
+        const int row = block * BR + mine + r, token = row / a.c.group, h = kvh * a.c.group + row % a.c.group;
+        RT *out = static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd;
+        bool wrong = false;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const float y = sum == 0.0f ? 0.0f : o[r][k] / sum;
+            if (lane * N + k < a.c.hd) {
+                paged_write(out + lane * N + k, y);
+                wrong |= !isfinite(y);
+            }
+        }
+        if (__any_sync(0xFFFFFFFFu, wrong)) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
+    }
 }
 
 // ---- host side ----
@@ -644,7 +840,7 @@ cudaError_t launch_many_as(const AttendCall &a, const ManyPlan &p, void *ws, int
         if (device < 64) known[device].store(true);
     }
     attend_many_kernel<HDP><<<p.blocks, MANY_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    attend_join_rows_kernel<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS><<<dim3(p.blocks, Shape::BLOCK_ROWS / 8), 256, 0, st>>>(f);
+    attend_join_rows_kernel<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS><<<dim3(p.blocks, Shape::BLOCK_ROWS / 32), 256, 0, st>>>(f);
     *launches += 2;
     return cudaGetLastError();
 }
