@@ -794,20 +794,34 @@ __global__ void __launch_bounds__(256) attend_join_rows_kernel(const ManyCall f)
             }
         }
     }
-    for (int r = 0; r < ROWS && mine + r < rows; r++) {
-        const float sum = paged_warp_sum(l[r]);
-        const int row = block * BR + mine + r, token = row / a.c.group, h = kvh * a.c.group + row % a.c.group;
-        RT *out = static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd;
-        bool wrong = false;
+    const unsigned first = (unsigned)(block * BR), token0 = first / (unsigned)a.c.group, head0 = first - token0 * (unsigned)a.c.group;
+    const bool mine_columns = lane * N < a.c.hd;
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) l[r] += __shfl_xor_sync(0xFFFFFFFFu, l[r], d);
+        if (mine + r >= rows) continue;
+        const unsigned n = head0 + (unsigned)(mine + r), t = a.c.group == 1 ? n : __umulhi(n, a.c.group_part);
+        const int token = (int)(token0 + t), h = kvh * a.c.group + (int)(n - t * (unsigned)a.c.group);
+        const float share = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        float odd = 0.0f; // zero times what is stored: NaN where that is not finite
 #pragma unroll
         for (int k = 0; k < N; k++) {
-            const float y = sum == 0.0f ? 0.0f : o[r][k] / sum;
-            if (lane * N + k < a.c.hd) {
-                paged_write(out + lane * N + k, y);
-                wrong |= !isfinite(y);
-            }
+            o[r][k] *= share;
+            odd = fmaf(o[r][k], 0.0f, odd);
         }
-        if (__any_sync(0xFFFFFFFFu, wrong)) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
+        RT *out = static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd + lane * N;
+        if (mine_columns) {
+            if constexpr (sizeof(RT) == 2 && N == 4)
+                *reinterpret_cast<uint2 *>(out) = make_uint2(pg_pack(o[r][0], o[r][1]), pg_pack(o[r][2], o[r][3]));
+            else if constexpr (sizeof(RT) == 2)
+                *reinterpret_cast<unsigned *>(out) = pg_pack(o[r][0], o[r][1]);
+            else if constexpr (N == 4)
+                *reinterpret_cast<float4 *>(out) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+            else
+                *reinterpret_cast<float2 *>(out) = make_float2(o[r][0], o[r][1]);
+        }
+        if (__any_sync(0xFFFFFFFFu, mine_columns && !(odd == 0.0f))) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
     }
 }
 
