@@ -19,15 +19,29 @@ changed. Rows and cache are float32 and float32, float32 and bfloat16, or bfloat
 Calls are asynchronous on the current stream. A page number outside the pool is treated as a page of zeros and not written,
 and reported by `torch_ops.check_status`.
 """
+import functools
 import math
 
 import torch
 
 from . import _native
-from .torch_ops import _on, _stream, _vp
+from .torch_ops import _bind_host_call, _host_call, _on, _stream, _vp
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 _NORMS = {"rmsnorm": 0, "rmsnorm_offset": 2}
+
+
+def _bind(name):
+    def first(*args):
+        if not _bind_host_call():
+            return None
+        globals()["_plain_" + name] = getattr(_host_call, "paged_" + name)
+        return globals()["_plain_" + name](*args)
+    return first if _host_call is not None else None
+
+
+#: the calls on plain device tensors in native code, or None where a call is anything else: those go through the checks below
+_plain_append, _plain_attention = _bind("append"), _bind("attention")
 
 
 def _rows(t, name, heads, head_dim, dtype, device, total):
@@ -75,6 +89,11 @@ def _vector(t, name, n, device):
     return t
 
 
+@functools.lru_cache(maxsize=None)
+def _scale(head_dim):
+    return 1.0 / math.sqrt(max(head_dim, 1))
+
+
 def _out(out, q):
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -92,6 +111,10 @@ def append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos=None, sin=Non
     `cos`, `sin` float32 [positions, rope_dim / 2] hold the rotation of every position (None: no rotation); columns from rope_dim on
     pass through. `q_norm`, `k_norm` float32 [head_dim]: an RMSNorm over each head's vector before the rotation, of weight w
     ("rmsnorm") or 1 + w ("rmsnorm_offset"). Rows past cu[-1] belong to no sequence: their part of the answer is not written."""
+    if out is None and norm in _NORMS and _plain_append is not None:
+        done = _plain_append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos, sin, q_norm, k_norm, eps, _NORMS[norm])
+        if done is not None:
+            return done
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _TYPES:
         raise TypeError("q must be a float32 or bfloat16 CUDA tensor")
     _cache(k_cache, v_cache, page_table, cu, lengths, q.dtype, q.device)
@@ -132,6 +155,10 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
     `max_new` and `max_length` are what the caller knows of the most new tokens of a sequence and of the longest cache (by default
     all rows and the whole table): the call is cut by them, and a sequence with more than `max_new` rows is reported by
     `torch_ops.check_status`. `scale` is 1 / sqrt(head_dim) by default. Rows past cu[-1] are not written."""
+    if out is None and max_new is not None and max_length is not None and _plain_attention is not None and isinstance(q, torch.Tensor):
+        done = _plain_attention(q, k_cache, v_cache, page_table, cu, lengths, max_new, max_length, _scale(q.shape[-1] if q.dim() else 1) if scale is None else scale, window, softcap)
+        if done is not None:
+            return done
     if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _TYPES:
         raise TypeError("q must be a float32 or bfloat16 CUDA tensor")
     _cache(k_cache, v_cache, page_table, cu, lengths, q.dtype, q.device)
@@ -148,7 +175,7 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
         need = int(_native.lib().b200i_paged_attention_workspace_bytes(q.device.index, *types, rows, batch, n_heads, n_kv, hd, max_new, max_length, int(window)))
         ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
         _native.call("b200i_paged_attention", q.device.index, _stream(q.device), _vp(out), _vp(q), ldq, _vp(k_cache), _vp(v_cache), *types, _vp(page_table), _vp(cu),
-                     _vp(lengths), rows, batch, n_heads, n_kv, hd, pages, page, max_pages, max_new, max_length, 1.0 / math.sqrt(hd) if scale is None else float(scale),
+                     _vp(lengths), rows, batch, n_heads, n_kv, hd, pages, page, max_pages, max_new, max_length, _scale(hd) if scale is None else float(scale),
                      int(window), float(softcap), _vp(ws), need)
     return out
 

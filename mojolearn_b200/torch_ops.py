@@ -107,14 +107,22 @@ ACT_NONE, ACT_GELU_ERF, ACT_GELU_TANH, ACT_SILU = 0, 1, 2, 3
 ACT_PAIR_SWIGLU, ACT_PAIR_GEGLU_ERF, ACT_PAIR_GEGLU_TANH = 4, 5, 6  # over interleaved (gate, up) weight rows: output [m, n / 2]
 
 
-def _bind_plain_product(*args):
-    global _plain_product
+def _bind_host_call():
+    """Give the native host side the library's entry points; False where there is none to give (the Python path then refuses)."""
     try:
         lib = _native.lib()
     except _native.NativeError:
-        return None  # the Python path's checks of the operands come first, then its own refusal
-    _host_call.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.b200i_gemm_w_plan, lib.b200i_product_workspace_bytes, lib.b200i_plan_workspace_bytes)),
+        return False
+    _host_call.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.b200i_gemm_w_plan, lib.b200i_product_workspace_bytes, lib.b200i_plan_workspace_bytes,
+                                                                      lib.b200i_paged_append, lib.b200i_paged_attention, lib.b200i_paged_attention_workspace_bytes)),
                     _native.NativeError)
+    return True
+
+
+def _bind_plain_product(*args):
+    global _plain_product
+    if not _bind_host_call():
+        return None  # the Python path's checks of the operands come first, then its own refusal
     _plain_product = _host_call.product
     return _plain_product(*args)
 
