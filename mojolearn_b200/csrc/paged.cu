@@ -54,20 +54,20 @@ int64_t enter(PagedCall *c, const char *who, int64_t device, int *dev, char *err
 // The kernel of a call and how its work is cut.
 struct AttendPlan {
     int few;      // rows of a sequence and key head, where they are few (else 0)
-    int hdp, nt;  // head_dim as it is laid out in shared memory; sets of eight rows
+    int hdp;      // head_dim as it is laid out in shared memory
     FewPlan cut;
     ManyPlan cut_many; // where they are many
     int64_t bytes() const { return few ? cut.bytes : cut_many.bytes; }
 };
-constexpr int FEW_ROWS = 16;
 
 AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
     AttendPlan p = {};
     p.hdp = head_dim <= 64 ? 64 : 128;
     const int64_t group = n_heads / n_kv;
-    if (max_new <= FEW_ROWS && max_new * group <= FEW_ROWS) {
-        p.few = (int)(max_new * group), p.nt = p.few <= 8 ? 1 : 2;
-        p.cut = few_plan(b200i_library::device_sms(device), (int)batch, (int)n_kv, p.hdp, p.nt, cache_type == B200I_T_F32 ? 32 : 64, max_new, max_length, (int)std::min(window, MOST));
+    if (max_new <= FEW_MOST && max_new * group <= FEW_MOST) {
+        p.few = (int)(max_new * group);
+        p.cut = few_plan(b200i_library::device_sms(device), row_type == B200I_T_F32, cache_type == B200I_T_F32, (int)batch, (int)n_kv, p.hdp, p.few, max_new, max_length,
+                         (int)std::min(window, MOST));
     } else {
         p.cut_many = many_plan(b200i_library::device_sms(device), row_type == B200I_T_BF16 ? ManyShape<128>::BLOCK_ROWS : FINE_ROWS, p.hdp);
     }
@@ -145,11 +145,11 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
     if (p.few) {
         if (row_type == B200I_T_BF16)
-            LIBRARY_CUDA_TRY((launch_few<__nv_bfloat16, __nv_bfloat16>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
+            LIBRARY_CUDA_TRY((launch_few<__nv_bfloat16, __nv_bfloat16>(a, p.cut, p.hdp, ws, dev, st, &launches)));
         else if (cache_type == B200I_T_BF16)
-            LIBRARY_CUDA_TRY((launch_few<float, __nv_bfloat16>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
+            LIBRARY_CUDA_TRY((launch_few<float, __nv_bfloat16>(a, p.cut, p.hdp, ws, dev, st, &launches)));
         else
-            LIBRARY_CUDA_TRY((launch_few<float, float>(a, p.cut, p.hdp, p.nt, ws, dev, st, &launches)));
+            LIBRARY_CUDA_TRY((launch_few<float, float>(a, p.cut, p.hdp, ws, dev, st, &launches)));
     } else {
         if (row_type == B200I_T_BF16)
             LIBRARY_CUDA_TRY(p.hdp == 64 ? launch_many_as<64>(a, p.cut_many, ws, dev, st, &launches) : launch_many_as<128>(a, p.cut_many, ws, dev, st, &launches));

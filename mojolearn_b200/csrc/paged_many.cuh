@@ -91,28 +91,6 @@ __device__ __forceinline__ void pg_st8(unsigned taddr, const unsigned *v) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), PG_R8(v, 0) : "memory");
 }
 
-// Two 32-bit words at a time.
-__device__ __forceinline__ unsigned long long pg_two(float x, float y) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void pg_one(unsigned long long v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ unsigned long long pg_fma2(unsigned long long x, unsigned long long y, unsigned long long z) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
-    return r;
-}
-__device__ __forceinline__ unsigned long long pg_add2(unsigned long long x, unsigned long long y) {
-    unsigned long long r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
-__device__ __forceinline__ unsigned long long pg_mul2(unsigned long long x, unsigned long long y) {
-    unsigned long long r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
-    return r;
-}
 __device__ __forceinline__ float pg_max3(float x, float y, float z) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
