@@ -98,6 +98,20 @@ __device__ __forceinline__ unsigned long long pg_mul2(unsigned long long x, unsi
     return r;
 }
 
+// A kernel that joins what the one before it left: its blocks are brought in while that one ends (pg_follow_early there lets them), and go on from
+// pg_follow when it has ended and what it wrote is to be seen.
+__device__ __forceinline__ void pg_follow_early() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pg_follow() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename F>
+inline cudaError_t launch_following(void (*kernel)(const F), dim3 grid, int threads, cudaStream_t st, const F &f) {
+    cudaLaunchConfig_t c = {};
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    c.gridDim = grid, c.blockDim = dim3(threads), c.stream = st, c.attrs = &early, c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, f);
+}
+
 // A cache as a matrix of rows of head_dim, in boxes of 128 bytes by `box_rows` rows, 128-byte swizzle, zeros outside.
 typedef CUresult (*PagedEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *, const cuuint32_t *,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

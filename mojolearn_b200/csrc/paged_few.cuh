@@ -47,7 +47,7 @@ struct FewCall {
     AttendCall a;
     float *part;       // [blocks][2][rows * HDP] outputs of parts, then [blocks][2][2 * rows] of m and l
     int *head;         // [blocks][8]: the item whose beginning a block left as a part: sequence (or -1), key head, tiles, tiles of the block before it, tiles a block
-    int whole;         // a block takes whole items: no parts
+    int whole;         // a block takes whole items, by steps of the grid: no parts
 };
 
 // Tiles of a sequence's key heads: from the first key that a row sees; one where rows see nothing, which makes them zero.
@@ -161,11 +161,21 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
         }
         return alive;
     };
-    int b = p.b, kvh = p.kvh, before = f.whole ? 0 : (int)p.in, line = -before;
+    int b = p.b, kvh = p.kvh, before = (int)p.in, line = -before;
     long long left = p.left;
     PagedSeq s = {};
     int t0 = 0, count = 0;
-    if (left > 0) s = paged_seq(a.c, b), count = few_tiles(a, s, KEYS, &t0);
+    const auto settle = [&] { // whole items: the first from (b, kvh) on, by steps of the grid, that has rows
+        for (; b < a.c.batch; kvh += gridDim.x, b += kvh / a.c.kv, kvh %= a.c.kv) {
+            s = paged_seq(a.c, b), count = few_tiles(a, s, KEYS, &t0);
+            if (count > 0) return;
+        }
+        left = 0;
+    };
+    if (f.whole)
+        settle();
+    else if (left > 0)
+        s = paged_seq(a.c, b), count = few_tiles(a, s, KEYS, &t0);
     for (; alive; number++) {
         const int at = number % FEW_ITEMS;
         if (!wait(&sm.item_empty[at], ((number / FEW_ITEMS) & 1u) ^ 1u)) break; // a fresh barrier counts as released
@@ -197,7 +207,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
         // what follows is asked for while this item's tiles come in
         const int b1 = kvh + 1 < a.c.kv ? b : b + 1;
         PagedSeq s1 = s;
-        if (b1 != b && b1 < a.c.batch) s1 = paged_seq(a.c, b1);
+        if (!f.whole && b1 != b && b1 < a.c.batch) s1 = paged_seq(a.c, b1);
         for (int t = 0; t < tiles; t++, it++) {
             const int slot = (int)(it % SLOTS), pos = (t0 + before + t) * KEYS;
             if (!wait(&sm.empty[slot], ((it / SLOTS) & 1u) ^ 1u)) break;
@@ -226,7 +236,12 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
                 }
             }
         }
-        left -= f.whole ? 1 : tiles;
+        if (f.whole) {
+            kvh += gridDim.x, b += kvh / a.c.kv, kvh %= a.c.kv;
+            settle();
+            continue;
+        }
+        left -= tiles;
         line += count, before = 0;
         if (left <= 0) continue;
         if (++kvh >= a.c.kv) {
@@ -256,11 +271,19 @@ __device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory
         if (!f.whole) f.head[blockIdx.x * 8] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    const auto tiles = [&](int b) {
-        int t0;
-        return few_tiles(f.a, paged_seq(f.a.c, b), FewKeys<CT>::N, &t0);
-    };
-    const LinePlace p = line_place(f.a.c, [&](int b) -> long long { return f.whole ? (long long)(tiles(b) > 0) : (long long)tiles(b); }, blockIdx.x, gridDim.x, place);
+    LinePlace p;
+    if (!f.whole) pg_follow_early();
+    if (f.whole) {
+        p.b = (int)blockIdx.x / f.a.c.kv, p.kvh = (int)blockIdx.x % f.a.c.kv, p.in = 0, p.left = 1, p.per = 0;
+    } else {
+        p = line_place(
+            f.a.c,
+            [&](int b) -> long long {
+                int t0;
+                return few_tiles(f.a, paged_seq(f.a.c, b), FewKeys<CT>::N, &t0);
+            },
+            blockIdx.x, gridDim.x, place);
+    }
     __syncthreads();
     return p;
 }
@@ -299,7 +322,7 @@ template <int HDP, int NT>
 using FewMmaShape = FewShape<HDP, 3 * HDP * NT * 8 * 4, NT * 8 * HDP * 2>;
 
 template <int HDP, int NT>
-__global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const FewCall f) {
+__global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FewCall f) {
     using T = __nv_bfloat16;
     using Shape = FewMmaShape<HDP, NT>;
     constexpr int KEYS = FewKeys<T>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, KS = HDP / 16, ROWS = NT * 8;
@@ -600,7 +623,7 @@ template <> struct FewRow<__nv_bfloat16> {
 
 template <typename CT, int HDP, int R>
 __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
-    attend_few_fma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const FewCall f) {
+    attend_few_fma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FewCall f) {
     using Shape = FewFmaShape<CT, HDP, R>;
     constexpr int KEYS = FewKeys<CT>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, MINE = KEYS / FEW_WARPS, SPLIT = 32 / MINE, COLS = HDP / 32, N = FewRow<CT>::N;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -784,39 +807,70 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
     }
 }
 
-// The parts of an item that several blocks share. blockIdx.x: the block that began it; blockIdx.y: the row.
+// The parts of an item that several blocks share, in the order of its keys: a block a row, a warp every eighth part, a lane the statistics of a part
+// and HDP / 32 columns of its output. blockIdx.x: the block that began the item; blockIdx.y: the row. What it costs is the way there: code that
+// is fetched from L2, and a chain of loads.
 template <typename RT, typename CT, int HDP, int ROWS>
-__global__ void __launch_bounds__(HDP) attend_join_kernel(const FewCall f) {
+__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ FewCall f) {
+    constexpr int N = HDP / 32;
+    __shared__ float met[8][HDP];
     const AttendCall &a = f.a;
-    const int c0 = blockIdx.x, r = blockIdx.y, col = threadIdx.x;
-    const int b = f.head[c0 * 8];
+    const int c0 = blockIdx.x, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int token = a.c.group == 1 ? r : (int)__umulhi((unsigned)r, a.c.group_part);
+    pg_follow();
+    const int4 head = *reinterpret_cast<const int4 *>(f.head + c0 * 8);
+    const int per = f.head[c0 * 8 + 4], b = head.x;
     if (b < 0) return;
-    const int kvh = f.head[c0 * 8 + 1], count = f.head[c0 * 8 + 2], from = f.head[c0 * 8 + 3], per = f.head[c0 * 8 + 4];
     const PagedSeq s = paged_seq(a.c, b);
-    if (r >= min(s.n, a.max_new) * a.c.group) return;
-    const int parts = min(1 + (int)((from + (long long)count - 1) / per), (int)gridDim.x - c0);
-    const float *stats = f.part + (long long)gridDim.x * 2 * ROWS * HDP;
-    float top = -INFINITY;
-    for (int i = 0; i < parts; i++) top = fmaxf(top, stats[((long long)(c0 + i) * 2 + (i == 0)) * 2 * ROWS + r]);
-    float l = 0.0f, o = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < parts; i++) {
-        const long long slot = (long long)(c0 + i) * 2 + (i == 0);
-        const float m = stats[slot * 2 * ROWS + r], keep = m == -INFINITY ? 0.0f : paged_exp2(m - top);
-        l = fmaf(stats[slot * 2 * ROWS + ROWS + r], keep, l);
-        o = fmaf(f.part[(slot * ROWS + r) * HDP + col], keep, o);
+    if (token >= min(s.n, a.max_new)) return;
+    const int parts = min(1 + (int)((unsigned)(head.w + head.z - 1) / (unsigned)per), (int)gridDim.x - c0);
+    const float *stats = f.part + (long long)gridDim.x * 2 * ROWS * HDP + r, *outputs = f.part + r * HDP + lane * N;
+    const auto slot = [&](int i) { return (unsigned)((c0 + i) * 2 + (i == 0)); };
+    float top = -INFINITY, l = 0.0f, o[N] = {};
+#pragma unroll 1
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, stats[slot(i) * (2 * ROWS)]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+#pragma unroll 1
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        float keep = 0.0f;
+        if (i0 + lane < parts) {
+            const float *at = stats + slot(i0 + lane) * (2 * ROWS);
+            keep = *at == -INFINITY ? 0.0f : paged_exp2(*at - top);
+            l = fmaf(at[ROWS], keep, l);
+        }
+        const int here = min(32, parts - i0);
+#pragma unroll 2
+        for (int i = warp; i < here; i += 8) {
+            const float k = __shfl_sync(0xFFFFFFFFu, keep, i);
+            const float *at = outputs + (long long)slot(i0 + i) * (ROWS * HDP);
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                const float2 v = *reinterpret_cast<const float2 *>(at + e);
+                o[e] = fmaf(v.x, k, o[e]), o[e + 1] = fmaf(v.y, k, o[e + 1]);
+            }
+        }
     }
-    const int row = s.first + r / a.c.group, h = kvh * a.c.group + r % a.c.group;
-    const float y = l == 0.0f ? 0.0f : o / l;
-    if (col < a.c.hd) paged_write(static_cast<RT *>(a.out) + ((long long)row * a.c.heads + h) * a.c.hd + col, y);
-    if (__syncthreads_or(col < a.c.hd && !isfinite(y)) && threadIdx.x < 32) attend_row_plain<RT, CT>(a, b, row, s.pos0 + r / a.c.group, s.length, h);
+    l = paged_warp_sum(l);
+#pragma unroll
+    for (int k = 0; k < N; k++) met[warp][lane * N + k] = o[k];
+    __syncthreads();
+    const int col = threadIdx.x, h = (head.y - token) * a.c.group + r;
+    float y = 0.0f;
+    if (col < a.c.hd) {
+#pragma unroll
+        for (int w = 0; w < 8; w++) y += met[w][col];
+        y *= l == 0.0f ? 0.0f : __frcp_rn(l);
+        paged_write(static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd + col, y);
+    }
+    if (__syncthreads_or(!(y * 0.0f == 0.0f)) && warp == 0) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
 }
 
 // ---- host side ----
 
 // How a call is cut: from what the host knows of the lengths, so nothing waits for the device.
 struct FewPlan {
-    int blocks, whole, rows;      // rows: what an item is laid out for
+    int blocks, whole, most, rows; // most rows of an item; what it is laid out for
     long long part_floats, bytes; // of the workspace
 };
 constexpr int FEW_LEAST = 4;  // tiles that a block takes at least
@@ -828,7 +882,7 @@ template <bool F32, typename CT, int HDP, int R> constexpr int few_blocks_per_sm
 inline FewPlan few_plan(int sms, bool f32_rows, bool f32_cache, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     FewPlan p;
     const int keys = f32_cache ? FewKeys<float>::N : FewKeys<__nv_bfloat16>::N;
-    p.rows = f32_rows ? 1 : 8; // laid out for 1, 2, 4, 8 or 16 float32 rows, for 8 or 16 of bfloat16
+    p.most = rows, p.rows = f32_rows ? 1 : 8; // laid out for 1, 2, 4, 8 or 16 float32 rows, for 8 or 16 of bfloat16
     while (p.rows < rows) p.rows *= 2;
     const int per_sm = p.rows < 16 ? 2 : (!f32_rows ? few_blocks_per_sm<false, __nv_bfloat16, 128, 16>() : (hdp == 64 ? few_blocks_per_sm<true, float, 64, 16>() : few_blocks_per_sm<true, float, 128, 16>()));
     long long span = max_length;
@@ -867,8 +921,8 @@ cudaError_t launch_few_as(const AttendCall &a, const FewPlan &p, void *ws, int d
     kernel<<<p.blocks, FEW_THREADS, smem, st>>>(map_k, map_v, f);
     *launches += 1;
     if (!p.whole) {
-        attend_join_kernel<RT, CT, HDP, R><<<dim3(p.blocks, R), HDP, 0, st>>>(f);
         *launches += 1;
+        return launch_following<FewCall>(attend_join_kernel<RT, CT, HDP, R>, dim3(p.blocks, p.most), 256, st, f);
     }
     return cudaGetLastError();
 }

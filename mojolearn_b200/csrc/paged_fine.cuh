@@ -30,7 +30,7 @@ template <typename CT, int HDP> struct FineShape {
 };
 
 template <typename CT, int HDP>
-__global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ManyCall f) {
+__global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyCall f) {
     using Shape = FineShape<CT, HDP>;
     using Walk = ManyWalk<FINE_ROWS, FINE_KEYS, 1>;
     constexpr int SLOTS = Shape::SLOTS, SLOT = Shape::SLOT, TILE = Shape::TILE, CP = Shape::PIECES, BOXES = HDP / 64, HALF_COLS = FINE_KEYS * 128, BR = FINE_ROWS;
@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_smem(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pg_follow_early();
     const LinePlace line = line_place(a.c, [&](int b) { return Walk::steps_of(a, b); }, blockIdx.x, gridDim.x, place);
     pg_fence_before();
     __syncthreads();
@@ -449,9 +450,9 @@ cudaError_t launch_fine_as(const AttendCall &a, const ManyPlan &p, void *ws, int
         if (device < 64) known[device].store(true);
     }
     attend_fine_kernel<CT, HDP><<<p.blocks, FINE_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    attend_join_rows_kernel<float, CT, HDP, FINE_ROWS><<<dim3(p.blocks, FINE_ROWS / 32), 256, 0, st>>>(f);
     *launches += 2;
-    return cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? e : launch_following<ManyCall>(attend_join_rows_kernel<float, CT, HDP, FINE_ROWS>, dim3(p.blocks, FINE_ROWS / 32), 256, st, f);
 }
 
 } // namespace b200i

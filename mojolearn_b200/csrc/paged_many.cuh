@@ -335,7 +335,7 @@ __device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some)
 }
 
 template <int HDP>
-__global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const ManyCall f) {
+__global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyCall f) {
     using Shape = ManyShape<HDP>;
     constexpr int SLOTS = Shape::SLOTS, TILE = Shape::TILE, BOXES = HDP / 64, BR = Shape::BLOCK_ROWS, HALF_COLS = 128 * 128; // bytes of a tile's 64 columns
     using T = __nv_bfloat16; // of rows and cache
@@ -370,6 +370,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(pg_smem(&tmem_slot)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    pg_follow_early();
     const LinePlace line = line_place(a.c, [&](int b) { return Walk::steps_of(a, b); }, blockIdx.x, gridDim.x, place);
     pg_fence_before();
     __syncthreads();
@@ -712,10 +713,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
 // The parts of an item that several blocks share, in the order of its keys: a warp four rows, a lane the statistics of a part and HDP / 32 columns.
 // blockIdx.x: the block that began the item.
 template <typename RT, typename CT, int HDP, int BR>
-__global__ void __launch_bounds__(256) attend_join_rows_kernel(const ManyCall f) {
+__global__ void __launch_bounds__(256) attend_join_rows_kernel(const __grid_constant__ ManyCall f) {
     constexpr int ROWS = 4, N = HDP / 32;
     const AttendCall &a = f.a;
     const int c0 = blockIdx.x, lane = threadIdx.x & 31, mine = (blockIdx.y * 8 + (threadIdx.x >> 5)) * ROWS;
+    pg_follow();
     const int *head = f.head + c0 * 8;
     const int b = head[0], kvh = head[1], block = head[2], count = head[3], from = head[4], per = head[5];
     if (b < 0) return;
@@ -832,9 +834,9 @@ cudaError_t launch_many_as(const AttendCall &a, const ManyPlan &p, void *ws, int
         if (device < 64) known[device].store(true);
     }
     attend_many_kernel<HDP><<<p.blocks, MANY_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    attend_join_rows_kernel<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS><<<dim3(p.blocks, Shape::BLOCK_ROWS / 32), 256, 0, st>>>(f);
     *launches += 2;
-    return cudaGetLastError();
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? e : launch_following<ManyCall>(attend_join_rows_kernel<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS>, dim3(p.blocks, Shape::BLOCK_ROWS / 32), 256, st, f);
 }
 
 } // namespace b200i
