@@ -97,16 +97,16 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
     if (norm_kind != 0 && norm_kind != 2) return refuse(err, err_cap, "paged_append: norm kind %lld is not 0 (weight w) or 2 (weight 1 + w)", (long long)norm_kind);
     a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.k_cache = k_cache, a.v_cache = v_cache, a.ldq = ldq, a.ldk = ldk, a.ldv = ldv;
     a.cosv = cosv, a.sinv = sinv, a.q_norm = q_norm, a.k_norm = k_norm, a.rope_dim = (int)rope_dim, a.positions = (int)positions;
-    a.eps = (float)eps, a.norm_shift = norm_kind == 2 ? 1.0f : 0.0f;
+    a.part_of_head = 1.0f / (float)head_dim, a.eps = (float)eps, a.norm_shift = norm_kind == 2 ? 1.0f : 0.0f;
     int dev;
     if (enter(&a.c, "paged_append", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (row_type == B200I_T_BF16)
-        LIBRARY_CUDA_TRY((launch_append<__nv_bfloat16, __nv_bfloat16>(a, st)));
+        LIBRARY_CUDA_TRY((launch_append<__nv_bfloat16, __nv_bfloat16>(a, b200i_library::device_sms(dev), st)));
     else if (cache_type == B200I_T_BF16)
-        LIBRARY_CUDA_TRY((launch_append<float, __nv_bfloat16>(a, st)));
+        LIBRARY_CUDA_TRY((launch_append<float, __nv_bfloat16>(a, b200i_library::device_sms(dev), st)));
     else
-        LIBRARY_CUDA_TRY((launch_append<float, float>(a, st)));
+        LIBRARY_CUDA_TRY((launch_append<float, float>(a, b200i_library::device_sms(dev), st)));
     b200i_library::count_launches(1);
     b200i_library::accept(err, err_cap);
     return 0;
