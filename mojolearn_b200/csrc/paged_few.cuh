@@ -27,14 +27,14 @@ namespace b200i {
 
 constexpr int FEW_WARPS = 4, FEW_THREADS = 32 * (FEW_WARPS + 1), FEW_ITEMS = 2; // items whose queries are held
 
-// keys of a ring slot: 64 of bfloat16, 32 of float32, so that a slot is head_dim (padded) x 256 bytes of keys and values
-template <typename CT> struct FewKeys { static constexpr int N = 64; };
-template <> struct FewKeys<float> { static constexpr int N = 32; };
+// keys of a ring slot, which is 32 KB of keys and values: 64 of bfloat16 and 32 of float32 at head_dim 128, twice as many at 64
+constexpr int FEW_SLOT = 32 * 1024;
+template <typename CT, int HDP> struct FewKeys { static constexpr int N = FEW_SLOT / (2 * HDP * (int)sizeof(CT)); };
 
 // Shared memory of a block: the ring, `meet` bytes for the warps' results, the queries, barriers. Two blocks on an SM (113 KB each) where
 // that leaves two slots.
 template <int HDP, int MEET_BYTES, int QUERY_BYTES> struct FewShape {
-    static constexpr int SLOT = HDP * 256, MEET = MEET_BYTES, QUERY = QUERY_BYTES;
+    static constexpr int SLOT = FEW_SLOT, MEET = MEET_BYTES, QUERY = QUERY_BYTES;
     static constexpr int REST = 1024 + 512 + MEET + FEW_ITEMS * QUERY;
     static constexpr int BLOCKS = (110 * 1024 - REST) / SLOT >= 2 ? 2 : 1;
     static constexpr int ROOM = ((BLOCKS == 2 ? 112 : 220) * 1024 - REST) / SLOT;
@@ -149,7 +149,7 @@ template <typename Shape> struct FewMemory {
 // The copying warp. `items`: FEW_ITEMS of them in shared memory.
 template <typename RT, typename CT, int HDP, typename Shape>
 __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUtensorMap *map_v, const FewCall &f, const FewMemory<Shape> &sm, FewItem *items, const LinePlace &p) {
-    constexpr int KEYS = FewKeys<CT>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, BOX_COLS = 128 / (int)sizeof(CT), BOXES = HDP / BOX_COLS;
+    constexpr int KEYS = FewKeys<CT, HDP>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, BOX_COLS = 128 / (int)sizeof(CT), BOXES = HDP / BOX_COLS;
     const AttendCall &a = f.a;
     const int lane = threadIdx.x & 31, page = 1 << a.c.page_shift, box_rows = min(page, KEYS), pieces = KEYS / box_rows;
     unsigned it = 0, number = 0;
@@ -216,7 +216,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
             if (lane == 0) pg_bar_expect(&sm.full[slot], (unsigned)(there * box_rows * 128 * BOXES * 2));
             __syncwarp();
             const int first = pos >> a.c.page_shift;
-            if (first + pieces - 1 >= base + 32 && there > 0) { // a tile's pages (at most four) lie in one set of 32: sets begin at its own
+            if (first + pieces - 1 >= base + 32 && there > 0) { // a tile's pages (at most eight) lie in one set of 32: sets begin at its own
                 base += 32;
                 id = ahead;
                 ahead = base + 32 + lane <= last_page ? ids[base + 32 + lane] : 0;
@@ -256,7 +256,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
 }
 
 // The beginning of a block: barriers, and its place on the line.
-template <typename CT, typename Shape>
+template <typename CT, int HDP, typename Shape>
 __device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory<Shape> &sm, long long *place, unsigned *bad_rows, int *dead) {
     if (threadIdx.x == 0) {
         for (int s = 0; s < Shape::SLOTS; s++) {
@@ -280,7 +280,7 @@ __device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory
             f.a.c,
             [&](int b) -> long long {
                 int t0;
-                return few_tiles(f.a, paged_seq(f.a.c, b), FewKeys<CT>::N, &t0);
+                return few_tiles(f.a, paged_seq(f.a.c, b), FewKeys<CT, HDP>::N, &t0);
             },
             blockIdx.x, gridDim.x, place);
     }
@@ -308,14 +308,16 @@ __device__ __forceinline__ void few_again(const AttendCall &a, const FewItem &i,
 // ---- bfloat16 rows ----
 
 // 16 keys by 16 columns of the tile as a fragment: rows are keys.
+template <int KEYS>
 __device__ __forceinline__ void few_keys(unsigned (&f)[4], const unsigned char *tile, int key0, int ks, int lane) {
     const int mi = lane >> 3, row = key0 + (lane & 7) + (mi & 1) * 8, chunk = 2 * ks + (mi >> 1);
-    pg_ldmatrix(f, pg_smem(tile) + (unsigned)((chunk >> 3) * (FewKeys<__nv_bfloat16>::N * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)));
+    pg_ldmatrix(f, pg_smem(tile) + (unsigned)((chunk >> 3) * (KEYS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)));
 }
 // The same of the values, turned: rows are columns of the tile (16 of them), columns its keys.
+template <int KEYS>
 __device__ __forceinline__ void few_values(unsigned (&f)[4], const unsigned char *tile, int key0, int mt, int lane) {
     const int mi = lane >> 3, row = key0 + (lane & 7) + (mi >> 1) * 8, chunk = 2 * mt + (mi & 1);
-    pg_ldmatrix_t(f, pg_smem(tile) + (unsigned)((chunk >> 3) * (FewKeys<__nv_bfloat16>::N * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)));
+    pg_ldmatrix_t(f, pg_smem(tile) + (unsigned)((chunk >> 3) * (KEYS * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)));
 }
 
 template <int HDP, int NT>
@@ -325,7 +327,7 @@ template <int HDP, int NT>
 __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) attend_few_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FewCall f) {
     using T = __nv_bfloat16;
     using Shape = FewMmaShape<HDP, NT>;
-    constexpr int KEYS = FewKeys<T>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, KS = HDP / 16, ROWS = NT * 8;
+    constexpr int KEYS = FewKeys<T, HDP>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, KS = HDP / 16, ROWS = NT * 8;
     extern __shared__ __align__(128) unsigned char smem[];
     const FewMemory<Shape> sm(smem);
     __shared__ float ml[FEW_WARPS][2][ROWS];
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
     __shared__ int dead;
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const LinePlace p = few_begin<T>(f, sm, place, &bad_rows, &dead);
+    const LinePlace p = few_begin<T, HDP>(f, sm, place, &bad_rows, &dead);
     if (warp == FEW_WARPS) {
         few_copies<T, T, HDP>(&map_k, &map_v, f, sm, items, p);
         return;
@@ -390,9 +392,12 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
             for (int mt = 0; mt < KS; mt++) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
         }
         for (int t = 0; t < item.tiles; t++, it++) {
-            const int slot = (int)(it % SLOTS), key0 = warp * 16, j0 = item.pos + t * KEYS + key0;
+            const int slot = (int)(it % SLOTS);
             if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot], (it / SLOTS) & 1u))) give_up();
-            if (alive && j0 < s.length) {
+#pragma unroll 1
+            for (int key0 = warp * 16; key0 < KEYS; key0 += 16 * FEW_WARPS) {
+                const int j0 = item.pos + t * KEYS + key0;
+                if (!alive || j0 >= s.length) break;
                 const unsigned char *kt = sm.ring + slot * Shape::SLOT, *vt = kt + HALF;
                 float z[NT][4];
 #pragma unroll
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++) {
                     unsigned k[4];
-                    few_keys(k, kt, key0, ks, lane);
+                    few_keys<KEYS>(k, kt, key0, ks, lane);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) pg_mma(z[nt], k, q0[nt][ks], q1[nt][ks]);
                 }
@@ -462,7 +467,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
 #pragma unroll
                 for (int mt = 0; mt < KS; mt++) {
                     unsigned v[4];
-                    few_values(v, vt, key0, mt, lane);
+                    few_values<KEYS>(v, vt, key0, mt, lane);
                     v[0] &= mask[0], v[1] &= mask[0], v[2] &= mask[1], v[3] &= mask[1];
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
@@ -581,9 +586,9 @@ using FewFmaShape = FewShape<HDP, FEW_WARPS * R * HDP * 4, R * HDP * 4>;
 
 // Four 32-bit words of a key at 16-byte chunk c of its row (a row's chunks are permuted by its number: the tensor maps' swizzle); of bfloat16
 // eight.
-template <typename CT> struct FewRow;
-template <> struct FewRow<float> {
-    static constexpr int N = 4, KEYS = FewKeys<float>::N;
+template <typename CT, int KEYS> struct FewRow;
+template <int KEYS> struct FewRow<float, KEYS> {
+    static constexpr int N = 4;
     static __device__ __forceinline__ void load(float *x, const unsigned char *tile, int row, int c) {
         const float4 v = *reinterpret_cast<const float4 *>(tile + (c >> 3) * (KEYS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
         x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
@@ -601,8 +606,8 @@ template <> struct FewRow<float> {
         }
     }
 };
-template <> struct FewRow<__nv_bfloat16> {
-    static constexpr int N = 8, KEYS = FewKeys<__nv_bfloat16>::N;
+template <int KEYS> struct FewRow<__nv_bfloat16, KEYS> {
+    static constexpr int N = 8;
     static __device__ __forceinline__ void two(float *x, unsigned v) { x[0] = __uint_as_float(v << 16), x[1] = __uint_as_float(v & 0xFFFF0000u); }
     static __device__ __forceinline__ void load(float *x, const unsigned char *tile, int row, int c) {
         const uint4 v = *reinterpret_cast<const uint4 *>(tile + (c >> 3) * (KEYS * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4));
@@ -625,7 +630,7 @@ template <typename CT, int HDP, int R>
 __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
     attend_few_fma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ FewCall f) {
     using Shape = FewFmaShape<CT, HDP, R>;
-    constexpr int KEYS = FewKeys<CT>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, MINE = KEYS / FEW_WARPS, SPLIT = 32 / MINE, COLS = HDP / 32, N = FewRow<CT>::N;
+    constexpr int KEYS = FewKeys<CT, HDP>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, MINE = KEYS / FEW_WARPS, SPLIT = 32 / MINE, COLS = HDP / 32, N = FewRow<CT, KEYS>::N;
     extern __shared__ __align__(128) unsigned char smem[];
     const FewMemory<Shape> sm(smem);
     __shared__ float ml[FEW_WARPS][2][R];
@@ -635,7 +640,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
     __shared__ int dead;
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const LinePlace p = few_begin<CT>(f, sm, place, &bad_rows, &dead);
+    const LinePlace p = few_begin<CT, HDP>(f, sm, place, &bad_rows, &dead);
     if (warp == FEW_WARPS) {
         few_copies<float, CT, HDP>(&map_k, &map_v, f, sm, items, p);
         return;
@@ -681,7 +686,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
 #pragma unroll 4
                 for (int c = share; c < chunks; c += SPLIT) {
                     float k[N];
-                    FewRow<CT>::load(k, kt, key0 + key, c);
+                    FewRow<CT, KEYS>::load(k, kt, key0 + key, c);
 #pragma unroll
                     for (int r = 0; r < R; r++)
 #pragma unroll
@@ -722,7 +727,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
                 __syncwarp();
                 const auto add = [&](int k, const float (&w)[R]) {
                     float v[COLS];
-                    FewRow<CT>::template columns<COLS>(v, vt, key0 + k, lane);
+                    FewRow<CT, KEYS>::template columns<COLS>(v, vt, key0 + k, lane);
 #pragma unroll
                     for (int r = 0; r < R; r++)
 #pragma unroll
@@ -881,7 +886,7 @@ template <bool F32, typename CT, int HDP, int R> constexpr int few_blocks_per_sm
 
 inline FewPlan few_plan(int sms, bool f32_rows, bool f32_cache, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     FewPlan p;
-    const int keys = f32_cache ? FewKeys<float>::N : FewKeys<__nv_bfloat16>::N;
+    const int keys = FEW_SLOT / (2 * hdp * (f32_cache ? 4 : 2));
     p.most = rows, p.rows = f32_rows ? 1 : 8; // laid out for 1, 2, 4, 8 or 16 float32 rows, for 8 or 16 of bfloat16
     while (p.rows < rows) p.rows *= 2;
     const int per_sm = p.rows < 16 ? 2 : (!f32_rows ? few_blocks_per_sm<false, __nv_bfloat16, 128, 16>() : (hdp == 64 ? few_blocks_per_sm<true, float, 64, 16>() : few_blocks_per_sm<true, float, 128, 16>()));
@@ -899,7 +904,7 @@ inline FewPlan few_plan(int sms, bool f32_rows, bool f32_cache, int batch, int k
 template <typename RT, typename CT, int HDP, int R>
 cudaError_t launch_few_as(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
     constexpr bool F32 = sizeof(RT) == 4;
-    constexpr int KEYS = FewKeys<CT>::N;
+    constexpr int KEYS = FewKeys<CT, HDP>::N;
     FewCall f;
     f.a = a, f.whole = p.whole, f.part = static_cast<float *>(ws), f.head = p.whole ? nullptr : reinterpret_cast<int *>(static_cast<float *>(ws) + p.part_floats);
     alignas(64) CUtensorMap map_k, map_v;
