@@ -11,7 +11,9 @@
 // has 128 rows and one stream of 64-key tiles, and two S in tensor memory, so that the softmax of one tile runs under the products of its
 // neighbours; the output of a tile is read while the next score is made. The pieces of Q are in tensor memory (192 columns of 512 at head_dim 128) beside O (128) and two S that their P is
 // written over (96 each): the products read only keys and values from shared memory, whose 64 rows a product would not pay for Q's.
-// A bfloat16 cache comes in by tensor-map copies; of a float32 one four warps read the rows and write their pieces.
+// A bfloat16 cache comes in by tensor-map copies; of a float32 one four warps read the rows and write their pieces. An item's rows come in by bulk
+// copies while the item before is worked on, are cut into pieces as soon as that one's last score is made, and its output goes out by bulk copies
+// from the same place: rows read and written by their threads, 512 bytes apart, had taken 16000 of 35000 cycles of an item of 1024 keys.
 #pragma once
 #include "paged_many.cuh"
 
@@ -24,9 +26,12 @@ template <typename CT, int HDP> struct FineShape {
     static constexpr int PIECES = sizeof(CT) == 4 ? 3 : 1;
     static constexpr int TILE = HDP * 128;               // bytes of 64 rows of bfloat16
     static constexpr int SLOT = PIECES * TILE;
-    static constexpr int ROOM = 216 * 1024 / SLOT;
+    static constexpr int PITCH = HDP * 4 + 16;           // of a row's words on their way in and out: eight rows' 16 bytes fall into different banks
+    static constexpr int STAGE = FINE_ROWS * PITCH;
+    static constexpr int ROOM = (224 * 1024 - STAGE) / SLOT;
     static constexpr int SLOTS = ROOM > 8 ? 8 : ROOM;
-    static constexpr int SMEM = 1024 + SLOTS * SLOT + 256;
+    static constexpr int SMEM = 1024 + SLOTS * SLOT + STAGE + 256;
+    static_assert(SLOTS >= 3, "two keys and a value");
 };
 
 template <typename CT, int HDP>
@@ -37,9 +42,9 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
     constexpr int Q_COLS = HDP / 2, O_AT = 3 * Q_COLS, S_AT = O_AT + HDP, S_COLS = 96; // columns of tensor memory
     static_assert(S_AT + 2 * S_COLS <= 512, "tensor memory");
     extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char *ring = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u);
-    unsigned long long *full = reinterpret_cast<unsigned long long *>(ring + SLOTS * SLOT), *empty = full + SLOTS;
-    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *o_free = o_full + 1, *q_full = o_free + 1, *tail = q_full + 1; // 2 SLOTS + 8 <= 32 words
+    unsigned char *ring = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u), *stage = ring + SLOTS * SLOT;
+    unsigned long long *full = reinterpret_cast<unsigned long long *>(stage + Shape::STAGE), *empty = full + SLOTS;
+    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *o_free = o_full + 1, *q_full = o_free + 1, *tail = q_full + 1, *stage_full = tail + 1, *stage_empty = stage_full + 1; // 2 SLOTS + 10 <= 32 words
     __shared__ long long place[32];
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
@@ -58,6 +63,8 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         pg_bar_init(o_free, 128);
         pg_bar_init(q_full, 128);
         pg_bar_init(tail, 1);
+        pg_bar_init(stage_full, 1);
+        pg_bar_init(stage_empty, 128);
         dead = 0;
         f.head[blockIdx.x * 8] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -259,6 +266,29 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             }
             if (!alive) atomicExch(a.c.status, PAGED_WAIT);
         }
+        if (warp == 9) { // ---------------- the queries of the next item, while this one's keys are worked on ----------------
+            unsigned items = 0;
+            while (w.left > 0) {
+                const PagedSeq s = paged_seq(a.c, w.b);
+                const ManyItem item = w.item(a, s);
+                if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(stage_empty, (items & 1u) ^ 1u))) {
+                    if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
+                    break;
+                }
+                if (lane == 0) pg_bar_expect(stage_full, (unsigned)(item.rows * a.c.hd * 4));
+                __syncwarp();
+                for (int r = lane; r < item.rows; r += 32) {
+                    const int2 at = many_row(a, item, r);
+                    const float *src = static_cast<const float *>(a.q) + (long long)(s.first + at.x) * a.ldq + (w.kvh * a.c.group + at.y) * a.c.hd;
+                    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(stage + r * Shape::PITCH)), "l"(src),
+                                 "r"(a.c.hd * 4), "r"(pg_smem(stage_full))
+                                 : "memory");
+                }
+                items++;
+                w.next(a);
+            }
+            if (w.left > 0 && items > 0) pg_bar_wait(stage_full, (items - 1) & 1u); // copies in flight end before the block does
+        }
         __syncwarp();
     } else { // ---------------- the softmax: a thread a row ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(FINE_REGS));
@@ -270,20 +300,20 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
             alive = false; // it goes on without waiting; nothing of the block is stored from here on
         };
-        while (w.left > 0) {
-            const PagedSeq s = paged_seq(a.c, w.b);
-            const ManyItem item = w.item(a, s);
-            const int tiles = w.tiles(item), first = w.first(item), row = item.row0 + tid;
-            const bool valid = tid < item.rows;
-            if (s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
-            const float *src = static_cast<const float *>(a.q) + (long long)(s.first + row / a.c.group) * a.ldq + (long long)(w.kvh * a.c.group + row % a.c.group) * a.c.hd;
+        unsigned char *const mine = stage + tid * Shape::PITCH;
+        unsigned items = 0;
+        const auto queries = [&](int rows) { // an item's rows from where they were brought to, as pieces into tensor memory: a thread its own
+            if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(stage_full, items & 1u))) give_up();
+            items++;
+            if (!alive) return;
+            const bool valid = tid < rows;
 #pragma unroll 1
-            for (int c = 0; c < HDP; c += 32) { // the row's pieces into tensor memory
-                unsigned p[3][16];
+            for (int c = 0; c < HDP; c += 16) {
+                unsigned p[3][8];
 #pragma unroll
-                for (int i = 0; i < 32; i += 4) {
+                for (int i = 0; i < 16; i += 4) {
                     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (valid && c + i < a.c.hd) x = *reinterpret_cast<const float4 *>(src + c + i);
+                    if (valid && c + i < a.c.hd) x = *reinterpret_cast<const float4 *>(mine + (c + i) * 4);
                     if (a.flip) x = make_float4(-x.x, -x.y, -x.z, -x.w);
                     unsigned lo[3], hi[3];
                     pg_split<3>(lo, x.x, x.y);
@@ -292,12 +322,24 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                     for (int k = 0; k < 3; k++) p[k][i / 2] = lo[k], p[k][i / 2 + 1] = hi[k];
                 }
 #pragma unroll
-                for (int k = 0; k < 3; k++) pg_st16(at + k * Q_COLS + c / 2, p[k]);
+                for (int k = 0; k < 3; k++) pg_st8(at + k * Q_COLS + c / 2, p[k]);
             }
             pg_wait_st();
             pg_fence_before();
             pg_bar_arrive(q_full);
-            const int hi = valid ? s.pos0 + row / a.c.group + 1 : 0, lo = a.window ? hi - a.window : 0;
+        };
+        if (w.left > 0) {
+            queries(w.item(a, paged_seq(a.c, w.b)).rows);
+            pg_bar_arrive(stage_empty); // for the second item's; the place is free again for the one after next when an item's output has left it
+        }
+        while (w.left > 0) {
+            const PagedSeq s = paged_seq(a.c, w.b);
+            const ManyItem item = w.item(a, s);
+            const int tiles = w.tiles(item), first = w.first(item);
+            const bool valid = tid < item.rows;
+            const int2 place = many_row(a, item, tid);
+            if (s.n > a.max_new && tid == 0) atomicExch(a.c.status, PAGED_BAD_BOUND);
+            const int hi = valid ? s.pos0 + place.x + 1 : 0, lo = a.window ? hi - a.window : 0;
             float m = -INFINITY, l = 0.0f;
             unsigned long long o[HDP / 2]; // two columns each
 #pragma unroll
@@ -386,46 +428,55 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 m = to;
             }
             tile_count += tiles;
-            take(tile_count - 1);
-
-            // ---- the item's (or its part's) end ----
             const bool is_whole = w.skip == 0 && w.steps(item) == item.steps;
             const long long slot = (long long)blockIdx.x * 2 + (first_part && w.skip > 0 ? 0 : 1);
-            bool wrong = false;
-            if (valid && alive && !dead) {
-                float *out = static_cast<float *>(a.out) + ((long long)(s.first + row / a.c.group) * a.c.heads + w.kvh * a.c.group + row % a.c.group) * a.c.hd;
-                float4 *part = reinterpret_cast<float4 *>(f.part + (slot * BR + tid) * HDP);
-#pragma unroll
-                for (int c = 0; c < HDP; c += 4) {
-                    float4 y;
-                    pg_one(o[c / 2], y.x, y.y), pg_one(o[c / 2 + 1], y.z, y.w);
-                    if (!is_whole) {
-                        part[c / 4] = y;
-                    } else if (c < a.c.hd) {
-                        const float share = l == 0.0f ? 0.0f : 1.0f / l;
-                        y = l == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(y.x * share, y.y * share, y.z * share, y.w * share);
-                        *reinterpret_cast<float4 *>(out + c) = y;
-                        wrong |= !isfinite(y.x) || !isfinite(y.y) || !isfinite(y.z) || !isfinite(y.w);
-                    }
-                }
-                if (!is_whole) {
-                    float *ml = f.part + (long long)gridDim.x * 2 * BR * HDP + slot * 2 * BR;
-                    ml[tid] = m, ml[BR + tid] = l;
-                }
+            if (!is_whole && valid) {
+                float *ml = f.part + (long long)gridDim.x * 2 * BR * HDP + slot * 2 * BR;
+                ml[tid] = m, ml[BR + tid] = l;
             }
             if (!is_whole && tid == 0 && w.skip == 0 && alive && !dead) {
                 int *head = f.head + blockIdx.x * 8;
                 head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = w.line, head[5] = (int)line.per;
             }
-            unsigned rest = __ballot_sync(0xFFFFFFFFu, wrong);
-            while (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
-                const int k = __ffs(rest) - 1, bad = __shfl_sync(0xFFFFFFFFu, row, k);
-                rest &= rest - 1;
-                attend_row_plain<float, CT>(a, w.b, s.first + bad / a.c.group, s.pos0 + bad / a.c.group, s.length, w.kvh * a.c.group + bad % a.c.group);
+            const int b = w.b, kvh = w.kvh;
+            w.next(a);
+            if (w.left > 0) queries(w.item(a, paged_seq(a.c, w.b)).rows); // the scores that read the last ones are done: the next item's begin under what follows
+            take(tile_count - 1);
+
+            // ---- the item's (or its part's) end: the row goes out the way its query came ----
+            const float share = !is_whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l); // (where nothing is seen, O is zero, or not finite and done again)
+            unsigned long long odd = 0; // zero times what is stored: NaN where that is not finite
+            const unsigned long long share2 = pg_two(share, share);
+#pragma unroll
+            for (int c = 0; c < HDP; c += 4) {
+                const unsigned long long y0 = pg_mul2(o[c / 2], share2), y1 = pg_mul2(o[c / 2 + 1], share2);
+                odd = pg_fma2(y0, 0, odd), odd = pg_fma2(y1, 0, odd);
+                *reinterpret_cast<ulonglong2 *>(mine + c * 4) = make_ulonglong2(y0, y1);
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            const bool store = valid && alive && !dead;
+            if (store) {
+                float *to = is_whole ? static_cast<float *>(a.out) + ((long long)(s.first + place.x) * a.c.heads + kvh * a.c.group + place.y) * a.c.hd : f.part + (slot * BR + tid) * HDP;
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(pg_smem(mine)), "r"(is_whole ? a.c.hd * 4 : HDP * 4) : "memory");
+            }
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            pg_bar_arrive(stage_empty);
+            float odd0, odd1;
+            pg_one(odd, odd0, odd1);
+            unsigned rest = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
+            if (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
+                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); // what is there is written over
+                __syncwarp();
+                while (rest) {
+                    const int k = __ffs(rest) - 1, token = __shfl_sync(0xFFFFFFFFu, place.x, k), head = __shfl_sync(0xFFFFFFFFu, place.y, k);
+                    rest &= rest - 1;
+                    attend_row_plain<float, CT>(a, b, s.first + token, s.pos0 + token, s.length, kvh * a.c.group + head);
+                }
             }
             first_part = false;
-            w.next(a);
         }
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); // what leaves shared memory has left it
     }
     pg_fence_before();
     __syncthreads();
