@@ -20,7 +20,7 @@ import os
 import numpy as np
 import torch
 
-from . import _native, _prof, lowbit
+from . import _native, _prof, lowbit, paged
 from .linalg import OP_NT, W_BF16, W_F32, W_INT8_EXP, W_INT8_SCALE
 from . import torch_ops
 from .parallel import gather_columns, shard_bounds
@@ -553,6 +553,16 @@ class TransformerBlock(object):
             with _prof.span("gather"):
                 ctx = gather_columns(ctx, self.group, self.exchange)  # heads are rank-major, so the gathered columns are in head order
         r1, n2 = add_norm(x2, self.o(ctx), self.norm2_w, self.norm2_b, self.norm_eps, self.norm_kind)
+        d = self._mlp(n2)
+        state.cached_tokens = used
+        if defer_add:
+            return r1.reshape(b, l, dm), d
+        return add(r1, d).reshape(b, l, dm)
+
+    def _mlp(self, n2):
+        """The block's MLP on normed rows n2 [m, d_model]: the update that is left to add."""
+        dev, m = n2.device, n2.shape[0]
+        st = _stream(dev)
         if not self.gated:
             # an ungated MLP's activation is elementwise on the up projection: it rides in that product's store
             # (mlp kinds 1, 2, 3 = gelu, gelu_tanh, silu are the store's activation codes)
@@ -583,11 +593,27 @@ class TransformerBlock(object):
         if self.by_heads and not gathered:
             with _prof.span("gather"):
                 act = gather_columns(act, self.group, self.exchange)
-        d = self.down(act)
-        state.cached_tokens = used
-        if defer_add:
-            return r1.reshape(b, l, dm), d
-        return add(r1, d).reshape(b, l, dm)
+        return self.down(act)
+
+    def forward_rows(self, x2, delta, k_cache, v_cache, page_table, cu, lengths, cos, sin, max_new, max_length):
+        """The block on the new rows x2 [rows, d_model] of sequences of their own lengths, keys and values in a paged cache (see
+        `paged`): (r, d), the output being r + d, left to the next norm. `delta`: a residual update of x2 not yet added."""
+        if delta is None:
+            n1 = norm(x2, self.norm1_w, self.norm1_b, self.norm_eps, self.norm_kind)
+        else:
+            x2, n1 = add_norm(x2, delta, self.norm1_w, self.norm1_b, self.norm_eps, self.norm_kind)
+        if self.qkv is not None:
+            q, k, v = self.qkv(n1).split(self.widths, dim=1)  # column blocks: they are read where they are
+        else:
+            q, k, v = self.q(n1), self.k(n1), self.v(n1)
+        q, k, v = (t.unflatten(1, (-1, self.head_dim)) for t in (q, k, v))
+        with _prof.span("rope_cache"):
+            q = paged.append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos, sin, q_norm=self.q_norm_w, k_norm=self.k_norm_w, eps=self.norm_eps,
+                             norm="rmsnorm_offset" if self.norm_kind == 2 else "rmsnorm")
+        with _prof.span("attention"):
+            ctx = paged.attention(q, k_cache, v_cache, page_table, cu, lengths, max_new=max_new, max_length=max_length, window=self.window, softcap=self.attn_softcap)
+        r1, n2 = add_norm(x2, self.o(ctx.flatten(1)), self.norm2_w, self.norm2_b, self.norm_eps, self.norm_kind)
+        return r1, self._mlp(n2)
 
     def _run(self, x, state):
         host = not isinstance(x, torch.Tensor)
