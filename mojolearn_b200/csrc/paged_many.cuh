@@ -10,9 +10,10 @@
 // of up to 128 gives both streams the rows, and every other tile of keys each, and joins the two at the end. One thread issues
 // the products: S = Q K^T from shared memory, O += P V with P (bfloat16, over the columns of S that it came from) read from tensor
 // memory and V as it lies, keys down. One warp copies keys and values: tensor-map boxes of 128 bytes by a page's rows into a ring.
-// The running maximum is moved, and O multiplied by what that costs, only when a row's maximum has grown by more than 2^8: weights
-// up to 2^8 are as exact, and a product of O by one is saved. S of the next tile is signalled after the products before it are done,
-// so O stands still while a softmax warp has an S in hand.
+// A row's weights are taken from the largest score of the tiles before, and that is moved, O multiplied by what it costs, only when it has grown
+// by more than 2^8: larger weights are as exact (up to 2^100, from where the row is done again), the scores are read once, and nothing is
+// exchanged between their reading and P. S of the next tile is signalled after the products before it are done, so O stands still while a
+// softmax warp has an S in hand.
 // Work is cut as in paged_few.cuh: all items' steps on one line, an equal piece a block, parts joined by attend_join_rows_kernel.
 #pragma once
 #include "paged_few.cuh"
@@ -96,25 +97,6 @@ __device__ __forceinline__ float pg_max3(float x, float y, float z) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
     return r;
 }
-// 2^x of two words of at most 8 without the exponential unit: x = n + f, f in [-1/2, 1/2], a cubic of f (its largest relative error, 2^-13.7, made least
-// by reweighted least squares; for weights that are rounded to 8 bits), and n added to the exponent. NaN gives a huge word or NaN, never a small one.
-constexpr float EXP_C0 = 0.99992806f, EXP_C1 = 0.69326097f, EXP_C2 = 0.24261115f, EXP_C3 = 0.05517167f;
-__device__ __forceinline__ float pg_max_nan(float x, float y) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ void pg_exp2_cubic(unsigned long long v, float &x, float &y) {
-    pg_one(v, x, y);
-    const unsigned long long c = pg_two(pg_max_nan(x, -126.0f), pg_max_nan(y, -126.0f)), round = pg_two(12582912.0f, 12582912.0f), back = pg_two(-12582912.0f, -12582912.0f);
-    const unsigned long long n = pg_add2(c, round), f = pg_fma2(pg_add2(n, back), pg_two(-1.0f, -1.0f), c);
-    unsigned long long p = pg_fma2(f, pg_two(EXP_C3, EXP_C3), pg_two(EXP_C2, EXP_C2));
-    p = pg_fma2(p, f, pg_two(EXP_C1, EXP_C1)), p = pg_fma2(p, f, pg_two(EXP_C0, EXP_C0));
-    float nx, ny, px, py;
-    pg_one(n, nx, ny), pg_one(p, px, py);
-    x = __uint_as_float((__float_as_uint(nx) << 23) + __float_as_uint(px)), y = __uint_as_float((__float_as_uint(ny) << 23) + __float_as_uint(py));
-}
-
 // Capped scores before their scale: x = tanh(x inner) / inner, inner = scale / softcap, so that the scale that follows is the uncapped one's.
 // Far from zero as sign(x) (1 - 2 / (1 + e^{2 |x inner|})); both forms for every score where one of the warp's is far, and no branch between them.
 __device__ __forceinline__ float pg_cap_far(float x, float inner, float outer) {
@@ -253,8 +235,8 @@ template <int BR, int KEYS, int STREAMS> struct ManyWalk {
 // 64 scores of a row, in tensor memory at s_at: their largest, and then their weights, of which the sum is returned and the bfloat16 words put
 // at p_at. Apart by what a tile needs, so that the common one is a straight run of instructions (scores that are capped; keys that are not
 // seen: the row sees columns lo .. hi - 1), and loops of 32 columns, so that the code of a tile that comes seldom is not long: fetched from L2 it
-// took 8000 cycles where all columns were written out. A quarter of the exponentials of the common uncapped tile is made beside the unit that
-// makes the others (16 a clock).
+// took 8000 cycles where all columns were written out. A quarter of the exponentials by a cubic beside the unit that
+// makes them (16 a clock) cost 8 %: 2048 tokens over 16384 keys 558 -> 601 us.
 template <bool EDGE>
 __device__ __forceinline__ float many_largest(unsigned s_at, int lo, int hi) {
     float top[2] = {-INFINITY, -INFINITY};
@@ -275,43 +257,47 @@ __device__ __forceinline__ float many_largest(unsigned s_at, int lo, int hi) {
     return fmaxf(top[0], top[1]);
 }
 template <bool CAP, bool EDGE>
-__device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at, unsigned p_at, float unit, float base, int lo, int hi) {
+__device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at, unsigned p_at, float unit, float base, int lo, int hi, float &largest) {
     const unsigned long long unit2 = pg_two(unit, unit), base2 = pg_two(-base, -base);
+    float top[2] = {-INFINITY, -INFINITY};
     unsigned long long sum[2] = {0, 0};
-#pragma unroll 1
+    unsigned z[2][16]; // 16 columns, and the next 16 on their way
+    pg_ld16(z[0], s_at);
+    pg_wait_ld16(z[0]);
+#pragma unroll(CAP || EDGE ? 1 : 2)
     for (int h = 0; h < 2; h++, lo -= 32, hi -= 32) {
-        unsigned z[32], p[16];
-        float *x = reinterpret_cast<float *>(z);
-        pg_ld32(z, s_at + 32 * h);
-        pg_wait_ld(z);
-        if (CAP) {
-            if (EDGE) { // what is not seen may be anything
 #pragma unroll
-                for (int i = 0; i < 32; i++)
-                    if (i >= hi || i < lo) x[i] = 0.0f;
-            }
-            pg_cap<32>(x, a);
-        }
+        for (int c = 0; c < 32; c += 16) {
+            float *x = reinterpret_cast<float *>(z[c / 16]);
+            unsigned p[8];
+            if (c == 0 || h == 0) pg_ld16(z[1 - c / 16], s_at + 32 * h + c + 16);
+            if (CAP) {
+                if (EDGE) { // what is not seen may be anything
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-            if (EDGE) {
-                if (i >= hi || i < lo) x[i] = -INFINITY;
-                if (i + 1 >= hi || i + 1 < lo) x[i + 1] = -INFINITY;
+                    for (int i = 0; i < 16; i++)
+                        if (c + i >= hi || c + i < lo) x[i] = 0.0f;
+                }
+                pg_cap<16>(x, a);
             }
-            const unsigned long long v = pg_fma2(pg_two(x[i], x[i + 1]), unit2, base2);
-            float w0, w1;
-            if (!EDGE && !CAP && i % 8 == 6) {
-                pg_exp2_cubic(v, w0, w1);
-            } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                if (EDGE) {
+                    if (c + i >= hi || c + i < lo) x[i] = -INFINITY;
+                    if (c + i + 1 >= hi || c + i + 1 < lo) x[i + 1] = -INFINITY;
+                }
+                top[(i / 2) & 1] = pg_max3(top[(i / 2) & 1], x[i], x[i + 1]);
+                const unsigned long long v = pg_fma2(pg_two(x[i], x[i + 1]), unit2, base2);
+                float w0, w1;
                 pg_one(v, w0, w1);
                 w0 = paged_exp2(w0), w1 = paged_exp2(w1);
+                sum[(i / 2) & 1] = pg_add2(sum[(i / 2) & 1], pg_two(w0, w1));
+                p[i / 2] = pg_pack(w0, w1);
             }
-            sum[(i / 2) & 1] = pg_add2(sum[(i / 2) & 1], pg_two(w0, w1));
-            p[i / 2] = pg_pack(w0, w1);
+            if (c == 0 || h == 0) pg_wait_ld16(z[1 - c / 16]);
+            pg_st8(p_at + 16 * h + c / 2, p); // over columns that have been read
         }
-        // the first columns' words wait for nobody: they lie over scores that both threads of the row have read twice or keep in registers
-        pg_st16(p_at + 16 * h, p);
     }
+    largest = fmaxf(top[0], top[1]);
     float s0, s1;
     pg_one(pg_add2(sum[0], sum[1]), s0, s1);
     return s0 + s1;
@@ -344,13 +330,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     unsigned char *query = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u), *ring = query + Shape::QUERY;
     unsigned long long *full = reinterpret_cast<unsigned long long *>(ring + SLOTS * TILE), *empty = full + SLOTS;
     unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 4, *q_full = o_full + 2, *tail = q_full + 1; // 2 SLOTS + 10 <= 32 words
-    __shared__ float stats[2][2][128], half_stat[2][2][128]; // m and l of a stream's rows; what the two threads of a row tell each other
+    __shared__ float stats[2][2][128], half_stat[3][2][2][128]; // m and l of a stream's rows; what the two threads of a row tell each other
     __shared__ long long place[32];
+    __shared__ unsigned long long pair_bars[8];
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
+        for (int i = 0; i < 8; i++) pg_bar_init(&pair_bars[i], 64);
         for (int s = 0; s < SLOTS; s++) {
             pg_bar_init(&full[s], 1);
             pg_bar_init(&empty[s], 1);
@@ -528,7 +516,17 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         const float unit = a.scale * PAGED_LOG2E;
         unsigned s_count = 0, o_count = 0;
         bool alive = true, first_part = true;
-        const auto meet = [&] { asm volatile("bar.sync %0, 256;" ::"r"(1 + stream) : "memory"); }; // of the stream's threads
+        unsigned told = 0;
+        const auto tell = [&] { // the same within the loop, where one of the two may have given up: with a bound
+            unsigned long long *bar = &pair_bars[stream * 4 + (warp & 3)];
+            pg_bar_arrive(bar);
+            if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(bar, told & 1u))) {
+                if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
+                alive = false;
+            }
+            told++;
+        };
+        const auto meet = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + stream * 4 + (warp & 3)) : "memory"); }; // of the two warps of the same rows: each comes here once an item, whatever happened
         while (w.left > 0) {
             const PagedSeq s = paged_seq(a.c, w.b);
             const ManyItem item = w.item(a, s);
@@ -566,7 +564,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
             int hi = valid ? s.pos0 + place.x + 1 : 0, lo = a.window ? hi - a.window : 0;
             const int begin = (item.t0 + w.first(item) + (item.pair ? 0 : stream)) * MANY_KEYS + 64 * half, step = (item.pair ? 1 : 2) * MANY_KEYS;
             hi -= begin, lo -= begin;
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f, known = -INFINITY; // known: the largest score of the tile before, of this thread's columns
             const int all = item.pair ? tiles : (tiles + 1 - stream) / 2;
             for (int j = 0; j < all; j++, hi -= step, lo -= step) {
                 if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&s_full[stream], s_count & 1u))) {
@@ -575,19 +573,27 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 }
                 s_count++;
                 pg_fence_after();
-                const bool edge = __any_sync(0xFFFFFFFFu, valid && (hi < 64 || lo > 0));
-                float most = -INFINITY;
-                if (alive) most = edge ? many_largest<true>(s_at, lo, hi) : many_largest<false>(s_at, lo, hi);
-                half_stat[stream][half][r] = most;
-                meet();
                 if (!alive) continue;
-                most = fmaxf(most, half_stat[stream][1 - half][r]); // (not written again before both have given their weights)
-                if (a.softcap > 0.0f) {
-                    float capped[2] = {most, 0.0f};
-                    pg_cap<2>(capped, a);
-                    most = most == -INFINITY ? most : capped[0]; // (nothing is seen)
+                const bool edge = __any_sync(0xFFFFFFFFu, valid && (hi < 64 || lo > 0));
+                // The largest score of the tiles before this one, of both halves, is what a row's weights are taken from, so that the scores are read
+                // once and nobody waits: a tile's own may exceed it, which costs range and no exactness. Rows that have seen nothing yet have none:
+                // there the two threads of each row look for this tile's first (alike in both halves: they hold the same rows and the same m).
+                float most = -INFINITY;
+                if (__any_sync(0xFFFFFFFFu, valid && m == -INFINITY)) {
+                    most = edge ? many_largest<true>(s_at, lo, hi) : many_largest<false>(s_at, lo, hi);
+                    half_stat[0][stream][half][r] = most;
+                    tell();
+                    most = fmaxf(most, half_stat[0][stream][1 - half][r]);
+                    tell(); // read, before it is written again
+                    if (!alive) continue;
+                    if (a.softcap > 0.0f) {
+                        float capped[2] = {most, 0.0f};
+                        pg_cap<2>(capped, a);
+                        most = most == -INFINITY ? most : capped[0]; // (nothing is seen)
+                    }
+                    most *= unit;
                 }
-                most *= unit;
+                if (j > 0) most = fmaxf(most, fmaxf(known, half_stat[1 + ((j - 1) & 1)][stream][1 - half][r])); // (this tile's scores come after both have left them)
                 if (__any_sync(0xFFFFFFFFu, most > m + 8.0f)) { // alike in both halves
                     const float to = most > m ? most : m, keep = m == -INFINITY ? 0.0f : paged_exp2(m - to);
                     m = to, l *= keep;
@@ -604,10 +610,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     }
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
+                float largest;
                 if (a.softcap > 0.0f)
-                    l += edge ? many_weights<true, true>(a, s_at, s_at, unit, base, lo, hi) : many_weights<true, false>(a, s_at, s_at, unit, base, lo, hi);
+                    l += edge ? many_weights<true, true>(a, s_at, s_at, unit, base, lo, hi, largest) : many_weights<true, false>(a, s_at, s_at, unit, base, lo, hi, largest);
                 else
-                    l += edge ? many_weights<false, true>(a, s_at, s_at, unit, base, lo, hi) : many_weights<false, false>(a, s_at, s_at, unit, base, lo, hi);
+                    l += edge ? many_weights<false, true>(a, s_at, s_at, unit, base, lo, hi, largest) : many_weights<false, false>(a, s_at, s_at, unit, base, lo, hi, largest);
+                known = largest * unit;
+                if (known > base + 100.0f && valid) l = NAN; // weights out of range: the row is done again like one that is not finite
+                half_stat[1 + (j & 1)][stream][half][r] = known;
                 pg_wait_st();
                 pg_fence_before();
                 pg_bar_arrive(&p_full[2 * stream + half]);
@@ -622,10 +632,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 o_count++;
                 pg_fence_after();
             }
-            meet(); // the last largest scores are read
-            half_stat[stream][half][r] = l;
+            half_stat[0][stream][half][r] = l;
             meet();
-            l = half_stat[stream][0][r] + half_stat[stream][1][r];
+            l = half_stat[0][stream][0][r] + half_stat[0][stream][1][r];
             const bool is_whole = w.skip == 0 && w.steps(item) == item.steps, some = all > 0 && alive;
             const long long slot = (long long)blockIdx.x * 2 + (first_part && w.skip > 0 ? 0 : 1);
             // the columns that this thread finishes: half of its row's, or where the streams share rows a quarter
@@ -634,7 +643,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
             float keep = 1.0f;
             if (!item.pair) { // the streams' results meet where the queries were
                 if (half == 0) stats[stream][0][r] = m, stats[stream][1][r] = l;
-                asm volatile("bar.sync 3, 512;" ::: "memory"); // both streams are done with their products, so with the queries too
+                asm volatile("bar.sync 9, 512;" ::: "memory"); // both streams are done with their products, so with the queries too
                 const float other_m = stats[1 - stream][0][r], other_l = stats[1 - stream][1][r], top = fmaxf(m, other_m);
                 keep = m == -INFINITY ? 0.0f : paged_exp2(m - top);
                 l = l * keep + (other_m == -INFINITY ? 0.0f : other_l * paged_exp2(other_m - top));
@@ -649,7 +658,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                         reinterpret_cast<float4 *>(query)[((c + i) / 4) * 128 + r] = make_float4(__uint_as_float(o[i]) * keep, __uint_as_float(o[i + 1]) * keep, __uint_as_float(o[i + 2]) * keep,
                                                                                                 __uint_as_float(o[i + 3]) * keep);
                 }
-                asm volatile("bar.sync 3, 512;" ::: "memory");
+                asm volatile("bar.sync 9, 512;" ::: "memory");
             }
             const float share = !is_whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l); // (where nothing is seen, O is zero, or not finite and done again)
             const unsigned long long keep2 = pg_two(keep * share, keep * share), share2 = pg_two(share, share);
@@ -700,7 +709,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 attend_row_plain<T, T>(a, w.b, s.first + token, s.pos0 + token, s.length, w.kvh * a.c.group + head);
             }
             pg_fence_before();
-            asm volatile("bar.sync 3, 512;" ::: "memory"); // `query` and the statistics are read
+            asm volatile("bar.sync 9, 512;" ::: "memory"); // `query` and the statistics are read
             first_part = false;
             w.next(a);
         }
