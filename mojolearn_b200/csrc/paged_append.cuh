@@ -9,6 +9,7 @@
 // idle where the head has an odd number of units). Sums and products are in 32 bits, two words an instruction, and a word is rounded once, at
 // its store. With many rows a warp takes several sets of heads of its row one after another, the next one's words asked for before this one's
 // are worked on: 350 instructions a set, most of them to find its place, had taken 60 us where the bytes need 33.
+// Measured: 16 prompts of 33 to 1024 tokens, 32 + 2 x 8 heads of 128, with norms, bfloat16: 45 us (0.72 of the HBM rate; 0.68 instructions a cycle).
 #pragma once
 #include <algorithm>
 

@@ -15,13 +15,14 @@
 // exchanged between their reading and P. S of the next tile is signalled after the products before it are done, so O stands still while a
 // softmax warp has an S in hand.
 // Work is cut as in paged_few.cuh: all items' steps on one line, an equal piece a block, parts joined by attend_join_rows_kernel.
+// Measured: 2048 tokens behind 14336, 32 heads on 8 of 128, 569 us (908 TFLOP/s of 1627, at 990 of 1000 W); each stream's score, softmax and sum
+// follow one another, and two streams fill the tensor pipe to 0.56. 12 chunks of up to 509 tokens, window 1024, capped, 187 us.
 #pragma once
 #include "paged_few.cuh"
 
 namespace b200i {
 
 constexpr int MANY_THREADS = 640, MANY_KEYS = 128; // two groups of four warps a stream, and one of which one warp copies and one issues
-constexpr int MANY_REGS = 96, MANY_REGS_LESS = 96;
 
 template <int HDP> struct ManyShape {
     static constexpr int TILE = HDP * 256;     // bytes of 128 rows of bfloat16
@@ -233,7 +234,7 @@ template <int BR, int KEYS, int STREAMS> struct ManyWalk {
 };
 
 // 64 scores of a row, in tensor memory at s_at: their largest, and then their weights, of which the sum is returned and the bfloat16 words put
-// at p_at. Apart by what a tile needs, so that the common one is a straight run of instructions (scores that are capped; keys that are not
+// over them. Apart by what a tile needs, so that the common one is a straight run of instructions (scores that are capped; keys that are not
 // seen: the row sees columns lo .. hi - 1), and loops of 32 columns, so that the code of a tile that comes seldom is not long: fetched from L2 it
 // took 8000 cycles where all columns were written out. A quarter of the exponentials by a cubic beside the unit that
 // makes them (16 a clock) cost 8 %: 2048 tokens over 16384 keys 558 -> 601 us.
@@ -257,7 +258,7 @@ __device__ __forceinline__ float many_largest(unsigned s_at, int lo, int hi) {
     return fmaxf(top[0], top[1]);
 }
 template <bool CAP, bool EDGE>
-__device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at, unsigned p_at, float unit, float base, int lo, int hi, float &largest) {
+__device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at, float unit, float base, int lo, int hi, float &largest) {
     const unsigned long long unit2 = pg_two(unit, unit), base2 = pg_two(-base, -base);
     float top[2] = {-INFINITY, -INFINITY};
     unsigned long long sum[2] = {0, 0};
@@ -294,7 +295,7 @@ __device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at
                 p[i / 2] = pg_pack(w0, w1);
             }
             if (c == 0 || h == 0) pg_wait_ld16(z[1 - c / 16]);
-            pg_st8(p_at + 16 * h + c / 2, p); // over columns that have been read
+            pg_st8(s_at + 16 * h + c / 2, p); // over columns that have been read
         }
     }
     largest = fmaxf(top[0], top[1]);
@@ -368,148 +369,148 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     Walk w;
     w.begin(a, line);
 
-    if (warp >= 16) {
-    if (warp == 16) { // ---------------- the copies ----------------
-        unsigned ld = 0, tails = 0;
-        bool alive = true;
-        while (w.left > 0 && alive) {
-            const ManyItem item = w.item(a, paged_seq(a.c, w.b));
-            const int tiles = w.tiles(item), first = w.first(item), last_page = (item.high - 1) >> a.c.page_shift;
-            const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
-            // in the order of their first use: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 K3 ... where the streams have tiles of their own
-            const int lead = min(item.pair ? 1 : 2, tiles);
-            for (int u = 0; u < 2 * tiles && alive; u++, ld++) {
-                const int v = u - lead; // after the first keys: values, then keys, as long as there are any
-                const bool paired = v < 2 * (tiles - lead);
-                const bool is_v = v >= 0 && (paired ? (v & 1) == 0 : true);
-                const int tile = v < 0 ? u : (paired ? (is_v ? v / 2 : v / 2 + lead) : (tiles - lead) + (v - 2 * (tiles - lead)));
-                const int slot = (int)(ld % SLOTS), pos = (item.t0 + first + tile) * MANY_KEYS;
-                if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u))) {
-                    if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
-                    alive = false;
-                    break;
-                }
-                const int there = min(MANY_KEYS / box_rows, max(0, (item.high - pos + box_rows - 1) / box_rows)); // pieces that hold positions that some row sees
-                unsigned char *dst = ring + slot * TILE;
-                const bool clean = is_v && (pos + MANY_KEYS > item.high || pos < item.low); // rows of values that no row sees are to be zero
-                unsigned long long *bar = clean ? tail : &full[slot];
-                if (lane == 0) pg_bar_expect(bar, (unsigned)(there * box_rows * 128 * BOXES));
-                __syncwarp();
-                for (int x = lane; x < there * BOXES; x += 32) {
-                    const int piece = x / BOXES, box = x % BOXES, at = pos + piece * box_rows, index = at >> a.c.page_shift;
-                    int row = a.c.pages * a.c.kv * page; // past the pool: zeros
-                    const int id = index <= last_page ? ids[index] : -1;
-                    if ((unsigned)id < (unsigned)a.c.pages)
-                        row = ((id * a.c.kv + w.kvh) << a.c.page_shift) + (at & (page - 1));
-                    else
-                        atomicExch(a.c.status, PAGED_BAD_PAGE);
-                    pg_tma_load(dst + box * HALF_COLS + piece * (box_rows * 128), is_v ? &map_v : &map_k, bar, box * 64, row);
-                }
-                if (clean) {
-                    if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(tail, tails & 1u))) {
+    if (warp >= 16) { // apart in this order: with the three as one chain of conditions the compiler's code took 190 us for 186 (12 chunks, capped)
+        if (warp == 16) { // ---------------- the copies ----------------
+            unsigned ld = 0, tails = 0;
+            bool alive = true;
+            while (w.left > 0 && alive) {
+                const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                const int tiles = w.tiles(item), first = w.first(item), last_page = (item.high - 1) >> a.c.page_shift;
+                const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
+                // in the order of their first use: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 K3 ... where the streams have tiles of their own
+                const int lead = min(item.pair ? 1 : 2, tiles);
+                for (int u = 0; u < 2 * tiles && alive; u++, ld++) {
+                    const int v = u - lead; // after the first keys: values, then keys, as long as there are any
+                    const bool paired = v < 2 * (tiles - lead);
+                    const bool is_v = v >= 0 && (paired ? (v & 1) == 0 : true);
+                    const int tile = v < 0 ? u : (paired ? (is_v ? v / 2 : v / 2 + lead) : (tiles - lead) + (v - 2 * (tiles - lead)));
+                    const int slot = (int)(ld % SLOTS), pos = (item.t0 + first + tile) * MANY_KEYS;
+                    if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u))) {
                         if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
                         alive = false;
                         break;
                     }
-                    tails++;
-                    for (int x = lane; x < 128 * 8 * BOXES; x += 32) { // 16 bytes each; a row's are in one swizzle atom, so their order does not matter
-                        const int at = pos + ((x >> 3) & 127);
-                        if (at >= item.high || at < item.low) *reinterpret_cast<uint4 *>(dst + (x >> 10) * HALF_COLS + (x & 1023) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    const int there = min(MANY_KEYS / box_rows, max(0, (item.high - pos + box_rows - 1) / box_rows)); // pieces that hold positions that some row sees
+                    unsigned char *dst = ring + slot * TILE;
+                    const bool clean = is_v && (pos + MANY_KEYS > item.high || pos < item.low); // rows of values that no row sees are to be zero
+                    unsigned long long *bar = clean ? tail : &full[slot];
+                    if (lane == 0) pg_bar_expect(bar, (unsigned)(there * box_rows * 128 * BOXES));
                     __syncwarp();
-                    if (lane == 0) pg_bar_arrive(&full[slot]);
+                    for (int x = lane; x < there * BOXES; x += 32) {
+                        const int piece = x / BOXES, box = x % BOXES, at = pos + piece * box_rows, index = at >> a.c.page_shift;
+                        int row = a.c.pages * a.c.kv * page; // past the pool: zeros
+                        const int id = index <= last_page ? ids[index] : -1;
+                        if ((unsigned)id < (unsigned)a.c.pages)
+                            row = ((id * a.c.kv + w.kvh) << a.c.page_shift) + (at & (page - 1));
+                        else
+                            atomicExch(a.c.status, PAGED_BAD_PAGE);
+                        pg_tma_load(dst + box * HALF_COLS + piece * (box_rows * 128), is_v ? &map_v : &map_k, bar, box * 64, row);
+                    }
+                    if (clean) {
+                        if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(tail, tails & 1u))) {
+                            if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
+                            alive = false;
+                            break;
+                        }
+                        tails++;
+                        for (int x = lane; x < 128 * 8 * BOXES; x += 32) { // 16 bytes each; a row's are in one swizzle atom, so their order does not matter
+                            const int at = pos + ((x >> 3) & 127);
+                            if (at >= item.high || at < item.low) *reinterpret_cast<uint4 *>(dst + (x >> 10) * HALF_COLS + (x & 1023) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) pg_bar_arrive(&full[slot]);
+                    }
                 }
+                if (alive) w.next(a);
             }
-            if (alive) w.next(a);
-        }
-        if (!alive) // copies in flight end before the block does
-            for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
-    } else if (warp == 17) { // ---------------- the products ----------------
-        if (lane == 0) {
-            unsigned ld = 0, items = 0, p_count[2] = {0, 0};
-            bool alive = true;
-            const unsigned q0 = pg_smem(query), r0 = pg_smem(ring);
-            const auto here = [&](unsigned i) { // a load is there
-                if (alive && !pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u)) alive = false;
-                pg_fence_after();
-            };
-            const auto score = [&](int stream, unsigned i, bool pair) { // S = Q K^T, K being load i
-                const unsigned k = pg_desc_low(r0 + (i % SLOTS) * TILE), d = tmem + stream * 128;
-                const unsigned q = pg_desc_low(q0 + (pair ? stream : 0) * TILE);
-#pragma unroll
-                for (int ks = 0; ks < HDP / 16; ks++)
-                    pg_mma_ss(d, pg_desc(q + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_desc(k + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_idesc(128, false), ks > 0);
-                pg_commit(&s_full[stream]);
-            };
-            const auto value = [&](int stream, unsigned i, bool add) { // O += P V, V being load i, as the two halves of P come; false where they do not
-                const unsigned v = pg_desc_low(r0 + (i % SLOTS) * TILE, HALF_COLS), d = tmem + 256 + stream * 128;
-                for (int half = 0; half < 2; half++) {
-                    if (alive && !pg_bar_wait(&p_full[2 * stream + half], p_count[stream] & 1u)) alive = false;
-                    if (!alive) return false;
+            if (!alive) // copies in flight end before the block does
+                for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
+        } else if (warp == 17) { // ---------------- the products ----------------
+            if (lane == 0) {
+                unsigned ld = 0, items = 0, p_count[2] = {0, 0};
+                bool alive = true;
+                const unsigned q0 = pg_smem(query), r0 = pg_smem(ring);
+                const auto here = [&](unsigned i) { // a load is there
+                    if (alive && !pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u)) alive = false;
                     pg_fence_after();
+                };
+                const auto score = [&](int stream, unsigned i, bool pair) { // S = Q K^T, K being load i
+                    const unsigned k = pg_desc_low(r0 + (i % SLOTS) * TILE), d = tmem + stream * 128;
+                    const unsigned q = pg_desc_low(q0 + (pair ? stream : 0) * TILE);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ks++)
-                        pg_mma_ts(d, tmem + stream * 128 + half * 64 + ks * 8, pg_desc(v + half * (64 * 128 / 16) + ks * 2048 / 16), pg_idesc(HDP, true), add || half > 0 || ks > 0);
-                }
-                p_count[stream]++;
-                return true;
-            };
-            while (w.left > 0 && alive) {
-                const ManyItem item = w.item(a, paged_seq(a.c, w.b));
-                const int tiles = w.tiles(item);
-                if (!pg_bar_wait(q_full, items & 1u)) alive = false;
-                items++;
-                pg_fence_after();
-                if (item.pair) {
-                    unsigned k = ld++, v;
-                    here(k);
-                    if (alive) score(0, k, true), score(1, k, true), pg_commit(&empty[k % SLOTS]);
-                    for (int j = 0; j < tiles && alive; j++) {
-                        v = ld++;
-                        here(v);
-                        if (j + 1 < tiles) k = ld++;
-                        for (int stream = 0; stream < 2 && alive; stream++) {
-                            if (!value(stream, v, j > 0)) break;
-                            if (stream == 1) pg_commit(&empty[v % SLOTS]);
-                            if (j + 1 < tiles) {
-                                if (stream == 0) here(k);
+                    for (int ks = 0; ks < HDP / 16; ks++)
+                        pg_mma_ss(d, pg_desc(q + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_desc(k + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_idesc(128, false), ks > 0);
+                    pg_commit(&s_full[stream]);
+                };
+                const auto value = [&](int stream, unsigned i, bool add) { // O += P V, V being load i, as the two halves of P come; false where they do not
+                    const unsigned v = pg_desc_low(r0 + (i % SLOTS) * TILE, HALF_COLS), d = tmem + 256 + stream * 128;
+                    for (int half = 0; half < 2; half++) {
+                        if (alive && !pg_bar_wait(&p_full[2 * stream + half], p_count[stream] & 1u)) alive = false;
+                        if (!alive) return false;
+                        pg_fence_after();
+#pragma unroll
+                        for (int ks = 0; ks < 4; ks++)
+                            pg_mma_ts(d, tmem + stream * 128 + half * 64 + ks * 8, pg_desc(v + half * (64 * 128 / 16) + ks * 2048 / 16), pg_idesc(HDP, true), add || half > 0 || ks > 0);
+                    }
+                    p_count[stream]++;
+                    return true;
+                };
+                while (w.left > 0 && alive) {
+                    const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                    const int tiles = w.tiles(item);
+                    if (!pg_bar_wait(q_full, items & 1u)) alive = false;
+                    items++;
+                    pg_fence_after();
+                    if (item.pair) {
+                        unsigned k = ld++, v;
+                        here(k);
+                        if (alive) score(0, k, true), score(1, k, true), pg_commit(&empty[k % SLOTS]);
+                        for (int j = 0; j < tiles && alive; j++) {
+                            v = ld++;
+                            here(v);
+                            if (j + 1 < tiles) k = ld++;
+                            for (int stream = 0; stream < 2 && alive; stream++) {
+                                if (!value(stream, v, j > 0)) break;
+                                if (stream == 1) pg_commit(&empty[v % SLOTS]);
+                                if (j + 1 < tiles) {
+                                    if (stream == 0) here(k);
+                                    if (!alive) break;
+                                    score(stream, k, true);
+                                    if (stream == 1) pg_commit(&empty[k % SLOTS]);
+                                } else {
+                                    pg_commit(&o_full[stream]);
+                                }
+                            }
+                        }
+                    } else {
+                        for (int j = 0; j < min(2, tiles) && alive; j++, ld++) {
+                            here(ld);
+                            if (alive) score(j, ld, false), pg_commit(&empty[ld % SLOTS]);
+                        }
+                        for (int j = 0; j < tiles && alive; j++) {
+                            const int stream = j & 1;
+                            here(ld);
+                            if (!value(stream, ld, j > 1)) break;
+                            pg_commit(&empty[ld % SLOTS]);
+                            ld++;
+                            if (j + 2 < tiles) {
+                                here(ld);
                                 if (!alive) break;
-                                score(stream, k, true);
-                                if (stream == 1) pg_commit(&empty[k % SLOTS]);
+                                score(stream, ld, false);
+                                pg_commit(&empty[ld % SLOTS]);
+                                ld++;
                             } else {
                                 pg_commit(&o_full[stream]);
                             }
                         }
                     }
-                } else {
-                    for (int j = 0; j < min(2, tiles) && alive; j++, ld++) {
-                        here(ld);
-                        if (alive) score(j, ld, false), pg_commit(&empty[ld % SLOTS]);
-                    }
-                    for (int j = 0; j < tiles && alive; j++) {
-                        const int stream = j & 1;
-                        here(ld);
-                        if (!value(stream, ld, j > 1)) break;
-                        pg_commit(&empty[ld % SLOTS]);
-                        ld++;
-                        if (j + 2 < tiles) {
-                            here(ld);
-                            if (!alive) break;
-                            score(stream, ld, false);
-                            pg_commit(&empty[ld % SLOTS]);
-                            ld++;
-                        } else {
-                            pg_commit(&o_full[stream]);
-                        }
-                    }
+                    if (alive) w.next(a);
                 }
-                if (alive) w.next(a);
+                if (!alive) atomicExch(a.c.status, PAGED_WAIT);
             }
-            if (!alive) atomicExch(a.c.status, PAGED_WAIT);
+            __syncwarp();
         }
-        __syncwarp();
-    }
     } else { // ---------------- the softmax of a stream: two threads a row, 64 columns of a tile each ----------------
         const int stream = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, s_at = tmem + lanes + stream * 128 + 64 * half, o_at = tmem + lanes + 256 + stream * 128;
@@ -612,9 +613,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 const float base = m == -INFINITY ? 0.0f : m;
                 float largest;
                 if (a.softcap > 0.0f)
-                    l += edge ? many_weights<true, true>(a, s_at, s_at, unit, base, lo, hi, largest) : many_weights<true, false>(a, s_at, s_at, unit, base, lo, hi, largest);
+                    l += edge ? many_weights<true, true>(a, s_at, unit, base, lo, hi, largest) : many_weights<true, false>(a, s_at, unit, base, lo, hi, largest);
                 else
-                    l += edge ? many_weights<false, true>(a, s_at, s_at, unit, base, lo, hi, largest) : many_weights<false, false>(a, s_at, s_at, unit, base, lo, hi, largest);
+                    l += edge ? many_weights<false, true>(a, s_at, unit, base, lo, hi, largest) : many_weights<false, false>(a, s_at, unit, base, lo, hi, largest);
                 known = largest * unit;
                 if (known > base + 100.0f && valid) l = NAN; // weights out of range: the row is done again like one that is not finite
                 half_stat[1 + (j & 1)][stream][half][r] = known;
