@@ -97,7 +97,12 @@ struct AttendCall {
     int max_new;    // a sequence's rows past these are not computed
 };
 
+// What an output's sum is multiplied by, l the sum of its weights: zero where the row, at position pos, sees nothing (a row that sees
+// anything sees itself); NaN where all that it sees are scores of -infinity.
+__device__ __forceinline__ float paged_share(float l, int pos) { return l != 0.0f ? 1.0f / l : (pos < 0 ? 0.0f : NAN); }
+
 // softmax(z) . V of one (row, head) by one warp, key by key: z = scale * q.k, capped to softcap * tanh(z / softcap).
+// Rows that see nothing are zero; scores that are all -infinity have no softmax: NaN.
 // A key that the row does not see is not read at all, so nothing that stands there (an infinity, a NaN) can reach the row.
 // Every other path comes here with a row that did not come out finite: a masked key has weight zero there, but is multiplied.
 template <typename RT, typename CT>
@@ -142,7 +147,7 @@ __device__ __noinline__ void attend_row_plain(const AttendCall &a, int b, int ro
     RT *out = static_cast<RT *>(a.out) + ((long long)row * a.c.heads + h) * hd;
 #pragma unroll
     for (int i = 0; i < PAGED_MAX_HD / 32; i++)
-        if (lane + 32 * i < hd) paged_write(out + lane + 32 * i, l == 0.0f ? 0.0f : (acc[i] + part[i]) / l);
+        if (lane + 32 * i < hd) paged_write(out + lane + 32 * i, l != 0.0f ? (acc[i] + part[i]) / l : paged_share(l, pos));
 }
 
 } // namespace b200i

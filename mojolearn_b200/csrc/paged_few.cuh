@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 keep[e] = m[nt][e] == -INFINITY ? 0.0f : paged_exp2(m[nt][e] - mm[nt][e]);
-                if (is_whole) keep[e] *= ll[nt][e] == 0.0f ? 0.0f : 1.0f / ll[nt][e];
+                if (is_whole) keep[e] *= paged_share(ll[nt][e], s.pos0 + (nt * 8 + (lane & 3) * 2 + e) / a.c.group);
             }
 #pragma unroll
             for (int mt = 0; mt < KS; mt++) {
@@ -795,7 +795,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
             }
             if (dead) continue;
             if (is_whole) {
-                x *= sum == 0.0f ? 0.0f : 1.0f / sum;
+                x *= paged_share(sum, s.pos0 + token);
                 if (col < a.c.hd) static_cast<float *>(a.out)[((long long)(s.first + token) * a.c.heads + item.kvh * a.c.group + r - token * a.c.group) * a.c.hd + col] = x;
                 if (!(x * 0.0f == 0.0f)) wrong |= 1u << r; // (past head_dim there are zeros)
             } else {
@@ -867,7 +867,7 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
     if (col < a.c.hd) {
 #pragma unroll
         for (int w = 0; w < 8; w++) y += met[w][col];
-        y *= l == 0.0f ? 0.0f : __frcp_rn(l);
+        y *= l != 0.0f ? __frcp_rn(l) : paged_share(l, s.pos0 + token);
         paged_write(static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd + col, y);
     }
     if (__syncthreads_or(!(y * 0.0f == 0.0f)) && warp == 0) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);

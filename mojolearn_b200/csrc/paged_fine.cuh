@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                     for (int i = 0; i < 32; i += 4) top[0] = pg_max3(top[0], x[i], x[i + 1]), top[1] = pg_max3(top[1], x[i + 2], x[i + 3]);
                 }
                 float most = fmaxf(top[0], top[1]);
-                if (a.softcap > 0.0f) pg_cap_fine<2>(top, a), most = most == -INFINITY ? most : fmaxf(top[0], top[1]); // (-infinity: nothing is seen)
+                if (a.softcap > 0.0f) pg_cap_fine<2>(top, a), most = max(lo, pos) < min(hi, pos + FINE_KEYS) ? fmaxf(top[0], top[1]) : -INFINITY; // (nothing is seen)
                 most *= unit;
                 const float to = most > m ? most : m, keep = m == -INFINITY ? 0.0f : paged_exp2(m - to), base = to == -INFINITY ? 0.0f : to;
                 const unsigned long long unit2 = pg_two(unit, unit), base2 = pg_two(-base, -base);
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             take(tile_count - 1);
 
             // ---- the item's (or its part's) end: the row goes out the way its query came ----
-            const float share = !is_whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l); // (where nothing is seen, O is zero, or not finite and done again)
+            const float share = !is_whole ? 1.0f : paged_share(l, s.pos0 + place.x); // (where nothing is seen, O is zero, or not finite and done again)
             unsigned long long odd = 0; // zero times what is stored: NaN where that is not finite
             const unsigned long long share2 = pg_two(share, share);
 #pragma unroll

@@ -590,7 +590,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     if (a.softcap > 0.0f) {
                         float capped[2] = {most, 0.0f};
                         pg_cap<2>(capped, a);
-                        most = most == -INFINITY ? most : capped[0]; // (nothing is seen)
+                        const int at = 64 * half; // a score of -infinity is capped as well; a row that sees nothing of the tile stays without
+                        most = max(lo + at, 0) < min(hi + at, MANY_KEYS) ? capped[0] : -INFINITY;
                     }
                     most *= unit;
                 }
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 }
                 asm volatile("bar.sync 9, 512;" ::: "memory");
             }
-            const float share = !is_whole ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l); // (where nothing is seen, O is zero, or not finite and done again)
+            const float share = !is_whole ? 1.0f : paged_share(l, s.pos0 + place.x); // (where nothing is seen, O is zero, or not finite and done again)
             const unsigned long long keep2 = pg_two(keep * share, keep * share), share2 = pg_two(share, share);
             unsigned long long odd = 0; // zero times what is stored: NaN where that is not finite
             T *out = static_cast<T *>(a.out) + ((long long)(s.first + place.x) * a.c.heads + w.kvh * a.c.group + place.y) * a.c.hd;
@@ -793,7 +794,7 @@ __global__ void __launch_bounds__(256) attend_join_rows_kernel(const __grid_cons
         if (mine + r >= rows) continue;
         const unsigned n = head0 + (unsigned)(mine + r), t = a.c.group == 1 ? n : __umulhi(n, a.c.group_part);
         const int token = (int)(token0 + t), h = kvh * a.c.group + (int)(n - t * (unsigned)a.c.group);
-        const float share = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        const float share = paged_share(l[r], s.pos0 + token);
         float odd = 0.0f; // zero times what is stored: NaN where that is not finite
 #pragma unroll
         for (int k = 0; k < N; k++) {

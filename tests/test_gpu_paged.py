@@ -108,6 +108,21 @@ def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(rows, cache, n
 
 
 @pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 150])
+def test_scores_of_minus_infinity(rows, cache, new):
+    """Infinite keys: a capped score is the cap; uncapped, a row whose scores are all -infinity has no softmax: NaN. A row without keys is zero."""
+    c = Case([new, new], [0, 300], 4, 2, 64, 32, rows, cache, lengths=[new, 0])
+    c.q[:, :, 3] = 1.0
+    c.k_cache[int(c.table[0, 0]), :, 0, 3] = float("-inf")
+    capped = attend(c, softcap=30.0)
+    check(capped, c.attention(softcap=30.0), rows, c.most())
+    got = attend(c)
+    assert bool(torch.isnan(got[0]).all()) and not bool(got[new:].any())
+    if new > 1:
+        check(got[1:new], c.attention()[1:new], rows, c.most())
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
 @pytest.mark.parametrize("new", [1, 200])
 def test_scores_far_apart(rows, cache, new):
     """Scores of hundreds, rising and falling along the keys: the running maximum moves, and most weights are zero."""
