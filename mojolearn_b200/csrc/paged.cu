@@ -137,6 +137,8 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     a.cap_inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f, a.cap_outer = a.softcap > 0.0f ? a.softcap / a.scale : 0.0f;
     float power = 1.0f;
     for (int i = 0; i < 4; i++) power *= a.cap_inner * a.cap_inner, a.cap_near[i] = CAP_NEAR[i] * power;
+    // the polynomial's eighth power has to stay within 32 bits; where it does not, all scores go the other way (unless they are as good as zero)
+    a.cap_from = a.cap_outer > 3e38f || (a.cap_inner > 1e-4f && a.cap_inner < 1e4f) ? a.cap_outer : -1.0f;
     a.window = (int)std::min(window, MOST), a.max_new = (int)std::min(max_new, MOST);
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;

@@ -93,6 +93,7 @@ struct AttendCall {
     float scale, softcap;  // scale > 0: a negative one is the queries' sign (flip)
     int flip;
     float cap_inner, cap_outer, cap_near[4]; // of capped scores (paged_many.cuh): scale / softcap, its inverse, its even powers times the polynomial's coefficients
+    float cap_from;                          // the polynomial is for scores up to this
     int window;     // 0: none
     int max_new;    // a sequence's rows past these are not computed
 };

@@ -121,7 +121,7 @@ __device__ __forceinline__ void pg_cap(float *x, const AttendCall &a) {
         p = pg_fma2(q, p, k[1]), p = pg_fma2(q, p, k[0]);
         pg_one(pg_fma2(pg_mul2(v, q), p, v), y0, y1);
     };
-    if (!__any_sync(0xFFFFFFFFu, most > a.cap_outer)) {
+    if (!__any_sync(0xFFFFFFFFu, most > a.cap_from)) {
 #pragma unroll
         for (int c = 0; c < N; c += 2) near(c, x[c], x[c + 1]);
     } else {
@@ -130,7 +130,7 @@ __device__ __forceinline__ void pg_cap(float *x, const AttendCall &a) {
             float y0, y1;
             near(c, y0, y1);
             const float f0 = pg_cap_far(x[c], a.cap_inner, a.cap_outer), f1 = pg_cap_far(x[c + 1], a.cap_inner, a.cap_outer);
-            x[c] = fabsf(x[c]) > a.cap_outer ? f0 : y0, x[c + 1] = fabsf(x[c + 1]) > a.cap_outer ? f1 : y1;
+            x[c] = fabsf(x[c]) > a.cap_from ? f0 : y0, x[c + 1] = fabsf(x[c + 1]) > a.cap_from ? f1 : y1;
         }
     }
 }

@@ -108,6 +108,16 @@ def test_a_value_that_is_not_finite_reaches_only_rows_that_see_it(rows, cache, n
 
 
 @pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("size", [2.0 ** -66, 2.0 ** -20, 2.0 ** 20, 2.0 ** 50])
+def test_capped_scores_of_any_size(rows, cache, new, size):
+    """Keys of any magnitude whose scale brings the scores back to ordinary ones."""
+    c = Case([new] * 3, [0, 65, 400], 8, 2, 64, 32, rows, cache)
+    c.k_cache.mul_(size)
+    held_to_64_bits(c, softcap=3.0, scale=0.25 / size)
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
 @pytest.mark.parametrize("new", [1, 3, 150])
 def test_scores_of_minus_infinity(rows, cache, new):
     """Infinite keys: a capped score is the cap; uncapped, a row whose scores are all -infinity has no softmax: NaN. A row without keys is zero."""
