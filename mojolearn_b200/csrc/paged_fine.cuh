@@ -14,7 +14,7 @@
 // A bfloat16 cache comes in by tensor-map copies; of a float32 one four warps read the rows and write their pieces. An item's rows come in by bulk
 // copies while the item before is worked on, are cut into pieces as soon as that one's last score is made, and its output goes out by bulk copies
 // from the same place: rows read and written by their threads, 512 bytes apart, had taken 16000 of 35000 cycles of an item of 1024 keys.
-// Measured: 4 prompts of 1024 tokens, 16 heads of 128: 128 us on a bfloat16 cache, 214 on a float32 one (32 and 64 at the tensor rate of their products):
+// Measured: 4 prompts of 1024 tokens, 16 heads of 128: 130 us on a bfloat16 cache, 214 on a float32 one (32 and 64 at the tensor rate of their products):
 // the issuing thread waits, three barriers between two products, and a product of 64 columns takes 45 cycles, not 32.
 #pragma once
 #include "paged_many.cuh"

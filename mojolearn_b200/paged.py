@@ -150,7 +150,7 @@ def append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos=None, sin=Non
 def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max_length=None, scale=None, window=0, softcap=0.0, out=None):
     """softmax(scale q.k) v of the rows q [rows, n_heads, head_dim] over the cached positions that each sees: those up to its own
     and, with `window`, the last `window` of them. `softcap` caps every score as cap * tanh(score / cap). A row that sees nothing
-    is zero; what stands in places that a row does not see, or past a sequence's length, never reaches it.
+    is zero (one whose scores are all -infinity has no softmax: NaN); what stands in places that a row does not see, or past a sequence's length, never reaches it.
 
     `max_new` and `max_length` are what the caller knows of the most new tokens of a sequence and of the longest cache (by default
     all rows and the whole table): the call is cut by them, and a sequence with more than `max_new` rows is reported by
