@@ -88,7 +88,7 @@ __device__ __forceinline__ LinePlace line_place(const PagedCall &c, F size_of, i
     const long long per = line_div(total + blocks - 1, blocks), start = per * block;
     __syncthreads();
     if (tid == 0) sh[28] = -1;
-    long long before = 0; // of the sequences before this round's
+    long long before = 0; // of the sequences before those that the block looks at
     for (int b0 = 0; b0 < c.batch && start < total; b0 += blockDim.x) {
         const int b = b0 + tid;
         long long here = mine; // what the first loop left, where that saw the whole batch
