@@ -12,8 +12,8 @@
 // memory and V as it lies, keys down. One warp copies keys and values: tensor-map boxes of 128 bytes by a page's rows into a ring.
 // A row's weights are taken from the largest score of the tiles before, and that is moved, O multiplied by what it costs, only when it has grown
 // by more than 2^8: larger weights are as exact (up to 2^100, from where the row is done again), the scores are read once, and nothing is
-// exchanged between their reading and P. S of the next tile is signalled after the products before it are done, so O stands still while a
-// softmax warp has an S in hand.
+// exchanged between their reading and P. S of the next tile is signalled after the products before it are done, and this tile's products begin
+// when the first half of P has been stored AND both halves of O have been multiplied, so O stands still while it is.
 // Work is cut as in paged_few.cuh: all items' steps on one line, an equal piece a block, parts joined by attend_join_rows_kernel.
 // Measured: 2048 tokens behind 14336, 32 heads on 8 of 128, 569 us (908 TFLOP/s of 1627, at 990 of 1000 W); each stream's score, softmax and sum
 // follow one another, and two streams fill the tensor pipe to 0.56. 12 chunks of up to 509 tokens, window 1024, capped, 187 us.
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         }
         for (int i = 0; i < 2; i++) {
             pg_bar_init(&s_full[i], 1);
-            pg_bar_init(&p_full[2 * i], 128), pg_bar_init(&p_full[2 * i + 1], 128);
+            pg_bar_init(&p_full[2 * i], 256), pg_bar_init(&p_full[2 * i + 1], 128);
             pg_bar_init(&o_full[i], 1);
         }
         pg_bar_init(q_full, 512);
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                         pg_mma_ss(d, pg_desc(q + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_desc(k + ((ks >> 2) * HALF_COLS + (ks & 3) * 32) / 16), pg_idesc(128, false), ks > 0);
                     pg_commit(&s_full[stream]);
                 };
-                const auto value = [&](int stream, unsigned i, bool add) { // O += P V, V being load i, as the two halves of P come; false where they do not
+                const auto value = [&](int stream, unsigned i, bool add) { // O += P V, V being load i, as the two halves of P come (the first with word from both that O may be added to); false where they do not
                     const unsigned v = pg_desc_low(r0 + (i % SLOTS) * TILE, HALF_COLS), d = tmem + 256 + stream * 128;
                     for (int half = 0; half < 2; half++) {
                         if (alive && !pg_bar_wait(&p_full[2 * stream + half], p_count[stream] & 1u)) alive = false;
@@ -609,7 +609,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                             for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
                             pg_st16(o_at + c, o);
                         }
+                        pg_wait_st();
                     }
+                }
+                if (half) { // the first half's products add to all columns of O, so they wait for this half's too to be multiplied
+                    pg_fence_before();
+                    pg_bar_arrive(&p_full[2 * stream]);
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
                 float largest;

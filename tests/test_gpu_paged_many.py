@@ -1,0 +1,34 @@
+"""Attention of many bfloat16 rows where the largest score keeps growing, so that the running output is multiplied tile after tile."""
+import pytest
+import torch
+
+from paged_ref import BF16, Case, check
+
+pytestmark = pytest.mark.gpu
+if torch.cuda.is_available():
+    from mojolearn_b200 import paged, torch_ops
+
+
+def climbing(new, past, heads, kv, hd, page, per_tile):
+    """A case whose scores climb by about `per_tile` (a factor of e to that) from one 128 keys to the next, along one column."""
+    c = Case(new, past, heads, kv, hd, page, BF16, BF16, seed=hd)
+    c.q[:, :, 7] = 1.0
+    for b, n in enumerate(c.length):
+        slope = torch.arange(n, device="cuda") * (per_tile / 128 * hd ** 0.5)
+        for i in range(-(-n // page)):
+            c.k_cache[int(c.table[b, i]), :, :min(page, n - i * page), 7] = slope[i * page:(i + 1) * page].to(BF16)
+    return c
+
+
+@pytest.mark.parametrize("new,heads,kv", [([300], 4, 4), ([40, 3], 8, 2), ([128, 129], 2, 2), ([70, 20], 8, 1)])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("per_tile", [7.0, 30.0])
+def test_an_output_that_is_multiplied_in_every_tile(new, heads, kv, hd, per_tile):
+    """Both halves of a row's output are multiplied before a tile's products are added: right, and the same words however the warps run."""
+    c = climbing(new, [1500 + 77 * i for i in range(len(new))], heads, kv, hd, 64, per_tile)
+    call = lambda: paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), max_new=max(new))  # noqa: E731
+    got = call()
+    check(got, c.attention(), BF16, c.most())
+    for _ in range(20):
+        assert torch.equal(call(), got)
+    torch_ops.check_status()
