@@ -321,6 +321,19 @@ __device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some)
     }
 }
 
+// An item's rows whose bits are set, done again: dealt out to the sixteen softmax warps.
+template <typename T, int BR, int KEYS, int STREAMS>
+__device__ __noinline__ void many_again(const AttendCall &a, const unsigned *bad, int b, int kvh, int block) {
+    const PagedSeq s = paged_seq(a.c, b);
+    const ManyItem item = many_item<BR, KEYS, STREAMS>(a, s, min(s.n, a.max_new), block);
+    int number = 0;
+    for (int row = 0; row < item.rows; row++) {
+        if (!(bad[row / 32] >> (row % 32) & 1u) || (number++ & 15) != (threadIdx.x >> 5)) continue;
+        const int2 at = many_row(a, item, row);
+        attend_row_plain<T, T>(a, b, s.first + at.x, s.pos0 + at.x, s.length, kvh * a.c.group + at.y);
+    }
+}
+
 template <int HDP>
 __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyCall f) {
     using Shape = ManyShape<HDP>;
@@ -334,6 +347,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     __shared__ float stats[2][2][128], half_stat[3][2][2][128]; // m and l of a stream's rows; what the two threads of a row tell each other
     __shared__ long long place[32];
     __shared__ unsigned long long pair_bars[8];
+    __shared__ uint4 bad[2][2]; // rows that did not come out finite, a bit each: of this item and of the one before
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
     const AttendCall &a = f.a;
@@ -515,8 +529,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         const int stream = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16, s_at = tmem + lanes + stream * 128 + 64 * half, o_at = tmem + lanes + 256 + stream * 128;
         const float unit = a.scale * PAGED_LOG2E;
-        unsigned s_count = 0, o_count = 0;
-        bool alive = true, first_part = true;
+        unsigned s_count = 0, o_count = 0, items = 0;
+        bool alive = true;
         unsigned told = 0;
         const auto tell = [&] { // the same within the loop, where one of the two may have given up: with a bound
             unsigned long long *bar = &pair_bars[stream * 4 + (warp & 3)];
@@ -555,6 +569,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                         *reinterpret_cast<uint4 *>(query + tile * TILE + (chunk >> 3) * HALF_COLS + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
                             make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
                 }
+                if (tid < 2) bad[items & 1u][tid] = make_uint4(0, 0, 0, 0); // before the queries are there, so before any row of this item is finished
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 pg_bar_arrive(q_full);
             }
@@ -643,7 +658,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
             meet();
             l = half_stat[0][stream][0][r] + half_stat[0][stream][1][r];
             const bool is_whole = w.skip == 0 && w.steps(item) == item.steps, some = all > 0 && alive;
-            const long long slot = (long long)blockIdx.x * 2 + (first_part && w.skip > 0 ? 0 : 1);
+            const long long slot = (long long)blockIdx.x * 2 + (items == 0 && w.skip > 0 ? 0 : 1);
             // the columns that this thread finishes: half of its row's, or where the streams share rows a quarter
             constexpr int Q4 = HDP / 4;
             const int from = item.pair ? half * (HDP / 2) : (stream * 2 + half) * Q4, to = from + (item.pair ? HDP / 2 : Q4);
@@ -709,15 +724,16 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
             }
             float odd0, odd1;
             pg_one(odd, odd0, odd1);
-            unsigned rest = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
-            while (rest) { // a masked key's zero weight met a value that is not finite. Every thread of a row that sees it so does the whole row: the same words.
-                const int k = __ffs(rest) - 1, token = __shfl_sync(0xFFFFFFFFu, place.x, k), head = __shfl_sync(0xFFFFFFFFu, place.y, k);
-                rest &= rest - 1;
-                attend_row_plain<T, T>(a, w.b, s.first + token, s.pos0 + token, s.length, w.kvh * a.c.group + head);
-            }
+            // A masked key's zero weight met a value that is not finite, or the weights left their range: the row is done again, by one warp, and not
+            // before all threads of the row have stored: each sees its own columns only.
+            const unsigned odd_rows = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
+            if (odd_rows && lane == 0) atomicOr(reinterpret_cast<unsigned *>(bad[items & 1u]) + mine / 32, odd_rows);
             pg_fence_before();
-            asm volatile("bar.sync 9, 512;" ::: "memory"); // `query` and the statistics are read
-            first_part = false;
+            asm volatile("bar.sync 9, 512;" ::: "memory"); // `query` and the statistics are read, and the rows stored
+            const uint4 some_bad = bad[items & 1u][0], more_bad = bad[items & 1u][1];
+            if (some_bad.x | some_bad.y | some_bad.z | some_bad.w | more_bad.x | more_bad.y | more_bad.z | more_bad.w)
+                many_again<T, BR, MANY_KEYS, 2>(a, reinterpret_cast<const unsigned *>(bad[items & 1u]), w.b, w.kvh, w.block);
+            items++;
             w.next(a);
         }
     }
@@ -817,7 +833,9 @@ __global__ void __launch_bounds__(256) attend_join_rows_kernel(const __grid_cons
             else
                 *reinterpret_cast<float2 *>(out) = make_float2(o[r][0], o[r][1]);
         }
-        if (__any_sync(0xFFFFFFFFu, mine_columns && !(odd == 0.0f))) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
+        const bool again = __any_sync(0xFFFFFFFFu, mine_columns && !(odd == 0.0f));
+        __syncwarp(); // the row's words are stored, in this order, by other lanes too
+        if (again) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
     }
 }
 

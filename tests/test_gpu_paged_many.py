@@ -32,3 +32,22 @@ def test_an_output_that_is_multiplied_in_every_tile(new, heads, kv, hd, per_tile
     for _ in range(20):
         assert torch.equal(call(), got)
     torch_ops.check_status()
+
+
+@pytest.mark.parametrize("new,past", [(300, 40), (60, 200), (7, 9000), (130, 12000)])
+@pytest.mark.parametrize("column", [5, 100])
+def test_a_row_done_again_is_written_after_its_other_words(new, past, column):
+    """A value that is not finite in one column only, which some rows of a block see and others do not: those are done again as a whole, and
+    the same words come out however the warps that store them run."""
+    c = Case([new], [past], 8, 2, 128, 32, BF16, BF16, seed=new)
+    for back in (1, new // 2, new - 2):
+        pos = c.length[0] - back
+        c.v_cache[int(c.table[0, pos // 32]), :, pos % 32, column] = float("nan")
+    call = lambda: paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), max_new=new)  # noqa: E731
+    want, got = c.attention(), call()
+    seen = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), seen) and bool(seen.any()) and not bool(seen.all(-1).any())
+    check(torch.where(seen, torch.zeros_like(got), got), torch.where(seen, 0.0, want), BF16, 6.0)
+    for _ in range(20):
+        assert torch.equal(call().view(torch.int16), got.view(torch.int16))
+    torch_ops.check_status()
