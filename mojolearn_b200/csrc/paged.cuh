@@ -12,6 +12,8 @@
 
 #include <cstdint>
 
+#include "paged_place.cuh"
+
 namespace b200i {
 
 constexpr int PAGED_MAX_HD = 128;
@@ -28,22 +30,7 @@ struct PagedCall {
     unsigned group_part;   // 2^32 / group + 1, rounded down: the upper half of a product with it is a quotient
 };
 
-// One sequence's part of a call.
-struct PagedSeq {
-    int first, n;  // its rows
-    int length;    // positions in its cache, the new ones among them
-    int pos0;      // position of its first row (negative where a table says that fewer are cached than are new)
-};
-
-__device__ __forceinline__ PagedSeq paged_seq(const PagedCall &c, int b) {
-    PagedSeq s;
-    const int lo = c.cu[b], hi = c.cu[b + 1], most = (int)c.rows;
-    s.first = min(max(lo, 0), most);
-    s.n = max(min(hi, most) - s.first, 0);
-    s.length = (int)min((long long)max(c.lengths[b], 0), (long long)c.max_pages << c.page_shift);
-    s.pos0 = s.length - s.n;
-    return s;
-}
+__device__ __forceinline__ PagedSeq paged_seq(const PagedCall &c, int b) { return paged_place(c.cu[b], c.cu[b + 1], c.lengths[b], (int)c.rows, c.max_pages << c.page_shift); }
 
 // The sequence of row t, or -1: a warp looks at 32 entries of cu at a time. All lanes call it with one t.
 __device__ __forceinline__ int paged_row_seq(const PagedCall &c, long long t) {
