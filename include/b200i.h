@@ -448,7 +448,7 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
  * positions that a row does not see, or past a sequence's length, has no influence on it. max_new and max_length bound the
  * sequences' new tokens and lengths as the host knows them (max_new is held to: a sequence with more rows sets the status word to
  * 12 and its further rows are not written; max_length only chooses how the work is cut). A device-side wait that ran out sets the
- * status word to 13. `ws`: the scratch that b200i_paged_attention_workspace_bytes asks for, 256-byte aligned. */
+ * status word to 13. `ws`: the scratch that b200i_paged_attention_workspace_bytes asks for, on a 16-byte boundary. */
 int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache,
                               const void *v_cache, int64_t row_type, int64_t cache_type, const int32_t *page_table,
                               const int32_t *cu, const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv,

@@ -132,6 +132,7 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (max_new <= 0 || max_length <= 0) return refuse(err, err_cap, "paged_attention: the bounds on new tokens and lengths must be positive");
     if (window < 0 || !(softcap >= 0.0) || softcap > 1e30 || !(scale > -1e30 && scale < 1e30)) return refuse(err, err_cap, "paged_attention: window, softcap or scale is out of range");
     if (ws_bytes < 0 || (ws_bytes > 0 && !ws)) return refuse(err, err_cap, "paged_attention: a workspace size without a workspace");
+    if (ws_bytes > 0 && !aligned16(ws)) return refuse(err, err_cap, "paged_attention: the workspace must start on a 16-byte boundary");
     a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.flip = scale < 0.0, a.softcap = (float)softcap;
     a.scale = std::max(fabsf((float)scale), 1e-30f); // none makes all weights alike, as does next to none
     a.cap_inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f, a.cap_outer = a.softcap > 0.0f ? a.softcap / a.scale : 0.0f;
