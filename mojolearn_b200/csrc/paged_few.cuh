@@ -296,6 +296,12 @@ __device__ __forceinline__ void few_head(const FewCall &f, const FewItem &i) {
     head[0] = i.b, head[1] = i.kvh, head[2] = i.count, head[3] = i.line, head[4] = i.per;
 }
 __device__ __forceinline__ void few_meet() { asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_WARPS) : "memory"); } // the computing warps
+// They meet, and know alike whether one of them brings a yes: a word in shared memory could change before the slower ones have read it.
+__device__ __forceinline__ bool few_vote(bool yes) {
+    unsigned some;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(some) : "r"((unsigned)yes), "n"(32 * FEW_WARPS) : "memory");
+    return some != 0;
+}
 // Rows that did not come out finite, done again: a masked key's zero weight met a value that is not finite.
 template <typename RT, typename CT>
 __device__ __forceinline__ void few_again(const AttendCall &a, const FewItem &i, unsigned *bad_rows, int rows) {
@@ -355,8 +361,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
     for (unsigned number = 0;; number++) {
         const int which = number % FEW_ITEMS;
         if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.item_full[which], (number / FEW_ITEMS) & 1u))) give_up();
-        few_meet(); // and nobody goes on where one has given up: what the item is would not be known
-        if (dead) break;
+        if (few_vote(!alive)) break; // nobody goes on where one has given up: what the item is would not be known
         const FewItem item = items[which];
         if (!item.more) break;
         const PagedSeq s = item.s;
@@ -660,8 +665,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
     for (unsigned number = 0;; number++) {
         const int which = number % FEW_ITEMS;
         if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.item_full[which], (number / FEW_ITEMS) & 1u))) give_up();
-        few_meet(); // and nobody goes on where one has given up: what the item is would not be known
-        if (dead) break;
+        if (few_vote(!alive)) break; // nobody goes on where one has given up: what the item is would not be known
         const FewItem item = items[which];
         if (!item.more) break;
         const PagedSeq s = item.s;
