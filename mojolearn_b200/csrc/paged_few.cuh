@@ -154,7 +154,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
     constexpr int KEYS = FewKeys<CT, HDP>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, BOX_COLS = 128 / (int)sizeof(CT), BOXES = HDP / BOX_COLS;
     const AttendCall &a = f.a;
     const int lane = threadIdx.x & 31, page = 1 << a.c.page_shift, box_rows = min(page, KEYS), pieces = KEYS / box_rows;
-    unsigned it = 0, number = 0;
+    unsigned it = 0, number = 0, sent = 0; // tiles, items looked at, phases of item_full that were begun
     bool alive = true;
     const auto wait = [&](unsigned long long *bar, unsigned parity) {
         if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(bar, parity))) {
@@ -186,6 +186,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
                 items[at].more = 0;
                 pg_bar_arrive(&sm.item_full[at]);
             }
+            sent++;
             break;
         }
         const int tiles = f.whole ? count : (int)min((long long)(count - before), left), n = min(s.n, a.max_new);
@@ -195,6 +196,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
             if (s.n > a.max_new) atomicExch(a.c.status, PAGED_BAD_BOUND);
             pg_bar_expect(&sm.item_full[at], row_bytes * (unsigned)n);
         }
+        sent++;
         __syncwarp();
         if (lane < n) {
             const RT *src = static_cast<const RT *>(a.q) + (long long)(s.first + lane) * a.ldq + (long long)kvh * a.c.group * a.c.hd;
@@ -251,10 +253,9 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
             while (count == 0 && b + 1 < a.c.batch) s = paged_seq(a.c, ++b), count = few_tiles(a, s, KEYS, &t0);
         }
     }
-    if (!alive) { // copies in flight end before the block does
-        for (unsigned i = it > (unsigned)SLOTS ? it - SLOTS : 0; i < it; i++) pg_bar_wait(&sm.full[i % SLOTS], (i / SLOTS) & 1u);
-        for (unsigned i = number > FEW_ITEMS ? number - FEW_ITEMS : 0; i <= number; i++) pg_bar_wait(&sm.item_full[i % FEW_ITEMS], (i / FEW_ITEMS) & 1u);
-    }
+    // copies in flight end before the block does, whoever has given up
+    for (unsigned i = it > (unsigned)SLOTS ? it - SLOTS : 0; i < it; i++) pg_bar_wait(&sm.full[i % SLOTS], (i / SLOTS) & 1u);
+    for (unsigned i = sent > FEW_ITEMS ? sent - FEW_ITEMS : 0; i < sent; i++) pg_bar_wait(&sm.item_full[i % FEW_ITEMS], (i / FEW_ITEMS) & 1u);
 }
 
 // The beginning of a block: barriers, and its place on the line.
@@ -484,7 +485,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
                 }
             }
             __syncwarp();
-            if (lane == 0) pg_bar_arrive(&sm.empty[slot]);
+            if (lane == 0 && alive) pg_bar_arrive(&sm.empty[slot]); // (what it has not waited for is not given back)
         }
 
         // ---- the item's (or its part's) end: the four warps' results meet ----
@@ -497,7 +498,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
                 if (lane < 4) ml[warp][0][nt * 8 + lane * 2 + e] = m[nt][e], ml[warp][1][nt * 8 + lane * 2 + e] = l[nt][e];
             }
         few_meet();
-        if (lane == 0) pg_bar_arrive(&sm.item_empty[which]);
+        if (lane == 0 && alive) pg_bar_arrive(&sm.item_empty[which]);
         float mm[NT][2], ll[NT][2];
         constexpr int MINE = KS / FEW_WARPS; // a warp joins this many of the 16-column pieces
 #pragma unroll
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
                 }
             }
             __syncwarp();
-            if (lane == 0) pg_bar_arrive(&sm.empty[slot]);
+            if (lane == 0 && alive) pg_bar_arrive(&sm.empty[slot]); // (what it has not waited for is not given back)
         }
 
         // ---- the item's (or its part's) end: the four warps' results meet, [warp][row][column] ----
@@ -779,7 +780,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
                 *reinterpret_cast<float2 *>(to) = make_float2(o[r][0], o[r][1]);
         }
         few_meet();
-        if (lane == 0) pg_bar_arrive(&sm.item_empty[which]);
+        if (lane == 0 && alive) pg_bar_arrive(&sm.item_empty[which]);
         const bool is_whole = item.before == 0 && item.tiles == item.count;
         const long long slot = (long long)blockIdx.x * 2 + (first_part && item.before > 0 ? 0 : 1);
         constexpr int AT_ONCE = 32 * FEW_WARPS / HDP; // rows that the threads take at once, a column each

@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *ring = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u), *stage = ring + SLOTS * SLOT;
     unsigned long long *full = reinterpret_cast<unsigned long long *>(stage + Shape::STAGE), *empty = full + SLOTS;
-    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *o_free = o_full + 1, *q_full = o_free + 1, *tail = q_full + 1, *stage_full = tail + 1, *stage_empty = stage_full + 1; // 2 SLOTS + 10 <= 32 words
+    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 2, *o_free = o_full + 1, *q_full = o_free + 1, *tail = q_full + 1, *stage_full = tail + 1, *stage_empty = stage_full + 1, *done = stage_empty + 1; // 2 SLOTS + 11 <= 32 words
     __shared__ long long place[32];
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
@@ -67,6 +67,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         pg_bar_init(tail, 1);
         pg_bar_init(stage_full, 1);
         pg_bar_init(stage_empty, 128);
+        pg_bar_init(done, 1);
         dead = 0;
         f.head[blockIdx.x * 8] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         bool alive = true;
         if (CP == 1 && warp == 4) {
             unsigned tails = 0;
+            bool tail_lost = false;
             const int box_rows = min(page, FINE_KEYS);
             while (w.left > 0 && alive) {
                 const ManyItem item = w.item(a, paged_seq(a.c, w.b));
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                     }
                     if (clean) {
                         if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(tail, tails & 1u))) {
-                            alive = false;
+                            alive = false, tail_lost = true;
                             break;
                         }
                         tails++;
@@ -143,10 +145,10 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 }
                 if (alive) w.next(a);
             }
-            if (!alive) { // copies in flight end before the block does
-                if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
-                for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
-            }
+            if (!alive && lane == 0) atomicExch(a.c.status, PAGED_WAIT);
+            // copies in flight end before the block does, whoever has given up
+            if (tail_lost) pg_bar_wait(tail, tails & 1u);
+            for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
         } else if (CP == 3) {
             constexpr int CHUNKS = HDP / 8, ROWS_AT_ONCE = 128 / CHUNKS, N = FINE_KEYS / ROWS_AT_ONCE; // a thread: N pieces of 8 columns, of rows ROWS_AT_ONCE apart
             const int mine = tid - 128, chunk = mine % CHUNKS, row0 = mine / CHUNKS;
@@ -266,7 +268,11 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 tile_count += tiles;
                 if (alive) w.next(a);
             }
-            if (!alive) atomicExch(a.c.status, PAGED_WAIT);
+            if (!alive) { // products in flight end before their tensor memory is given back
+                atomicExch(a.c.status, PAGED_WAIT);
+                pg_commit(done);
+                pg_bar_wait(done, 0);
+            }
         }
         if (warp == 9) { // ---------------- the queries of the next item, while this one's keys are worked on ----------------
             unsigned items = 0;
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 items++;
                 w.next(a);
             }
-            if (w.left > 0 && items > 0) pg_bar_wait(stage_full, (items - 1) & 1u); // copies in flight end before the block does
+            if (items > 0) pg_bar_wait(stage_full, (items - 1) & 1u); // copies in flight end before the block does, whoever has given up
         }
         __syncwarp();
     } else { // ---------------- the softmax: a thread a row ----------------
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         };
         if (w.left > 0) {
             queries(w.item(a, paged_seq(a.c, w.b)).rows);
-            pg_bar_arrive(stage_empty); // for the second item's; the place is free again for the one after next when an item's output has left it
+            if (alive) pg_bar_arrive(stage_empty); // for the second item's; the place is free again for the one after next when an item's output has left it
         }
         while (w.left > 0) {
             const PagedSeq s = paged_seq(a.c, w.b);
@@ -463,7 +469,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             }
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            pg_bar_arrive(stage_empty);
+            if (alive) pg_bar_arrive(stage_empty); // (a place whose rows it has not waited for is not given back)
             float odd0, odd1;
             pg_one(odd, odd0, odd1);
             unsigned rest = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));

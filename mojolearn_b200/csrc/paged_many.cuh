@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *query = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u), *ring = query + Shape::QUERY;
     unsigned long long *full = reinterpret_cast<unsigned long long *>(ring + SLOTS * TILE), *empty = full + SLOTS;
-    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 4, *q_full = o_full + 2, *tail = q_full + 1; // 2 SLOTS + 10 <= 32 words
+    unsigned long long *s_full = empty + SLOTS, *p_full = s_full + 2, *o_full = p_full + 4, *q_full = o_full + 2, *tail = q_full + 1, *done = tail + 1; // 2 SLOTS + 11 <= 32 words
     __shared__ float stats[2][2][128], half_stat[3][2][2][128]; // m and l of a stream's rows; what the two threads of a row tell each other
     __shared__ long long place[32];
     __shared__ unsigned long long pair_bars[8];
@@ -365,6 +365,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         }
         pg_bar_init(q_full, 512);
         pg_bar_init(tail, 1);
+        pg_bar_init(done, 1);
         dead = 0;
         f.head[blockIdx.x * 8] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     if (warp >= 16) { // apart in this order: with the three as one chain of conditions the compiler's code took 190 us for 186 (12 chunks, capped)
         if (warp == 16) { // ---------------- the copies ----------------
             unsigned ld = 0, tails = 0;
-            bool alive = true;
+            bool alive = true, tail_lost = false;
             while (w.left > 0 && alive) {
                 const ManyItem item = w.item(a, paged_seq(a.c, w.b));
                 const int tiles = w.tiles(item), first = w.first(item), last_page = (item.high - 1) >> a.c.page_shift;
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     if (clean) {
                         if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(tail, tails & 1u))) {
                             if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
-                            alive = false;
+                            alive = false, tail_lost = true;
                             break;
                         }
                         tails++;
@@ -438,8 +439,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 }
                 if (alive) w.next(a);
             }
-            if (!alive) // copies in flight end before the block does
-                for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
+            // copies in flight end before the block does, whoever has given up
+            if (tail_lost) pg_bar_wait(tail, tails & 1u);
+            for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
         } else if (warp == 17) { // ---------------- the products ----------------
             if (lane == 0) {
                 unsigned ld = 0, items = 0, p_count[2] = {0, 0};
@@ -521,7 +523,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     }
                     if (alive) w.next(a);
                 }
-                if (!alive) atomicExch(a.c.status, PAGED_WAIT);
+                if (!alive) { // products in flight end before their tensor memory is given back
+                    atomicExch(a.c.status, PAGED_WAIT);
+                    pg_commit(done);
+                    pg_bar_wait(done, 0);
+                }
             }
             __syncwarp();
         }
