@@ -135,11 +135,12 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (ws_bytes > 0 && !aligned16(ws)) return refuse(err, err_cap, "paged_attention: the workspace must start on a 16-byte boundary");
     a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.flip = scale < 0.0, a.softcap = (float)softcap;
     a.scale = std::max(fabsf((float)scale), 1e-30f); // none makes all weights alike, as does next to none
-    a.cap_inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f, a.cap_outer = a.softcap > 0.0f ? a.softcap / a.scale : 0.0f;
+    // scale / softcap and its inverse, held to what 32 bits have: there next to every score is far below the cap, or far above it
+    const auto within = [](double x) { return (float)std::min(std::max(x, 1.2e-38), 3.4e38); };
+    a.cap_inner = a.softcap > 0.0f ? within((double)a.scale / a.softcap) : 0.0f, a.cap_outer = a.softcap > 0.0f ? within((double)a.softcap / a.scale) : 0.0f;
+    a.cap_far = !(a.cap_inner > 1e-4f && a.cap_inner < 1e4f);
     float power = 1.0f;
-    for (int i = 0; i < 4; i++) power *= a.cap_inner * a.cap_inner, a.cap_near[i] = CAP_NEAR[i] * power;
-    // the polynomial's eighth power has to stay within 32 bits; where it does not, all scores go the other way (unless they are as good as zero)
-    a.cap_from = a.cap_outer > 3e38f || (a.cap_inner > 1e-4f && a.cap_inner < 1e4f) ? a.cap_outer : -1.0f;
+    for (int i = 0; i < 4; i++) power *= a.cap_far ? 1.0f : a.cap_inner * a.cap_inner, a.cap_near[i] = CAP_NEAR[i] * power;
     a.window = (int)std::min(window, MOST), a.max_new = (int)std::min(max_new, MOST);
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;

@@ -79,8 +79,8 @@ struct AttendCall {
     long long ldq;  // elements between rows of q
     float scale, softcap;  // scale > 0: a negative one is the queries' sign (flip)
     int flip;
-    float cap_inner, cap_outer, cap_near[4]; // of capped scores (paged_many.cuh): scale / softcap, its inverse, its even powers times the polynomial's coefficients
-    float cap_from;                          // the polynomial is for scores up to this
+    float cap_inner, cap_outer, cap_near[4]; // of capped scores (paged_many.cuh): scale / softcap and its inverse, both within 32 bits; the polynomial's coefficients
+    int cap_far;                             // 0: with the even powers of cap_inner in them
     int window;     // 0: none
     int max_new;    // a sequence's rows past these are not computed
 };

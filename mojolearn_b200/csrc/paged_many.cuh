@@ -104,10 +104,13 @@ __device__ __forceinline__ float pg_cap_far(float x, float inner, float outer) {
     const float e = paged_exp2(fabsf(x) * (inner * 2.0f * PAGED_LOG2E));
     return copysignf((1.0f - __fdividef(2.0f, 1.0f + e)) * outer, x); // (the quotient of a huge or infinite e is zero)
 }
-// Near zero by x + x^3 P(x^2): for weights of 8 bits a polynomial over |x inner| <= 1, whose largest error, 4e-6, was made least by reweighted
-// least squares (CAP_NEAR; with inner's powers in AttendCall); a warp whose scores are all below the cap, as they mostly are, does only this.
-constexpr float CAP_NEAR[4] = {-0.33297876f, 0.13021576f, -0.04450673f, 0.00886790f};
-template <int N>
+// Up to |y| = 1, y = x inner, as x + x q P(q), q = y^2: for weights of 8 bits P has four coefficients, the largest error being 4.5e-6 of the cap; they
+// were chosen by least maximum among those that meet tanh(1), so that there is no step between the two forms that large caps would turn into a step of
+// a score. Which form a score takes goes by y alone, so a small score under a large cap stays as exact as it is. A warp whose scores are all
+// below the cap, as they mostly are, does only this one. With inner's powers in the coefficients (cap_near, in AttendCall) the product y is saved:
+// 12 capped chunks 191 us against 194. FAR has it, for an inner whose eighth power would leave 32 bits.
+constexpr float CAP_NEAR[4] = {-0.33295240f, 0.13005409f, -0.04421596f, 0.00870843f};
+template <int N, bool FAR>
 __device__ __forceinline__ void pg_cap(float *x, const AttendCall &a) {
     float most = 0.0f;
 #pragma unroll
@@ -115,13 +118,14 @@ __device__ __forceinline__ void pg_cap(float *x, const AttendCall &a) {
     unsigned long long k[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) k[i] = pg_two(a.cap_near[i], a.cap_near[i]);
+    const unsigned long long inner = pg_two(a.cap_inner, a.cap_inner);
     const auto near = [&](int c, float &y0, float &y1) {
-        const unsigned long long v = pg_two(x[c], x[c + 1]), q = pg_mul2(v, v);
+        const unsigned long long v = pg_two(x[c], x[c + 1]), y = FAR ? pg_mul2(v, inner) : v, q = pg_mul2(y, y);
         unsigned long long p = pg_fma2(q, k[3], k[2]);
         p = pg_fma2(q, p, k[1]), p = pg_fma2(q, p, k[0]);
         pg_one(pg_fma2(pg_mul2(v, q), p, v), y0, y1);
     };
-    if (!__any_sync(0xFFFFFFFFu, most > a.cap_from)) {
+    if (!__any_sync(0xFFFFFFFFu, most > a.cap_outer)) {
 #pragma unroll
         for (int c = 0; c < N; c += 2) near(c, x[c], x[c + 1]);
     } else {
@@ -130,7 +134,7 @@ __device__ __forceinline__ void pg_cap(float *x, const AttendCall &a) {
             float y0, y1;
             near(c, y0, y1);
             const float f0 = pg_cap_far(x[c], a.cap_inner, a.cap_outer), f1 = pg_cap_far(x[c + 1], a.cap_inner, a.cap_outer);
-            x[c] = fabsf(x[c]) > a.cap_from ? f0 : y0, x[c + 1] = fabsf(x[c + 1]) > a.cap_from ? f1 : y1;
+            x[c] = fabsf(x[c]) > a.cap_outer ? f0 : y0, x[c + 1] = fabsf(x[c + 1]) > a.cap_outer ? f1 : y1;
         }
     }
 }
@@ -257,7 +261,7 @@ __device__ __forceinline__ float many_largest(unsigned s_at, int lo, int hi) {
     }
     return fmaxf(top[0], top[1]);
 }
-template <bool CAP, bool EDGE>
+template <int CAP, bool EDGE> // CAP: 0 none, 1 capped, 2 capped with FAR
 __device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at, float unit, float base, int lo, int hi, float &largest) {
     const unsigned long long unit2 = pg_two(unit, unit), base2 = pg_two(-base, -base);
     float top[2] = {-INFINITY, -INFINITY};
@@ -278,7 +282,7 @@ __device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at
                     for (int i = 0; i < 16; i++)
                         if (c + i >= hi || c + i < lo) x[i] = 0.0f;
                 }
-                pg_cap<16>(x, a);
+                pg_cap<16, CAP == 2>(x, a);
             }
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
@@ -610,7 +614,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                     if (!alive) continue;
                     if (a.softcap > 0.0f) {
                         float capped[2] = {most, 0.0f};
-                        pg_cap<2>(capped, a);
+                        a.cap_far ? pg_cap<2, true>(capped, a) : pg_cap<2, false>(capped, a);
                         const int at = 64 * half; // a score of -infinity is capped as well; a row that sees nothing of the tile stays without
                         most = max(lo + at, 0) < min(hi + at, MANY_KEYS) ? capped[0] : -INFINITY;
                     }
@@ -639,10 +643,12 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 }
                 const float base = m == -INFINITY ? 0.0f : m;
                 float largest;
-                if (a.softcap > 0.0f)
-                    l += edge ? many_weights<true, true>(a, s_at, unit, base, lo, hi, largest) : many_weights<true, false>(a, s_at, unit, base, lo, hi, largest);
+                if (a.softcap > 0.0f && !a.cap_far)
+                    l += edge ? many_weights<1, true>(a, s_at, unit, base, lo, hi, largest) : many_weights<1, false>(a, s_at, unit, base, lo, hi, largest);
+                else if (a.softcap > 0.0f)
+                    l += many_weights<2, true>(a, s_at, unit, base, lo, hi, largest);
                 else
-                    l += edge ? many_weights<false, true>(a, s_at, unit, base, lo, hi, largest) : many_weights<false, false>(a, s_at, unit, base, lo, hi, largest);
+                    l += edge ? many_weights<0, true>(a, s_at, unit, base, lo, hi, largest) : many_weights<0, false>(a, s_at, unit, base, lo, hi, largest);
                 known = largest * unit;
                 if (known > base + 100.0f && valid) l = NAN; // weights out of range: the row is done again like one that is not finite
                 half_stat[1 + (j & 1)][stream][half][r] = known;
