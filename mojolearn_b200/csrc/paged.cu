@@ -133,7 +133,8 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (window < 0 || !(softcap >= 0.0) || softcap > 1e30 || !(scale > -1e30 && scale < 1e30)) return refuse(err, err_cap, "paged_attention: window, softcap or scale is out of range");
     if (ws_bytes < 0 || (ws_bytes > 0 && !ws)) return refuse(err, err_cap, "paged_attention: a workspace size without a workspace");
     if (ws_bytes > 0 && !aligned16(ws)) return refuse(err, err_cap, "paged_attention: the workspace must start on a 16-byte boundary");
-    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.flip = scale < 0.0, a.softcap = (float)softcap;
+    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.ldq = ldq, a.flip = scale < 0.0;
+    a.softcap = softcap > 0.0 ? std::max((float)softcap, 1e-30f) : 0.0f; // (a cap of next to nothing is still one: all weights alike)
     a.scale = std::max(fabsf((float)scale), 1e-30f); // none makes all weights alike, as does next to none
     // scale / softcap and its inverse, held to what 32 bits have: there next to every score is far below the cap, or far above it
     const auto within = [](double x) { return (float)std::min(std::max(x, 1.2e-38), 3.4e38); };

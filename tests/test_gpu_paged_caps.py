@@ -49,3 +49,14 @@ def test_scores_about_where_the_formula_changes(rows, cache, new, part):
     got = paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), max_new=new, softcap=65536.0, scale=1.0)
     off = (got.double() - c.attention(softcap=65536.0, scale=1.0)).abs().max()
     assert float(off) <= (2.0 ** -5 + 2.0 ** -7) * c.most()
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("cap,scale", [(1e-20, 1e20), (1e-25, 1.0), (1e-40, 1.0), (1e-300, 0.125)])
+def test_caps_next_to_nothing(rows, cache, new, cap, scale):
+    """Scores capped to next to nothing weigh all keys alike, whatever the scale; a product of zero among them too."""
+    c = Case([new] * 2, [0, 300], 4, 2, 64, 32, rows, cache)
+    for b in range(2):
+        c.k_cache[int(c.table[b, 0]), :, 0] = 0.0
+    held(c, softcap=cap, scale=scale)
