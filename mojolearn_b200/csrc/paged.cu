@@ -138,6 +138,7 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     a.scale = std::max(fabsf((float)scale), 1e-30f); // none makes all weights alike, as does next to none
     // scale / softcap and its inverse, held to what 32 bits have: there next to every score is far below the cap, or far above it
     const auto within = [](double x) { return (float)std::min(std::max(x, 1.2e-38), 3.4e38); };
+    a.cap_part = a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
     a.cap_inner = a.softcap > 0.0f ? within((double)a.scale / a.softcap) : 0.0f, a.cap_outer = a.softcap > 0.0f ? within((double)a.softcap / a.scale) : 0.0f;
     a.cap_far = !(a.cap_inner > 1e-4f && a.cap_inner < 1e4f);
     float power = 1.0f;

@@ -78,6 +78,7 @@ struct AttendCall {
     void *out;
     long long ldq;  // elements between rows of q
     float scale, softcap;  // scale > 0: a negative one is the queries' sign (flip)
+    float cap_part;        // 1 / softcap
     int flip;
     float cap_inner, cap_outer, cap_near[4]; // of capped scores (paged_many.cuh): scale / softcap and its inverse, both within 32 bits; the polynomial's coefficients
     int cap_far;                             // 0: with the even powers of cap_inner in them

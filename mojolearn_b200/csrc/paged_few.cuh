@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
         return;
     }
 
-    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E;
     unsigned it = 0;
     bool alive = true, first_part = true;
     const auto give_up = [&] {
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         float x = z[nt][i];
-                        x = unit * (a.softcap > 0.0f ? tanhf(x * inner) : x);
+                        x = unit * (a.softcap > 0.0f ? tanhf(x * a.scale * a.cap_part) : x); // (scale / softcap may leave 32 bits)
                         if (edge) {
                             const int j = j0 + (lane >> 2) + (i >> 1) * 8;
                             if (j >= hi[nt][i & 1] || j < lo[nt][i & 1]) x = -INFINITY;
@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
 
     float *const weights = sm.meet + warp * R * HDP; // [R][MINE], where this warp's results will be
     const int key = lane % MINE, share = lane / MINE;  // of a tile a warp takes MINE keys; SPLIT lanes have a key's columns between them
-    const float sign = a.flip ? -1.0f : 1.0f, unit = sign * (a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E), inner = a.softcap > 0.0f ? a.scale / a.softcap : 0.0f;
+    const float sign = a.flip ? -1.0f : 1.0f, unit = sign * (a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E);
     unsigned it = 0;
     bool alive = true, first_part = true;
     const auto give_up = [&] {
@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
                     z += z1;
 #pragma unroll
                     for (int d = MINE; d < 32; d <<= 1) z += __shfl_xor_sync(0xFFFFFFFFu, z, d);
-                    z = unit * (a.softcap > 0.0f ? tanhf(z * inner) : z);
+                    z = unit * (a.softcap > 0.0f ? tanhf(z * a.scale * a.cap_part) : z);
                     if (edge) {
                         const int seen = s.pos0 + r / a.c.group;
                         if (j > seen || (a.window && j <= seen - a.window)) z = -INFINITY;

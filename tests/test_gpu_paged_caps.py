@@ -60,3 +60,11 @@ def test_caps_next_to_nothing(rows, cache, new, cap, scale):
     for b in range(2):
         c.k_cache[int(c.table[b, 0]), :, 0] = 0.0
     held(c, softcap=cap, scale=scale)
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 90])
+def test_a_scale_and_a_cap_whose_quotient_leaves_32_bits(rows, cache, new):
+    c = Case([new] * 2, [0, 300], 4, 2, 64, 32, rows, cache)
+    c.k_cache.mul_(2.0 ** 50)
+    held(c, softcap=1e30, scale=2.0 ** -52)
