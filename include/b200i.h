@@ -428,7 +428,8 @@ int64_t b200i_launch_count(void);
  * lengths[b] (int32) counts what its cache holds with them: its row i is at position lengths[b] - (cu[b + 1] - cu[b]) + i.
  * Rows past cu[batch] belong to no sequence: nothing is read for them and nothing written. The three arrays are read on
  * the device; a page number outside the pool counts as a page of zeros, is not written, and sets the status word
- * (b200i_decode_status) to 11. Row and cache types: float32 and float32, float32 and bfloat16, bfloat16 and bfloat16. */
+ * (b200i_decode_status) to 11. A sequence of more than max_pages * page positions, or with offsets that descend or leave 0 .. rows,
+ * is left out (nothing is written for its rows) and sets it to 14. Row and cache types: float32 and float32, float32 and bfloat16, bfloat16 and bfloat16. */
 
 /* Rows q [rows, n_heads * head_dim], k and v [rows, n_kv * head_dim] with row pitches ldq, ldk, ldv in elements (column blocks
  * of a fused product), starting on 16-byte boundaries. q_out [rows, n_heads * head_dim] receives the rotated queries in the row

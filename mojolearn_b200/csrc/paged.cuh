@@ -5,7 +5,8 @@
 // sequence b's are cu[b] .. cu[b + 1], and lengths[b] counts what its cache holds with them, so that its row i is at
 // position lengths[b] - n + i. All three arrays live on the device and are read there; what they say is bounded by the
 // extents of the tensors before it is used as an index, so that no table makes a kernel read or write outside of them: a page
-// number outside the pool reads as zeros, is not written, and sets the library's status word to PAGED_BAD_PAGE.
+// number outside the pool reads as zeros, is not written, and sets the library's status word to PAGED_BAD_PAGE; a sequence whose length
+// its page table has no room for, or whose row offsets are not the call's, is left out and sets it to PAGED_BAD_TABLE.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -19,6 +20,7 @@ namespace b200i {
 constexpr int PAGED_MAX_HD = 128;
 constexpr int PAGED_BAD_PAGE = 11; // the status word: a page number outside the pool
 constexpr int PAGED_BAD_BOUND = 12; // the status word: more new tokens in a sequence than the call's bound
+constexpr int PAGED_BAD_TABLE = 14; // the status word: a length past the page table, or row offsets that are not the call's
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 struct PagedCall {
@@ -31,6 +33,13 @@ struct PagedCall {
 };
 
 __device__ __forceinline__ PagedSeq paged_seq(const PagedCall &c, int b) { return paged_place(c.cu[b], c.cu[b + 1], c.lengths[b], (int)c.rows, c.max_pages << c.page_shift); }
+
+// The same, and the status word where the tables do not hold the sequence: each kernel looks at every sequence once in this way.
+__device__ __forceinline__ PagedSeq paged_seq_checked(const PagedCall &c, int b) {
+    const int lo = c.cu[b], hi = c.cu[b + 1], length = c.lengths[b], capacity = c.max_pages << c.page_shift;
+    if (!paged_holds(lo, hi, length, (int)c.rows, capacity)) atomicExch(c.status, PAGED_BAD_TABLE);
+    return paged_place(lo, hi, length, (int)c.rows, capacity);
+}
 
 // The sequence of row t, or -1: a warp looks at 32 entries of cu at a time. All lanes call it with one t.
 __device__ __forceinline__ int paged_row_seq(const PagedCall &c, long long t) {

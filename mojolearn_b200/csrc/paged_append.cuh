@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(128) append_units_kernel(const AppendCall a, i
 
     const int b = paged_row_seq(a.c, t);
     if (b < 0) return; // a row of no sequence: nothing is written for it
-    const PagedSeq s = paged_seq(a.c, b);
+    const PagedSeq s = paged_seq_checked(a.c, b);
+    if (s.n == 0) return; // its tables do not hold it
     const int pos = s.pos0 + (int)(t - s.first);
     // the position's place in the caches, of key head 0; -1: none
     const long long place = pos < 0 ? -1 : paged_offset(a.c, b, 0, pos);
@@ -193,7 +194,8 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
     const int lane = threadIdx.x & 31, b = paged_row_seq(a.c, t);
     int head = blockIdx.y * 8 + (threadIdx.x >> 5);
     if (b < 0 || head >= a.c.heads + 2 * a.c.kv) return;
-    const PagedSeq s = paged_seq(a.c, b);
+    const PagedSeq s = paged_seq_checked(a.c, b);
+    if (s.n == 0) return; // its tables do not hold it
     const int pos = s.pos0 + (int)(t - s.first), part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2);
     head -= part == 0 ? 0 : (part == 1 ? a.c.heads : a.c.heads + a.c.kv);
     const RT *src = part == 0 ? static_cast<const RT *>(a.q) + t * a.ldq : (part == 1 ? static_cast<const RT *>(a.k) + t * a.ldk : static_cast<const RT *>(a.v) + t * a.ldv);

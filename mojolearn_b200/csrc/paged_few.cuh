@@ -169,7 +169,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
     int t0 = 0, count = 0;
     const auto settle = [&] { // whole items: the first from (b, kvh) on, by steps of the grid, that has rows
         for (; b < a.c.batch; kvh += gridDim.x, b += kvh / a.c.kv, kvh %= a.c.kv) {
-            s = paged_seq(a.c, b), count = few_tiles(a, s, KEYS, &t0);
+            s = paged_seq_checked(a.c, b), count = few_tiles(a, s, KEYS, &t0);
             if (count > 0) return;
         }
         left = 0;
@@ -283,7 +283,7 @@ __device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory
             f.a.c,
             [&](int b) -> long long {
                 int t0;
-                return few_tiles(f.a, paged_seq(f.a.c, b), FewKeys<CT, HDP>::N, &t0);
+                return few_tiles(f.a, paged_seq_checked(f.a.c, b), FewKeys<CT, HDP>::N, &t0);
             },
             blockIdx.x, gridDim.x, place);
     }

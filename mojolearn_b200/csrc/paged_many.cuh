@@ -202,7 +202,7 @@ template <int BR, int KEYS, int STREAMS> struct ManyWalk {
 
     static __device__ __forceinline__ int rows_of(const AttendCall &a, const PagedSeq &s) { return min(s.n, a.max_new); } // tokens that are computed
     static __device__ __forceinline__ long long steps_of(const AttendCall &a, int b) {
-        const PagedSeq s = paged_seq(a.c, b);
+        const PagedSeq s = paged_seq_checked(a.c, b);
         const int n = rows_of(a, s), blocks = many_blocks(a, n, BR);
         long long sum = 0;
         for (int i = 0; i < blocks; i++) sum += many_item<BR, KEYS, STREAMS>(a, s, n, i).steps;

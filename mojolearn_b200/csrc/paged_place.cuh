@@ -15,13 +15,15 @@ struct PagedSeq {
     int pos0;      // position of its first row (negative where a table says that fewer are cached than are new)
 };
 
-// Rows lo .. hi - 1 of `rows` in all and `length` positions, of `capacity` that the page table has room for. Whatever the tables say, the rows lie
-// within the call's and the length within the capacity.
+// Whether rows lo .. hi - 1 lie within the call's `rows` and, where there are any, `length` positions within the `capacity` of the page table.
+PAGED_HD bool paged_holds(int lo, int hi, int length, int rows, int capacity) { return 0 <= lo && lo <= hi && hi <= rows && (lo == hi || length <= capacity); }
+
+// Where they are. A sequence that is not held has no rows: to move its positions to where there is room would put new keys over old ones.
 PAGED_HD PagedSeq paged_place(int lo, int hi, int length, int rows, int capacity) {
     PagedSeq s;
-    s.first = lo < 0 ? 0 : (lo > rows ? rows : lo);
-    hi = hi < rows ? hi : rows;
-    s.n = hi > s.first ? hi - s.first : 0; // compared first: a difference of any two words leaves 32 bits
+    const bool held = paged_holds(lo, hi, length, rows, capacity);
+    s.first = held ? lo : 0;
+    s.n = held ? hi - lo : 0;
     s.length = length < 0 ? 0 : (length > capacity ? capacity : length);
     s.pos0 = s.length - s.n;
     return s;

@@ -16,8 +16,9 @@ what its cache holds with them, so that its last row is at position `lengths[b] 
 device tensors and are read by the kernels only, so a call can be captured in a CUDA graph and replayed after they have
 changed. Rows and cache are float32 and float32, float32 and bfloat16, or bfloat16 and bfloat16.
 
-Calls are asynchronous on the current stream. A page number outside the pool is treated as a page of zeros and not written,
-and reported by `torch_ops.check_status`.
+Calls are asynchronous on the current stream. A page number outside the pool is treated as a page of zeros and not written; a
+sequence with more positions than its row of the page table has room for, or with offsets that are not the call's, is left
+out. Both are reported by `torch_ops.check_status`.
 """
 import functools
 import math

@@ -1,0 +1,49 @@
+"""What a call's tables may say and what is made of it: lengths past the page table, offsets past the rows, positions past the rotation, windows of
+any size, pages that nobody reads."""
+import pytest
+import torch
+
+from paged_ref import BF16, TYPES, Case, check
+
+pytestmark = pytest.mark.gpu
+if torch.cuda.is_available():
+    from mojolearn_b200 import _native, paged, torch_ops
+
+
+def both(c, lengths, cu, **kw):
+    """Append and attention into outputs of sevens, and the caches before."""
+    before = c.k_cache.clone(), c.v_cache.clone()
+    q, out = (torch.full((c.total, c.heads, c.hd), 7.0, dtype=c.rows, device="cuda") for _ in range(2))
+    paged.append(c.q, c.k, c.v, c.k_cache, c.v_cache, c.table, cu, lengths, out=q)
+    appended = int(_native.lib().b200i_decode_status(torch.cuda.current_device()))
+    paged.attention(c.q, c.k_cache, c.v_cache, c.table, cu, lengths, max_new=max(c.new), out=out, **kw)
+    return before, q, out, appended
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("what", ["length", "length at the limit", "offset"])
+def test_a_sequence_that_its_tables_do_not_hold_is_left_out(rows, cache, new, what):
+    """The second of three says more positions than its table has room for, or the last more rows than the call has: nothing of it is written, and
+    that is reported; the others are as they were."""
+    c = Case([new] * 3, [10, 64 * 3 - new, 40], 4, 2, 64, 64, rows, cache, seed=new)
+    c.table = c.table[:, :3].contiguous()
+    bad = 2 if what == "offset" else 1
+    lengths, cu = c.lengths.clone(), c.cu.clone()
+    if what == "offset":
+        cu[3] += 5
+    else:
+        lengths[1] = 64 * 3 + 1 if what == "length at the limit" else 1 << 30
+    (kb, vb), q, out, appended = both(c, lengths, cu)
+    assert appended == 14
+    with pytest.raises(_native.NativeError, match="more positions than its page table"):
+        torch_ops.check_status()
+    want = c.attention()
+    mine = slice(bad * new, bad * new + new)
+    assert bool((q[mine] == 7.0).all()) and bool((out[mine] == 7.0).all())
+    pages = [int(p) for p in c.table[bad] if p >= 0]
+    assert torch.equal(kb[pages], c.k_cache[pages]) and torch.equal(vb[pages], c.v_cache[pages])
+    for b in {0, 1, 2} - {bad}:
+        at = slice(b * new, b * new + new)
+        assert torch.equal(q[at], c.q[at])
+        check(out[at], want[at], rows, c.most())

@@ -46,3 +46,10 @@ def test_tables_of_any_words_stay_inside(place):
 
 def test_ordinary_tables(place):
     assert place([(0, 3, 20, 10, 64), (3, 10, 64, 10, 64), (5, 5, 7, 10, 64), (2, 9, 3, 10, 64)]) == [(0, 3, 20, 17), (3, 7, 64, 57), (5, 0, 7, 7), (2, 7, 3, -4)]
+
+
+def test_a_sequence_that_is_not_held_has_no_rows(place):
+    """More positions than the table has room for, or offsets that are not the call's: its rows are not moved to other positions."""
+    for case in [(0, 3, 65, 10, 64), (0, 3, HIGH, 10, 64), (8, 11, 20, 10, 64), (-1, 3, 20, 10, 64), (5, 2, 20, 10, 64), (LOW, HIGH, 20, 10, 64)]:
+        assert place([case])[0][1] == 0, case
+    assert place([(0, 3, 64, 10, 64), (4, 4, 65, 10, 64)]) == [(0, 3, 64, 61), (4, 0, 64, 64)]
