@@ -21,6 +21,7 @@ constexpr int PAGED_MAX_HD = 128;
 constexpr int PAGED_BAD_PAGE = 11; // the status word: a page number outside the pool
 constexpr int PAGED_BAD_BOUND = 12; // the status word: more new tokens in a sequence than the call's bound
 constexpr int PAGED_BAD_TABLE = 14; // the status word: a length past the page table, or row offsets that are not the call's
+constexpr int PAGED_BAD_POSITION = 15; // the status word: a position past the rotation's table
 constexpr float PAGED_LOG2E = 1.4426950408889634f;
 
 struct PagedCall {

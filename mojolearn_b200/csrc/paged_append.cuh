@@ -82,6 +82,13 @@ __device__ __forceinline__ bool append_place(const AppendCall &a, long long t, i
     return true;
 }
 
+// Whether the rotation's table has no row for a position: nothing is written for the row then, and that is reported.
+__device__ __forceinline__ bool append_past(const AppendCall &a, int pos) {
+    if (!a.cosv || pos < a.positions) return false;
+    atomicExch(a.c.status, PAGED_BAD_POSITION);
+    return true;
+}
+
 // N words of 32 bits, 16-byte aligned, two by two.
 template <int N>
 __device__ __forceinline__ void append_words(unsigned long long *x, const float *p) {
@@ -124,13 +131,14 @@ __global__ void __launch_bounds__(128) append_units_kernel(const AppendCall a, i
     const PagedSeq s = paged_seq_checked(a.c, b);
     if (s.n == 0) return; // its tables do not hold it
     const int pos = s.pos0 + (int)(t - s.first);
+    if (append_past(a, pos)) return;
     // the position's place in the caches, of key head 0; -1: none
     const long long place = pos < 0 ? -1 : paged_offset(a.c, b, 0, pos);
     const int head_words = a.c.hd << a.c.page_shift;
     unsigned long long c[N / 2], sn[N / 2];
     const bool turns = turned && a.cosv != nullptr;
     if (turns) {
-        const long long row = (long long)min(max(pos, 0), a.positions - 1) * half + at0;
+        const long long row = (long long)max(pos, 0) * half + at0;
         append_words<N>(c, a.cosv + row);
         append_words<N>(sn, a.sinv + row);
     }
@@ -197,6 +205,7 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
     const PagedSeq s = paged_seq_checked(a.c, b);
     if (s.n == 0) return; // its tables do not hold it
     const int pos = s.pos0 + (int)(t - s.first), part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2);
+    if (append_past(a, pos)) return;
     head -= part == 0 ? 0 : (part == 1 ? a.c.heads : a.c.heads + a.c.kv);
     const RT *src = part == 0 ? static_cast<const RT *>(a.q) + t * a.ldq : (part == 1 ? static_cast<const RT *>(a.k) + t * a.ldk : static_cast<const RT *>(a.v) + t * a.ldv);
     src += (long long)head * a.c.hd;
@@ -214,7 +223,7 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
     CT *dst_cache;
     if (!append_place<RT, CT>(a, t, b, pos, part, head, &dst_row, &dst_cache)) return;
     const int half = a.rope_dim / 2;
-    const long long row = (long long)min(max(pos, 0), a.positions - 1) * half;
+    const long long row = (long long)max(pos, 0) * half;
     for (int i = lane; i < a.c.hd; i += 32) {
         float x = paged_read(src + i);
         if (w) x = x * r * (w[i] + a.norm_shift);

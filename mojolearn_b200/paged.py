@@ -110,7 +110,7 @@ def append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos=None, sin=Non
     given as they are): the rotated queries [rows, n_heads, head_dim], keys and values put in their pages.
 
     `cos`, `sin` float32 [positions, rope_dim / 2] hold the rotation of every position (None: no rotation); columns from rope_dim on
-    pass through. `q_norm`, `k_norm` float32 [head_dim]: an RMSNorm over each head's vector before the rotation, of weight w
+    pass through, and a row whose position they do not hold is not written and reported by `torch_ops.check_status`. `q_norm`, `k_norm` float32 [head_dim]: an RMSNorm over each head's vector before the rotation, of weight w
     ("rmsnorm") or 1 + w ("rmsnorm_offset"). Rows past cu[-1] belong to no sequence: their part of the answer is not written."""
     if out is None and norm in _NORMS and _plain_append is not None:
         done = _plain_append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos, sin, q_norm, k_norm, eps, _NORMS[norm])

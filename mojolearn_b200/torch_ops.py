@@ -97,6 +97,8 @@ def check_status(device=None):
         raise _native.NativeError("mojolearn_b200: a sequence has more new tokens than the call's max_new (status 12); the further rows were not written")
     if v == 14:
         raise _native.NativeError("mojolearn_b200: a sequence has more positions than its page table has room for, or row offsets that are not the call's (status 14); nothing was written for it")
+    if v == 15:
+        raise _native.NativeError("mojolearn_b200: a new token's position is past the rotation's table (status 15); nothing was written for it")
     if v != 0:
         raise _native.NativeError("mojolearn_b200: a bounded device-side wait ran out (status %d); results computed "
                                   "since the last check are incomplete" % v)

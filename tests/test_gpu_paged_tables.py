@@ -10,6 +10,11 @@ if torch.cuda.is_available():
     from mojolearn_b200 import _native, paged, torch_ops
 
 
+def tables(positions, half):
+    a = torch.arange(positions, device="cuda")[:, None] * 0.01 * (1 + torch.arange(half, device="cuda"))
+    return a.cos(), a.sin()
+
+
 def both(c, lengths, cu, **kw):
     """Append and attention into outputs of sevens, and the caches before."""
     before = c.k_cache.clone(), c.v_cache.clone()
@@ -47,3 +52,23 @@ def test_a_sequence_that_its_tables_do_not_hold_is_left_out(rows, cache, new, wh
         at = slice(b * new, b * new + new)
         assert torch.equal(q[at], c.q[at])
         check(out[at], want[at], rows, c.most())
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("hd,half", [(64, 32), (64, 2), (24, 12)])
+def test_a_position_past_the_rotation_is_not_written(rows, cache, hd, half):
+    c = Case([1, 20], [30, 25], 4, 2, hd, 16, rows, cache)
+    cos, sin = tables(40, half)
+    whole = tables(60, half)
+    kb, vb = c.k_cache.clone(), c.v_cache.clone()
+    want = paged.append(c.q, c.k, c.v, kw := c.k_cache.clone(), vw := c.v_cache.clone(), *c.args(), *whole)
+    torch_ops.check_status()
+    out = torch.full((21, 4, hd), 7.0, dtype=rows, device="cuda")
+    paged.append(c.q, c.k, c.v, c.k_cache, c.v_cache, *c.args(), cos, sin, out=out)
+    with pytest.raises(_native.NativeError, match="past the rotation"):
+        torch_ops.check_status()
+    assert torch.equal(out[:16], want[:16]) and bool((out[16:] == 7.0).all())
+    for pos in range(25, 45):  # of the second sequence
+        page, slot = int(c.table[1, pos // 16]), pos % 16
+        for got, before, after in ((c.k_cache, kb, kw), (c.v_cache, vb, vw)):
+            assert torch.equal(got[page, :, slot], (after if pos < 40 else before)[page, :, slot])
