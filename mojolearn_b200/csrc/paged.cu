@@ -143,7 +143,8 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     a.cap_far = !(a.cap_inner > 1e-4f && a.cap_inner < 1e4f);
     float power = 1.0f;
     for (int i = 0; i < 4; i++) power *= a.cap_far ? 1.0f : a.cap_inner * a.cap_inner, a.cap_near[i] = CAP_NEAR[i] * power;
-    a.window = (int)std::min(window, MOST), a.max_new = (int)std::min(max_new, MOST);
+    // a window as wide as the table is none; so a position and a window's difference stays in 32 bits
+    a.window = window < max_pages * page ? (int)window : 0, a.max_new = (int)std::min(max_new, MOST);
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -72,3 +72,15 @@ def test_a_position_past_the_rotation_is_not_written(rows, cache, hd, half):
         page, slot = int(c.table[1, pos // 16]), pos % 16
         for got, before, after in ((c.k_cache, kb, kw), (c.v_cache, vb, vw)):
             assert torch.equal(got[page, :, slot], (after if pos < 40 else before)[page, :, slot])
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new", [9, 90])
+@pytest.mark.parametrize("window", [(1 << 31) - 1, 1 << 31, (1 << 63) - 1])
+def test_windows_wider_than_any_cache(rows, cache, new, window):
+    """No window at all, also where some rows stand before the beginning of their cache."""
+    c = Case([new] * 2, [0, 300], 4, 4, 64, 16, rows, cache, lengths=[2, new + 300])
+    kw = {"max_new": new}
+    want = paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), **kw)
+    assert torch.equal(paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), window=window, **kw), want)
+    check(want, c.attention(), rows, c.most())
