@@ -204,7 +204,7 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
                          "r"(row_bytes), "r"(pg_smem(&sm.item_full[at]))
                          : "memory");
         }
-        const int last_page = (s.length - 1) >> a.c.page_shift;
+        const int last_page = (s.length - 1) >> a.c.page_shift, low = a.window ? max(0, s.pos0 + 1 - a.window) : 0; // no row sees what is below
         const int *ids = a.c.table + (long long)b * a.c.max_pages;
         int base = ((t0 + before) * KEYS) >> a.c.page_shift; // the first page that `id` holds, a lane each; `ahead` the 32 after
         int id = base + lane <= last_page ? ids[base + lane] : 0, ahead = base + 32 + lane <= last_page ? ids[base + 32 + lane] : 0;
@@ -230,10 +230,12 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
                 const int mine = __shfl_sync(0xFFFFFFFFu, id, (first + min(piece, there - 1) - base) & 31);
                 if (piece < there) {
                     int row = a.c.pages * a.c.kv * page; // past the pool: zeros
-                    if ((unsigned)mine < (unsigned)a.c.pages)
-                        row = ((mine * a.c.kv + kvh) << a.c.page_shift) + ((pos + piece * box_rows) & (page - 1));
-                    else
-                        atomicExch(a.c.status, PAGED_BAD_PAGE);
+                    if (low - pos < (piece + 1) * box_rows) { // a page that nobody sees any more may be anyone's
+                        if ((unsigned)mine < (unsigned)a.c.pages)
+                            row = ((mine * a.c.kv + kvh) << a.c.page_shift) + ((pos + piece * box_rows) & (page - 1));
+                        else
+                            atomicExch(a.c.status, PAGED_BAD_PAGE);
+                    }
                     const bool is_v = box >= BOXES;
                     const int cb = is_v ? box - BOXES : box;
                     pg_tma_load(dst + (is_v ? HALF : 0) + cb * (KEYS * 128) + piece * (box_rows * 128), is_v ? map_v : map_k, &sm.full[slot], cb * BOX_COLS, row);

@@ -121,11 +121,13 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                     for (int x = lane; x < there * BOXES; x += 32) {
                         const int piece = x / BOXES, box = x % BOXES, at = pos + piece * box_rows, index = at >> a.c.page_shift;
                         int row = a.c.pages * a.c.kv * page; // past the pool: zeros
-                        const int id = index <= last_page ? ids[index] : -1;
-                        if ((unsigned)id < (unsigned)a.c.pages)
-                            row = ((id * a.c.kv + w.kvh) << a.c.page_shift) + (at & (page - 1));
-                        else
-                            atomicExch(a.c.status, PAGED_BAD_PAGE);
+                        if (item.low - at < box_rows) { // a page that nobody sees any more may be anyone's
+                            const int id = index <= last_page ? ids[index] : -1;
+                            if ((unsigned)id < (unsigned)a.c.pages)
+                                row = ((id * a.c.kv + w.kvh) << a.c.page_shift) + (at & (page - 1));
+                            else
+                                atomicExch(a.c.status, PAGED_BAD_PAGE);
+                        }
                         pg_tma_load(dst + box * HALF_COLS + piece * (box_rows * 128), is_v ? &map_v : &map_k, bar, box * 64, row);
                     }
                     if (clean) {

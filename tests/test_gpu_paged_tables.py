@@ -84,3 +84,18 @@ def test_windows_wider_than_any_cache(rows, cache, new, window):
     want = paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), **kw)
     assert torch.equal(paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), window=window, **kw), want)
     check(want, c.attention(), rows, c.most())
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("page", [16, 32, 128])
+@pytest.mark.parametrize("new", [1, 4, 70, 300])
+@pytest.mark.parametrize("nobody", [-1, 1 << 30])
+def test_pages_below_the_window_need_no_number(rows, cache, page, new, nobody):
+    """Pages that no row sees any more may be given to others: their place in the table is not read as a page."""
+    c = Case([new] * 3, [0, 100, 700], 4, 2, 64, page, rows, cache, seed=new)
+    call = lambda: paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), max_new=new, window=50)  # noqa: E731
+    want = call()
+    for b, n in enumerate(c.length):
+        c.table[b, :max(0, n - new + 1 - 50) // page] = nobody
+    assert torch.equal(call(), want)
+    torch_ops.check_status()
