@@ -210,11 +210,12 @@ PyObject *paged_append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     }
     if (!vector_of(args[10], wq, c.hd, dev, &pq) || !vector_of(args[11], wk, c.hd, dev, &pk) || !real(args[12], &eps) || !integer(args[13], &kind)) Py_RETURN_NONE;
     at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous));
+    // written, so storage that is shared until then (a lazy clone) becomes this tensor's own, before addresses into it are taken
+    void *const k_cache = c.k.mutable_data_ptr(), *const v_cache = c.v.mutable_data_ptr();
     char message[ERR_CAP] = "";
     int64_t status;
     Py_BEGIN_ALLOW_THREADS;
-    status = g_append(dev.index(), c10::cuda::getCurrentCUDAStream(dev.index()).stream(), out.data_ptr(), const_cast<void *>(c.k.const_data_ptr()),
-                      const_cast<void *>(c.v.const_data_ptr()), q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), ldq, ldk, ldv, type, c.type, pcos, psin, 2 * half, positions, pq, pk, eps,
+    status = g_append(dev.index(), c10::cuda::getCurrentCUDAStream(dev.index()).stream(), out.data_ptr(), k_cache, v_cache, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), ldq, ldk, ldv, type, c.type, pcos, psin, 2 * half, positions, pq, pk, eps,
                       kind, static_cast<const int32_t *>(c.table.const_data_ptr()), static_cast<const int32_t *>(c.cu.const_data_ptr()), static_cast<const int32_t *>(c.lengths.const_data_ptr()),
                       rows, c.batch, heads, c.kv, c.hd, c.pages, c.page, c.table.size(1), message, ERR_CAP);
     Py_END_ALLOW_THREADS;

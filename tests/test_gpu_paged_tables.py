@@ -99,3 +99,13 @@ def test_pages_below_the_window_need_no_number(rows, cache, page, new, nobody):
         c.table[b, :max(0, n - new + 1 - 50) // page] = nobody
     assert torch.equal(call(), want)
     torch_ops.check_status()
+
+
+def test_a_lazily_copied_cache_is_written_alone():
+    """Storage that two tensors share until one of them is written."""
+    c = Case([3], [20], 4, 2, 64, 16, BF16, BF16)
+    k, v = torch._lazy_clone(c.k_cache), torch._lazy_clone(c.v_cache)
+    kb, vb = c.k_cache.clone(), c.v_cache.clone()
+    paged.append(c.q, c.k, c.v, k, v, *c.args())
+    assert torch.equal(c.k_cache, kb) and torch.equal(c.v_cache, vb)
+    assert not torch.equal(k, kb) and not torch.equal(v, vb)
