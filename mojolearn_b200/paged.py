@@ -224,18 +224,23 @@ class PagedCache(object):
         need = [self.pages_for(s, n) for s, n in zip(sequences, counts)]
         if sum(need) > len(self.free):
             raise ValueError("paged cache: %d pages are wanted and %d are free REFUSED" % (sum(need), len(self.free)))
-        for s, n, m in zip(sequences, counts, need):
-            self.held[s].extend(self.free.pop() for _ in range(m))
-            self.length[s] += n
-        width = max(1, max(len(self.held[s]) for s in sequences))
+        at, held = len(self.free), []
+        for s, m in zip(sequences, need):
+            held.append(self.held[s] + self.free[at - m:at][::-1])
+            at -= m
+        lengths, width = [self.length[s] + n for s, n in zip(sequences, counts)], max(1, max(len(h) for h in held))
         cu = [0]
         for n in counts:
             cu.append(cu[-1] + n)
-        # one copy to the device for all three
-        flat = cu + [self.length[s] for s in sequences]
-        for s in sequences:
-            flat.extend(self.held[s])
-            flat.extend([-1] * (width - len(self.held[s])))
+        # one copy to the device for all three, and nothing is taken before it is on its way
+        flat = cu + lengths
+        for h in held:
+            flat.extend(h)
+            flat.extend([-1] * (width - len(h)))
         t = torch.tensor(flat, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
         b = len(sequences)
-        return t[2 * b + 1:].view(b, width), t[:b + 1], t[b + 1:2 * b + 1]
+        tables = t[2 * b + 1:].view(b, width), t[:b + 1], t[b + 1:2 * b + 1]
+        for s, h, n in zip(sequences, held, lengths):
+            self.held[s], self.length[s] = h, n
+        del self.free[at:]
+        return tables

@@ -1,0 +1,39 @@
+"""`PagedCache` and `PagedLM` where a call fails or is refused, and at long positions."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+if torch.cuda.is_available():
+    from mojolearn_b200 import paged
+    from mojolearn_b200.models import CausalLM, CausalLMConfig, PagedLM
+
+
+def model(layers=3, **kw):
+    cfg = CausalLMConfig(vocab=256, d_model=128, n_layers=layers, **dict({"n_heads": 4, "n_kv_heads": 2, "head_dim": 32, "intermediate": 256, "max_positions": 1024}, **kw))
+    r = np.random.default_rng(5)
+    hd = cfg.head_dim
+    w = {"model.embed_tokens.weight": r.standard_normal((256, 128)) * 0.5, "model.norm.weight": np.ones(128), "lm_head.weight": r.standard_normal((256, 128)) * 0.1}
+    for i in range(layers):
+        p = "model.layers.%d." % i
+        for n in ("input_layernorm", "post_attention_layernorm"):
+            w[p + n + ".weight"] = np.ones(128)
+        for n, rows, cols in (("self_attn.q_proj", 4 * hd, 128), ("self_attn.k_proj", 2 * hd, 128), ("self_attn.v_proj", 2 * hd, 128), ("self_attn.o_proj", 128, 4 * hd),
+                              ("mlp.gate_proj", 256, 128), ("mlp.up_proj", 256, 128), ("mlp.down_proj", 128, 256)):
+            w[p + n + ".weight"] = r.standard_normal((rows, cols)) * 0.08
+    return CausalLM(cfg, {k: np.asarray(v, dtype=np.float32) for k, v in w.items()})
+
+
+def test_tables_that_cannot_be_made_take_no_pages(monkeypatch):
+    cache = paged.PagedCache(8, 2, 64, page=16)
+    a = cache.open()
+    cache.extend([a], [5])
+
+    def fail(*args, **kw):
+        raise RuntimeError("no pinned memory, say")
+
+    with monkeypatch.context() as m:
+        m.setattr(paged.torch, "tensor", fail)
+        with pytest.raises(RuntimeError, match="say"):
+            cache.extend([a], [40])
+    assert cache.length[a] == 5 and len(cache.held[a]) == 1 and len(cache.free) == 7
