@@ -42,8 +42,10 @@ class PagedLM(object):
         return self.cache.length[sequence]
 
     def feed(self, sequences, ids):
-        """New tokens ids[i] (each at least one) of sequences[i]: logits (len(sequences), vocab) on the device, of each one's last."""
-        lm, cfg, dev = self.lm, self.lm.config, self.lm.device
+        """New tokens ids[i] (each at least one) of sequences[i]: logits (len(sequences), vocab) on the device, of each one's last.
+        A call that fails leaves the sequences as they were."""
+        lm, cfg = self.lm, self.lm.config
+        sequences = list(sequences)
         ids = [np.asarray(x, dtype=np.int32).reshape(-1) for x in ids]
         counts = [x.size for x in ids]
         if len(ids) != len(sequences) or not ids or min(counts) < 1:
@@ -54,7 +56,15 @@ class PagedLM(object):
         if lm.pos_table is not None and longest > lm.pos_table.shape[0]:
             raise ValueError("position table of %d rows is too short" % lm.pos_table.shape[0])
         before = [self.cache.length[s] for s in sequences]
-        table, cu, lengths = self.cache.extend(sequences, counts)
+        tables = self.cache.extend(sequences, counts)
+        try:
+            return self._forward(ids, counts, before, longest, *tables)
+        except BaseException:  # the tokens were not (all) written: they do not count
+            self.cache.retract(sequences, counts)
+            raise
+
+    def _forward(self, ids, counts, before, longest, table, cu, lengths):
+        lm, cfg, dev = self.lm, self.lm.config, self.lm.device
         total, st = sum(counts), _stream(dev)
         host = np.concatenate(ids + [np.arange(p, p + n, dtype=np.int32) for p, n in zip(before, counts)] + [np.cumsum(counts) - 1]).astype(np.int32)
         words = torch.from_numpy(host).pin_memory().to(dev, non_blocking=True)

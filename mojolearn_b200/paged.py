@@ -215,6 +215,17 @@ class PagedCache(object):
         """How many further pages `count` more tokens of a sequence take."""
         return max(0, -(-(self.length[sequence] + count) // self.page) - len(self.held[sequence]))
 
+    def retract(self, sequences, counts):
+        """Take back an `extend` whose tokens were not written: the lengths and pages are as before it. What was queued on the device for
+        them may still run; pages go to later calls on the same stream."""
+        for s, n in reversed(list(zip(sequences, counts))):
+            if not 0 <= n <= self.length[s]:
+                raise ValueError("sequence %r has %d tokens, not %d to take back" % (s, self.length[s], n))
+            self.length[s] -= n
+            keep = -(-self.length[s] // self.page)
+            self.free.extend(reversed(self.held[s][keep:]))
+            del self.held[s][keep:]
+
     def extend(self, sequences, counts):
         """Room for counts[i] more tokens of sequences[i]: (page_table, cu, lengths) on the device. Refused as a whole, with no
         page taken, where the pool has too few left."""

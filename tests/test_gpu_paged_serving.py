@@ -24,6 +24,30 @@ def model(layers=3, **kw):
     return CausalLM(cfg, {k: np.asarray(v, dtype=np.float32) for k, v in w.items()})
 
 
+@pytest.mark.parametrize("block", [0, 1, 2])
+def test_a_call_that_fails_leaves_its_sequences_as_they_were(block, monkeypatch):
+    lm = model()
+    served, clean = PagedLM(lm, 20, page=16), PagedLM(lm, 20, page=16)
+    first, more = np.arange(10), np.arange(40) + 3
+    names = []
+    for s in (served, clean):
+        a, b = s.open(), s.open()
+        s.feed([a], [first])
+        names.append((a, b))
+    free, held = list(served.cache.free), list(served.cache.held[names[0][0]])
+
+    def fail(*args, **kw):
+        raise RuntimeError("out of memory, say")
+
+    with monkeypatch.context() as m:
+        m.setattr(lm.blocks[block], "forward_rows", fail)
+        with pytest.raises(RuntimeError, match="say"):
+            served.feed(list(names[0]), [more, first])
+    assert [served.length(n) for n in names[0]] == [10, 0]
+    assert sorted(served.cache.free) == sorted(free) and served.cache.held[names[0][0]] == held
+    assert torch.equal(served.feed(list(names[0]), [more[:7], first]), clean.feed(list(names[1]), [more[:7], first]))
+
+
 def test_tables_that_cannot_be_made_take_no_pages(monkeypatch):
     cache = paged.PagedCache(8, 2, 64, page=16)
     a = cache.open()
