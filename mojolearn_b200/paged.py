@@ -191,8 +191,12 @@ class PagedCache(object):
     def __init__(self, n_pages, n_kv_heads, head_dim, *, page=64, layers=1, dtype=torch.bfloat16, device=None):
         if dtype not in _TYPES:
             raise TypeError("a cache is float32 or bfloat16, got %s" % dtype)
-        if n_pages < 1 or layers < 1:
-            raise ValueError("a cache has at least one page and one layer")
+        if n_pages < 1 or layers < 1 or n_kv_heads < 1:
+            raise ValueError("a cache has at least one page, one key head and one layer")
+        if page < 16 or page > 256 or page & (page - 1):
+            raise ValueError("a page holds a power of two from 16 to 256 positions, got %r" % (page,))
+        if head_dim < 8 or head_dim > 128 or head_dim % 8:
+            raise ValueError("head_dim must be a multiple of 8 up to 128, got %r" % (head_dim,))
         _native.require_device()
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.page, self.pages, self.dtype = int(page), int(n_pages), dtype

@@ -61,3 +61,16 @@ def test_tables_that_cannot_be_made_take_no_pages(monkeypatch):
         with pytest.raises(RuntimeError, match="say"):
             cache.extend([a], [40])
     assert cache.length[a] == 5 and len(cache.held[a]) == 1 and len(cache.free) == 7
+
+
+@pytest.mark.parametrize("kw", [{"page": 24}, {"page": 8}, {"page": 512}, {"page": 0}, {"head_dim": 12}, {"head_dim": 136}, {"head_dim": 0}, {"n_kv_heads": 0}])
+def test_a_pool_that_no_call_would_take_is_refused(kw):
+    with pytest.raises(ValueError):
+        paged.PagedCache(4, kw.pop("n_kv_heads", 2), kw.pop("head_dim", 64), **kw)
+
+
+def test_a_model_whose_heads_no_call_would_take_is_refused():
+    with pytest.raises(ValueError, match="head_dim"):
+        PagedLM(model(layers=1, head_dim=12), 4)
+    with pytest.raises(ValueError, match="page"):
+        PagedLM(model(layers=1), 4, page=24)
