@@ -27,9 +27,10 @@ class PagedLM(object):
         cfg = lm.config
         self.lm = lm
         self.cache = paged.PagedCache(n_pages, cfg.n_kv_heads, cfg.head_dim, page=page, layers=cfg.n_layers, dtype=CACHES[cache], device=lm.device)
+        self.positions = min([cfg.max_positions] + [blk.ceiling for blk in lm.blocks])  # as far as the contiguous model goes
         self.cos = self.sin = None
-        if lm.blocks and lm.blocks[0].rope:  # of every position: a row takes its own
-            self.cos, self.sin = lm.blocks[0].rope_tables(0, cfg.max_positions)
+        if lm.blocks and lm.blocks[0].rope and self.positions:  # of every position: a row takes its own
+            self.cos, self.sin = lm.blocks[0].rope_tables(0, self.positions)
 
     def open(self):
         """A new, empty sequence: its name for `feed` and `close`."""
@@ -44,15 +45,15 @@ class PagedLM(object):
     def feed(self, sequences, ids):
         """New tokens ids[i] (each at least one) of sequences[i]: logits (len(sequences), vocab) on the device, of each one's last.
         A call that fails leaves the sequences as they were."""
-        lm, cfg = self.lm, self.lm.config
+        lm = self.lm
         sequences = list(sequences)
         ids = [np.asarray(x, dtype=np.int32).reshape(-1) for x in ids]
         counts = [x.size for x in ids]
         if len(ids) != len(sequences) or not ids or min(counts) < 1:
             raise ValueError("feed takes at least one token for each sequence")
         longest = max(self.cache.length[s] + n for s, n in zip(sequences, counts))
-        if longest > cfg.max_positions:
-            raise ValueError("absolute position %d is at or beyond max_positions %d" % (longest - 1, cfg.max_positions))
+        if longest > self.positions:
+            raise ValueError("absolute position %d is at or beyond max_positions %d" % (longest - 1, self.positions))
         if lm.pos_table is not None and longest > lm.pos_table.shape[0]:
             raise ValueError("position table of %d rows is too short" % lm.pos_table.shape[0])
         before = [self.cache.length[s] for s in sequences]

@@ -469,6 +469,11 @@ class TransformerBlock(object):
         return ({"linear": 1, "llama3": 2}[kind], float(rope_scaling["factor"]), float(rope_scaling.get("low_freq_factor", 1.0)),
                 float(rope_scaling.get("high_freq_factor", 4.0)), int(rope_scaling.get("original_max_position_embeddings", 8192)))
 
+    @property
+    def ceiling(self):
+        """The positions that a call may reach: the model's, within the domain of the rotation's sine and cosine."""
+        return min(self.max_positions, MAX_POSITIONS * (int(self.rope_scaling[1]) if self.rope_scaling[0] == 1 else 1))
+
     def rope_tables(self, pos0, l, position=None):
         """cos and sin [l, rope_dim / 2] for this call's positions; the same for every block of a model."""
         dev, st = self.device, _stream(self.device)
@@ -501,9 +506,8 @@ class TransformerBlock(object):
         if pos0 + l > state.max_tokens:
             raise ValueError("transformer: this call would use %d KV slots and the cache holds %d REFUSED" %
                              (pos0 + l, state.max_tokens))
-        ceiling = min(self.max_positions, MAX_POSITIONS * (int(self.rope_scaling[1]) if self.rope_scaling[0] == 1 else 1))
-        if pos0 + l > ceiling:
-            raise ValueError("transformer: absolute position %d is at or beyond %d" % (pos0 + l - 1, ceiling))
+        if pos0 + l > self.ceiling:
+            raise ValueError("transformer: absolute position %d is at or beyond %d" % (pos0 + l - 1, self.ceiling))
         dev, st = x.device, _stream(x.device)
         x2 = x.reshape(m, dm).contiguous()
         if delta is None:

@@ -74,3 +74,25 @@ def test_a_model_whose_heads_no_call_would_take_is_refused():
         PagedLM(model(layers=1, head_dim=12), 4)
     with pytest.raises(ValueError, match="page"):
         PagedLM(model(layers=1), 4, page=24)
+
+
+def test_a_model_of_more_positions_than_its_rotation_has():
+    """`CausalLM` takes such a model and refuses the positions past the rotation's domain; so does `PagedLM`."""
+    lm = model(layers=1, max_positions=20000)
+    served = PagedLM(lm, 600, page=16, cache="float32")
+    a = served.open()
+    ids = np.arange(30, dtype=np.int32)
+    row, want = served.feed([a], [ids])[0], torch.from_numpy(lm.forward(ids[None])[0, -1]).cuda()
+    assert float((row - want).norm() / want.norm()) <= 2e-5
+    for n in (8192 - 30 + 1, 9000):
+        with pytest.raises(ValueError, match="absolute position"):
+            served.feed([a], [np.zeros(n, dtype=np.int32)])
+    assert served.length(a) == 30
+    served.feed([a], [np.zeros(8192 - 30, dtype=np.int32)])
+    lm.check_status()
+    stretched = PagedLM(model(layers=1, max_positions=20000, rope_scaling={"rope_type": "linear", "factor": 2.0}), 1200, page=16)
+    b = stretched.open()
+    stretched.feed([b], [np.zeros(9000, dtype=np.int32)])
+    stretched.lm.check_status()
+    with pytest.raises(ValueError, match="absolute position"):
+        stretched.feed([b], [np.zeros(16384 - 9000 + 1, dtype=np.int32)])
