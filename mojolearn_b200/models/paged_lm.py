@@ -17,6 +17,12 @@ from ..transformer import NORM_KINDS, _stream, _vp, add, add_norm, norm
 CACHES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
 
+def _integers(x):
+    if x.dtype.kind not in "iu":
+        raise TypeError("token ids must be integers")
+    return x.astype(np.int32)
+
+
 class PagedLM(object):
     def __init__(self, lm, n_pages, *, page=64, cache="bfloat16"):
         """`lm`: a CausalLM on one device. `n_pages` pages of `page` positions for each of its layers."""
@@ -47,7 +53,7 @@ class PagedLM(object):
         A call that fails leaves the sequences as they were."""
         lm = self.lm
         sequences = list(sequences)
-        ids = [np.asarray(x, dtype=np.int32).reshape(-1) for x in ids]
+        ids = [np.asarray(x).reshape(-1) for x in ids]
         counts = [x.size for x in ids]
         if len(ids) != len(sequences) or not ids or min(counts) < 1:
             raise ValueError("feed takes at least one token for each sequence")
@@ -56,6 +62,7 @@ class PagedLM(object):
             raise ValueError("absolute position %d is at or beyond max_positions %d" % (longest - 1, self.positions))
         if lm.pos_table is not None and longest > lm.pos_table.shape[0]:
             raise ValueError("position table of %d rows is too short" % lm.pos_table.shape[0])
+        ids = [_integers(x) for x in ids]
         before = [self.cache.length[s] for s in sequences]
         tables = self.cache.extend(sequences, counts)
         try:
@@ -91,9 +98,10 @@ class PagedLM(object):
     def generate(self, prompts, max_new_tokens, chunk=512):
         """Greedy continuations of prompts of any lengths: a list of int32 arrays, prompt and continuation. Prompts are fed `chunk` tokens
         at a time, and sequences whose prompt is through go on one token a call beside them."""
-        prompts = [np.asarray(p, dtype=np.int32).reshape(-1) for p in prompts]
+        prompts = [np.asarray(p).reshape(-1) for p in prompts]
         if not prompts or min(p.size for p in prompts) < 1:
             raise ValueError("a prompt has at least one token")
+        prompts = [_integers(p) for p in prompts]
         names = [self.open() for _ in prompts]
         try:
             out = [list(p) for p in prompts]

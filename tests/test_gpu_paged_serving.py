@@ -96,3 +96,16 @@ def test_a_model_of_more_positions_than_its_rotation_has():
     stretched.lm.check_status()
     with pytest.raises(ValueError, match="absolute position"):
         stretched.feed([b], [np.zeros(16384 - 9000 + 1, dtype=np.int32)])
+
+
+def test_ids_that_are_no_integers():
+    lm = model(layers=1)
+    served = PagedLM(lm, 8, page=16)
+    a = served.open()
+    for ids in (np.array([1.5, 2.0]), [0.5], np.array([True])):
+        with pytest.raises(TypeError, match="integers"):
+            served.feed([a], [ids])
+        with pytest.raises(TypeError, match="integers"):
+            served.generate([ids], 2)
+    assert served.length(a) == 0 and len(served.cache.free) == 8
+    assert torch.equal(served.feed([a], [[1, 2]]), served.feed([served.open()], [np.array([1, 2], dtype=np.int64)]))
