@@ -444,7 +444,7 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
                            const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
                            int64_t pages, int64_t page, int64_t max_pages, char *err, int64_t err_cap);
 
-/* out [rows, n_heads, head_dim] in the row type: softmax over the keys a row sees of scale * q.k (capped to
+/* out [rows, n_heads, head_dim] in the row type, not over q: softmax over the keys a row sees of scale * q.k (capped to
  * softcap * tanh(z / softcap) where softcap > 0), times the values. A row at position p sees the positions up to p and, where
  * window > 0, after p - window; one that sees none is zero (one whose scores are all -infinity has no softmax: NaN). What stands in
  * positions that a row does not see, or past a sequence's length, has no influence on it. max_new and max_length bound the

@@ -19,6 +19,13 @@ constexpr int64_t MOST = 0x7FFFFFFF;
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// Whether `bytes` from `at` on meet one of the rows of `width` bytes, `pitch` apart, from `row` on.
+bool meets_rows(const void *at, long long bytes, const void *row, long long width, long long pitch, long long rows) {
+    const long long off = (long long)reinterpret_cast<uintptr_t>(at) - (long long)reinterpret_cast<uintptr_t>(row); // of the region from the first row
+    const long long first = off < width ? 0 : (off - width) / pitch + 1;                                            // the first row that ends behind its beginning
+    return first < rows && first * pitch < off + bytes;
+}
+
 // What both calls check, and the part of the arguments that they share. `who` names the call in messages.
 int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cache_type, const void *page_table, const void *cu, const void *lengths, int64_t rows,
                     int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t pages, int64_t page, int64_t max_pages, char *err, int64_t err_cap) {
@@ -129,6 +136,9 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     if (!out || !q || !k_cache || !v_cache) return refuse(err, err_cap, "paged_attention: null storage");
     if (!aligned16(out) || !aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !rows_fit(ldq, n_heads * head_dim, row_type))
         return refuse(err, err_cap, "paged_attention: rows must start on 16-byte boundaries and hold their heads side by side");
+    const long long row_bytes = n_heads * head_dim * (row_type == B200I_T_F32 ? 4 : 2);
+    if (meets_rows(out, rows * row_bytes, q, row_bytes, ldq * (row_type == B200I_T_F32 ? 4 : 2), rows))
+        return refuse(err, err_cap, "paged_attention: the output may not lie over the queries, which may be read again");
     if (max_new <= 0 || max_length <= 0) return refuse(err, err_cap, "paged_attention: the bounds on new tokens and lengths must be positive");
     if (window < 0 || !(softcap >= 0.0) || softcap > 1e30 || !(scale > -1e30 && scale < 1e30)) return refuse(err, err_cap, "paged_attention: window, softcap or scale is out of range");
     if (ws_bytes < 0 || (ws_bytes > 0 && !ws)) return refuse(err, err_cap, "paged_attention: a workspace size without a workspace");

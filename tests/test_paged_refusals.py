@@ -8,7 +8,7 @@ from mojolearn_b200 import _native
 PLACE = ctypes.c_void_p(1 << 20)  # never read: the calls are refused first
 
 
-def attend(out=PLACE, q=PLACE, ldq=256, rows=2, ws=None, ws_bytes=0, window=0, softcap=0.0, scale=0.1):
+def attend(out=ctypes.c_void_p(1 << 22), q=PLACE, ldq=256, rows=2, ws=None, ws_bytes=0, window=0, softcap=0.0, scale=0.1):
     buf = ctypes.create_string_buffer(256)
     status = _native.lib().b200i_paged_attention(-1, None, out, q, ldq, PLACE, PLACE, 0, 1, PLACE, PLACE, PLACE, rows, 1, 4, 2, 64, 3, 16, 2, 2, 32, scale, window, softcap, ws, ws_bytes,
                                                  ctypes.cast(buf, ctypes.c_void_p), 256)
@@ -19,3 +19,16 @@ def attend(out=PLACE, q=PLACE, ldq=256, rows=2, ws=None, ws_bytes=0, window=0, s
 def test_a_workspace_between_16_byte_boundaries(off):
     status, message = attend(ws=ctypes.c_void_p((1 << 21) + off), ws_bytes=1 << 20)
     assert status == 1 and b"workspace" in message and b"16-byte" in message
+
+
+@pytest.mark.parametrize("out,q,ldq,rows", [(0, 0, 256, 2), (1024, 0, 256, 2), (2032, 0, 256, 2), (0, 2032, 256, 2), (2048, 4096, 1024, 3), (4096, 0, 1024, 3)])
+def test_an_output_over_the_queries(out, q, ldq, rows):
+    """A row that does not come out finite is done again from its query, so that has to be there still."""
+    status, message = attend(out=ctypes.c_void_p((1 << 20) + out), q=ctypes.c_void_p((1 << 20) + q), ldq=ldq, rows=rows)
+    assert status == 1 and b"output" in message and b"queries" in message
+
+
+@pytest.mark.parametrize("out,q,ldq,rows", [(2048, 0, 256, 2), (0, 2048, 256, 2), (1024, 0, 2048, 2), (5120, 4096, 1024, 3)])
+def test_an_output_beside_the_queries(out, q, ldq, rows):
+    """Column blocks of one matrix, and rows one after another: whatever refuses this call, it is not that."""
+    assert b"queries" not in attend(out=ctypes.c_void_p((1 << 20) + out), q=ctypes.c_void_p((1 << 20) + q), ldq=ldq, rows=rows, ws=PLACE, ws_bytes=8)[1]
