@@ -433,10 +433,11 @@ int64_t b200i_launch_count(void);
 
 /* Rows q [rows, n_heads * head_dim], k and v [rows, n_kv * head_dim] with row pitches ldq, ldk, ldv in elements (column blocks
  * of a fused product), starting on 16-byte boundaries. q_out [rows, n_heads * head_dim] receives the rotated queries in the row
- * type, the caches the rotated keys and the values in theirs. q_norm, k_norm (float32 [head_dim], may be NULL): an RMSNorm
- * over each head's vector before the rotation, norm_kind 0 with weight w, 2 with 1 + w. cosv, sinv (float32
- * [positions, rope_dim / 2], both NULL = no rotation): row p is position p's, and a new token at a position from
- * `positions` on sets the status word to 15 and has nothing written for it; rope_dim as in b200i_qkv_rope_cache (0 = head_dim). */
+ * type, the caches the rotated keys and the values in theirs; q_out may be q itself where that has no wider pitch, and lies over no
+ * other rows. q_norm, k_norm (float32 [head_dim], may be NULL): an RMSNorm over each head's vector before the rotation, norm_kind 0
+ * with weight w, 2 with 1 + w. cosv, sinv (float32 [positions, rope_dim / 2], both NULL = no rotation): row p is position p's, and a
+ * new token at a position from `positions` on sets the status word to 15 and has nothing written for it; rope_dim as in
+ * b200i_qkv_rope_cache (0 = head_dim). */
 int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_cache, void *v_cache, const void *q, const void *k,
                            const void *v, int64_t ldq, int64_t ldk, int64_t ldv, int64_t row_type, int64_t cache_type,
                            const float *cosv, const float *sinv, int64_t rope_dim, int64_t positions, const float *q_norm,

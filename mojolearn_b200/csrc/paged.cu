@@ -97,6 +97,11 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
     if (!aligned16(q_out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
         !rows_fit(ldq, n_heads * head_dim, row_type) || !rows_fit(ldk, n_kv * head_dim, row_type) || !rows_fit(ldv, n_kv * head_dim, row_type))
         return refuse(err, err_cap, "paged_append: rows must start on 16-byte boundaries and hold their heads side by side");
+    const long long es = row_type == B200I_T_F32 ? 4 : 2, q_bytes = n_heads * head_dim * es, kv_bytes = n_kv * head_dim * es;
+    const bool in_place = q_out == q && (ldq == n_heads * head_dim || rows == 1); // a head's words are read and written by one warp
+    if ((!in_place && meets_rows(q_out, rows * q_bytes, q, q_bytes, ldq * es, rows)) || meets_rows(q_out, rows * q_bytes, k, kv_bytes, ldk * es, rows) ||
+        meets_rows(q_out, rows * q_bytes, v, kv_bytes, ldv * es, rows))
+        return refuse(err, err_cap, "paged_append: the output lies over rows that are read, other than queries in their very place");
     if ((cosv == nullptr) != (sinv == nullptr)) return refuse(err, err_cap, "paged_append: cos without sin, or sin without cos");
     if (rope_dim == 0 || !cosv) rope_dim = head_dim;
     if (rope_dim < 0 || rope_dim > head_dim || rope_dim % 2 != 0) return refuse(err, err_cap, "paged_append: rope_dim %lld does not fit head_dim %lld", (long long)rope_dim, (long long)head_dim);

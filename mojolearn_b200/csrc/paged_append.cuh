@@ -224,7 +224,11 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
     if (!append_place<RT, CT>(a, t, b, pos, part, head, &dst_row, &dst_cache)) return;
     const int half = a.rope_dim / 2;
     const long long row = (long long)max(pos, 0) * half;
-    for (int i = lane; i < a.c.hd; i += 32) {
+    float out[PAGED_MAX_HD / 32];
+#pragma unroll
+    for (int k = 0; k < PAGED_MAX_HD / 32; k++) {
+        const int i = lane + 32 * k;
+        if (i >= a.c.hd) break;
         float x = paged_read(src + i);
         if (w) x = x * r * (w[i] + a.norm_shift);
         if (part < 2 && a.cosv && i < a.rope_dim) {
@@ -234,10 +238,17 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
             const float c = a.cosv[row + j], sn = a.sinv[row + j];
             x = i < half ? fmaf(x, c, -(y * sn)) : fmaf(x, c, y * sn);
         }
+        out[k] = x;
+    }
+    __syncwarp(); // all is read before any of it is written: the queries may be rotated in their place
+#pragma unroll
+    for (int k = 0; k < PAGED_MAX_HD / 32; k++) {
+        const int i = lane + 32 * k;
+        if (i >= a.c.hd) break;
         if (dst_row)
-            paged_write(dst_row + i, x);
+            paged_write(dst_row + i, out[k]);
         else
-            paged_write(dst_cache + i, x);
+            paged_write(dst_cache + i, out[k]);
     }
 }
 

@@ -109,3 +109,15 @@ def test_a_lazily_copied_cache_is_written_alone():
     paged.append(c.q, c.k, c.v, k, v, *c.args())
     assert torch.equal(c.k_cache, kb) and torch.equal(c.v_cache, vb)
     assert not torch.equal(k, kb) and not torch.equal(v, vb)
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("heads,hd,half", [(4, 72, 36), (4, 64, 32), (5, 128, 3)])
+def test_queries_rotated_in_their_place(rows, cache, heads, hd, half):
+    c = Case([1, 20], [30, 25], heads, 1, hd, 16, rows, cache)
+    cos, sin = tables(60, half)
+    q, want = c.q.contiguous(), paged.append(c.q, c.k, c.v, c.k_cache, c.v_cache, *c.args(), cos, sin)
+    kb, vb = c.k_cache.clone(), c.v_cache.clone()
+    assert paged.append(q, c.k, c.v, c.k_cache, c.v_cache, *c.args(), cos, sin, out=q) is q
+    assert torch.equal(q, want) and torch.equal(c.k_cache, kb) and torch.equal(c.v_cache, vb)
+    torch_ops.check_status()

@@ -32,3 +32,23 @@ def test_an_output_over_the_queries(out, q, ldq, rows):
 def test_an_output_beside_the_queries(out, q, ldq, rows):
     """Column blocks of one matrix, and rows one after another: whatever refuses this call, it is not that."""
     assert b"queries" not in attend(out=ctypes.c_void_p((1 << 20) + out), q=ctypes.c_void_p((1 << 20) + q), ldq=ldq, rows=rows, ws=PLACE, ws_bytes=8)[1]
+
+
+def append(out, q=1 << 20, k=1 << 21, v=1 << 22, ldq=256):
+    buf = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p
+    # norm kind 7 is refused, before the device and after the places
+    status = _native.lib().b200i_paged_append(-1, None, p(out), PLACE, PLACE, p(q), p(k), p(v), ldq, 128, 128, 0, 1, None, None, 0, 0, None, None, 1e-6, 7, PLACE, PLACE, PLACE, 2, 1, 4, 2, 64,
+                                              3, 16, 2, ctypes.cast(buf, ctypes.c_void_p), 256)
+    assert status == 1
+    return buf.value
+
+
+@pytest.mark.parametrize("out,ldq", [((1 << 20) + 1024, 256), ((1 << 20) - 16, 256), (1 << 20, 512), (1 << 21, 256), ((1 << 22) + 512, 256)])
+def test_rotated_queries_over_rows_that_are_read(out, ldq):
+    assert b"output" in append(out, ldq=ldq)
+
+
+def test_rotated_queries_beside_the_rows_or_in_their_place():
+    for out in (1 << 23, 1 << 20, (1 << 20) + 2048, (1 << 21) + 1024):
+        assert b"norm kind" in append(out)
