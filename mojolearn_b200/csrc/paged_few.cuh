@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
 // and HDP / 32 columns of its output. blockIdx.x: the block that began the item; blockIdx.y: the row. What it costs is the way there: code that
 // is fetched from L2, and a chain of loads.
 template <typename RT, typename CT, int HDP, int ROWS>
-__global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant__ FewCall f) {
+__global__ void __launch_bounds__(256, 4) attend_join_kernel(const __grid_constant__ FewCall f) {
     constexpr int N = HDP / 32;
     __shared__ float met[8][HDP];
     const AttendCall &a = f.a;
@@ -877,7 +877,25 @@ __global__ void __launch_bounds__(256) attend_join_kernel(const __grid_constant_
         y *= l != 0.0f ? __frcp_rn(l) : paged_share(l, s.pos0 + token);
         paged_write(static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd + col, y);
     }
-    if (__syncthreads_or(!(y * 0.0f == 0.0f)) && warp == 0) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
+    if (!__syncthreads_or(!(y * 0.0f == 0.0f))) return;
+    // done again, an eighth of its keys a warp
+    __shared__ float again[8][2];
+    const int pos = s.pos0 + token, begin = attend_begin(a, pos), end = attend_end(pos, s.length), step = (max(end - begin, 0) + 255) / 256 * 32;
+    const RowSums sums = attend_keys_plain<RT, CT>(a, b, s.first + token, h, begin + warp * step, min(begin + (warp + 1) * step, end));
+    if (lane == 0) again[warp][0] = sums.m, again[warp][1] = sums.l;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (4 * lane + k < HDP) met[warp][4 * lane + k] = sums.o[k];
+    __syncthreads();
+    if (col >= a.c.hd) return;
+    top = again[0][0];
+    for (int w = 1; w < 8; w++) top = fmaxf(top, again[w][0]);
+    l = y = 0.0f;
+    for (int w = 0; w < 8; w++) {
+        const float keep = again[w][0] == -INFINITY ? 0.0f : paged_exp2((again[w][0] - top) * PAGED_LOG2E);
+        l = fmaf(again[w][1], keep, l), y = fmaf(met[w][col], keep, y);
+    }
+    paged_write(static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + h) * a.c.hd + col, l != 0.0f ? y / l : paged_share(l, pos));
 }
 
 // ---- host side ----

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         pg_bar_init(stage_empty, 128);
         pg_bar_init(done, 1);
         dead = 0;
-        f.head[blockIdx.x * 8] = -1;
+        f.head[blockIdx.x * 8] = -1, f.head[blockIdx.x * 8 + 6] = 0x7FFFFFFF, f.head[blockIdx.x * 8 + 7] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 8) {
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 int *head = f.head + blockIdx.x * 8;
                 head[0] = w.b, head[1] = w.kvh, head[2] = w.block, head[3] = item.steps, head[4] = w.line, head[5] = (int)line.per;
             }
-            const int b = w.b, kvh = w.kvh;
+            const int kvh = w.kvh;
             w.next(a);
             if (w.left > 0) queries(w.item(a, paged_seq(a.c, w.b)).rows); // the scores that read the last ones are done: the next item's begin under what follows
             take(tile_count - 1);
@@ -475,14 +475,10 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             float odd0, odd1;
             pg_one(odd, odd0, odd1);
             unsigned rest = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
-            if (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
-                asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); // what is there is written over
-                __syncwarp();
-                while (rest) {
-                    const int k = __ffs(rest) - 1, token = __shfl_sync(0xFFFFFFFFu, place.x, k), head = __shfl_sync(0xFFFFFFFFu, place.y, k);
-                    rest &= rest - 1;
-                    attend_row_plain<float, CT>(a, b, s.first + token, s.pos0 + token, s.length, kvh * a.c.group + head);
-                }
+            while (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
+                const int k = __ffs(rest) - 1, token = __shfl_sync(0xFFFFFFFFu, place.x, k), head = __shfl_sync(0xFFFFFFFFu, place.y, k);
+                rest &= rest - 1;
+                many_mark(f.head + blockIdx.x * 8 + 6, (s.first + token) * a.c.heads + kvh * a.c.group + head);
             }
             first_part = false;
         }
@@ -511,9 +507,7 @@ cudaError_t launch_fine_as(const AttendCall &a, const ManyPlan &p, void *ws, int
         if (device < 64) known[device].store(true);
     }
     attend_fine_kernel<CT, HDP><<<p.blocks, FINE_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    *launches += 2;
-    const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? e : launch_following<ManyCall>(attend_join_rows_kernel<float, CT, HDP, FINE_ROWS>, dim3(p.blocks, FINE_ROWS / 32), 256, st, f);
+    return many_after<float, CT, HDP, FINE_ROWS, FINE_KEYS, 1>(f, p.blocks, st, launches);
 }
 
 } // namespace b200i

@@ -311,8 +311,11 @@ __device__ __forceinline__ float many_weights(const AttendCall &a, unsigned s_at
 struct ManyCall {
     AttendCall a;
     float *part; // [blocks][2][BLOCK_ROWS][HDP], then [blocks][2][2][BLOCK_ROWS] of m and l
-    int *head;   // [blocks][8]: sequence (or -1), key head, block of rows, steps, steps of the block before it, steps a block
+    int *head;   // [blocks][8]: sequence (or -1), key head, block of rows, steps, steps of the block before it, steps a block, the first and the last row that did not come out finite
 };
+
+// A row did not come out finite: it is done again by attend_again_kernel.
+__device__ __noinline__ void many_mark(int *at, int row) { atomicMin(at, row), atomicMax(at + 1, row); } // rows and heads of the output, one after another
 
 // 16 columns of an output that is there, or zeros.
 __device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some) {
@@ -322,19 +325,6 @@ __device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some)
     } else {
 #pragma unroll
         for (int i = 0; i < 16; i++) o[i] = 0;
-    }
-}
-
-// An item's rows whose bits are set, done again: dealt out to the sixteen softmax warps.
-template <typename T, int BR, int KEYS, int STREAMS>
-__device__ __noinline__ void many_again(const AttendCall &a, const unsigned *bad, int b, int kvh, int block) {
-    const PagedSeq s = paged_seq(a.c, b);
-    const ManyItem item = many_item<BR, KEYS, STREAMS>(a, s, min(s.n, a.max_new), block);
-    int number = 0;
-    for (int row = 0; row < item.rows; row++) {
-        if (!(bad[row / 32] >> (row % 32) & 1u) || (number++ & 15) != (threadIdx.x >> 5)) continue;
-        const int2 at = many_row(a, item, row);
-        attend_row_plain<T, T>(a, b, s.first + at.x, s.pos0 + at.x, s.length, kvh * a.c.group + at.y);
     }
 }
 
@@ -351,7 +341,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     __shared__ float stats[2][2][128], half_stat[3][2][2][128]; // m and l of a stream's rows; what the two threads of a row tell each other
     __shared__ long long place[32];
     __shared__ unsigned long long pair_bars[8];
-    __shared__ uint4 bad[2][2]; // rows that did not come out finite, a bit each: of this item and of the one before
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
     const AttendCall &a = f.a;
@@ -371,7 +360,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
         pg_bar_init(tail, 1);
         pg_bar_init(done, 1);
         dead = 0;
-        f.head[blockIdx.x * 8] = -1;
+        f.head[blockIdx.x * 8] = -1, f.head[blockIdx.x * 8 + 6] = 0x7FFFFFFF, f.head[blockIdx.x * 8 + 7] = -1;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 17) {
@@ -581,7 +570,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                         *reinterpret_cast<uint4 *>(query + tile * TILE + (chunk >> 3) * HALF_COLS + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) =
                             make_uint4(x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip);
                 }
-                if (tid < 2) bad[items & 1u][tid] = make_uint4(0, 0, 0, 0); // before the queries are there, so before any row of this item is finished
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 pg_bar_arrive(q_full);
             }
@@ -738,15 +726,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
             }
             float odd0, odd1;
             pg_one(odd, odd0, odd1);
-            // A masked key's zero weight met a value that is not finite, or the weights left their range: the row is done again, by one warp, and not
-            // before all threads of the row have stored: each sees its own columns only.
-            const unsigned odd_rows = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
-            if (odd_rows && lane == 0) atomicOr(reinterpret_cast<unsigned *>(bad[items & 1u]) + mine / 32, odd_rows);
+            // a masked key's zero weight met a value that is not finite, or the weights left their range: the row is done again after this kernel
+            if (store && is_whole && !(odd0 + odd1 == 0.0f)) many_mark(f.head + blockIdx.x * 8 + 6, (s.first + place.x) * a.c.heads + w.kvh * a.c.group + place.y);
             pg_fence_before();
-            asm volatile("bar.sync 9, 512;" ::: "memory"); // `query` and the statistics are read, and the rows stored
-            const uint4 some_bad = bad[items & 1u][0], more_bad = bad[items & 1u][1];
-            if (some_bad.x | some_bad.y | some_bad.z | some_bad.w | more_bad.x | more_bad.y | more_bad.z | more_bad.w)
-                many_again<T, BR, MANY_KEYS, 2>(a, reinterpret_cast<const unsigned *>(bad[items & 1u]), w.b, w.kvh, w.block);
+            asm volatile("bar.sync 9, 512;" ::: "memory"); // `query` and the statistics are read
             items++;
             w.next(a);
         }
@@ -757,14 +740,14 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
 }
 
 // The parts of an item that several blocks share, in the order of its keys: a warp four rows, a lane the statistics of a part and HDP / 32 columns.
-// blockIdx.x: the block that began the item.
+// blockIdx.x: the block that began the item; blockIdx.y: 32 rows of it.
 template <typename RT, typename CT, int HDP, int BR>
 __global__ void __launch_bounds__(256) attend_join_rows_kernel(const __grid_constant__ ManyCall f) {
     constexpr int ROWS = 4, N = HDP / 32;
     const AttendCall &a = f.a;
     const int c0 = blockIdx.x, lane = threadIdx.x & 31, mine = (blockIdx.y * 8 + (threadIdx.x >> 5)) * ROWS;
     pg_follow();
-    const int *head = f.head + c0 * 8;
+    int *head = f.head + c0 * 8;
     const int b = head[0], kvh = head[1], block = head[2], count = head[3], from = head[4], per = head[5];
     if (b < 0) return;
     const PagedSeq s = paged_seq(a.c, b);
@@ -847,9 +830,37 @@ __global__ void __launch_bounds__(256) attend_join_rows_kernel(const __grid_cons
             else
                 *reinterpret_cast<float2 *>(out) = make_float2(o[r][0], o[r][1]);
         }
-        const bool again = __any_sync(0xFFFFFFFFu, mine_columns && !(odd == 0.0f));
-        __syncwarp(); // the row's words are stored, in this order, by other lanes too
-        if (again) attend_row_plain<RT, CT>(a, b, s.first + token, s.pos0 + token, s.length, h);
+        if (mine_columns && !(odd == 0.0f)) many_mark(head + 6, (s.first + token) * a.c.heads + h);
+    }
+}
+
+// The rows that did not come out finite, done again: of each block's items, whose way along the line is gone once more, those between the first and the
+// last that were marked are looked at. A kernel by itself: in the one that makes the parts the other warps' waits (about a second at most) ran while
+// rows were done again, and its registers would be this one's. Where no row is marked it costs 2 to 6 us of a call.
+// blockIdx.x: the block whose items these are; blockIdx.y: eight rows of them, by steps of 8 gridDim.y.
+template <typename RT, typename CT, int BR, int KEYS, int STREAMS>
+__global__ void __launch_bounds__(256) attend_again_kernel(const __grid_constant__ ManyCall f) {
+    using Walk = ManyWalk<BR, KEYS, STREAMS>;
+    __shared__ long long place[32];
+    const AttendCall &a = f.a;
+    const int lane = threadIdx.x & 31;
+    pg_follow();
+    const int first = f.head[blockIdx.x * 8 + 6], last = f.head[blockIdx.x * 8 + 7];
+    if (last < first) return;
+    const LinePlace line = line_place(a.c, [&](int b) { return Walk::steps_of(a, b); }, blockIdx.x, gridDim.x, place);
+    Walk w;
+    for (w.begin(a, line); w.left > 0; w.next(a)) {
+        const PagedSeq s = paged_seq(a.c, w.b);
+        if (w.skip > 0 || (s.first + s.n) * a.c.heads <= first || s.first * a.c.heads > last) continue; // another block began it, or none of its rows is marked
+        const ManyItem item = w.item(a, s);
+        for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < item.rows; r += gridDim.y * 8) {
+            const int2 at = many_row(a, item, r);
+            const int h = w.kvh * a.c.group + at.y;
+            const RT *out = static_cast<const RT *>(a.out) + ((long long)(s.first + at.x) * a.c.heads + h) * a.c.hd;
+            bool odd = false;
+            for (int c = lane; c < a.c.hd; c += 32) odd |= !(paged_read(out + c) * 0.0f == 0.0f);
+            if (__any_sync(0xFFFFFFFFu, odd)) attend_row_plain<RT, CT>(a, w.b, s.first + at.x, s.pos0 + at.x, s.length, h);
+        }
     }
 }
 
@@ -864,6 +875,15 @@ inline ManyPlan many_plan(int sms, int block_rows, int hdp) {
     p.part_floats = (long long)p.blocks * 2 * block_rows * (hdp + 2);
     p.bytes = p.part_floats * 4 + (long long)p.blocks * 32;
     return p;
+}
+
+// What follows the kernel that makes the parts.
+template <typename RT, typename CT, int HDP, int BR, int KEYS, int STREAMS>
+cudaError_t many_after(const ManyCall &f, int blocks, cudaStream_t st, int *launches) {
+    *launches += 3;
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = launch_following<ManyCall>(attend_join_rows_kernel<RT, CT, HDP, BR>, dim3(blocks, BR / 32), 256, st, f);
+    return e != cudaSuccess ? e : launch_following<ManyCall>(attend_again_kernel<RT, CT, BR, KEYS, STREAMS>, dim3(blocks, 8), 256, st, f);
 }
 
 template <int HDP>
@@ -882,9 +902,7 @@ cudaError_t launch_many_as(const AttendCall &a, const ManyPlan &p, void *ws, int
         if (device < 64) known[device].store(true);
     }
     attend_many_kernel<HDP><<<p.blocks, MANY_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    *launches += 2;
-    const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? e : launch_following<ManyCall>(attend_join_rows_kernel<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS>, dim3(p.blocks, Shape::BLOCK_ROWS / 32), 256, st, f);
+    return many_after<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS, MANY_KEYS, 2>(f, p.blocks, st, launches);
 }
 
 } // namespace b200i

@@ -1,8 +1,8 @@
-"""Attention of many bfloat16 rows where the largest score keeps growing, so that the running output is multiplied tile after tile."""
+"""Attention where a row's output is multiplied tile after tile, and where rows do not come out finite and are done again."""
 import pytest
 import torch
 
-from paged_ref import BF16, Case, check
+from paged_ref import BF16, TYPES, Case, check
 
 pytestmark = pytest.mark.gpu
 if torch.cuda.is_available():
@@ -51,3 +51,26 @@ def test_a_row_done_again_is_written_after_its_other_words(new, past, column):
     for _ in range(20):
         assert torch.equal(call().view(torch.int16), got.view(torch.int16))
     torch_ops.check_status()
+
+
+@pytest.mark.parametrize("rows,cache", TYPES)
+@pytest.mark.parametrize("new,past", [(1, 131000), (5, 30000), (300, 9000), (40, 60000)])
+@pytest.mark.parametrize("what", ["value", "key", "masked value"])
+def test_what_is_not_finite_in_a_long_past(rows, cache, new, past, what):
+    """Every row that sees it, or is beside it, is done again over the whole past: right, without a wait that runs out, and in a time that a wait for
+    the others bears (a kernel's waits run out after about a second)."""
+    c = Case([new, 1], [past, 700], 8, 2, 128, 64, rows, cache, seed=new)
+    pos = c.length[0] - 1 if what == "masked value" else 3
+    (c.k_cache if what == "key" else c.v_cache)[int(c.table[0, pos // 64]), :, pos % 64, 9] = float("nan")
+    call = lambda: paged.attention(c.q, c.k_cache, c.v_cache, *c.args(), max_new=new)  # noqa: E731
+    call()
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    begin.record()
+    got = call()
+    end.record()
+    torch_ops.check_status()
+    assert begin.elapsed_time(end) < 250.0
+    want = c.attention()
+    seen = torch.isnan(want)
+    assert torch.equal(torch.isnan(got), seen) and int(seen.any(-1).sum()) == (8 if what == "masked value" else 8 * new)
+    check(torch.where(seen, torch.zeros_like(got), got), torch.where(seen, 0.0, want), rows, 6.0)
