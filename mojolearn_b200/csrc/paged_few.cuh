@@ -16,8 +16,8 @@
 // and the kernel waits for memory. A weight goes in as two bfloat16 pieces, so that the output's own rounding is the only one of 8 bits.
 // float32 rows (attend_few_fma_kernel): two or four lanes a key for the scores, a lane four columns for the values, in fused multiply-adds. Products of
 // three bfloat16 pieces on the tensor cores took 5000 cycles for 16 keys of a float32 cache, of which splitting was most.
-// Measured, kernel and join, of the HBM rate: 32 sequences of 1216 to 1279 float32 keys, 16 heads, 109 us (0.92); 64 of 91 to 8192 bfloat16 keys, 32
-// heads on 8, 200 us (0.87); one of 131000, 95 us (0.87); one of 200 keys 8.4 us a call.
+// Measured, kernel and join, of the HBM rate: 32 sequences of 1216 to 1279 float32 keys, 16 heads, 111 us (0.90); 64 of 91 to 8192 bfloat16 keys, 32
+// heads on 8, 202 us (0.86); one of 131000, 95 us (0.87); one of 200 keys 8.5 us a call.
 #pragma once
 #include <algorithm>
 #include <atomic>

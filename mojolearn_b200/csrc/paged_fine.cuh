@@ -14,7 +14,8 @@
 // A bfloat16 cache comes in by tensor-map copies; of a float32 one four warps read the rows and write their pieces. An item's rows come in by bulk
 // copies while the item before is worked on, are cut into pieces as soon as that one's last score is made, and its output goes out by bulk copies
 // from the same place: rows read and written by their threads, 512 bytes apart, had taken 16000 of 35000 cycles of an item of 1024 keys.
-// Measured: 4 prompts of 1024 tokens, 16 heads of 128: 130 us on a bfloat16 cache, 214 on a float32 one (32 and 64 at the tensor rate of their products):
+// Measured, with what follows it: 4 prompts of 1024 tokens, 16 heads of 128: 142 us on a bfloat16 cache, 223 on a float32 one (32 and 64 at the tensor rate
+// of their products):
 // the issuing thread waits, three barriers between two products, and a product of 64 columns takes 45 cycles, not 32.
 #pragma once
 #include "paged_many.cuh"
@@ -475,7 +476,9 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             float odd0, odd1;
             pg_one(odd, odd0, odd1);
             unsigned rest = __ballot_sync(0xFFFFFFFFu, store && is_whole && !(odd0 + odd1 == 0.0f));
-            while (rest) { // a masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range
+            // A masked key's zero weight met a value that is not finite, or a 32-bit word left bfloat16's range: the row is done again after this kernel. Row by
+            // row with its place: where a thread only stores a word, the compiler's code for the softmax of float32 caches takes 293 us for 222.
+            while (rest) {
                 const int k = __ffs(rest) - 1, token = __shfl_sync(0xFFFFFFFFu, place.x, k), head = __shfl_sync(0xFFFFFFFFu, place.y, k);
                 rest &= rest - 1;
                 many_mark(f.head + blockIdx.x * 8 + 6, (s.first + token) * a.c.heads + kvh * a.c.group + head);

@@ -15,8 +15,8 @@
 // exchanged between their reading and P. S of the next tile is signalled after the products before it are done, and this tile's products begin
 // when the first half of P has been stored AND both halves of O have been multiplied, so O stands still while it is.
 // Work is cut as in paged_few.cuh: all items' steps on one line, an equal piece a block, parts joined by attend_join_rows_kernel.
-// Measured: 2048 tokens behind 14336, 32 heads on 8 of 128, 569 us (908 TFLOP/s of 1627, at 990 of 1000 W); each stream's score, softmax and sum
-// follow one another, and two streams fill the tensor pipe to 0.56. 12 chunks of up to 509 tokens, window 1024, capped, 187 us.
+// Measured, with what follows it: 2048 tokens behind 14336, 32 heads on 8 of 128, 588 us (876 TFLOP/s of 1627, at 990 of 1000 W); each stream's score,
+// softmax and sum follow one another, and two streams fill the tensor pipe to 0.54. 12 chunks of up to 509 tokens, window 1024, capped, 194 us.
 #pragma once
 #include "paged_few.cuh"
 
