@@ -67,7 +67,7 @@ struct AttendPlan {
     int64_t bytes() const { return few ? cut.bytes : cut_many.bytes; }
 };
 
-AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
+AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
     AttendPlan p = {};
     p.hdp = head_dim <= 64 ? 64 : 128;
     const int64_t group = n_heads / n_kv;
@@ -76,7 +76,9 @@ AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t
         p.cut = few_plan(b200i_library::device_sms(device), row_type == B200I_T_F32, cache_type == B200I_T_F32, (int)batch, (int)n_kv, p.hdp, p.few, max_new, max_length,
                          (int)std::min(window, MOST));
     } else {
-        p.cut_many = many_plan(b200i_library::device_sms(device), row_type == B200I_T_BF16 ? ManyShape<128>::BLOCK_ROWS : FINE_ROWS, p.hdp);
+        const bool wide = row_type == B200I_T_BF16;
+        p.cut_many = many_plan(b200i_library::device_sms(device), wide ? ManyShape<128>::BLOCK_ROWS : FINE_ROWS, p.hdp, wide ? MANY_KEYS : FINE_KEYS, rows, batch, n_kv, group, max_new,
+                               std::min(max_length, MOST));
     }
     return p;
 }
@@ -129,7 +131,7 @@ int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, 
     if (rows <= 0 || batch <= 0 || n_kv <= 0 || n_heads < n_kv || head_dim <= 0 || max_new <= 0 || max_length <= 0 || window < 0) return 0;
     int dev = (int)device;
     if (device < 0 && cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); dev = -1; }
-    return attend_plan(dev, row_type, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window).bytes();
+    return attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window).bytes();
 }
 
 int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, int64_t row_type, int64_t cache_type,
@@ -163,7 +165,7 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const AttendPlan p = attend_plan(dev, row_type, cache_type, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
+    const AttendPlan p = attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
     if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
     if (p.few) {
         if (row_type == B200I_T_BF16)

@@ -52,3 +52,17 @@ def test_rotated_queries_over_rows_that_are_read(out, ldq):
 def test_rotated_queries_beside_the_rows_or_in_their_place():
     for out in (1 << 23, 1 << 20, (1 << 20) + 2048, (1 << 21) + 1024):
         assert b"norm kind" in append(out)
+
+
+def workspace(rows, batch, max_new, max_length, row_type=1, heads=32, kv=8):
+    return _native.lib().b200i_paged_attention_workspace_bytes(-1, row_type, 1, rows, batch, heads, kv, 128, max_new, max_length, 0)
+
+
+@pytest.mark.parametrize("row_type,block", [(0, 2 * 128 * 130 * 4 + 32), (1, 2 * 256 * 130 * 4 + 32)])
+def test_a_short_call_has_a_short_workspace(row_type, block):
+    """Parts of as many blocks as the call can have steps: 17 tokens over 300 keys, 8 key heads, tiles of 64 or 128 keys."""
+    tiles = -(-300 // (128 if row_type else 64)) + 1
+    assert workspace(17, 1, 17, 300, row_type) == min(148, 8 * tiles) * block
+    assert workspace(5, 1, 5, 1, row_type) == 8 * 2 * block
+    for call in ((2048, 1, 2048, 16384), (4096, 4, 1024, 1024), (17, 1, 17, 1 << 31), (1 << 30, 1, 1 << 30, 1 << 62), (40, 30, 17, 100)):
+        assert workspace(*call, row_type) == 148 * block
