@@ -42,6 +42,7 @@ extern "C" {
 /* types of the paged cache and of the rows that meet it */
 #define B200I_T_F32 0
 #define B200I_T_BF16 1
+#define B200I_T_INT4 2 /* of a paged cache only */
 
 /* --- identity of the loaded binary ---------------------------------------------------
  * Replace linalg_numeric_mode / linalg_profile_version / linalg_numerical_profile /
@@ -429,7 +430,15 @@ int64_t b200i_launch_count(void);
  * Rows past cu[batch] belong to no sequence: nothing is read for them and nothing written. The three arrays are read on
  * the device; a page number outside the pool counts as a page of zeros, is not written, and sets the status word
  * (b200i_decode_status) to 11. A sequence of more than max_pages * page positions, or with offsets that descend or leave 0 .. rows,
- * is left out (nothing is written for its rows) and sets it to 14. Row and cache types: float32 and float32, float32 and bfloat16, bfloat16 and bfloat16. */
+ * is left out (nothing is written for its rows) and sets it to 14. Row and cache types: float32 and float32, float32 and bfloat16, bfloat16 and bfloat16,
+ * and either with a cache in 4 bits.
+ *
+ * A cache in 4 bits (B200I_T_INT4) is [pages, n_kv] runs of page * 18 * groups bytes, groups = ceil(head_dim / 32) being the groups of 32 columns of a head, a last
+ * one filled up with zeros. A run holds the codes of its positions, 16 bytes a group, and then their scales, a bfloat16 word a group. Column c of a group has
+ * the four bits 4 (i / 2) + 16 (i % 2) and up, i = c % 8, of the group's 32-bit word c / 8, and code n of scale s is s (n - 8). Written are n from 1 to 15, and for s the smallest
+ * number of five significant bits with 7 s >= the group's largest magnitude, from 2^-100 to 2^90 (larger words are cut to 7 s); n - 8 is the 64-bit value of the key or value over s to the
+ * nearest, ties to even. The scale of a group with a word that is not finite is NaN. What s (n - 8) is with such a scale is a bfloat16 word; scales of more
+ * significant bits, which are never written, have it rounded. */
 
 /* Rows q [rows, n_heads * head_dim], k and v [rows, n_kv * head_dim] with row pitches ldq, ldk, ldv in elements (column blocks
  * of a fused product), starting on 16-byte boundaries. q_out [rows, n_heads * head_dim] receives the rotated queries in the row
@@ -444,6 +453,14 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
                            const float *k_norm, double eps, int64_t norm_kind, const int32_t *page_table, const int32_t *cu,
                            const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
                            int64_t pages, int64_t page, int64_t max_pages, char *err, int64_t err_cap);
+
+/* Rows read back: k_out and v_out [rows, n_kv, head_dim] in out_type receive what the caches hold at the positions of the rows that cu and lengths name (with cu the running
+ * sums of the lengths, all of each sequence). A row whose position is negative, or whose page is outside the pool, is zeros; one of no sequence is not written. Types as a
+ * row and a cache type. */
+int64_t b200i_paged_read(int64_t device, void *stream, void *k_out, void *v_out, const void *k_cache, const void *v_cache,
+                         int64_t out_type, int64_t cache_type, const int32_t *page_table, const int32_t *cu, const int32_t *lengths,
+                         int64_t rows, int64_t batch, int64_t n_kv, int64_t head_dim, int64_t pages, int64_t page, int64_t max_pages,
+                         char *err, int64_t err_cap);
 
 /* out [rows, n_heads, head_dim] in the row type, not over q: softmax over the keys a row sees of scale * q.k (capped to
  * softcap * tanh(z / softcap) where softcap > 0), times the values. A row at position p sees the positions up to p and, where

@@ -99,6 +99,7 @@ SIGNATURES = {
     "b200i_add_positions_at": [I64, VP, VP, VP, I64, I64, VP, I64, VP, I64],
     "b200i_advance_position": [I64, VP, VP, I64, VP, I64],
     "b200i_paged_append": [I64] + [VP] * 7 + [I64] * 5 + [VP, VP, I64, I64, VP, VP, F64, I64, VP, VP, VP] + [I64] * 8 + [VP, I64],
+    "b200i_paged_read": [I64] + [VP] * 5 + [I64, I64, VP, VP, VP] + [I64] * 7 + [VP, I64],
     "b200i_paged_attention": [I64, VP, VP, VP, I64, VP, VP, I64, I64, VP, VP, VP] + [I64] * 10 + [F64, I64, F64, VP, I64, VP, I64],
     "b200i_paged_attention_workspace_bytes": [I64] * 11,
     "b200i_ffma_probe": [I64, VP, VP, I64, I64, I64, VP, I64],

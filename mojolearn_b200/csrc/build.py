@@ -15,10 +15,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB = os.path.join(HERE, "libb200i.so")
 #: the negative-control build: every window admitted (-DB200I_SABOTAGE_ADMIT_ALWAYS); loaded only by the tests
 SABOTAGE_LIB = os.path.join(HERE, "libb200i_sabotage_admit.so")
-SOURCES = ["b200i.cu", "paged.cu"]
-HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".cuh")) + ["library.h", os.path.join("..", "..", "include", "b200i.h")]
+SOURCES = ["b200i.cu", "paged.cu", "paged_int4.cu"]
+HEADERS = sorted(f for f in os.listdir(HERE) if f.endswith(".cuh")) + ["library.h", "paged_int4.h", os.path.join("..", "..", "include", "b200i.h")]
 #: which headers a source includes: an object is compiled again where one of its own is newer (the paged cache's kernels stand apart)
 OWN_HEADERS = {"paged.cu": [f for f in HEADERS if f.startswith("paged") or not f.endswith(".cuh")],
+               "paged_int4.cu": [f for f in HEADERS if f.startswith("paged") or not f.endswith(".cuh")],
                "b200i.cu": [f for f in HEADERS if not f.startswith("paged")]}
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

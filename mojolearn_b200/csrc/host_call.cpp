@@ -1,5 +1,5 @@
-// The host side of calls on device tensors, in native code: torch_ops.product without bias, activation or `out`, and paged.append and
-// paged.attention.
+// The host side of calls on device tensors, in native code: torch_ops.product without bias, activation or `out`, and paged.append,
+// paged.attention and paged.read.
 //
 // The checks, allocations and argument conversions of a one-row product take 15.5 us of host time a call in Python and ctypes and
 // 6.5 here, on the tensors themselves, with output and workspace from torch's allocator and the C ABI called directly. A loop of
@@ -43,6 +43,9 @@ using AttendNeedFn = int64_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t, in
 AppendFn g_append = nullptr;            // b200i_paged_append
 AttendFn g_attend = nullptr;            // b200i_paged_attention
 AttendNeedFn g_attend_need = nullptr;   // b200i_paged_attention_workspace_bytes
+using ReadFn = int64_t (*)(int64_t, void *, void *, void *, const void *, const void *, int64_t, int64_t, const int32_t *, const int32_t *, const int32_t *, int64_t, int64_t, int64_t,
+                           int64_t, int64_t, int64_t, int64_t, char *, int64_t);
+ReadFn g_read = nullptr;                // b200i_paged_read
 PyObject *g_error = nullptr;  // the package's exception for a refusal
 
 // Workspace sizes by the call's form: a pure function of it and of the device's SM count. Reached with the GIL held; bounded.
@@ -61,12 +64,13 @@ bool plain(PyObject *o, at::Tensor &t, bool contiguous = true) {
 }
 
 PyObject *bind(PyObject *, PyObject *args) {
-    unsigned long long gemm, auto_need, plan_need, append, attend, attend_need;
+    unsigned long long gemm, auto_need, plan_need, append, attend, attend_need, read;
     PyObject *error;
-    if (!PyArg_ParseTuple(args, "KKKKKKO", &gemm, &auto_need, &plan_need, &append, &attend, &attend_need, &error)) return nullptr;
+    if (!PyArg_ParseTuple(args, "KKKKKKKO", &gemm, &auto_need, &plan_need, &append, &attend, &attend_need, &read, &error)) return nullptr;
     g_append = reinterpret_cast<AppendFn>(static_cast<uintptr_t>(append));
     g_attend = reinterpret_cast<AttendFn>(static_cast<uintptr_t>(attend));
     g_attend_need = reinterpret_cast<AttendNeedFn>(static_cast<uintptr_t>(attend_need));
+    g_read = reinterpret_cast<ReadFn>(static_cast<uintptr_t>(read));
     g_gemm = reinterpret_cast<GemmFn>(static_cast<uintptr_t>(gemm));
     g_auto_need = reinterpret_cast<NeedFn>(static_cast<uintptr_t>(auto_need));
     g_plan_need = reinterpret_cast<NeedFn>(static_cast<uintptr_t>(plan_need));
@@ -137,15 +141,17 @@ PyObject *product(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
 
 bool modes() { return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::impl::PythonTorchFunctionTLS::stack_len() > 0; }
 
-// What the two calls share. Each part is false where the call is not a plain one, which the Python path then looks at.
+// What the calls share. Each part is false where the call is not a plain one, which the Python path then looks at.
 struct Pages {
     at::Tensor k, v, table, cu, lengths;
     int64_t batch = 0, pages = 0, kv = 0, page = 0, hd = 0, type = 0;
-    bool read(PyObject *const *args, c10::Device dev) { // k_cache, v_cache, page_table, cu, lengths
+    bool read(PyObject *const *args, c10::Device dev, int64_t head_dim) { // k_cache, v_cache, page_table, cu, lengths; head_dim as the rows have it
         if (!plain(args[0], k) || !plain(args[1], v) || !plain(args[2], table) || !plain(args[3], cu) || !plain(args[4], lengths)) return false;
-        if (k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || (k.scalar_type() != at::kFloat && k.scalar_type() != at::kBFloat16)) return false;
+        const bool four = k.scalar_type() == at::kByte; // 4 bits
+        if (k.dim() != 4 || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || (k.scalar_type() != at::kFloat && k.scalar_type() != at::kBFloat16 && !four)) return false;
+        if (k.size(3) != (four ? (head_dim + 31) / 32 * 18 : head_dim)) return false;
         if (table.scalar_type() != at::kInt || cu.scalar_type() != at::kInt || lengths.scalar_type() != at::kInt || table.dim() != 2 || cu.dim() != 1 || lengths.dim() != 1) return false;
-        batch = lengths.size(0), pages = k.size(0), kv = k.size(1), page = k.size(2), hd = k.size(3), type = k.scalar_type() == at::kBFloat16;
+        batch = lengths.size(0), pages = k.size(0), kv = k.size(1), page = k.size(2), hd = head_dim, type = four ? 2 : k.scalar_type() == at::kBFloat16;
         return table.size(0) == batch && cu.size(0) == batch + 1 && k.device() == dev && v.device() == dev && table.device() == dev && cu.device() == dev && lengths.device() == dev;
     }
 };
@@ -191,7 +197,7 @@ PyObject *paged_append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     if (!plain(args[0], q, false) || q.dim() != 3 || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
     const c10::Device dev = q.device();
     Pages c;
-    if (!c.read(args + 3, dev) || c10::cuda::current_device() != dev.index()) Py_RETURN_NONE;
+    if (!c.read(args + 3, dev, q.size(2)) || c10::cuda::current_device() != dev.index()) Py_RETURN_NONE;
     int64_t heads, kv1, kv2, ldq, ldk, ldv, kind, half = 0, positions = 0;
     double eps;
     const int64_t rows = q.size(0), type = q.scalar_type() == at::kBFloat16;
@@ -229,10 +235,10 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (nargs != 11 || !g_attend || !g_attend_need || modes()) Py_RETURN_NONE;
     at::Tensor q;
-    if (!plain(args[0], q, false) || q.dim() != 3 || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
+    if (!plain(args[0], q, false) || q.dim() != 3 || q.dim() != 3 || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
     const c10::Device dev = q.device();
     Pages c;
-    if (!c.read(args + 1, dev) || c10::cuda::current_device() != dev.index()) Py_RETURN_NONE;
+    if (!c.read(args + 1, dev, q.size(2)) || c10::cuda::current_device() != dev.index()) Py_RETURN_NONE;
     int64_t heads, ldq, max_new, max_length, window;
     double scale, softcap;
     const int64_t rows = q.size(0), type = q.scalar_type() == at::kBFloat16;
@@ -253,10 +259,38 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// paged_read(k_cache, v_cache, page_table, cu, lengths, rows, head_dim, type of the output) -> keys and values, or None
+PyObject *paged_read(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 8 || !g_read || modes()) Py_RETURN_NONE;
+    at::Tensor first;
+    int64_t rows, hd, type;
+    if (!plain(args[0], first) || !integer(args[5], &rows) || !integer(args[6], &hd) || !integer(args[7], &type) || rows <= 0 || hd <= 0 || hd > 128) Py_RETURN_NONE;
+    const c10::Device dev = first.device();
+    Pages c;
+    if (!c.read(args, dev, hd) || c10::cuda::current_device() != dev.index() || type > c.type) Py_RETURN_NONE;
+    const auto options = first.options().requires_grad(false).dtype(type ? at::kBFloat16 : at::kFloat);
+    at::Tensor k = at::empty({rows, c.kv, hd}, options), v = at::empty({rows, c.kv, hd}, options);
+    char message[ERR_CAP] = "";
+    int64_t status;
+    Py_BEGIN_ALLOW_THREADS;
+    status = g_read(dev.index(), c10::cuda::getCurrentCUDAStream(dev.index()).stream(), k.data_ptr(), v.data_ptr(), c.k.const_data_ptr(), c.v.const_data_ptr(), type, c.type,
+                    static_cast<const int32_t *>(c.table.const_data_ptr()), static_cast<const int32_t *>(c.cu.const_data_ptr()), static_cast<const int32_t *>(c.lengths.const_data_ptr()), rows,
+                    c.batch, c.kv, hd, c.pages, c.page, c.table.size(1), message, ERR_CAP);
+    Py_END_ALLOW_THREADS;
+    if (status != 0) return refusal(message, "b200i_paged_read failed");
+    PyObject *of_k = THPVariable_Wrap(std::move(k)), *of_v = of_k ? THPVariable_Wrap(std::move(v)) : nullptr, *both = of_v ? PyTuple_Pack(2, of_k, of_v) : nullptr;
+    Py_XDECREF(of_k);
+    Py_XDECREF(of_v);
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef METHODS[] = {{"bind", bind, METH_VARARGS, "addresses of the C entry points, and the exception of a refusal"},
                          {"product", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(product)), METH_FASTCALL, "a product of plain device tensors, or None"},
                          {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_append)), METH_FASTCALL, "rows into a paged cache, or None"},
                          {"paged_attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_attention)), METH_FASTCALL, "attention over a paged cache, or None"},
+                         {"paged_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(paged_read)), METH_FASTCALL, "rows of a paged cache, or None"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef MODULE = {PyModuleDef_HEAD_INIT, "_host_call", "native host side of a product call", -1, METHODS, nullptr, nullptr, nullptr, nullptr};
 

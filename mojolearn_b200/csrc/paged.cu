@@ -8,7 +8,9 @@
 #include "paged_append.cuh"
 #include "paged_few.cuh"
 #include "paged_fine.cuh"
+#include "paged_int4.h"
 #include "paged_many.cuh"
+#include "paged_read.cuh"
 
 using namespace b200i;
 using b200i_library::refuse;
@@ -37,9 +39,9 @@ int64_t shared_part(PagedCall *c, const char *who, int64_t row_type, int64_t cac
     if (n_heads % n_kv != 0 || n_heads > 32767) return refuse(err, err_cap, "%s: n_heads must be a multiple of n_kv and below 32768", who);
     if (head_dim % 8 != 0 || head_dim > PAGED_MAX_HD) return refuse(err, err_cap, "%s: head_dim must be a multiple of 8 up to %d", who, PAGED_MAX_HD);
     if (page < 16 || page > 256 || (page & (page - 1)) != 0) return refuse(err, err_cap, "%s: a page holds a power of two from 16 to 256 positions", who);
-    if ((row_type != B200I_T_F32 && row_type != B200I_T_BF16) || (cache_type != B200I_T_F32 && cache_type != B200I_T_BF16) ||
+    if ((row_type != B200I_T_F32 && row_type != B200I_T_BF16) || (cache_type != B200I_T_F32 && cache_type != B200I_T_BF16 && cache_type != B200I_T_INT4) ||
         (row_type == B200I_T_BF16 && cache_type == B200I_T_F32))
-        return refuse(err, err_cap, "%s: rows and cache are float32 and float32, float32 and bfloat16, or bfloat16 and bfloat16", who);
+        return refuse(err, err_cap, "%s: rows and cache are float32 and float32, float32 and bfloat16, bfloat16 and bfloat16, or either and 4 bits", who);
     if (pages * n_kv * page > MOST) return refuse(err, err_cap, "%s: a pool of more than 2^31 - 1 rows of head_dim", who);
     if (!page_table || !cu || !lengths) return refuse(err, err_cap, "%s: null page table, row offsets or lengths", who);
     int shift = 0;
@@ -73,7 +75,10 @@ AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t
     const int64_t group = n_heads / n_kv;
     if (max_new <= FEW_MOST && max_new * group <= FEW_MOST) {
         p.few = (int)(max_new * group);
-        p.cut = few_plan(b200i_library::device_sms(device), row_type == B200I_T_F32, cache_type == B200I_T_F32, (int)batch, (int)n_kv, p.hdp, p.few, max_new, max_length,
+        if (cache_type == B200I_T_INT4)
+            p.cut = int4_few_plan(b200i_library::device_sms(device), row_type == B200I_T_F32, (int)batch, (int)n_kv, p.hdp, p.few, max_new, max_length, (int)std::min(window, MOST));
+        else
+            p.cut = few_plan(b200i_library::device_sms(device), row_type == B200I_T_F32, cache_type == B200I_T_F32, (int)batch, (int)n_kv, p.hdp, p.few, max_new, max_length,
                          (int)std::min(window, MOST));
     } else {
         const bool wide = row_type == B200I_T_BF16;
@@ -82,6 +87,9 @@ AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t
     }
     return p;
 }
+
+// Bytes of a position of a head.
+long long cache_row_bytes(int64_t type, int64_t head_dim) { return type == B200I_T_INT4 ? INT4_BYTES * int4_groups((int)head_dim) : head_dim * (type == B200I_T_F32 ? 4 : 2); }
 
 bool rows_fit(int64_t ld, int64_t width, int64_t type) { return ld >= width && (ld * (type == B200I_T_F32 ? 4 : 2)) % 16 == 0; }
 
@@ -115,12 +123,41 @@ int64_t b200i_paged_append(int64_t device, void *stream, void *q_out, void *k_ca
     int dev;
     if (enter(&a.c, "paged_append", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (row_type == B200I_T_BF16)
+    if (cache_type == B200I_T_INT4)
+        LIBRARY_CUDA_TRY(int4_append(a, row_type == B200I_T_F32, eps, b200i_library::device_sms(dev), st));
+    else if (row_type == B200I_T_BF16)
         LIBRARY_CUDA_TRY((launch_append<__nv_bfloat16, __nv_bfloat16>(a, b200i_library::device_sms(dev), st)));
     else if (cache_type == B200I_T_BF16)
         LIBRARY_CUDA_TRY((launch_append<float, __nv_bfloat16>(a, b200i_library::device_sms(dev), st)));
     else
         LIBRARY_CUDA_TRY((launch_append<float, float>(a, b200i_library::device_sms(dev), st)));
+    b200i_library::count_launches(1);
+    b200i_library::accept(err, err_cap);
+    return 0;
+}
+
+int64_t b200i_paged_read(int64_t device, void *stream, void *k_out, void *v_out, const void *k_cache, const void *v_cache, int64_t out_type, int64_t cache_type, const int32_t *page_table,
+                         const int32_t *cu, const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_kv, int64_t head_dim, int64_t pages, int64_t page, int64_t max_pages, char *err,
+                         int64_t err_cap) {
+    ReadCall a;
+    if (shared_part(&a.c, "paged_read", out_type, cache_type, page_table, cu, lengths, rows, batch, n_kv, n_kv, head_dim, pages, page, max_pages, err, err_cap)) return 1;
+    if (!k_out || !v_out || !k_cache || !v_cache) return refuse(err, err_cap, "paged_read: null storage");
+    if (!aligned16(k_out) || !aligned16(v_out) || !aligned16(k_cache) || !aligned16(v_cache)) return refuse(err, err_cap, "paged_read: storage must start on 16-byte boundaries");
+    const long long bytes = rows * n_kv * head_dim * (out_type == B200I_T_F32 ? 4 : 2), held = pages * n_kv * page * cache_row_bytes(cache_type, head_dim);
+    if (meets_rows(k_out, bytes, v_out, bytes, bytes, 1) || meets_rows(k_out, bytes, k_cache, held, held, 1) || meets_rows(k_out, bytes, v_cache, held, held, 1) ||
+        meets_rows(v_out, bytes, k_cache, held, held, 1) || meets_rows(v_out, bytes, v_cache, held, held, 1))
+        return refuse(err, err_cap, "paged_read: the outputs may lie neither over one another nor over the caches");
+    a.k_cache = k_cache, a.v_cache = v_cache, a.k_out = k_out, a.v_out = v_out;
+    int dev;
+    if (enter(&a.c, "paged_read", device, &dev, err, err_cap)) return 1;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int sms = b200i_library::device_sms(dev);
+    if (cache_type == B200I_T_INT4)
+        LIBRARY_CUDA_TRY((out_type == B200I_T_F32 ? launch_read<Int4, float>(a, sms, st) : launch_read<Int4, __nv_bfloat16>(a, sms, st)));
+    else if (cache_type == B200I_T_BF16)
+        LIBRARY_CUDA_TRY((out_type == B200I_T_F32 ? launch_read<__nv_bfloat16, float>(a, sms, st) : launch_read<__nv_bfloat16, __nv_bfloat16>(a, sms, st)));
+    else
+        LIBRARY_CUDA_TRY((launch_read<float, float>(a, sms, st)));
     b200i_library::count_launches(1);
     b200i_library::accept(err, err_cap);
     return 0;
@@ -167,7 +204,9 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const AttendPlan p = attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
     if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
-    if (p.few) {
+    if (cache_type == B200I_T_INT4) {
+        LIBRARY_CUDA_TRY(p.few ? int4_few(a, row_type == B200I_T_F32, p.cut, p.hdp, ws, dev, st, &launches) : int4_many(a, row_type == B200I_T_F32, p.cut_many, p.hdp, ws, dev, st, &launches));
+    } else if (p.few) {
         if (row_type == B200I_T_BF16)
             LIBRARY_CUDA_TRY((launch_few<__nv_bfloat16, __nv_bfloat16>(a, p.cut, p.hdp, ws, dev, st, &launches)));
         else if (cache_type == B200I_T_BF16)
@@ -176,7 +215,7 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
             LIBRARY_CUDA_TRY((launch_few<float, float>(a, p.cut, p.hdp, ws, dev, st, &launches)));
     } else {
         if (row_type == B200I_T_BF16)
-            LIBRARY_CUDA_TRY(p.hdp == 64 ? launch_many_as<64>(a, p.cut_many, ws, dev, st, &launches) : launch_many_as<128>(a, p.cut_many, ws, dev, st, &launches));
+            LIBRARY_CUDA_TRY((p.hdp == 64 ? launch_many_as<__nv_bfloat16, 64>(a, p.cut_many, ws, dev, st, &launches) : launch_many_as<__nv_bfloat16, 128>(a, p.cut_many, ws, dev, st, &launches)));
         else if (cache_type == B200I_T_BF16)
             LIBRARY_CUDA_TRY((p.hdp == 64 ? launch_fine_as<__nv_bfloat16, 64>(a, p.cut_many, ws, dev, st, &launches) : launch_fine_as<__nv_bfloat16, 128>(a, p.cut_many, ws, dev, st, &launches)));
         else

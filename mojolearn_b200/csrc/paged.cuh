@@ -126,6 +126,14 @@ template <> struct PagedWords<__nv_bfloat16> {
     static __device__ __forceinline__ float4 upper(const Eight &x) { return two(x.z, x.w); }
     static __device__ __forceinline__ float4 words(const Four &x) { return two(x.x, x.y); }
 };
+// The rows of a cache (of paged_cache_row): eight or four of their columns. (A cache in 4 bits: paged_int4.cuh.)
+template <typename T> struct PagedRows : PagedWords<T> {
+    const T *base;
+    int hd;
+    __device__ __forceinline__ PagedRows(const void *p, const PagedCall &c) : base(static_cast<const T *>(p)), hd(c.hd) {}
+    __device__ __forceinline__ typename PagedWords<T>::Eight eight(int row, int col) const { return PagedWords<T>::eight(base + (long long)row * hd + col); }
+    __device__ __forceinline__ typename PagedWords<T>::Four four(int row, int col) const { return PagedWords<T>::four(base + (long long)row * hd + col); }
+};
 __device__ __forceinline__ float paged_dot(const float4 &x, const float4 &y, float z) { return fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, fmaf(x.x, y.x, z)))); }
 
 // A (row, head) over some of its keys: the largest score (-infinity: none), the weights' sum and four columns of the weighted sum of values,
@@ -145,11 +153,11 @@ struct RowSums {
 template <typename RT, typename CT>
 __device__ __noinline__ RowSums attend_keys_plain(const AttendCall &a, int b, int row, int h, int begin, int end) {
     using QW = PagedWords<RT>;
-    using W = PagedWords<CT>;
+    using W = PagedRows<CT>;
     constexpr int ASK = sizeof(CT) == 2 ? 4 : 2, ASK_V = 2 * ASK; // keys a lane asks for at once
     // What the loop needs of the arguments is read before it: they are behind an address here, and read again after every store that might be to them.
     const PagedCall c = a.c;
-    const CT *const keys = static_cast<const CT *>(a.k), *const values = static_cast<const CT *>(a.v);
+    const W keys(a.k, c), values(a.v, c);
     const float scale = a.flip ? -a.scale : a.scale, softcap = a.softcap;
     const int lane = threadIdx.x & 31, part = lane & 7, hd = c.hd, kvh = h / c.group, c0 = 4 * lane;
     const RT *q = static_cast<const RT *>(a.q) + (long long)row * a.ldq + (long long)h * hd;
@@ -172,7 +180,7 @@ __device__ __noinline__ RowSums attend_keys_plain(const AttendCall &a, int b, in
                 for (int i = 0; i < ASK; i++) {
                     const int key = __shfl_sync(0xFFFFFFFFu, at, 4 * (i0 + i) + (lane >> 3));
                     y[i] = {};
-                    if (key >= 0 && col < hd) y[i] = W::eight(keys + (long long)key * hd + col);
+                    if (key >= 0 && col < hd) y[i] = keys.eight(key, col);
                 }
 #pragma unroll
                 for (int i = 0; i < ASK; i++) sums[i0 + i] = paged_dot(QW::upper(x), W::upper(y[i]), paged_dot(QW::lower(x), W::lower(y[i]), sums[i0 + i]));
@@ -205,7 +213,7 @@ __device__ __noinline__ RowSums attend_keys_plain(const AttendCall &a, int b, in
             for (int k = 0; k < ASK_V; k++) {
                 const int key = __shfl_sync(0xFFFFFFFFu, at, k0 + k);
                 v[k] = {};
-                if (key >= 0 && c0 < hd) v[k] = W::four(values + (long long)key * hd + c0);
+                if (key >= 0 && c0 < hd) v[k] = values.four(key, c0);
             }
 #pragma unroll
             for (int k = 0; k < ASK_V; k++) {

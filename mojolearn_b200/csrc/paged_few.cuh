@@ -36,7 +36,7 @@ template <typename CT, int HDP> struct FewKeys { static constexpr int N = FEW_SL
 // Shared memory of a block: the ring, `meet` bytes for the warps' results, the queries, barriers. Two blocks on an SM (113 KB each) where
 // that leaves two slots.
 template <int HDP, int MEET_BYTES, int QUERY_BYTES> struct FewShape {
-    static constexpr int SLOT = FEW_SLOT, MEET = MEET_BYTES, QUERY = QUERY_BYTES;
+    static constexpr int WARPS = FEW_WARPS, SLOT = FEW_SLOT, MEET = MEET_BYTES, QUERY = QUERY_BYTES;
     static constexpr int REST = 1024 + 512 + MEET + FEW_ITEMS * QUERY;
     static constexpr int BLOCKS = (110 * 1024 - REST) / SLOT >= 2 ? 2 : 1;
     static constexpr int ROOM = ((BLOCKS == 2 ? 112 : 220) * 1024 - REST) / SLOT;
@@ -148,10 +148,11 @@ template <typename Shape> struct FewMemory {
     }
 };
 
-// The copying warp. `items`: FEW_ITEMS of them in shared memory.
-template <typename RT, typename CT, int HDP, typename Shape>
-__device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUtensorMap *map_v, const FewCall &f, const FewMemory<Shape> &sm, FewItem *items, const LinePlace &p) {
-    constexpr int KEYS = FewKeys<CT, HDP>::N, SLOTS = Shape::SLOTS, HALF = Shape::SLOT / 2, BOX_COLS = 128 / (int)sizeof(CT), BOXES = HDP / BOX_COLS;
+// The copying warp. `items`: FEW_ITEMS of them in shared memory. `bring(to, full, pos, there, low, kvh, page_of)`, all lanes, asks for the `there` pieces (of
+// min(page, KEYS) positions) of a tile that begins at pos, as bytes that `full` counts: page_of(piece) is a piece's page, and positions below low are seen by no row.
+template <typename RT, int KEYS, typename Shape, typename F>
+__device__ __forceinline__ void few_copies(const FewCall &f, const FewMemory<Shape> &sm, FewItem *items, const LinePlace &p, F bring) {
+    constexpr int SLOTS = Shape::SLOTS;
     const AttendCall &a = f.a;
     const int lane = threadIdx.x & 31, page = 1 << a.c.page_shift, box_rows = min(page, KEYS), pieces = KEYS / box_rows;
     unsigned it = 0, number = 0, sent = 0; // tiles, items looked at, phases of item_full that were begun
@@ -216,31 +217,13 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
             const int slot = (int)(it % SLOTS), pos = (t0 + before + t) * KEYS;
             if (!wait(&sm.empty[slot], ((it / SLOTS) & 1u) ^ 1u)) break;
             const int there = min(pieces, max(0, (s.length - pos + box_rows - 1) / box_rows)); // pieces that hold positions of the sequence
-            unsigned char *dst = sm.ring + slot * Shape::SLOT;
-            if (lane == 0) pg_bar_expect(&sm.full[slot], (unsigned)(there * box_rows * 128 * BOXES * 2));
-            __syncwarp();
             const int first = pos >> a.c.page_shift;
             if (first + pieces - 1 >= base + 32 && there > 0) { // a tile's pages (at most eight) lie in one set of 32: sets begin at its own
                 base += 32;
                 id = ahead;
                 ahead = base + 32 + lane <= last_page ? ids[base + 32 + lane] : 0;
             }
-            for (int u = 0; u < there * 2 * BOXES; u += 32) {
-                const int v = u + lane, piece = v / (2 * BOXES), box = v % (2 * BOXES);
-                const int mine = __shfl_sync(0xFFFFFFFFu, id, (first + min(piece, there - 1) - base) & 31);
-                if (piece < there) {
-                    int row = a.c.pages * a.c.kv * page; // past the pool: zeros
-                    if (low - pos < (piece + 1) * box_rows) { // a page that nobody sees any more may be anyone's
-                        if ((unsigned)mine < (unsigned)a.c.pages)
-                            row = ((mine * a.c.kv + kvh) << a.c.page_shift) + ((pos + piece * box_rows) & (page - 1));
-                        else
-                            atomicExch(a.c.status, PAGED_BAD_PAGE);
-                    }
-                    const bool is_v = box >= BOXES;
-                    const int cb = is_v ? box - BOXES : box;
-                    pg_tma_load(dst + (is_v ? HALF : 0) + cb * (KEYS * 128) + piece * (box_rows * 128), is_v ? map_v : map_k, &sm.full[slot], cb * BOX_COLS, row);
-                }
-            }
+            bring(sm.ring + slot * Shape::SLOT, &sm.full[slot], pos, there, low, kvh, [&](int piece) { return __shfl_sync(0xFFFFFFFFu, id, (first + min(piece, there - 1) - base) & 31); });
         }
         if (f.whole) {
             kvh += gridDim.x, b += kvh / a.c.kv, kvh %= a.c.kv;
@@ -260,17 +243,44 @@ __device__ __forceinline__ void few_copies(const CUtensorMap *map_k, const CUten
     for (unsigned i = sent > FEW_ITEMS ? sent - FEW_ITEMS : 0; i < sent; i++) pg_bar_wait(&sm.item_full[i % FEW_ITEMS], (i / FEW_ITEMS) & 1u);
 }
 
-// The beginning of a block: barriers, and its place on the line.
+// What brings tiles of float32 or bfloat16 caches: boxes of 128 bytes by a piece's rows.
 template <typename CT, int HDP, typename Shape>
+__device__ __forceinline__ auto few_boxes(const CUtensorMap *map_k, const CUtensorMap *map_v, const PagedCall &c) {
+    return [map_k, map_v, &c](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
+        constexpr int KEYS = FewKeys<CT, HDP>::N, HALF = Shape::SLOT / 2, BOX_COLS = 128 / (int)sizeof(CT), BOXES = HDP / BOX_COLS;
+        const int lane = threadIdx.x & 31, page = 1 << c.page_shift, box_rows = min(page, KEYS);
+        if (lane == 0) pg_bar_expect(full, (unsigned)(there * box_rows * 128 * BOXES * 2));
+        __syncwarp();
+        for (int u = 0; u < there * 2 * BOXES; u += 32) {
+            const int v = u + lane, piece = v / (2 * BOXES), box = v % (2 * BOXES);
+            const int mine = page_of(piece);
+            if (piece < there) {
+                int row = c.pages * c.kv * page; // past the pool: zeros
+                if (low - pos < (piece + 1) * box_rows) { // a page that nobody sees any more may be anyone's
+                    if ((unsigned)mine < (unsigned)c.pages)
+                        row = ((mine * c.kv + kvh) << c.page_shift) + ((pos + piece * box_rows) & (page - 1));
+                    else
+                        atomicExch(c.status, PAGED_BAD_PAGE);
+                }
+                const bool is_v = box >= BOXES;
+                const int cb = is_v ? box - BOXES : box;
+                pg_tma_load(dst + (is_v ? HALF : 0) + cb * (KEYS * 128) + piece * (box_rows * 128), is_v ? map_v : map_k, full, cb * BOX_COLS, row);
+            }
+        }
+    };
+}
+
+// The beginning of a block: barriers, and its place on the line.
+template <int KEYS, typename Shape>
 __device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory<Shape> &sm, long long *place, unsigned *bad_rows, int *dead) {
     if (threadIdx.x == 0) {
         for (int s = 0; s < Shape::SLOTS; s++) {
             pg_bar_init(&sm.full[s], 1);
-            pg_bar_init(&sm.empty[s], FEW_WARPS);
+            pg_bar_init(&sm.empty[s], Shape::WARPS);
         }
         for (int i = 0; i < FEW_ITEMS; i++) {
             pg_bar_init(&sm.item_full[i], 1);
-            pg_bar_init(&sm.item_empty[i], FEW_WARPS);
+            pg_bar_init(&sm.item_empty[i], Shape::WARPS);
         }
         *bad_rows = 0, *dead = 0;
         if (!f.whole) f.head[blockIdx.x * 8] = -1;
@@ -285,7 +295,7 @@ __device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory
             f.a.c,
             [&](int b) -> long long {
                 int t0;
-                return few_tiles(f.a, paged_seq_checked(f.a.c, b), FewKeys<CT, HDP>::N, &t0);
+                return few_tiles(f.a, paged_seq_checked(f.a.c, b), KEYS, &t0);
             },
             blockIdx.x, gridDim.x, place);
     }
@@ -298,22 +308,22 @@ __device__ __forceinline__ void few_head(const FewCall &f, const FewItem &i) {
     int *head = f.head + blockIdx.x * 8;
     head[0] = i.b, head[1] = i.kvh, head[2] = i.count, head[3] = i.line, head[4] = i.per;
 }
-__device__ __forceinline__ void few_meet() { asm volatile("bar.sync 1, %0;" ::"n"(32 * FEW_WARPS) : "memory"); } // the computing warps
+template <int WARPS = FEW_WARPS> __device__ __forceinline__ void few_meet() { asm volatile("bar.sync 1, %0;" ::"n"(32 * WARPS) : "memory"); } // the computing warps
 // They meet, and know alike whether one of them brings a yes: a word in shared memory could change before the slower ones have read it.
-__device__ __forceinline__ bool few_vote(bool yes) {
+template <int WARPS = FEW_WARPS> __device__ __forceinline__ bool few_vote(bool yes) {
     unsigned some;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(some) : "r"((unsigned)yes), "n"(32 * FEW_WARPS) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(some) : "r"((unsigned)yes), "n"(32 * WARPS) : "memory");
     return some != 0;
 }
 // Rows that did not come out finite, done again: a masked key's zero weight met a value that is not finite.
-template <typename RT, typename CT>
+template <typename RT, typename CT, int WARPS = FEW_WARPS>
 __device__ __forceinline__ void few_again(const AttendCall &a, const FewItem &i, unsigned *bad_rows, int rows) {
     const unsigned rest = *bad_rows;
-    few_meet();
+    few_meet<WARPS>();
     if (threadIdx.x == 0) *bad_rows = 0;
-    for (int r = threadIdx.x >> 5; r < rows; r += FEW_WARPS)
+    for (int r = threadIdx.x >> 5; r < rows; r += WARPS)
         if (rest >> r & 1) attend_row_plain<RT, CT>(a, i.b, i.s.first + r / a.c.group, i.s.pos0 + r / a.c.group, i.s.length, i.kvh * a.c.group + r % a.c.group);
-    few_meet();
+    few_meet<WARPS>();
 }
 
 // ---- bfloat16 rows ----
@@ -348,9 +358,9 @@ __global__ void __launch_bounds__(FEW_THREADS, FewMmaShape<HDP, NT>::BLOCKS) att
     __shared__ int dead;
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const LinePlace p = few_begin<T, HDP>(f, sm, place, &bad_rows, &dead);
+    const LinePlace p = few_begin<KEYS>(f, sm, place, &bad_rows, &dead);
     if (warp == FEW_WARPS) {
-        few_copies<T, T, HDP>(&map_k, &map_v, f, sm, items, p);
+        few_copies<T, KEYS>(f, sm, items, p, few_boxes<T, HDP, Shape>(&map_k, &map_v, f.a.c));
         return;
     }
 
@@ -650,9 +660,9 @@ __global__ void __launch_bounds__(FEW_THREADS, FewFmaShape<CT, HDP, R>::BLOCKS)
     __shared__ int dead;
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const LinePlace p = few_begin<CT, HDP>(f, sm, place, &bad_rows, &dead);
+    const LinePlace p = few_begin<KEYS>(f, sm, place, &bad_rows, &dead);
     if (warp == FEW_WARPS) {
-        few_copies<float, CT, HDP>(&map_k, &map_v, f, sm, items, p);
+        few_copies<float, KEYS>(f, sm, items, p, few_boxes<CT, HDP, Shape>(&map_k, &map_v, f.a.c));
         return;
     }
 
@@ -911,20 +921,25 @@ constexpr int FEW_MOST = 16;  // rows of an item
 
 template <bool F32, typename CT, int HDP, int R> constexpr int few_blocks_per_sm() { return F32 ? FewFmaShape<CT, HDP, R>::BLOCKS : FewMmaShape<HDP, R <= 8 ? 1 : 2>::BLOCKS; }
 
+// Of at most `room` blocks at a time and tiles of `keys` keys; p->rows is set.
+inline void few_cut(FewPlan *p, int room, int keys, int batch, int kv, int hdp, long long max_new, long long max_length, int window) {
+    long long span = max_length;
+    if (window > 0) span = std::min(span, (long long)window + max_new + keys);
+    const long long items = (long long)batch * kv, tiles = (span + keys - 1) / keys;
+    p->whole = tiles <= FEW_WHOLE;
+    const long long want = p->whole ? items : (items * tiles + FEW_LEAST - 1) / FEW_LEAST;
+    p->blocks = (int)std::min<long long>(room, want);
+    p->part_floats = p->whole ? 0 : (long long)p->blocks * 2 * p->rows * (hdp + 2);
+    p->bytes = p->whole ? 0 : p->part_floats * 4 + (long long)p->blocks * 32;
+}
+
 inline FewPlan few_plan(int sms, bool f32_rows, bool f32_cache, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     FewPlan p;
     const int keys = FEW_SLOT / (2 * hdp * (f32_cache ? 4 : 2));
     p.most = rows, p.rows = f32_rows ? 1 : 8; // laid out for 1, 2, 4, 8 or 16 float32 rows, for 8 or 16 of bfloat16
     while (p.rows < rows) p.rows *= 2;
     const int per_sm = p.rows < 16 ? 2 : (!f32_rows ? few_blocks_per_sm<false, __nv_bfloat16, 128, 16>() : (hdp == 64 ? few_blocks_per_sm<true, float, 64, 16>() : few_blocks_per_sm<true, float, 128, 16>()));
-    long long span = max_length;
-    if (window > 0) span = std::min(span, (long long)window + max_new + keys);
-    const long long items = (long long)batch * kv, tiles = (span + keys - 1) / keys;
-    p.whole = tiles <= FEW_WHOLE;
-    const long long want = p.whole ? items : (items * tiles + FEW_LEAST - 1) / FEW_LEAST;
-    p.blocks = (int)std::min<long long>((long long)per_sm * sms, want);
-    p.part_floats = p.whole ? 0 : (long long)p.blocks * 2 * p.rows * (hdp + 2);
-    p.bytes = p.whole ? 0 : p.part_floats * 4 + (long long)p.blocks * 32;
+    few_cut(&p, per_sm * sms, keys, batch, kv, hdp, max_new, max_length, window);
     return p;
 }
 

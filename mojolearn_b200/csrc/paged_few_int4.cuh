@@ -1,0 +1,472 @@
+// Attention of few rows over a paged cache in 4 bits: a decode step's single tokens (and up to 16 rows a sequence and key head).
+//
+// The sums, the line of tiles, the copying warp and the join are those of paged_few.cuh. Bound: HBM, 4.5 bits a word of keys and values; next to that the
+// instructions that make bfloat16 words of codes (paged_int4.cuh), one and a half a word, of which an SM has 42 words a clock to do at the HBM rate. So eight warps
+// compute, two blocks on an SM, each on 16 keys of a 128-key tile, and a word is made once and meets all rows of its key head in one instruction:
+// m16n8k16 with the KEYS as rows, S^T = K Q^T and O^T = V^T P^T, the eight columns being rows. What a word's place is in an instruction is free where both factors agree on
+// it: of a key a lane takes a quarter of its columns, which is one group and one 16-byte load; of the values an eighth of the columns of four keys, whose codes become pairs along the
+// keys by one byte permutation for eight words.
+// PACK: up to four bfloat16 rows or two of float32 leave columns of the eight free. A weight is then two pieces of 8 bits in neighbouring columns (three in four
+// columns; and so are float32 queries), and one product serves where the others need one for each piece.
+// A tensor core cuts its 32-bit sums off where it adds to a large one: with float32 rows each 16 keys begin at zero and are added to the output to nearest.
+// Weights are taken from the largest score so far as it was when one last exceeded it by 2^8: larger ones are as exact, and the usual tile needs one vote.
+#pragma once
+#include <type_traits>
+
+#include "paged_few.cuh"
+#include "paged_int4.cuh"
+
+namespace b200i {
+
+constexpr int FEW4_WARPS = 8, FEW4_THREADS = 32 * (FEW4_WARPS + 1), FEW4_KEYS = 16 * FEW4_WARPS;
+
+template <typename RT, int HDP, int NT, bool PACK> struct Few4Shape {
+    static constexpr bool F32 = std::is_same_v<RT, float>;
+    static constexpr int WARPS = FEW4_WARPS, ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
+    static constexpr int CODES = FEW4_KEYS * HDP / 2, SCALES = FEW4_KEYS * HDP / INT4_GROUP * 2, SLOT = 2 * (CODES + SCALES); // codes of keys and of values, their scales
+    static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : 2;
+    static constexpr bool HELD = PACK || (!F32 && NT == 1); // the queries stay in registers; else they lie as fragments where the warps' results meet
+    static constexpr int PITCH = HDP + 8;                   // floats of a row of those
+    static constexpr int MEET = FEW4_WARPS / 2 * ROWS * PITCH * 4, QUERY = ROWS * HDP * (int)sizeof(RT);
+    static constexpr int REST = 1024 + 512 + MEET + FEW_ITEMS * QUERY;
+    static constexpr int ROOM = (112 * 1024 - REST) / SLOT, SLOTS = ROOM > 8 ? 8 : ROOM;
+    static constexpr int SMEM = REST + SLOTS * SLOT;
+    static_assert(SLOTS >= 2 && (HELD || Q_PIECES * NT * HDP / 16 * 256 <= MEET), "shared memory");
+};
+
+// What brings a tile: a lane one of a piece's four runs of bytes (codes of keys, of values, scales of keys, of values).
+template <typename Shape>
+__device__ __forceinline__ auto few4_runs(const AttendCall &a) {
+    return [&a](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
+        const PagedCall &c = a.c;
+        const int lane = threadIdx.x & 31, run = lane & 3, piece = lane >> 2, page = 1 << c.page_shift, rows = min(page, FEW4_KEYS), groups = int4_groups(c.hd);
+        const int id = page_of(piece), bytes = rows * groups * (run < 2 ? 16 : 2), first = piece * rows;
+        const bool want = piece < there && low - pos < first + rows; // a page that nobody sees any more may be anyone's
+        const bool some = want && (unsigned)id < (unsigned)c.pages;
+        unsigned char *const to = dst + (run & 1) * (run < 2 ? Shape::CODES : Shape::SCALES) + (run < 2 ? first * groups * 16 : 2 * Shape::CODES + first * groups * 2);
+        if (want && !some) { // a page of zeros
+            atomicExch(c.status, PAGED_BAD_PAGE);
+            if (run >= 2)
+                for (int i = 0; i < bytes; i += 16) *reinterpret_cast<uint4 *>(to + i) = make_uint4(0, 0, 0, 0);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        const unsigned all = __ballot_sync(0xFFFFFFFFu, some);
+        if (lane == 0) pg_bar_expect(full, (unsigned)(__popc(all) / 4 * rows * groups * 36));
+        __syncwarp();
+        if (!some) return;
+        const int in = (pos + first) & (page - 1);
+        const unsigned char *src = int4_page(run & 1 ? a.v : a.k, id * c.kv + kvh, groups, c.page_shift) + (run < 2 ? in * groups * 16 : ((16 * groups) << c.page_shift) + in * groups * 2);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(to)), "l"(src), "r"(bytes), "r"(pg_smem(full)) : "memory");
+    };
+}
+
+template <typename RT, int HDP, int NT, bool PACK>
+__global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
+    using Shape = Few4Shape<RT, HDP, NT, PACK>;
+    constexpr bool F32 = Shape::F32, HELD = Shape::HELD;
+    constexpr int KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = FEW4_WARPS, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
+    constexpr int E = PACK ? 1 : 2 * NT;                   // rows of a lane's scores
+    constexpr int K_WORDS = HDP / 32, V_WORDS = HDP / 64;  // of codes, of a key: a quarter of its columns, an eighth
+    extern __shared__ __align__(128) unsigned char smem[];
+    const FewMemory<Shape> sm(smem);
+    __shared__ float ml[WARPS][2][ROWS], joined[2][ROWS];
+    __shared__ long long place[32];
+    __shared__ FewItem items[FEW_ITEMS];
+    __shared__ unsigned bad_rows;
+    __shared__ int dead;
+    const AttendCall &a = f.a;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    const LinePlace p = few_begin<KEYS>(f, sm, place, &bad_rows, &dead);
+    if (warp == WARPS) {
+        few_copies<RT, KEYS>(f, sm, items, p, few4_runs<Shape>(a));
+        return;
+    }
+
+    const int groups = int4_groups(a.c.hd), stride = 16 * groups;
+    const int k_group = t4 * (HDP / 4) / INT4_GROUP, v_group = g * (HDP / 8) / INT4_GROUP; // of the lane's columns
+    const bool k_some = k_group < groups, v_some = v_group < groups;
+    // in a slot, of the warp's keys: the lane's codes and scales of keys g (and g + 8), and of values 2 t4 (and 1, 8 and 9 further on)
+    const int k_at = (warp * 16 + g) * stride + (k_some ? t4 * (HDP / 8) : 0), k_scale = 2 * Shape::CODES + ((warp * 16 + g) * groups + (k_some ? k_group : 0)) * 2;
+    const int v_at = Shape::CODES + (warp * 16 + 2 * t4) * stride + (v_some ? g * (HDP / 16) : 0);
+    const int v_scale = 2 * Shape::CODES + Shape::SCALES + ((warp * 16 + 2 * t4) * groups + (v_some ? v_group : 0)) * 2;
+    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E;
+    const auto row_of = [&](int e) { return PACK ? (F32 ? t4 >> 1 : t4) : (e >> 1) * 8 + 2 * t4 + (e & 1); };
+    uint2 *const fragments = reinterpret_cast<uint2 *>(sm.meet);
+    unsigned it = 0;
+    bool alive = true, first_part = true;
+    const auto give_up = [&] {
+        if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
+        alive = false; // it goes on without waiting, so that the others meet it; nothing of the block is stored from here on
+    };
+    for (unsigned number = 0;; number++) {
+        const int which = number % FEW_ITEMS;
+        if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.item_full[which], (number / FEW_ITEMS) & 1u))) give_up();
+        if (few_vote<WARPS>(!alive)) break; // nobody goes on where one has given up: what the item is would not be known
+        const FewItem item = items[which];
+        if (!item.more) break;
+        const PagedSeq s = item.s;
+        const int rows = min(item.n * a.c.group, ROWS);
+
+        // The rows as fragments: column n of row `row`, words col .. col + 3 of it, piece by piece.
+        const auto words = [&](uint2 (&q)[QP], int row, int col) {
+#pragma unroll
+            for (int k = 0; k < QP; k++) q[k] = make_uint2(0, 0);
+            if (row >= rows || col >= a.c.hd) return;
+            const unsigned char *src = sm.query + which * Shape::QUERY + (row * a.c.hd + col) * (int)sizeof(RT);
+            if constexpr (F32) {
+                float4 x = *reinterpret_cast<const float4 *>(src);
+                if (a.flip) x = make_float4(-x.x, -x.y, -x.z, -x.w);
+                unsigned lo[3], hi[3];
+                pg_split<3>(lo, x.x, x.y), pg_split<3>(hi, x.z, x.w);
+#pragma unroll
+                for (int k = 0; k < 3; k++) q[k] = make_uint2(lo[k], hi[k]);
+            } else {
+                const unsigned flip = a.flip ? 0x80008000u : 0u;
+                q[0] = *reinterpret_cast<const uint2 *>(src);
+                q[0].x ^= flip, q[0].y ^= flip;
+            }
+        };
+        uint2 held[HELD ? KS : 1];
+        if constexpr (HELD) {
+            const int row = !PACK ? g : (F32 ? g >> 2 : g >> 1), piece = !PACK ? 0 : (F32 ? g & 3 : g & 1);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                uint2 q[QP];
+                words(q, row, t4 * (HDP / 4) + 4 * ks);
+                held[ks] = piece == 0 ? q[0] : make_uint2(0, 0);
+                if constexpr (F32) held[ks] = piece == 1 ? q[1] : (piece == 2 ? q[2] : held[ks]);
+            }
+        } else {
+            for (int i = tid; i < NT * KS * 32; i += 32 * WARPS) {
+                const int of = i & 31, ks = (i >> 5) % KS, nt = (i >> 5) / KS;
+                uint2 q[QP];
+                words(q, nt * 8 + (of >> 2), (of & 3) * (HDP / 4) + 4 * ks);
+#pragma unroll
+                for (int k = 0; k < QP; k++) fragments[k * (NT * KS * 32) + i] = q[k];
+            }
+            few_meet<WARPS>();
+        }
+        int hi[E], lo[E]; // what a row sees: positions lo .. hi - 1
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            hi[e] = row_of(e) < rows ? s.pos0 + row_of(e) / a.c.group + 1 : 0;
+            lo[e] = a.window ? hi[e] - a.window : 0;
+        }
+        const int all_lo = a.window ? s.pos0 + item.n - a.window : 0, low = a.window ? s.pos0 + 1 - a.window : 0; // every row sees positions all_lo .. pos0; none sees what is below low
+
+        float o[NT][KS][4], m[E], l[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) m[e] = -INFINITY, l[e] = 0.0f;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int mt = 0; mt < KS; mt++) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
+        for (int t = 0; t < item.tiles; t++, it++) {
+            const unsigned char *const slot = sm.ring + (it % SLOTS) * Shape::SLOT;
+            const int j0 = item.pos + t * KEYS + warp * 16;
+            if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[it % SLOTS], (it / SLOTS) & 1u))) give_up();
+            if (alive && j0 < s.length && j0 + 16 > low) {
+                // ---- scores ----
+                float z[NT][4], z_small[F32 && !PACK ? NT : 1][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.0f;
+                if constexpr (F32 && !PACK) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) z_small[nt][0] = z_small[nt][1] = z_small[nt][2] = z_small[nt][3] = 0.0f;
+                }
+                {
+                    unsigned code[2][K_WORDS], scale[2], shift[2];
+#pragma unroll
+                    for (int h = 0; h < 2; h++) { // keys g and g + 8
+                        const unsigned char *at = slot + k_at + h * 8 * stride;
+                        if constexpr (K_WORDS == 4) {
+                            const uint4 w = *reinterpret_cast<const uint4 *>(at);
+                            code[h][0] = w.x, code[h][1] = w.y, code[h][2] = w.z, code[h][3] = w.w;
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(at);
+                            code[h][0] = w.x, code[h][1] = w.y;
+                        }
+                        scale[h] = *reinterpret_cast<const unsigned short *>(slot + k_scale + h * 16 * groups);
+                        if (!k_some) scale[h] = 0;
+                        scale[h] *= 0x10001u, shift[h] = int4_shift(scale[h]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < K_WORDS; w++) {
+                        unsigned x[2][4];
+                        int4_pairs(x[0], code[0][w], scale[0], shift[0]), int4_pairs(x[1], code[1][w], scale[1], shift[1]);
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            const unsigned k[4] = {x[0][2 * i], x[1][2 * i], x[0][2 * i + 1], x[1][2 * i + 1]};
+                            const int ks = 2 * w + i;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                if constexpr (HELD) {
+                                    pg_mma(z[nt], k, held[ks].x, held[ks].y);
+                                } else {
+#pragma unroll
+                                    for (int piece = QP - 1; piece >= 0; piece--) {
+                                        const uint2 q = fragments[piece * (NT * KS * 32) + (nt * KS + ks) * 32 + lane];
+                                        pg_mma(F32 && piece > 0 ? z_small[F32 && !PACK ? nt : 0] : z[nt], k, q.x, q.y);
+                                    }
+                                }
+                            }
+                        }
+                    }
+                }
+                float x[E][2]; // keys g and g + 8
+                if constexpr (PACK) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        x[0][h] = z[0][2 * h];
+                        if constexpr (F32) {
+                            x[0][h] += z[0][2 * h + 1]; // two pieces here, the third beside it
+                            x[0][h] += __shfl_xor_sync(0xFFFFFFFFu, x[0][h], 1);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            x[e][h] = z[e >> 1][2 * h + (e & 1)];
+                            if constexpr (F32) x[e][h] += z_small[e >> 1][2 * h + (e & 1)];
+                        }
+                }
+                const bool edge = j0 + 16 > s.pos0 + 1 || j0 < all_lo;
+                bool more = false;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float y = x[e][h];
+                        y = unit * (a.softcap > 0.0f ? tanhf(y * a.scale * a.cap_part) : y); // (scale / softcap may leave 32 bits)
+                        if (edge) {
+                            const int j = j0 + g + h * 8;
+                            if (j >= hi[e] || j < lo[e]) y = -INFINITY;
+                        }
+                        more |= y > m[e] + 8.0f;
+                        x[e][h] = y;
+                    }
+                if (__any_sync(0xFFFFFFFFu, more)) {
+                    float keep[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        float top = fmaxf(x[e][0], x[e][1]);
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                        top = fmaxf(m[e], top);
+                        keep[e] = m[e] == -INFINITY ? 0.0f : paged_exp2(m[e] - top);
+                        m[e] = top, l[e] *= keep[e];
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int mt = 0; mt < KS; mt++)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[nt][mt][i] *= keep[PACK ? 0 : 2 * nt + (i & 1)];
+                }
+                // ---- weights, as pieces and turned: keys down ----
+                unsigned w[NT][PACK ? 1 : WP][2];
+                float base[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) base[e] = m[e] == -INFINITY ? 0.0f : m[e];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float y[E];
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        y[e] = paged_exp2(x[e][h] - base[e]);
+                        l[e] += y[e];
+                    }
+                    if constexpr (PACK) {
+                        const float rest = y[0] - __uint_as_float(pg_pack(y[0], 0.0f) << 16);
+                        unsigned two = pg_pack(y[0], rest);
+                        if constexpr (F32) {
+                            const float last = rest - __uint_as_float(two & 0xFFFF0000u);
+                            if (t4 & 1) two = pg_pack(last, 0.0f);
+                        }
+                        w[0][0][h] = pg_transpose(two);
+                    } else {
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            unsigned piece[WP];
+                            pg_split<WP>(piece, y[2 * nt], y[2 * nt + 1]);
+#pragma unroll
+                            for (int k = 0; k < WP; k++) w[nt][k][h] = pg_transpose(piece[k]);
+                        }
+                    }
+                }
+                // ---- values ----
+                unsigned code[4][V_WORDS], scale[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) { // keys 2 t4, 2 t4 + 1, and eight further on
+                    const int key = (k & 1) + (k >> 1) * 8;
+                    const unsigned char *at = slot + v_at + key * stride;
+                    if constexpr (V_WORDS == 2) {
+                        const uint2 c = *reinterpret_cast<const uint2 *>(at);
+                        code[k][0] = c.x, code[k][1] = c.y;
+                    } else {
+                        code[k][0] = *reinterpret_cast<const unsigned *>(at);
+                    }
+                    scale[k] = *reinterpret_cast<const unsigned short *>(slot + v_scale + key * groups * 2);
+                    if (!v_some) scale[k] = 0;
+                    if (edge) { // what stands in positions that no row sees, or of no sequence, counts as zero
+                        const int j = j0 + 2 * t4 + key;
+                        if (j >= s.length || j < low) scale[k] = 0;
+                    }
+                }
+                const unsigned scale0 = scale[0] | scale[1] << 16, scale1 = scale[2] | scale[3] << 16, shift0 = int4_shift(scale0), shift1 = int4_shift(scale1);
+#pragma unroll
+                for (int v = 0; v < V_WORDS; v++) {
+                    unsigned even0[4], odd0[4], even1[4], odd1[4]; // columns 2 i and 2 i + 1, of two keys each
+                    int4_pairs(even0, __byte_perm(code[0][v], code[1][v], 0x5410), scale0, shift0);
+                    int4_pairs(odd0, __byte_perm(code[0][v], code[1][v], 0x7632), scale0, shift0);
+                    int4_pairs(even1, __byte_perm(code[2][v], code[3][v], 0x5410), scale1, shift1);
+                    int4_pairs(odd1, __byte_perm(code[2][v], code[3][v], 0x7632), scale1, shift1);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const unsigned x4[4] = {even0[i], odd0[i], even1[i], odd1[i]};
+                        const int mt = 4 * v + i;
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            if constexpr (F32) {
+                                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(d, x4, w[nt][k][0], w[nt][k][1]);
+#pragma unroll
+                                for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
+                            } else {
+#pragma unroll
+                                for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[nt][k][0], w[nt][k][1]);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0 && alive) pg_bar_arrive(&sm.empty[it % SLOTS]); // (what it has not waited for is not given back)
+        }
+
+        // ---- the item's (or its part's) end: the warps' results meet, [four warps][row][column], four of them adding to the others' ----
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], d);
+            if (g == 0 && !(PACK && F32 && (t4 & 1))) ml[warp][0][row_of(e)] = m[e], ml[warp][1][row_of(e)] = l[e];
+        }
+        few_meet<WARPS>();
+        if (lane == 0 && alive) pg_bar_arrive(&sm.item_empty[which]);
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const int r = row_of(e);
+            float top = ml[0][0][r], sum = 0.0f;
+#pragma unroll
+            for (int k = 1; k < WARPS; k++) top = fmaxf(top, ml[k][0][r]);
+            if (warp == 0) { // alike in all lanes that have the row
+#pragma unroll
+                for (int k = 0; k < WARPS; k++) sum = fmaf(ml[k][1][r], ml[k][0][r] == -INFINITY ? 0.0f : paged_exp2(ml[k][0][r] - top), sum);
+                joined[0][r] = top, joined[1][r] = sum;
+            }
+            const float keep = m[e] == -INFINITY ? 0.0f : paged_exp2(m[e] - top);
+#pragma unroll
+            for (int mt = 0; mt < KS; mt++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (PACK || (i & 1) == (e & 1)) o[PACK ? 0 : e >> 1][mt][i] *= keep;
+        }
+        const auto share_out = [&](int to, bool add) { // four neighbouring columns at a time
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+                for (int mt = 0; mt < KS; mt += 2) {
+                    float4 y;
+                    const float(&u)[4] = o[PACK ? 0 : e >> 1][mt], (&v)[4] = o[PACK ? 0 : e >> 1][mt + 1];
+                    if constexpr (PACK) {
+                        y = make_float4(u[0] + u[1], u[2] + u[3], v[0] + v[1], v[2] + v[3]); // the pieces
+                        if constexpr (F32) {
+                            y.x += __shfl_xor_sync(0xFFFFFFFFu, y.x, 1), y.y += __shfl_xor_sync(0xFFFFFFFFu, y.y, 1);
+                            y.z += __shfl_xor_sync(0xFFFFFFFFu, y.z, 1), y.w += __shfl_xor_sync(0xFFFFFFFFu, y.w, 1);
+                            if (t4 & 1) continue;
+                        }
+                    } else {
+                        y = make_float4(u[e & 1], u[2 + (e & 1)], v[e & 1], v[2 + (e & 1)]);
+                    }
+                    float4 *const at = reinterpret_cast<float4 *>(sm.meet + (to * ROWS + row_of(e)) * Shape::PITCH + g * (HDP / 8) + 2 * mt);
+                    if (add) {
+                        const float4 x4 = *at;
+                        y.x += x4.x, y.y += x4.y, y.z += x4.z, y.w += x4.w;
+                    }
+                    *at = y;
+                }
+        };
+        if (warp >= WARPS / 2) share_out(warp - WARPS / 2, false);
+        few_meet<WARPS>();
+        if (warp < WARPS / 2) share_out(warp, true);
+        few_meet<WARPS>();
+        const bool is_whole = item.before == 0 && item.tiles == item.count;
+        const long long part_slot = (long long)blockIdx.x * 2 + (first_part && item.before > 0 ? 0 : 1);
+        unsigned wrong = 0;
+#pragma unroll 1
+        for (int r = tid / HDP; r < rows && !dead; r += 32 * WARPS / HDP) {
+            const int col = tid % HDP, token = r / a.c.group;
+            const float *at = sm.meet + r * Shape::PITCH + col;
+            float y = (at[0] + at[ROWS * Shape::PITCH]) + (at[2 * ROWS * Shape::PITCH] + at[3 * ROWS * Shape::PITCH]);
+            if (is_whole) {
+                y *= paged_share(joined[1][r], s.pos0 + token);
+                if (col < a.c.hd) paged_write(static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + item.kvh * a.c.group + r - token * a.c.group) * a.c.hd + col, y);
+                if (col < a.c.hd && !(y * 0.0f == 0.0f)) wrong |= 1u << r;
+            } else {
+                f.part[(part_slot * ROWS + r) * HDP + col] = y;
+                if (col == 0) {
+                    float *stats = f.part + (long long)gridDim.x * 2 * ROWS * HDP + part_slot * 2 * ROWS;
+                    stats[r] = joined[0][r], stats[ROWS + r] = joined[1][r];
+                }
+            }
+        }
+        if (!is_whole && tid == 0 && item.before == 0 && !dead) few_head(f, item);
+        if (wrong) atomicOr(&bad_rows, wrong);
+        few_meet<WARPS>(); // what met is read, `bad_rows` is whole
+        if (bad_rows) few_again<RT, Int4, WARPS>(a, item, &bad_rows, rows);
+        first_part = false;
+    }
+}
+
+// ---- host side ----
+inline FewPlan few4_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
+    FewPlan p;
+    p.most = rows, p.rows = rows <= (f32_rows ? 2 : 4) ? (f32_rows ? 2 : 4) : (rows <= 8 ? 8 : 16);
+    few_cut(&p, 2 * sms, FEW4_KEYS, batch, kv, hdp, max_new, max_length, window);
+    return p;
+}
+
+template <typename RT, int HDP, int NT, bool PACK>
+cudaError_t launch_few4_as(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
+    using Shape = Few4Shape<RT, HDP, NT, PACK>;
+    FewCall f;
+    f.a = a, f.whole = p.whole, f.part = static_cast<float *>(ws), f.head = p.whole ? nullptr : reinterpret_cast<int *>(static_cast<float *>(ws) + p.part_floats);
+    const auto kernel = attend_few_int4_kernel<RT, HDP, NT, PACK>;
+    static std::atomic<bool> known[64];
+    if (device >= 64 || !known[device].load()) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+        if (e != cudaSuccess) return e;
+        if (device < 64) known[device].store(true);
+    }
+    kernel<<<p.blocks, FEW4_THREADS, Shape::SMEM, st>>>(f);
+    *launches += 1;
+    if (!p.whole) {
+        *launches += 1;
+        return launch_following<FewCall>(attend_join_kernel<RT, Int4, HDP, Shape::ROWS>, dim3(p.blocks, p.most), 256, st, f);
+    }
+    return cudaGetLastError();
+}
+template <typename RT, int HDP>
+cudaError_t launch_few4_rows(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
+    if (p.rows < 8) return launch_few4_as<RT, HDP, 1, true>(a, p, ws, device, st, launches);
+    return p.rows == 8 ? launch_few4_as<RT, HDP, 1, false>(a, p, ws, device, st, launches) : launch_few4_as<RT, HDP, 2, false>(a, p, ws, device, st, launches);
+}
+template <typename RT>
+cudaError_t launch_few4(const AttendCall &a, const FewPlan &p, int hdp, void *ws, int device, cudaStream_t st, int *launches) {
+    return hdp == 64 ? launch_few4_rows<RT, 64>(a, p, ws, device, st, launches) : launch_few4_rows<RT, 128>(a, p, ws, device, st, launches);
+}
+
+} // namespace b200i

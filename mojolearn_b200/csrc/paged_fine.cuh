@@ -26,7 +26,7 @@ constexpr int FINE_THREADS = 384, FINE_KEYS = 64, FINE_ROWS = 128; // four warps
 constexpr int FINE_REGS = 232, FINE_REGS_LOAD = 144, FINE_REGS_LESS = 128; // a thread: together 504 = 3 x 168, what the block is launched with
 
 template <typename CT, int HDP> struct FineShape {
-    static constexpr int PIECES = sizeof(CT) == 4 ? 3 : 1;
+    static constexpr int PIECES = std::is_same_v<CT, float> ? 3 : 1;
     static constexpr int TILE = HDP * 128;               // bytes of 64 rows of bfloat16
     static constexpr int SLOT = PIECES * TILE;
     static constexpr int PITCH = HDP * 4 + 16;           // of a row's words on their way in and out: eight rows' 16 bytes fall into different banks
@@ -41,7 +41,7 @@ template <typename CT, int HDP>
 __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyCall f) {
     using Shape = FineShape<CT, HDP>;
     using Walk = ManyWalk<FINE_ROWS, FINE_KEYS, 1>;
-    constexpr int SLOTS = Shape::SLOTS, SLOT = Shape::SLOT, TILE = Shape::TILE, CP = Shape::PIECES, BOXES = HDP / 64, HALF_COLS = FINE_KEYS * 128, BR = FINE_ROWS;
+    constexpr int SLOTS = Shape::SLOTS, SLOT = Shape::SLOT, TILE = Shape::TILE, CP = Shape::PIECES, LOADERS = std::is_same_v<CT, __nv_bfloat16> ? 1 : 128, BOXES = HDP / 64, HALF_COLS = FINE_KEYS * 128, BR = FINE_ROWS;
     constexpr int Q_COLS = HDP / 2, O_AT = 3 * Q_COLS, S_AT = O_AT + HDP, S_COLS = 96; // columns of tensor memory
     static_assert(S_AT + 2 * S_COLS <= 512, "tensor memory");
     extern __shared__ __align__(128) unsigned char smem[];
@@ -55,7 +55,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int s = 0; s < SLOTS; s++) {
-            pg_bar_init(&full[s], CP == 1 ? 1 : 128);
+            pg_bar_init(&full[s], LOADERS);
             pg_bar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
         };
         unsigned ld = 0;
         bool alive = true;
-        if (CP == 1 && warp == 4) {
+        if (LOADERS == 1 && warp == 4) {
             unsigned tails = 0;
             bool tail_lost = false;
             const int box_rows = min(page, FINE_KEYS);
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
             // copies in flight end before the block does, whoever has given up
             if (tail_lost) pg_bar_wait(tail, tails & 1u);
             for (unsigned i = ld > (unsigned)SLOTS ? ld - SLOTS : 0; i < ld; i++) pg_bar_wait(&full[i % SLOTS], (i / SLOTS) & 1u);
-        } else if (CP == 3) {
+        } else if constexpr (std::is_same_v<CT, float>) {
             constexpr int CHUNKS = HDP / 8, ROWS_AT_ONCE = 128 / CHUNKS, N = FINE_KEYS / ROWS_AT_ONCE; // a thread: N pieces of 8 columns, of rows ROWS_AT_ONCE apart
             const int mine = tid - 128, chunk = mine % CHUNKS, row0 = mine / CHUNKS;
             while (w.left > 0) {
@@ -204,6 +204,39 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                         for (int k = 0; k < 3; k++)
                             *reinterpret_cast<uint4 *>(dst + k * TILE + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = make_uint4(p[0][k], p[1][k], p[2][k], p[3][k]);
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    pg_bar_arrive(&full[slot]);
+                }
+                w.next(a);
+            }
+        } else if constexpr (std::is_same_v<CT, Int4>) { // the codes, written as bfloat16 words
+            using Tile = Int4Tile<HDP, FINE_KEYS, 4>;
+            const Tile mine(warp - 4, lane);
+            while (w.left > 0) {
+                const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                const int tiles = w.tiles(item), begin = (item.t0 + w.first(item)) * FINE_KEYS;
+                int id[Tile::N];
+                typename Tile::Codes next;
+                bool next_v;
+                int next_pos = begin + load_of(0, tiles, &next_v) * FINE_KEYS;
+                mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
+                next_pos = begin + load_of(1, tiles, &next_v) * FINE_KEYS;
+                mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                for (int u = 0; u < 2 * tiles; u++, ld++) {
+                    const int slot = (int)(ld % SLOTS);
+                    const typename Tile::Codes codes = next;
+                    if (u + 1 < 2 * tiles) mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
+                    if (u + 2 < 2 * tiles) {
+                        next_pos = begin + load_of(u + 2, tiles, &next_v) * FINE_KEYS;
+                        mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                    }
+                    if (alive && !pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u)) {
+                        atomicExch(a.c.status, PAGED_WAIT);
+                        alive = false; // it goes on without waiting and without writing
+                    }
+                    if (!alive) continue;
+                    mine.put(ring + slot * SLOT, codes);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     pg_bar_arrive(&full[slot]);
                 }
@@ -498,11 +531,12 @@ cudaError_t launch_fine_as(const AttendCall &a, const ManyPlan &p, void *ws, int
     using Shape = FineShape<CT, HDP>;
     ManyCall f;
     f.a = a, f.part = static_cast<float *>(ws), f.head = reinterpret_cast<int *>(static_cast<float *>(ws) + p.part_floats);
-    alignas(64) CUtensorMap map_k, map_v;
+    alignas(64) CUtensorMap map_k = {}, map_v = {}; // (of a cache in 4 bits nothing is copied by them)
     const long long rows = ((long long)a.c.pages * a.c.kv) << a.c.page_shift;
     const int box = std::min(1 << a.c.page_shift, FINE_KEYS);
-    constexpr bool f32 = sizeof(CT) == 4;
-    if (!paged_map(&map_k, a.k, rows, a.c.hd, f32, box) || !paged_map(&map_v, a.v, rows, a.c.hd, f32, box)) return cudaErrorNotSupported;
+    constexpr bool f32 = std::is_same_v<CT, float>;
+    if constexpr (!std::is_same_v<CT, Int4>)
+        if (!paged_map(&map_k, a.k, rows, a.c.hd, f32, box) || !paged_map(&map_v, a.v, rows, a.c.hd, f32, box)) return cudaErrorNotSupported;
     static std::atomic<bool> known[64];
     if (device >= 64 || !known[device].load()) {
         const cudaError_t e = cudaFuncSetAttribute(attend_fine_kernel<CT, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);

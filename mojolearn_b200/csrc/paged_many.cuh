@@ -18,11 +18,14 @@
 // Measured, with what follows it: 2048 tokens behind 14336, 32 heads on 8 of 128, 588 us (876 TFLOP/s of 1627, at 990 of 1000 W); each stream's score,
 // softmax and sum follow one another, and two streams fill the tensor pipe to 0.54. 12 chunks of up to 509 tokens, window 1024, capped, 194 us.
 #pragma once
+#include <type_traits>
+
 #include "paged_few.cuh"
+#include "paged_int4.cuh"
 
 namespace b200i {
 
-constexpr int MANY_THREADS = 640, MANY_KEYS = 128; // two groups of four warps a stream, and one of which one warp copies and one issues
+constexpr int MANY_THREADS = 640, MANY_KEYS = 128, MANY_LOAD_WARPS = 3; // two groups of four warps a stream, and one of which one warp copies and one issues
 
 template <int HDP> struct ManyShape {
     static constexpr int TILE = HDP * 256;     // bytes of 128 rows of bfloat16
@@ -315,7 +318,7 @@ struct ManyCall {
 };
 
 // A row did not come out finite: it is done again by attend_again_kernel.
-__device__ __noinline__ void many_mark(int *at, int row) { atomicMin(at, row), atomicMax(at + 1, row); } // rows and heads of the output, one after another
+static __device__ __noinline__ void many_mark(int *at, int row) { atomicMin(at, row), atomicMax(at + 1, row); } // rows and heads of the output, one after another
 
 // 16 columns of an output that is there, or zeros.
 __device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some) {
@@ -328,11 +331,12 @@ __device__ __forceinline__ void many_output(unsigned *o, unsigned at, bool some)
     }
 }
 
-template <int HDP>
+template <typename CT, int HDP>
 __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ManyCall f) {
     using Shape = ManyShape<HDP>;
     constexpr int SLOTS = Shape::SLOTS, TILE = Shape::TILE, BOXES = HDP / 64, BR = Shape::BLOCK_ROWS, HALF_COLS = 128 * 128; // bytes of a tile's 64 columns
-    using T = __nv_bfloat16; // of rows and cache
+    using T = __nv_bfloat16; // of rows, and of keys and values in shared memory
+    constexpr bool FOUR = std::is_same_v<CT, Int4>;
     using Walk = ManyWalk<BR, MANY_KEYS, 2>;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *query = smem + ((1024u - (pg_smem(smem) & 1023u)) & 1023u), *ring = query + Shape::QUERY;
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     if (tid == 0) {
         for (int i = 0; i < 8; i++) pg_bar_init(&pair_bars[i], 64);
         for (int s = 0; s < SLOTS; s++) {
-            pg_bar_init(&full[s], 1);
+            pg_bar_init(&full[s], FOUR ? 32 * MANY_LOAD_WARPS : 1);
             pg_bar_init(&empty[s], 1);
         }
         for (int i = 0; i < 2; i++) {
@@ -378,20 +382,62 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     w.begin(a, line);
 
     if (warp >= 16) { // apart in this order: with the three as one chain of conditions the compiler's code took 190 us for 186 (12 chunks, capped)
-        if (warp == 16) { // ---------------- the copies ----------------
+        // keys and values in the order of their first use: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 K3 ... where the streams have tiles of their own
+        const auto load_of = [](int u, int tiles, int lead, bool *is_v) {
+            const int v = u - lead; // after the first keys: values, then keys, as long as there are any
+            const bool paired = v < 2 * (tiles - lead);
+            *is_v = v >= 0 && (paired ? (v & 1) == 0 : true);
+            return v < 0 ? u : (paired ? (*is_v ? v / 2 : v / 2 + lead) : (tiles - lead) + (v - 2 * (tiles - lead)));
+        };
+        if (FOUR && warp != 17) { // ---------------- the cache's codes, written as bfloat16 words ----------------
+            if constexpr (FOUR) {
+                using Tile = Int4Tile<HDP, MANY_KEYS, MANY_LOAD_WARPS>;
+                const Tile mine(warp == 16 ? 0 : warp - 17, lane);
+                unsigned ld = 0;
+                bool alive = true;
+                while (w.left > 0) {
+                    const ManyItem item = w.item(a, paged_seq(a.c, w.b));
+                    const int tiles = w.tiles(item), begin = (item.t0 + w.first(item)) * MANY_KEYS, lead = min(item.pair ? 1 : 2, tiles);
+                    int id[Tile::N];
+                    typename Tile::Codes next;
+                    bool next_v;
+                    int next_pos = begin + load_of(0, tiles, lead, &next_v) * MANY_KEYS;
+                    mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                    mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
+                    next_pos = begin + load_of(1, tiles, lead, &next_v) * MANY_KEYS;
+                    mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                    for (int u = 0; u < 2 * tiles; u++, ld++) {
+                        const int slot = (int)(ld % SLOTS);
+                        const typename Tile::Codes codes = next;
+                        if (u + 1 < 2 * tiles) mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
+                        if (u + 2 < 2 * tiles) {
+                            next_pos = begin + load_of(u + 2, tiles, lead, &next_v) * MANY_KEYS;
+                            mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                        }
+                        if (alive && !pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u)) {
+                            atomicExch(a.c.status, PAGED_WAIT);
+                            alive = false; // it goes on without waiting and without writing
+                        }
+                        if (!alive) continue;
+                        mine.put(ring + slot * TILE, codes);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        pg_bar_arrive(&full[slot]);
+                    }
+                    w.next(a);
+                }
+                __syncwarp();
+            }
+        } else if (warp == 16) { // ---------------- the copies ----------------
             unsigned ld = 0, tails = 0;
             bool alive = true, tail_lost = false;
             while (w.left > 0 && alive) {
                 const ManyItem item = w.item(a, paged_seq(a.c, w.b));
                 const int tiles = w.tiles(item), first = w.first(item), last_page = (item.high - 1) >> a.c.page_shift;
                 const int *ids = a.c.table + (long long)w.b * a.c.max_pages;
-                // in the order of their first use: K0 V0 K1 V1 ..., or K0 K1 V0 K2 V1 K3 ... where the streams have tiles of their own
                 const int lead = min(item.pair ? 1 : 2, tiles);
                 for (int u = 0; u < 2 * tiles && alive; u++, ld++) {
-                    const int v = u - lead; // after the first keys: values, then keys, as long as there are any
-                    const bool paired = v < 2 * (tiles - lead);
-                    const bool is_v = v >= 0 && (paired ? (v & 1) == 0 : true);
-                    const int tile = v < 0 ? u : (paired ? (is_v ? v / 2 : v / 2 + lead) : (tiles - lead) + (v - 2 * (tiles - lead)));
+                    bool is_v;
+                    const int tile = load_of(u, tiles, lead, &is_v);
                     const int slot = (int)(ld % SLOTS), pos = (item.t0 + first + tile) * MANY_KEYS;
                     if (!__all_sync(0xFFFFFFFFu, pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u))) {
                         if (lane == 0) atomicExch(a.c.status, PAGED_WAIT);
@@ -890,23 +936,24 @@ cudaError_t many_after(const ManyCall &f, int blocks, cudaStream_t st, int *laun
     return e != cudaSuccess ? e : launch_following<ManyCall>(attend_again_kernel<RT, CT, BR, KEYS, STREAMS>, dim3(blocks, 8), 256, st, f);
 }
 
-template <int HDP>
+template <typename CT, int HDP>
 cudaError_t launch_many_as(const AttendCall &a, const ManyPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
     using Shape = ManyShape<HDP>;
     ManyCall f;
     f.a = a, f.part = static_cast<float *>(ws), f.head = reinterpret_cast<int *>(static_cast<float *>(ws) + p.part_floats);
-    alignas(64) CUtensorMap map_k, map_v;
+    alignas(64) CUtensorMap map_k = {}, map_v = {}; // (of a cache in 4 bits nothing is copied by them)
     const long long rows = ((long long)a.c.pages * a.c.kv) << a.c.page_shift;
     const int box = std::min(1 << a.c.page_shift, MANY_KEYS);
-    if (!paged_map(&map_k, a.k, rows, a.c.hd, false, box) || !paged_map(&map_v, a.v, rows, a.c.hd, false, box)) return cudaErrorNotSupported;
+    if constexpr (!std::is_same_v<CT, Int4>)
+        if (!paged_map(&map_k, a.k, rows, a.c.hd, false, box) || !paged_map(&map_v, a.v, rows, a.c.hd, false, box)) return cudaErrorNotSupported;
     static std::atomic<bool> known[64];
     if (device >= 64 || !known[device].load()) {
-        const cudaError_t e = cudaFuncSetAttribute(attend_many_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+        const cudaError_t e = cudaFuncSetAttribute(attend_many_kernel<CT, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
         if (e != cudaSuccess) return e;
         if (device < 64) known[device].store(true);
     }
-    attend_many_kernel<HDP><<<p.blocks, MANY_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
-    return many_after<__nv_bfloat16, __nv_bfloat16, HDP, Shape::BLOCK_ROWS, MANY_KEYS, 2>(f, p.blocks, st, launches);
+    attend_many_kernel<CT, HDP><<<p.blocks, MANY_THREADS, Shape::SMEM, st>>>(map_k, map_v, f);
+    return many_after<__nv_bfloat16, CT, HDP, Shape::BLOCK_ROWS, MANY_KEYS, 2>(f, p.blocks, st, launches);
 }
 
 } // namespace b200i

@@ -5,8 +5,9 @@ new tokens of any open sequences, a decode step's single tokens and chunks of pr
 the model's own products, norms and embedding one after another, and `paged.append` and `paged.attention` place and read keys
 and values sequence by sequence. Pages are taken as sequences grow and given back when they are closed.
 
-Keys and values are bfloat16 (half the memory and traffic of a decode step) or float32. Either way the attention's sums run in an
-order of the kernels' own choice, so logits agree with `CausalLM`'s to rounding, not to the bit.
+Keys and values are float32, bfloat16 (half the memory and traffic of a decode step) or "int4" (4.5 bits a word, a seventh of them: see `paged`
+for how a word is rounded). Either way the attention's sums run in an order of the kernels' own choice, so logits agree with `CausalLM`'s to rounding, not
+to the bit, and in 4 bits to what is left of its keys and values.
 """
 import numpy as np
 import torch
@@ -14,7 +15,7 @@ import torch
 from .. import _native, paged
 from ..transformer import NORM_KINDS, _stream, _vp, add, add_norm, norm
 
-CACHES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
+CACHES = {"bfloat16": torch.bfloat16, "float32": torch.float32, "int4": "int4"}
 
 
 def _integers(x):

@@ -2,8 +2,8 @@
 
 `append` takes the fresh query, key and value rows of a call, norms queries and keys per head where the model does,
 rotates them to their positions and places keys and values in the cache's pages; `attention` is the attention of the
-rotated queries over the pages: a prompt, a chunk of new tokens behind what is cached, or a decode step's single tokens.
-`PagedCache` keeps the pool of pages and hands them to sequences.
+rotated queries over the pages: a prompt, a chunk of new tokens behind what is cached, or a decode step's single tokens;
+`read` gives rows of the cache back. `PagedCache` keeps the pool of pages and hands them to sequences.
 
 The reference keeps one contiguous cache per batch (`TransformerState`, `_transformer_impl.py:194-236`) and has none of
 this. It is not part of the identical-mode contract either: sums run in 32 bits in an order that the kernels choose (the
@@ -14,7 +14,13 @@ Layout. A cache is `[pages, n_kv_heads, page, head_dim]`, keys and values apart,
 positions. The rows of all sequences stand one after another: sequence b's are `cu[b]:cu[b + 1]`, and `lengths[b]` counts
 what its cache holds with them, so that its last row is at position `lengths[b] - 1`. `cu`, `lengths` and `page_table` are
 device tensors and are read by the kernels only, so a call can be captured in a CUDA graph and replayed after they have
-changed. Rows and cache are float32 and float32, float32 and bfloat16, or bfloat16 and bfloat16.
+changed. Rows and cache are float32 and float32, float32 and bfloat16, or bfloat16 and bfloat16, and either with a cache in 4 bits.
+
+A cache in 4 bits is uint8 `[pages, n_kv_heads, page, row_bytes(head_dim)]`. A head's columns go by groups of 32 (a last one filled up with zeros): a
+column is a whole number from -7 to 7 and a group has a bfloat16 scale of five significant bits, the smallest (from 2^-100 to 2^90) of which 7 reach its
+largest magnitude; a key or value x is held as the whole number nearest to x / scale, ties to even, of the 64-bit value of x. The product of the two is
+a bfloat16 word, so what is held is rounded once and by nothing that reads it. A group with a word that is not finite is held as NaN; words beyond
+8.6e27 are cut to that. `include/b200i.h` gives the order of the bytes.
 
 Calls are asynchronous on the current stream. A page number outside the pool is treated as a page of zeros and not written; a
 sequence with more positions than its row of the page table has room for, or with offsets that are not the call's, is left
@@ -29,6 +35,7 @@ from . import _native
 from .torch_ops import _bind_host_call, _host_call, _on, _stream, _vp
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
+_CACHES = {torch.float32: 0, torch.bfloat16: 1, torch.uint8: 2}
 _NORMS = {"rmsnorm": 0, "rmsnorm_offset": 2}
 
 
@@ -42,7 +49,12 @@ def _bind(name):
 
 
 #: the calls on plain device tensors in native code, or None where a call is anything else: those go through the checks below
-_plain_append, _plain_attention = _bind("append"), _bind("attention")
+_plain_append, _plain_attention, _plain_read = _bind("append"), _bind("attention"), _bind("read")
+
+
+def row_bytes(head_dim):
+    """Bytes that a position of a head takes in a cache of 4 bits: 18 for each group of 32 columns."""
+    return -(-int(head_dim) // 32) * 18
 
 
 def _rows(t, name, heads, head_dim, dtype, device, total):
@@ -60,7 +72,7 @@ def _rows(t, name, heads, head_dim, dtype, device, total):
     return t.stride(0) if t.shape[0] > 1 else heads * head_dim
 
 
-def _cache(k_cache, v_cache, page_table, cu, lengths, row_dtype, device):
+def _cache(k_cache, v_cache, page_table, cu, lengths, row_dtype, device, head_dim):
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache"), (page_table, "page_table"), (cu, "cu"), (lengths, "lengths")):
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise TypeError("%s must be a CUDA tensor" % name)
@@ -68,11 +80,13 @@ def _cache(k_cache, v_cache, page_table, cu, lengths, row_dtype, device):
             raise ValueError("operands live on different devices")
         if not t.is_contiguous():
             raise ValueError("%s must be contiguous" % name)
-    if k_cache.dtype not in _TYPES or v_cache.dtype != k_cache.dtype or (row_dtype == torch.bfloat16 and k_cache.dtype != row_dtype):
-        raise TypeError("rows and caches must be float32 and float32, float32 and bfloat16, or bfloat16 and bfloat16: got %s, %s and %s" %
+    if k_cache.dtype not in _CACHES or v_cache.dtype != k_cache.dtype or (row_dtype == torch.bfloat16 and k_cache.dtype == torch.float32):
+        raise TypeError("rows and caches must be float32 and float32, float32 and bfloat16, bfloat16 and bfloat16, or either and uint8 (4 bits): got %s, %s and %s" %
                         (row_dtype, k_cache.dtype, v_cache.dtype))
     if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
         raise ValueError("the caches must both be (pages, n_kv_heads, page, head_dim)")
+    if k_cache.dtype == torch.uint8 and k_cache.shape[3] != row_bytes(head_dim):
+        raise ValueError("a cache in 4 bits must be (pages, n_kv_heads, page, %d) for a head_dim of %d, got %s" % (row_bytes(head_dim), head_dim, tuple(k_cache.shape)))
     for t, name in ((page_table, "page_table"), (cu, "cu"), (lengths, "lengths")):
         if t.dtype != torch.int32:
             raise TypeError("%s must be int32, got %s" % (name, t.dtype))
@@ -93,6 +107,14 @@ def _vector(t, name, n, device):
 @functools.lru_cache(maxsize=None)
 def _scale(head_dim):
     return 1.0 / math.sqrt(max(head_dim, 1))
+
+
+def _head_dim(q, k_cache):
+    """The columns of a head: what a cache of words has, or the rows of one in 4 bits."""
+    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _TYPES:
+        raise TypeError("q must be a float32 or bfloat16 CUDA tensor")
+    four = isinstance(k_cache, torch.Tensor) and k_cache.dtype == torch.uint8
+    return (q if four else k_cache).shape[-1] if isinstance(k_cache, torch.Tensor) and q.dim() and k_cache.dim() else 0
 
 
 def _out(out, q):
@@ -116,10 +138,9 @@ def append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos=None, sin=Non
         done = _plain_append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos, sin, q_norm, k_norm, eps, _NORMS[norm])
         if done is not None:
             return done
-    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _TYPES:
-        raise TypeError("q must be a float32 or bfloat16 CUDA tensor")
-    _cache(k_cache, v_cache, page_table, cu, lengths, q.dtype, q.device)
-    pages, n_kv, page, hd = k_cache.shape
+    hd = _head_dim(q, k_cache)
+    _cache(k_cache, v_cache, page_table, cu, lengths, q.dtype, q.device, hd)
+    pages, n_kv, page, _ = k_cache.shape
     rows, n_heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
     ldq = _rows(q, "q", n_heads, hd, q.dtype, q.device, rows)
     ldk, ldv = _rows(k, "k", n_kv, hd, q.dtype, q.device, rows), _rows(v, "v", n_kv, hd, q.dtype, q.device, rows)
@@ -143,7 +164,7 @@ def append(q, k, v, k_cache, v_cache, page_table, cu, lengths, cos=None, sin=Non
         return out
     with _on(q.device):
         _native.call("b200i_paged_append", q.device.index, _stream(q.device), _vp(out), _vp(k_cache), _vp(v_cache), _vp(q), _vp(k), _vp(v), ldq, ldk, ldv,
-                     _TYPES[q.dtype], _TYPES[k_cache.dtype], _vp(cos), _vp(sin), 2 * half, positions, _vp(q_norm), _vp(k_norm), float(eps), _NORMS[norm],
+                     _TYPES[q.dtype], _CACHES[k_cache.dtype], _vp(cos), _vp(sin), 2 * half, positions, _vp(q_norm), _vp(k_norm), float(eps), _NORMS[norm],
                      _vp(page_table), _vp(cu), _vp(lengths), rows, lengths.shape[0], n_heads, n_kv, hd, pages, page, page_table.shape[1])
     return out
 
@@ -160,10 +181,9 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
         done = _plain_attention(q, k_cache, v_cache, page_table, cu, lengths, max_new, max_length, _scale(q.shape[-1] if q.dim() else 1) if scale is None else scale, window, softcap)
         if done is not None:
             return done
-    if not isinstance(q, torch.Tensor) or not q.is_cuda or q.dtype not in _TYPES:
-        raise TypeError("q must be a float32 or bfloat16 CUDA tensor")
-    _cache(k_cache, v_cache, page_table, cu, lengths, q.dtype, q.device)
-    pages, n_kv, page, hd = k_cache.shape
+    hd = _head_dim(q, k_cache)
+    _cache(k_cache, v_cache, page_table, cu, lengths, q.dtype, q.device, hd)
+    pages, n_kv, page, _ = k_cache.shape
     rows, n_heads, batch, max_pages = q.shape[0], q.shape[1] if q.dim() == 3 else 0, lengths.shape[0], page_table.shape[1]
     ldq = _rows(q, "q", n_heads, hd, q.dtype, q.device, rows)
     max_new = max(rows, 1) if max_new is None else int(max_new)
@@ -172,7 +192,7 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
     if rows == 0:
         return out
     with _on(q.device):
-        types = _TYPES[q.dtype], _TYPES[k_cache.dtype]
+        types = _TYPES[q.dtype], _CACHES[k_cache.dtype]
         need = int(_native.lib().b200i_paged_attention_workspace_bytes(q.device.index, *types, rows, batch, n_heads, n_kv, hd, max_new, max_length, int(window)))
         ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
         _native.call("b200i_paged_attention", q.device.index, _stream(q.device), _vp(out), _vp(q), ldq, _vp(k_cache), _vp(v_cache), *types, _vp(page_table), _vp(cu),
@@ -181,16 +201,53 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
     return out
 
 
+def read(k_cache, v_cache, page_table, cu, lengths, *, rows, head_dim=None, dtype=None):
+    """What the caches hold at the positions of `rows` rows: keys and values [rows, n_kv_heads, head_dim]. Sequence b's rows are cu[b]:cu[b + 1], the last
+    of its lengths[b] positions as in a call that wrote them; with `cu` the running sums of `lengths` they are all of each sequence.
+
+    `head_dim` is the caches' own unless they are in 4 bits. `dtype` is float32 or, of caches in bfloat16 and 4 bits, bfloat16, which holds what they
+    hold exactly and is the default there. A row at a position before the first, or in a page outside the pool, is zeros; rows past cu[-1] are not written."""
+    if not isinstance(k_cache, torch.Tensor) or not k_cache.is_cuda or k_cache.dtype not in _CACHES:
+        raise TypeError("k_cache must be a float32, bfloat16 or uint8 CUDA tensor")
+    four = k_cache.dtype == torch.uint8
+    if head_dim is None:
+        if four:
+            raise ValueError("a cache in 4 bits does not say what its head_dim is")
+        head_dim = k_cache.shape[-1]
+    if dtype is None:
+        dtype = torch.bfloat16 if four else k_cache.dtype
+    if dtype not in _TYPES:
+        raise TypeError("rows are read as float32 or bfloat16, got %s" % (dtype,))
+    if _plain_read is not None:
+        done = _plain_read(k_cache, v_cache, page_table, cu, lengths, rows, head_dim, _TYPES[dtype])
+        if done is not None:
+            return done
+    rows, head_dim, device = int(rows), int(head_dim), k_cache.device
+    _cache(k_cache, v_cache, page_table, cu, lengths, dtype, device, head_dim)
+    pages, n_kv, page, width = k_cache.shape
+    if not four and width != head_dim:
+        raise ValueError("the caches have a head_dim of %d, not %d" % (width, head_dim))
+    if rows < 0:
+        raise ValueError("rows must not be negative, got %d" % rows)
+    k, v = (torch.empty((rows, n_kv, head_dim), dtype=dtype, device=device) for _ in range(2))
+    if rows == 0:
+        return k, v
+    with _on(device):
+        _native.call("b200i_paged_read", device.index, _stream(device), _vp(k), _vp(v), _vp(k_cache), _vp(v_cache), _TYPES[dtype], _CACHES[k_cache.dtype],
+                     _vp(page_table), _vp(cu), _vp(lengths), rows, lengths.shape[0], n_kv, head_dim, pages, page, page_table.shape[1])
+    return k, v
+
+
 class PagedCache(object):
     """A pool of pages for the layers of one model, and the sequences that hold them.
 
     `open()` begins a sequence, `extend(sequences, counts)` takes the pages that so many further tokens of each need and gives the
     (page_table, cu, lengths) of a call over them, `close(sequence)` gives its pages back. All layers share the page numbers; `k[i]`
-    and `v[i]` are layer i's caches. Sequences and free pages are kept on the host, so nothing here waits for the device."""
+    and `v[i]` are layer i's caches, of words of `dtype` or, with dtype "int4", in 4 bits. Sequences and free pages are kept on the host, so nothing here waits for the device."""
 
     def __init__(self, n_pages, n_kv_heads, head_dim, *, page=64, layers=1, dtype=torch.bfloat16, device=None):
-        if dtype not in _TYPES:
-            raise TypeError("a cache is float32 or bfloat16, got %s" % dtype)
+        if dtype not in _TYPES and dtype != "int4":
+            raise TypeError("a cache is float32, bfloat16 or \"int4\", got %s" % (dtype,))
         if n_pages < 1 or layers < 1 or n_kv_heads < 1:
             raise ValueError("a cache has at least one page, one key head and one layer")
         if page < 16 or page > 256 or page & (page - 1):
@@ -200,9 +257,10 @@ class PagedCache(object):
         _native.require_device()
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.page, self.pages, self.dtype = int(page), int(n_pages), dtype
-        shape = (self.pages, int(n_kv_heads), self.page, int(head_dim))
-        self.k = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
-        self.v = [torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(layers)]
+        self.head_dim, four = int(head_dim), dtype == "int4"
+        shape = (self.pages, int(n_kv_heads), self.page, row_bytes(head_dim) if four else self.head_dim)
+        self.k = [torch.zeros(shape, dtype=torch.uint8 if four else dtype, device=self.device) for _ in range(layers)]
+        self.v = [torch.zeros(shape, dtype=torch.uint8 if four else dtype, device=self.device) for _ in range(layers)]
         self.free = list(range(self.pages - 1, -1, -1))
         self.held, self.length, self._next = {}, {}, 0
 
