@@ -205,7 +205,7 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     const AttendPlan p = attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
     if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
     if (cache_type == B200I_T_INT4) {
-        LIBRARY_CUDA_TRY(p.few ? int4_few(a, row_type == B200I_T_F32, p.cut, p.hdp, ws, dev, st, &launches) : int4_many(a, row_type == B200I_T_F32, p.cut_many, p.hdp, ws, dev, st, &launches));
+        LIBRARY_CUDA_TRY(p.few ? int4_few(a, row_type == B200I_T_F32, p.cut, ws, dev, st, &launches) : int4_many(a, row_type == B200I_T_F32, p.cut_many, p.hdp, ws, dev, st, &launches));
     } else if (p.few) {
         if (row_type == B200I_T_BF16)
             LIBRARY_CUDA_TRY((launch_few<__nv_bfloat16, __nv_bfloat16>(a, p.cut, p.hdp, ws, dev, st, &launches)));

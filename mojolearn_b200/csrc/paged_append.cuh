@@ -194,22 +194,10 @@ __global__ void __launch_bounds__(128) append_units_kernel(const AppendCall a, i
     }
 }
 
-// Rotations whose halves are not whole units (a partial rotation of few columns), or tables and weights that are not 16-byte aligned: a warp a head, a
-// column a lane.
-template <typename RT, typename CT>
-__global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a) {
-    const long long t = blockIdx.x;
-    const int lane = threadIdx.x & 31, b = paged_row_seq(a.c, t);
-    int head = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (b < 0 || head >= a.c.heads + 2 * a.c.kv) return;
-    const PagedSeq s = paged_seq_checked(a.c, b);
-    if (s.n == 0) return; // its tables do not hold it
-    const int pos = s.pos0 + (int)(t - s.first), part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2);
-    if (append_past(a, pos)) return;
-    head -= part == 0 ? 0 : (part == 1 ? a.c.heads : a.c.heads + a.c.kv);
-    const RT *src = part == 0 ? static_cast<const RT *>(a.q) + t * a.ldq : (part == 1 ? static_cast<const RT *>(a.k) + t * a.ldk : static_cast<const RT *>(a.v) + t * a.ldv);
-    src += (long long)head * a.c.hd;
-    const float *w = part == 0 ? a.q_norm : (part == 1 ? a.k_norm : nullptr);
+// A head's columns by a warp, a column a lane: normed by w (nullptr: not) and, where it turns, rotated to pos.
+template <typename RT, typename DT>
+__device__ __forceinline__ void append_columns(const AppendCall &a, const RT *src, const float *w, int pos, bool turns, DT *dst) {
+    const int lane = threadIdx.x & 31;
     float r = 1.0f;
     if (w) {
         float sum = 0.0f;
@@ -219,9 +207,6 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
         }
         r = 1.0f / sqrtf(paged_warp_sum(sum) / (float)a.c.hd + a.eps);
     }
-    RT *dst_row;
-    CT *dst_cache;
-    if (!append_place<RT, CT>(a, t, b, pos, part, head, &dst_row, &dst_cache)) return;
     const int half = a.rope_dim / 2;
     const long long row = (long long)max(pos, 0) * half;
     float out[PAGED_MAX_HD / 32];
@@ -231,7 +216,7 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
         if (i >= a.c.hd) break;
         float x = paged_read(src + i);
         if (w) x = x * r * (w[i] + a.norm_shift);
-        if (part < 2 && a.cosv && i < a.rope_dim) {
+        if (turns && a.cosv && i < a.rope_dim) {
             const int j = i < half ? i : i - half, p = i < half ? i + half : i - half;
             float y = paged_read(src + p);
             if (w) y = y * r * (w[p] + a.norm_shift);
@@ -245,27 +230,59 @@ __global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a)
     for (int k = 0; k < PAGED_MAX_HD / 32; k++) {
         const int i = lane + 32 * k;
         if (i >= a.c.hd) break;
-        if (dst_row)
-            paged_write(dst_row + i, out[k]);
-        else
-            paged_write(dst_cache + i, out[k]);
+        paged_write(dst + i, out[k]);
     }
+}
+
+// Rotations whose halves are not whole units (a partial rotation of few columns), or tables and weights that are not 16-byte aligned.
+template <typename RT, typename CT>
+__global__ void __launch_bounds__(256) append_columns_kernel(const AppendCall a) {
+    const long long t = blockIdx.x;
+    const int b = paged_row_seq(a.c, t);
+    int head = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (b < 0 || head >= a.c.heads + 2 * a.c.kv) return;
+    const PagedSeq s = paged_seq_checked(a.c, b);
+    if (s.n == 0) return; // its tables do not hold it
+    const int pos = s.pos0 + (int)(t - s.first), part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2);
+    if (append_past(a, pos)) return;
+    head -= part == 0 ? 0 : (part == 1 ? a.c.heads : a.c.heads + a.c.kv);
+    const RT *src = part == 0 ? static_cast<const RT *>(a.q) + t * a.ldq : (part == 1 ? static_cast<const RT *>(a.k) + t * a.ldk : static_cast<const RT *>(a.v) + t * a.ldv);
+    src += (long long)head * a.c.hd;
+    const float *w = part == 0 ? a.q_norm : (part == 1 ? a.k_norm : nullptr);
+    RT *dst_row;
+    CT *dst_cache;
+    if (!append_place<RT, CT>(a, t, b, pos, part, head, &dst_row, &dst_cache)) return;
+    if (dst_row)
+        append_columns<RT, RT>(a, src, w, pos, true, dst_row);
+    else
+        append_columns<RT, CT>(a, src, w, pos, part < 2, dst_cache);
+}
+
+// Whether a call's heads go by units, and how they are cut: lanes a head, sets of heads a row, blocks a row.
+template <int N> bool append_by_units(const AppendCall &a) {
+    const uintptr_t words = reinterpret_cast<uintptr_t>(a.cosv) | reinterpret_cast<uintptr_t>(a.sinv) | reinterpret_cast<uintptr_t>(a.q_norm) | reinterpret_cast<uintptr_t>(a.k_norm);
+    return (a.rope_dim / 2) % N == 0 && (a.c.hd - a.rope_dim) % N == 0 && words % 16 == 0;
+}
+struct AppendCut {
+    int lanes_log2, sets, blocks;
+};
+template <int N> AppendCut append_cut(const AppendCall &a, int parts, int sms) {
+    const int need = a.rope_dim / 2 / N + ((a.c.hd - a.rope_dim) / N + 1) / 2;
+    int lg = 0;
+    while ((1 << lg) < need) lg++;
+    // with a few rows a warp takes one set of heads, so that none waits for another's; with many it takes all that the blocks of a row leave it
+    const int per_set = 32 >> lg, sets = (parts + per_set - 1) / per_set, blocks = (sets + 3) / 4;
+    const long long room = 8LL * sms; // blocks that fill the device
+    return {lg, sets, (int)std::max<long long>(1, std::min<long long>(blocks, room / a.c.rows))};
 }
 
 template <typename RT, typename CT>
 cudaError_t launch_append(const AppendCall &a, int sms, cudaStream_t st) {
     constexpr int N = Unit<RT>::N;
     const int parts = a.c.heads + 2 * a.c.kv;
-    const uintptr_t words = reinterpret_cast<uintptr_t>(a.cosv) | reinterpret_cast<uintptr_t>(a.sinv) | reinterpret_cast<uintptr_t>(a.q_norm) | reinterpret_cast<uintptr_t>(a.k_norm);
-    if ((a.rope_dim / 2) % N == 0 && (a.c.hd - a.rope_dim) % N == 0 && words % 16 == 0) {
-        const int need = a.rope_dim / 2 / N + ((a.c.hd - a.rope_dim) / N + 1) / 2;
-        int lg = 0;
-        while ((1 << lg) < need) lg++;
-        // with a few rows a warp takes one set of heads, so that none waits for another's; with many it takes all that the blocks of a row leave it
-        const int per_set = 32 >> lg, sets = (parts + per_set - 1) / per_set, blocks = (sets + 3) / 4;
-        const long long room = 8LL * sms; // blocks that fill the device
-        const int y = (int)std::max<long long>(1, std::min<long long>(blocks, room / a.c.rows));
-        append_units_kernel<RT, CT><<<dim3((unsigned)a.c.rows, (unsigned)y), 128, 0, st>>>(a, lg, sets);
+    if (append_by_units<N>(a)) {
+        const AppendCut cut = append_cut<N>(a, parts, sms);
+        append_units_kernel<RT, CT><<<dim3((unsigned)a.c.rows, (unsigned)cut.blocks), 128, 0, st>>>(a, cut.lanes_log2, cut.sets);
     } else {
         append_columns_kernel<RT, CT><<<dim3((unsigned)a.c.rows, (unsigned)((parts + 7) / 8)), 256, 0, st>>>(a);
     }

@@ -4,9 +4,9 @@
 // it of (the norm's sum, root and products: 2^-21.4; the rotation's: 2^-23), so where the largest magnitude of a group, or a word, is nearer than that to a border between
 // two scales or codes (about one group in 5000), the warp's keys are done again in 64 bits. Values, and keys without norm and rotation, have no such error: what a
 // code leaves is computed exactly.
-// Bound: HBM, and latency for a few rows. A lane takes four columns, eight lanes a group: its largest magnitude is three steps across lanes, and the partner of a rotated
-// column is in the lane half a rotation away. Rotations whose halves are not whole lanes, and tables that are not on 16-byte boundaries, go by a warp a head with a column of
-// each group a lane, keys and values in 64 bits.
+// Bound: HBM, and latency for a few rows. A lane takes the unit pairs of paged_append.cuh; the units of a group are in neighbouring lanes where half a rotation is
+// whole groups, and looked up else. What is not a warp's units goes by a warp a head, a column of each group a lane, in 64 bits: rotations whose halves are not whole
+// units, tables that are not on 16-byte boundaries, and the keys that are done again.
 #pragma once
 #include "paged_append.cuh"
 #include "paged_int4.cuh"
@@ -32,188 +32,13 @@ __device__ __forceinline__ bool append4_place(Append4Place *at, const PagedCall 
     return true;
 }
 
-template <typename T> struct Four4; // four columns of a row
-template <> struct Four4<float> {
-    using Raw = float4;
-    static __device__ __forceinline__ float4 words(const Raw &r) { return r; }
-    static __device__ __forceinline__ void store(float *p, const float (&x)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(x[0], x[1], x[2], x[3]); }
-};
-template <> struct Four4<__nv_bfloat16> {
-    using Raw = uint2;
-    static __device__ __forceinline__ float4 words(const Raw &r) { return PagedWords<__nv_bfloat16>::words(r); }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, const float (&x)[4]) { *reinterpret_cast<uint2 *>(p) = make_uint2(pg_pack(x[0], x[1]), pg_pack(x[2], x[3])); }
-};
-
-// Codes and scale of the lane's four columns by the 64-bit words of its key. All lanes; `lanes` of them a head.
-struct Append4Exact {
-    float x[4], w[4], c[4], sn[4];
-    float shift;
-    int lanes, from, sign; // the partner's lane, and whether the lane's columns are the rotation's first half (-1), its second (1) or none (0)
-    bool normed;
-    double eps;
-    int hd;
-};
-struct Append4Codes {
-    float n[4], scale;
-};
-static __device__ __noinline__ Append4Codes append4_exact(const Append4Exact &e) {
-    double x[4], y[4];
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < 4; i++) x[i] = e.x[i], sum = fma(x[i], x[i], sum);
-    if (e.normed) {
-        for (int o = e.lanes >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        const double r = sqrt(sum / (double)e.hd + e.eps);
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = x[i] / r * ((double)e.w[i] + (double)e.shift);
-    }
-    double most = 0.0;
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const double other = __shfl_sync(0xFFFFFFFFu, x[i], e.from);
-        y[i] = e.sign == 0 ? x[i] : fma(x[i], (double)e.c[i], (double)e.sign * (other * (double)e.sn[i]));
-        odd |= !(fabs(y[i]) <= 3.4e38);
-        most = fmax(most, fabs(y[i]));
-    }
-    if (odd) most = INFINITY;
-    for (int o = 1; o < 8; o <<= 1) most = fmax(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-    Append4Codes r;
-    r.scale = int4_scale(most);
-#pragma unroll
-    for (int i = 0; i < 4; i++) r.n[i] = r.scale == r.scale ? int4_code(y[i], r.scale) : 0.0f;
-    return r;
-}
-
-// blockIdx.x: the row; its heads in sets of 32 >> lanes_log2, a set a warp, by steps of the warps of gridDim.y blocks.
+// A row's head of keys or values (part 1 or 2) by a warp, in 64 bits: lane i has columns i, i + 32, ...
 template <typename RT>
-__global__ void __launch_bounds__(128) append_int4_kernel(const Append4Call f, int lanes_log2, int sets) {
-    using W = Four4<RT>;
+__device__ __noinline__ void append4_head(const Append4Call &f, long long t, int part, int head, int pos, const Append4Place &place) {
     const AppendCall &a = f.a;
-    const long long t = blockIdx.x;
-    const int all = threadIdx.x & 31, lane = all & ((1 << lanes_log2) - 1), in_set = all >> lanes_log2, col = 4 * lane;
-    const bool some = col < a.c.hd;
-    const int half = a.rope_dim / 2, parts = a.c.heads + 2 * a.c.kv;
-    const RT *const q = static_cast<const RT *>(a.q) + t * a.ldq, *const k = static_cast<const RT *>(a.k) + t * a.ldk, *const v = static_cast<const RT *>(a.v) + t * a.ldv;
-    typename W::Raw raw;
-    const auto ask = [&](int set) {
-        const int head = (set << (5 - lanes_log2)) + in_set;
-        const RT *src = head < a.c.heads ? q + head * a.c.hd : (head < a.c.heads + a.c.kv ? k + (head - a.c.heads) * a.c.hd : v + (head - a.c.heads - a.c.kv) * a.c.hd);
-        raw = {};
-        if (head < parts && some) raw = __ldg(reinterpret_cast<const typename W::Raw *>(src + col));
-    };
-    int set = blockIdx.y * 4 + (threadIdx.x >> 5);
-    const int step = gridDim.y * 4;
-    if (set < sets) ask(set);
-
-    const int b = paged_row_seq(a.c, t);
-    if (b < 0) return; // a row of no sequence: nothing is written for it
-    const PagedSeq s = paged_seq_checked(a.c, b);
-    if (s.n == 0) return; // its tables do not hold it
-    const int pos = s.pos0 + (int)(t - s.first);
-    if (append_past(a, pos)) return;
-    Append4Place place;
-    const bool placed = append4_place(&place, a.c, b, pos);
-    // The rotation: y = x c -+ other s, the other word being half a rotation of columns away.
-    const bool turns = a.cosv != nullptr && col < a.rope_dim;
-    const int sign = !turns ? 0 : (col < half ? -1 : 1), from = !turns ? all : (col < half ? all + half / 4 : all - half / 4);
-    float4 c = make_float4(1.0f, 1.0f, 1.0f, 1.0f), sn = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (turns) {
-        const long long row = (long long)max(pos, 0) * half + (col < half ? col : col - half);
-        c = __ldg(reinterpret_cast<const float4 *>(a.cosv + row)), sn = __ldg(reinterpret_cast<const float4 *>(a.sinv + row));
-    }
-    for (; set < sets; set += step) {
-        const int head = (set << (5 - lanes_log2)) + in_set, part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2); // q, k, v
-        const float4 r4 = W::words(raw);
-        float x[4] = {r4.x, r4.y, r4.z, r4.w}, y[4];
-        if (set + step < sets) ask(set + step);
-        Append4Exact e;
-#pragma unroll
-        for (int i = 0; i < 4; i++) e.x[i] = x[i], e.w[i] = 0.0f;
-        const float *w = part == 0 ? a.q_norm : (part == 1 ? a.k_norm : nullptr);
-        if (a.q_norm || a.k_norm) { // uniform over the grid: the reduction is a warp's
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) sum = fmaf(x[i], x[i], sum);
-            for (int o = (1 << lanes_log2) >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            if (w && some) {
-                const float r = rsqrtf(fmaf(sum, a.part_of_head, a.eps));
-                const float4 w4 = __ldg(reinterpret_cast<const float4 *>(w + col));
-                e.w[0] = w4.x, e.w[1] = w4.y, e.w[2] = w4.z, e.w[3] = w4.w;
-#pragma unroll
-                for (int i = 0; i < 4; i++) x[i] *= (e.w[i] + a.norm_shift) * r;
-            }
-        }
-        const bool turned = part < 2 && sign != 0;
-        const float cs[4] = {c.x, c.y, c.z, c.w}, sns[4] = {sn.x, sn.y, sn.z, sn.w};
-        float off[4]; // how far a word may be from its 64-bit value
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float other = __shfl_sync(0xFFFFFFFFu, x[i], from);
-            y[i] = turned ? fmaf(x[i], cs[i], sign < 0 ? -(other * sns[i]) : other * sns[i]) : x[i];
-            off[i] = part == 1 && (w || turned) ? 0x1p-20f * (fabsf(x[i]) + (turned ? fabsf(other) : 0.0f)) : 0.0f;
-        }
-        if (part == 0 && some) W::store(static_cast<RT *>(a.q_out) + (t * a.c.heads + head) * a.c.hd + col, y);
-        if (!__any_sync(0xFFFFFFFFu, part > 0)) continue;
-        // ---- the codes ----
-        unsigned most = 0;
-        float most_off = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; i++) most = max(most, __float_as_uint(y[i]) & 0x7FFFFFFFu), most_off = fmaxf(most_off, off[i]); // (a NaN's bits are larger than an infinity's)
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
-            most_off = fmaxf(most_off, __shfl_xor_sync(0xFFFFFFFFu, most_off, o));
-        }
-        Append4Codes n;
-        n.scale = int4_scale(__uint_as_float(most));
-        const float before = __uint_as_float(__float_as_uint(n.scale) - 0x80000u), inverse = 1.0f / n.scale;
-        bool near = most_off > 0.0f && (7.0f * n.scale - __uint_as_float(most) <= most_off || __uint_as_float(most) - 7.0f * before <= most_off);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float left;
-            n.n[i] = int4_code(y[i], n.scale, inverse, &left);
-            near |= off[i] > 0.0f && fabsf(fabsf(left) - 0.5f * n.scale) <= off[i];
-        }
-        if (most >= 0x7F800000u) n.n[0] = n.n[1] = n.n[2] = n.n[3] = 0.0f, near = false;
-        if (__any_sync(0xFFFFFFFFu, near)) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) e.c[i] = cs[i], e.sn[i] = sns[i];
-            e.shift = a.norm_shift, e.lanes = 1 << lanes_log2, e.from = from, e.sign = turned ? sign : 0, e.normed = a.k_norm != nullptr, e.eps = f.eps, e.hd = a.c.hd;
-            const Append4Codes exact = append4_exact(e);
-            if (part == 1) n = exact; // (of values nothing is normed)
-        }
-        // a lane has the first or the last four of a word's eight columns
-        const unsigned shift = (lane & 1) * 8;
-        unsigned word = 0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) word |= (unsigned)((int)n.n[i] + 8) << (shift + 4 * (i >> 1) + 16 * (i & 1));
-        word |= __shfl_xor_sync(0xFFFFFFFFu, word, 1);
-        if (part == 0 || head >= parts || !placed || lane >= 8 * int4_groups(a.c.hd)) continue;
-        unsigned char *const cache = static_cast<unsigned char *>(part == 1 ? a.k_cache : a.v_cache) + place.head * (head - a.c.heads - (part == 1 ? 0 : a.c.kv));
-        if ((lane & 1) == 0) *reinterpret_cast<unsigned *>(cache + place.codes + 2 * lane) = word;
-        if ((lane & 7) == 0) *reinterpret_cast<unsigned short *>(cache + place.scales + 2 * (lane >> 3)) = (unsigned short)(__float_as_uint(n.scale) >> 16);
-    }
-}
-
-// Any rotation: a warp a head, lane i the columns i, i + 32, ...: group by group.
-template <typename RT>
-__global__ void __launch_bounds__(256) append_int4_columns_kernel(const Append4Call f) {
-    const AppendCall &a = f.a;
-    const long long t = blockIdx.x;
-    const int lane = threadIdx.x & 31, b = paged_row_seq(a.c, t);
-    int head = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (b < 0 || head >= a.c.heads + 2 * a.c.kv) return;
-    const PagedSeq s = paged_seq_checked(a.c, b);
-    if (s.n == 0) return; // its tables do not hold it
-    const int pos = s.pos0 + (int)(t - s.first), part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2);
-    if (append_past(a, pos)) return;
-    head -= part == 0 ? 0 : (part == 1 ? a.c.heads : a.c.heads + a.c.kv);
-    Append4Place place;
-    if (part > 0 && !append4_place(&place, a.c, b, pos)) return;
-    const RT *src = part == 0 ? static_cast<const RT *>(a.q) + t * a.ldq : (part == 1 ? static_cast<const RT *>(a.k) + t * a.ldk : static_cast<const RT *>(a.v) + t * a.ldv);
-    src += (long long)head * a.c.hd;
-    const float *w = part == 0 ? a.q_norm : (part == 1 ? a.k_norm : nullptr);
+    const int lane = threadIdx.x & 31;
+    const RT *src = (part == 1 ? static_cast<const RT *>(a.k) + t * a.ldk : static_cast<const RT *>(a.v) + t * a.ldv) + (long long)head * a.c.hd;
+    const float *w = part == 1 ? a.k_norm : nullptr;
     double root = 1.0;
     if (w) {
         double sum = 0.0;
@@ -228,51 +53,262 @@ __global__ void __launch_bounds__(256) append_int4_columns_kernel(const Append4C
     const int half = a.rope_dim / 2;
     const long long row = (long long)max(pos, 0) * half;
     const auto word = [&](int i) { return w ? (double)paged_read(src + i) / root * ((double)w[i] + (double)a.norm_shift) : (double)paged_read(src + i); };
-    double out[PAGED_MAX_HD / 32];
-#pragma unroll
-    for (int k = 0; k < PAGED_MAX_HD / 32; k++) {
+    unsigned char *const cache = static_cast<unsigned char *>(part == 1 ? a.k_cache : a.v_cache) + place.head * head;
+#pragma unroll 1
+    for (int k = 0; 32 * k < a.c.hd; k++) {
         const int i = lane + 32 * k;
-        out[k] = 0.0;
-        if (i >= a.c.hd) continue;
-        out[k] = word(i);
-        if (part < 2 && a.cosv && i < a.rope_dim) {
-            const int j = i < half ? i : i - half;
-            const double other = word(i < half ? i + half : i - half), c = a.cosv[row + j], sn = a.sinv[row + j];
-            out[k] = i < half ? fma(out[k], c, -(other * sn)) : fma(out[k], c, other * sn);
+        double y = 0.0;
+        if (i < a.c.hd) {
+            y = word(i);
+            if (part == 1 && a.cosv && i < a.rope_dim) {
+                const int j = i < half ? i : i - half;
+                const double other = word(i < half ? i + half : i - half), c = a.cosv[row + j], sn = a.sinv[row + j];
+                y = i < half ? fma(y, c, -(other * sn)) : fma(y, c, other * sn);
+            }
         }
-    }
-    __syncwarp(); // all is read before any of it is written: the queries may be rotated in their place
-    unsigned char *const cache = static_cast<unsigned char *>(part == 1 ? a.k_cache : a.v_cache) + (part > 0 ? place.head * head : 0);
-#pragma unroll
-    for (int k = 0; k < PAGED_MAX_HD / 32; k++) {
-        if (32 * k >= a.c.hd) break;
-        const int i = lane + 32 * k;
-        if (part == 0) {
-            if (i < a.c.hd) paged_write(static_cast<RT *>(a.q_out) + (t * a.c.heads + head) * a.c.hd + i, (float)out[k]);
-            continue;
-        }
-        double most = fabs(out[k]) <= 3.4e38 ? fabs(out[k]) : INFINITY;
+        double most = fabs(y) <= 3.4e38 ? fabs(y) : INFINITY;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
         const float scale = int4_scale(most);
-        const unsigned n = (unsigned)((int)(scale == scale ? int4_code(out[k], scale) : 0.0f) + 8);
-        unsigned word4 = n << (4 * ((lane & 7) >> 1) + 16 * (lane & 1));
+        unsigned n = (unsigned)((int)(scale == scale ? int4_code(y, scale) : 0.0f) + 8) << (4 * ((lane & 7) >> 1) + 16 * (lane & 1));
 #pragma unroll
-        for (int o = 1; o < 8; o <<= 1) word4 |= __shfl_xor_sync(0xFFFFFFFFu, word4, o);
-        if ((lane & 7) == 0) *reinterpret_cast<unsigned *>(cache + place.codes + 16 * k + lane / 2) = word4;
+        for (int o = 1; o < 8; o <<= 1) n |= __shfl_xor_sync(0xFFFFFFFFu, n, o);
+        if ((lane & 7) == 0) *reinterpret_cast<unsigned *>(cache + place.codes + 16 * k + lane / 2) = n;
         if (lane == 0) *reinterpret_cast<unsigned short *>(cache + place.scales + 2 * k) = (unsigned short)(__float_as_uint(scale) >> 16);
     }
 }
 
+// The codes of a unit's columns, as their four bits in two halves of 16: those of even columns and of odd ones. *nearest: how near the nearest word is to a
+// border between two codes.
+template <int N>
+__device__ __forceinline__ uint2 append4_codes(const float (&y)[N], float s, float inverse, float *nearest) {
+    float q[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        // the quotient to nearest, so that one of eight bits by five is a tie if and only if it is one
+        float p = y[i] * inverse;
+        p = fmaf(fmaf(-p, s, y[i]), inverse, p);
+        q[i] = (p + 12582912.0f) - 12582912.0f;
+        *nearest = fminf(*nearest, fabsf(fabsf(fmaf(-q[i], s, y[i])) - 0.5f * s));
+    }
+    float half[2]; // 8388608 and the codes (each eight more than q) as digits of sixteen
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+        half[e] = q[e] + (N == 8 ? 8388608.0f + 34952.0f : 8388608.0f + 136.0f);
+#pragma unroll
+        for (int i = 1; i < N / 2; i++) half[e] = fmaf(q[2 * i + e], (float)(1 << (4 * i)), half[e]);
+    }
+    return make_uint2(__float_as_uint(half[0]), __float_as_uint(half[1]));
+}
+
+// blockIdx.x: the row; its heads in sets of 32 >> lanes_log2, a set a warp, by steps of the warps of gridDim.y blocks. (Queries, norms and rotation as in
+// append_units_kernel.)
+template <typename RT>
+__global__ void __launch_bounds__(128) append_int4_kernel(const __grid_constant__ Append4Call f, int lanes_log2, int sets) {
+    constexpr int N = Unit<RT>::N, OF = INT4_GROUP / N; // units of a group
+    const AppendCall &a = f.a;
+    const long long t = blockIdx.x;
+    const int all = threadIdx.x & 31, lane = all & ((1 << lanes_log2) - 1), in_set = all >> lanes_log2;
+    const int half = a.rope_dim / 2, pairs = half / N, rest = (a.c.hd - a.rope_dim) / N;
+    const bool turned = lane < pairs;
+    const int at0 = turned ? lane * N : a.rope_dim + (lane - pairs) * 2 * N, at1 = turned ? at0 + half : at0 + N;
+    const bool some0 = lane < pairs + (rest + 1) / 2, some1 = some0 && (turned || (lane - pairs) * 2 + 1 < rest);
+    const bool straight = rest == 0 && pairs % OF == 0; // a group's units are OF neighbouring lanes' first, or second
+    const RT *const q = static_cast<const RT *>(a.q) + t * a.ldq, *const k = static_cast<const RT *>(a.k) + t * a.ldk, *const v = static_cast<const RT *>(a.v) + t * a.ldv;
+    const int parts = a.c.heads + 2 * a.c.kv, groups = int4_groups(a.c.hd);
+
+    typename Unit<RT>::Raw raw0, raw1;
+    const auto ask = [&](int set) {
+        const int head = (set << (5 - lanes_log2)) + in_set;
+        const RT *src = head < a.c.heads ? q + head * a.c.hd : (head < a.c.heads + a.c.kv ? k + (head - a.c.heads) * a.c.hd : v + (head - a.c.heads - a.c.kv) * a.c.hd);
+        raw0 = raw1 = typename Unit<RT>::Raw{};
+        if (head < parts && some0) raw0 = Unit<RT>::ask(src + at0);
+        if (head < parts && some1) raw1 = Unit<RT>::ask(src + at1);
+    };
+    int set = blockIdx.y * 4 + (threadIdx.x >> 5);
+    const int step = gridDim.y * 4;
+    if (set < sets) ask(set);
+
+    const int b = paged_row_seq(a.c, t);
+    if (b < 0) return; // a row of no sequence: nothing is written for it
+    const PagedSeq s = paged_seq_checked(a.c, b);
+    if (s.n == 0) return; // its tables do not hold it
+    const int pos = s.pos0 + (int)(t - s.first);
+    if (append_past(a, pos)) return;
+    Append4Place place;
+    const bool placed = append4_place(&place, a.c, b, pos);
+    unsigned long long c[N / 2], sn[N / 2];
+    const bool turns = turned && a.cosv != nullptr;
+    float turn_off = 0.0f; // of a rotated word, in units of the largest one that it is made of
+    if (turns) {
+        const long long row = (long long)max(pos, 0) * half + at0;
+        append_words<N>(c, a.cosv + row);
+        append_words<N>(sn, a.sinv + row);
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            float u[4];
+            pg_one(c[i], u[0], u[1]), pg_one(sn[i], u[2], u[3]);
+            turn_off = fmaxf(turn_off, fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))));
+        }
+        turn_off *= 0x1p-19f;
+    }
+    for (; set < sets; set += step) {
+        const int head = (set << (5 - lanes_log2)) + in_set, part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2); // q, k, v
+        unsigned long long x0[N / 2], x1[N / 2];
+        Unit<RT>::words(x0, raw0), Unit<RT>::words(x1, raw1);
+        if (set + step < sets) ask(set + step);
+        const float *w = part == 0 ? a.q_norm : (part == 1 ? a.k_norm : nullptr);
+        if (a.q_norm || a.k_norm) { // uniform over the grid: the reduction is a warp's
+            unsigned long long sums = 0;
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) sums = pg_fma2(x0[i], x0[i], pg_fma2(x1[i], x1[i], sums));
+            float sum, other;
+            pg_one(sums, sum, other);
+            sum += other;
+            for (int o = (1 << lanes_log2) >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+            if (w) {
+                const float r = rsqrtf(fmaf(sum, a.part_of_head, a.eps));
+                const unsigned long long r2 = pg_two(r, r), shift2 = pg_two(a.norm_shift * r, a.norm_shift * r);
+                unsigned long long weight[N / 2];
+                if (some0) {
+                    append_words<N>(weight, w + at0);
+#pragma unroll
+                    for (int i = 0; i < N / 2; i++) x0[i] = pg_mul2(x0[i], pg_fma2(weight[i], r2, shift2));
+                }
+                if (some1) {
+                    append_words<N>(weight, w + at1);
+#pragma unroll
+                    for (int i = 0; i < N / 2; i++) x1[i] = pg_mul2(x1[i], pg_fma2(weight[i], r2, shift2));
+                }
+            }
+        }
+        const bool held = __any_sync(0xFFFFFFFFu, part > 0); // keys or values among the warp's heads
+        // How far a word may be from its 64-bit value: by the largest words that it is made of. Of float32 values, and keys as they came, only what the quotient
+        // is off by; of bfloat16 ones that is nothing.
+        const bool moved = part == 1 && (w || turns);
+        float off = -1.0f;
+        if (held && (N == 4 || moved)) {
+            unsigned most = 0;
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) most = max(max(most, (unsigned)(x0[i] >> 32) & 0x7FFFFFFFu), max((unsigned)x0[i] & 0x7FFFFFFFu, max((unsigned)(x1[i] >> 32) & 0x7FFFFFFFu, (unsigned)x1[i] & 0x7FFFFFFFu)));
+            off = __uint_as_float(most) * (moved ? (turns ? turn_off : 0x1p-20f) : 0x1p-22f);
+        }
+        if (turns && part < 2) {
+            const unsigned long long minus = pg_two(-1.0f, -1.0f);
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                const unsigned long long u = x0[i], y = x1[i];
+                x0[i] = pg_fma2(u, c[i], pg_mul2(pg_mul2(y, sn[i]), minus));
+                x1[i] = pg_fma2(y, c[i], pg_mul2(u, sn[i]));
+            }
+        }
+        if (part == 0 && some0) {
+            RT *dst = static_cast<RT *>(a.q_out) + (t * a.c.heads + head) * a.c.hd;
+            Unit<RT>::store(dst + at0, x0);
+            if (some1) Unit<RT>::store(dst + at1, x1);
+        }
+        if (!held) continue;
+        // ---- the codes ----
+        float y0[N], y1[N], far0 = off, far1 = off;
+        unsigned most0 = 0, most1 = 0; // (a NaN's bits are larger than an infinity's)
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) pg_one(x0[i], y0[2 * i], y0[2 * i + 1]), pg_one(x1[i], y1[2 * i], y1[2 * i + 1]);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            most0 = max(most0, __float_as_uint(y0[i]) & 0x7FFFFFFFu), most1 = max(most1, __float_as_uint(y1[i]) & 0x7FFFFFFFu);
+        }
+        if (straight) {
+#pragma unroll
+            for (int o = 1; o < OF; o <<= 1) {
+                most0 = max(most0, __shfl_xor_sync(0xFFFFFFFFu, most0, o)), most1 = max(most1, __shfl_xor_sync(0xFFFFFFFFu, most1, o));
+                far0 = fmaxf(far0, __shfl_xor_sync(0xFFFFFFFFu, far0, o));
+            }
+            far1 = far0;
+        } else { // unit u of a head is lane u's first, lane u - pairs' second, or one of two neighbours behind the rotation
+            unsigned m0 = 0, m1 = 0;
+            float f0 = off, f1 = off;
+#pragma unroll 1
+            for (int i = 0; i < 2 * OF; i++) {
+                const int u = (i < OF ? at0 : at1) / N / OF * OF + i % OF, r = u - 2 * pairs;
+                const int from = (all - lane) + (r < 0 ? (u < pairs ? u : u - pairs) : pairs + r / 2);
+                const bool second = r < 0 ? u >= pairs : (r & 1) != 0, there = u * N < a.c.hd;
+                const unsigned p0 = __shfl_sync(0xFFFFFFFFu, most0, from), p1 = __shfl_sync(0xFFFFFFFFu, most1, from);
+                const float g = __shfl_sync(0xFFFFFFFFu, off, from);
+                if (there && i < OF) m0 = max(m0, second ? p1 : p0), f0 = fmaxf(f0, g);
+                if (there && i >= OF) m1 = max(m1, second ? p1 : p0), f1 = fmaxf(f1, g);
+            }
+            most0 = m0, most1 = m1, far0 = f0, far1 = f1;
+        }
+        bool near = false;
+        float scale[2];
+        uint2 code[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const unsigned most = h ? most1 : most0;
+            const float top = __uint_as_float(most), s5 = int4_scale(top), before = __uint_as_float(__float_as_uint(s5) - 0x80000u), far = h ? far1 : far0;
+            float inverse, nearest = INFINITY;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s5));
+            scale[h] = s5;
+            code[h] = append4_codes(h ? y1 : y0, s5, inverse, &nearest);
+            near |= nearest <= off;
+            if (moved) near |= 7.0f * s5 - top <= far || (s5 > 0x1p-100f && top - 7.0f * before <= far);
+            if (!(top <= 7.0f * s5)) near = true; // words that are cut, or not finite
+        }
+        near &= part > 0 && head < parts && some0 && placed; // (a lane without a second unit has zeros there, which are near nothing)
+        const unsigned again = __ballot_sync(0xFFFFFFFFu, near), mine = again >> (all - lane) & (unsigned)((1ull << (1 << lanes_log2)) - 1);
+        if (part > 0 && head < parts && placed && mine == 0) {
+            unsigned char *const cache = static_cast<unsigned char *>(part == 1 ? a.k_cache : a.v_cache) + place.head * (head - a.c.heads - (part == 1 ? 0 : a.c.kv));
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int at = h ? at1 : at0;
+                if (!(h ? some1 : some0)) continue;
+                if constexpr (N == 8) {
+                    *reinterpret_cast<unsigned *>(cache + place.codes + at / 2) = __byte_perm(code[h].x, code[h].y, 0x5410);
+                } else { // half a word: its first bytes, or its second ones
+                    unsigned char *const to = cache + place.codes + at / 8 * 4 + (at / 4 & 1);
+                    to[0] = (unsigned char)code[h].x, to[2] = (unsigned char)code[h].y;
+                }
+                if (at % INT4_GROUP == 0) *reinterpret_cast<unsigned short *>(cache + place.scales + at / INT4_GROUP * 2) = (unsigned short)(__float_as_uint(scale[h]) >> 16);
+            }
+            for (int at = a.c.hd + 8 * lane; at < INT4_GROUP * groups; at += 8 << lanes_log2) *reinterpret_cast<unsigned *>(cache + place.codes + at / 2) = 0x88888888u; // the last group's zeros
+        }
+        for (unsigned rest_of = again; rest_of;) { // the heads that are done again, one after another
+            const int first = (__ffs(rest_of) - 1) >> lanes_log2 << lanes_log2, which = (set << (5 - lanes_log2)) + (first >> lanes_log2);
+            rest_of &= ~(unsigned)(((1ull << (1 << lanes_log2)) - 1) << first);
+            const int of = which < a.c.heads + a.c.kv ? 1 : 2;
+            append4_head<RT>(f, t, of, which - a.c.heads - (of == 1 ? 0 : a.c.kv), pos, place);
+        }
+    }
+}
+
+// A warp a head: queries column by column, keys and values by append4_head.
+template <typename RT>
+__global__ void __launch_bounds__(256) append_int4_columns_kernel(const __grid_constant__ Append4Call f) {
+    const AppendCall &a = f.a;
+    const long long t = blockIdx.x;
+    const int head = blockIdx.y * 8 + (threadIdx.x >> 5), b = paged_row_seq(a.c, t);
+    if (b < 0 || head >= a.c.heads + 2 * a.c.kv) return;
+    const PagedSeq s = paged_seq_checked(a.c, b);
+    if (s.n == 0) return; // its tables do not hold it
+    const int pos = s.pos0 + (int)(t - s.first), part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2);
+    if (append_past(a, pos)) return;
+    if (part > 0) {
+        Append4Place place;
+        if (append4_place(&place, a.c, b, pos)) append4_head<RT>(f, t, part, head - a.c.heads - (part == 1 ? 0 : a.c.kv), pos, place);
+        return;
+    }
+    append_columns<RT, RT>(a, static_cast<const RT *>(a.q) + t * a.ldq + (long long)head * a.c.hd, a.q_norm, pos, true,
+                           static_cast<RT *>(a.q_out) + (t * a.c.heads + head) * a.c.hd);
+}
+
 template <typename RT>
 cudaError_t launch_append4(const AppendCall &a, double eps, int sms, cudaStream_t st) {
+    constexpr int N = Unit<RT>::N;
     const Append4Call f = {a, eps};
-    const int parts = a.c.heads + 2 * a.c.kv, groups = int4_groups(a.c.hd);
-    const uintptr_t words = reinterpret_cast<uintptr_t>(a.cosv) | reinterpret_cast<uintptr_t>(a.sinv) | reinterpret_cast<uintptr_t>(a.q_norm) | reinterpret_cast<uintptr_t>(a.k_norm);
-    if ((a.rope_dim / 2) % 4 == 0 && words % 16 == 0) {
-        const int lg = groups == 1 ? 3 : (groups == 2 ? 4 : 5), per_set = 32 >> lg, sets = (parts + per_set - 1) / per_set, blocks = (sets + 3) / 4;
-        const int y = (int)std::max<long long>(1, std::min<long long>(blocks, 8LL * sms / a.c.rows)); // as in launch_append
-        append_int4_kernel<RT><<<dim3((unsigned)a.c.rows, (unsigned)y), 128, 0, st>>>(f, lg, sets);
+    const int parts = a.c.heads + 2 * a.c.kv;
+    if (append_by_units<N>(a)) {
+        const AppendCut cut = append_cut<N>(a, parts, sms);
+        append_int4_kernel<RT><<<dim3((unsigned)a.c.rows, (unsigned)cut.blocks), 128, 0, st>>>(f, cut.lanes_log2, cut.sets);
     } else {
         append_int4_columns_kernel<RT><<<dim3((unsigned)a.c.rows, (unsigned)((parts + 7) / 8)), 256, 0, st>>>(f);
     }

@@ -18,55 +18,60 @@
 
 namespace b200i {
 
-constexpr int FEW4_WARPS = 8, FEW4_THREADS = 32 * (FEW4_WARPS + 1), FEW4_KEYS = 16 * FEW4_WARPS;
+constexpr int FEW4_WARPS = 8, FEW4_THREADS = 32 * (FEW4_WARPS + 2), FEW4_KEYS = 16 * FEW4_WARPS; // two warps copy, keys and values
 
-template <typename RT, int HDP, int NT, bool PACK> struct Few4Shape {
+template <typename RT, int GROUPS, int NT, bool PACK> struct Few4Shape {
     static constexpr bool F32 = std::is_same_v<RT, float>;
-    static constexpr int WARPS = FEW4_WARPS, ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
-    static constexpr int CODES = FEW4_KEYS * HDP / 2, SCALES = FEW4_KEYS * HDP / INT4_GROUP * 2, SLOT = 2 * (CODES + SCALES); // codes of keys and of values, their scales
+    static constexpr int HDP = GROUPS <= 2 ? 64 : 128; // head_dim as it is laid out for the products: a lane's quarter (eighth) of it lies in one group
+    static constexpr int WARPS = FEW4_WARPS, COPIERS = 2, ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
+    static constexpr int HALF = FEW4_KEYS * GROUPS * INT4_BYTES, SLOT = 2 * HALF; // keys, then values
     static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : 2;
     static constexpr bool HELD = PACK || (!F32 && NT == 1); // the queries stay in registers; else they lie as fragments where the warps' results meet
+    static constexpr int TOGETHER = 1;
     static constexpr int PITCH = HDP + 8;                   // floats of a row of those
     static constexpr int MEET = FEW4_WARPS / 2 * ROWS * PITCH * 4, QUERY = ROWS * HDP * (int)sizeof(RT);
     static constexpr int REST = 1024 + 512 + MEET + FEW_ITEMS * QUERY;
     static constexpr int ROOM = (112 * 1024 - REST) / SLOT, SLOTS = ROOM > 8 ? 8 : ROOM;
     static constexpr int SMEM = REST + SLOTS * SLOT;
-    static_assert(SLOTS >= 2 && (HELD || Q_PIECES * NT * HDP / 16 * 256 <= MEET), "shared memory");
+    static_assert(SLOTS > TOGETHER && (HELD || Q_PIECES * NT * HDP / 16 * 256 <= MEET), "shared memory");
 };
 
-// What brings a tile: a lane one of a piece's four runs of bytes (codes of keys, of values, scales of keys, of values).
+// What brings a tile's keys (or values): a lane a piece, whose codes and scales follow one another in the cache as in the slot. Of a page larger than a tile they do
+// not, and two lanes bring them.
 template <typename Shape>
-__device__ __forceinline__ auto few4_runs(const AttendCall &a) {
-    return [&a](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
+__device__ __forceinline__ auto few4_runs(const AttendCall &a, bool values) {
+    return [&a, values](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
         const PagedCall &c = a.c;
-        const int lane = threadIdx.x & 31, run = lane & 3, piece = lane >> 2, page = 1 << c.page_shift, rows = min(page, FEW4_KEYS), groups = int4_groups(c.hd);
-        const int id = page_of(piece), bytes = rows * groups * (run < 2 ? 16 : 2), first = piece * rows;
+        const int lane = threadIdx.x & 31, page = 1 << c.page_shift, rows = min(page, FEW4_KEYS), groups = int4_groups(c.hd), split = page > FEW4_KEYS;
+        const int piece = lane >> split, scales = lane & split; // this lane's
+        const int id = page_of(piece), first = piece * rows;
         const bool want = piece < there && low - pos < first + rows; // a page that nobody sees any more may be anyone's
         const bool some = want && (unsigned)id < (unsigned)c.pages;
-        unsigned char *const to = dst + (run & 1) * (run < 2 ? Shape::CODES : Shape::SCALES) + (run < 2 ? first * groups * 16 : 2 * Shape::CODES + first * groups * 2);
-        if (want && !some) { // a page of zeros
+        unsigned char *const to = dst + (values ? Shape::HALF : 0) + first * groups * INT4_BYTES;
+        if (want && !some) { // a page of zeros: scales of zero
             atomicExch(c.status, PAGED_BAD_PAGE);
-            if (run >= 2)
-                for (int i = 0; i < bytes; i += 16) *reinterpret_cast<uint4 *>(to + i) = make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < rows * groups * 2; i += 16) *reinterpret_cast<uint4 *>(to + rows * groups * 16 + i) = make_uint4(0, 0, 0, 0);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         const unsigned all = __ballot_sync(0xFFFFFFFFu, some);
-        if (lane == 0) pg_bar_expect(full, (unsigned)(__popc(all) / 4 * rows * groups * 36));
+        if (lane == 0) pg_bar_expect(full, (unsigned)((__popc(all) >> split) * rows * groups * INT4_BYTES));
         __syncwarp();
         if (!some) return;
-        const int in = (pos + first) & (page - 1);
-        const unsigned char *src = int4_page(run & 1 ? a.v : a.k, id * c.kv + kvh, groups, c.page_shift) + (run < 2 ? in * groups * 16 : ((16 * groups) << c.page_shift) + in * groups * 2);
-        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(to)), "l"(src), "r"(bytes), "r"(pg_smem(full)) : "memory");
+        const unsigned char *src = int4_page(values ? a.v : a.k, id * c.kv + kvh, groups, c.page_shift);
+        const int in = (pos + first) & (page - 1), codes = rows * groups * 16, bytes = !split ? rows * groups * INT4_BYTES : (scales ? rows * groups * 2 : codes);
+        src += !split ? 0 : (scales ? ((16 * groups) << c.page_shift) + in * groups * 2 : in * groups * 16);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(to + scales * codes)), "l"(src), "r"(bytes), "r"(pg_smem(full)) : "memory");
     };
 }
 
-template <typename RT, int HDP, int NT, bool PACK>
+template <typename RT, int GROUPS, int NT, bool PACK>
 __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
-    using Shape = Few4Shape<RT, HDP, NT, PACK>;
+    using Shape = Few4Shape<RT, GROUPS, NT, PACK>;
     constexpr bool F32 = Shape::F32, HELD = Shape::HELD;
-    constexpr int KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = FEW4_WARPS, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
+    constexpr int HDP = Shape::HDP, KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = FEW4_WARPS, QP = Shape::Q_PIECES, WP = Shape::W_PIECES, CH = Shape::TOGETHER;
     constexpr int E = PACK ? 1 : 2 * NT;                   // rows of a lane's scores
     constexpr int K_WORDS = HDP / 32, V_WORDS = HDP / 64;  // of codes, of a key: a quarter of its columns, an eighth
+    constexpr int STRIDE = 16 * GROUPS;                    // bytes of a key's codes
     extern __shared__ __align__(128) unsigned char smem[];
     const FewMemory<Shape> sm(smem);
     __shared__ float ml[WARPS][2][ROWS], joined[2][ROWS];
@@ -77,22 +82,26 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const LinePlace p = few_begin<KEYS>(f, sm, place, &bad_rows, &dead);
-    if (warp == WARPS) {
-        few_copies<RT, KEYS>(f, sm, items, p, few4_runs<Shape>(a));
+    if (warp >= WARPS) {
+        if (warp == WARPS)
+            few_copies<RT, KEYS, true>(f, sm, items, p, few4_runs<Shape>(a, false));
+        else
+            few_copies<RT, KEYS, false>(f, sm, items, p, few4_runs<Shape>(a, true));
         return;
     }
 
-    const int groups = int4_groups(a.c.hd), stride = 16 * groups;
-    const int k_group = t4 * (HDP / 4) / INT4_GROUP, v_group = g * (HDP / 8) / INT4_GROUP; // of the lane's columns
-    const bool k_some = k_group < groups, v_some = v_group < groups;
-    // in a slot, of the warp's keys: the lane's codes and scales of keys g (and g + 8), and of values 2 t4 (and 1, 8 and 9 further on)
-    const int k_at = (warp * 16 + g) * stride + (k_some ? t4 * (HDP / 8) : 0), k_scale = 2 * Shape::CODES + ((warp * 16 + g) * groups + (k_some ? k_group : 0)) * 2;
-    const int v_at = Shape::CODES + (warp * 16 + 2 * t4) * stride + (v_some ? g * (HDP / 16) : 0);
-    const int v_scale = 2 * Shape::CODES + Shape::SCALES + ((warp * 16 + 2 * t4) * groups + (v_some ? v_group : 0)) * 2;
-    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E;
+    // of the lane's columns: of a key's quarters and of its eighths, those that are in no group of the head's count as zeros
+    const int k_group = t4 * (HDP / 4) / INT4_GROUP, v_group = g * (HDP / 8) / INT4_GROUP;
+    const bool k_some = k_group < GROUPS, v_some = v_group < GROUPS;
+    // in a slot, of the warp's 16 keys: the lane's codes and scales of keys g (and g + 8), and of values 2 t4 (and 1, 8 and 9 further on)
+    const int box_rows = min(1 << a.c.page_shift, KEYS), in = (warp * 16) & (box_rows - 1), piece = (warp * 16 - in) * (GROUPS * INT4_BYTES); // the piece they lie in
+    const int k_at = piece + (in + g) * STRIDE + (k_some ? t4 * (HDP / 8) : 0), k_scale = piece + box_rows * STRIDE + (in + g) * (2 * GROUPS) + (k_some ? 2 * k_group : 0);
+    const int v_at = Shape::HALF + piece + (in + 2 * t4) * STRIDE + (v_some ? g * (HDP / 16) : 0);
+    const int v_scale = Shape::HALF + piece + box_rows * STRIDE + (in + 2 * t4) * (2 * GROUPS) + (v_some ? 2 * v_group : 0);
+    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, part_of_unit = 1.0f / unit;
     const auto row_of = [&](int e) { return PACK ? (F32 ? t4 >> 1 : t4) : (e >> 1) * 8 + 2 * t4 + (e & 1); };
     uint2 *const fragments = reinterpret_cast<uint2 *>(sm.meet);
-    unsigned it = 0;
+    unsigned slot_at = 0, parity = 0; // of the next tile
     bool alive = true, first_part = true;
     const auto give_up = [&] {
         if (lane == 0) atomicExch(a.c.status, PAGED_WAIT), dead = 1;
@@ -154,46 +163,61 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
         }
         const int all_lo = a.window ? s.pos0 + item.n - a.window : 0, low = a.window ? s.pos0 + 1 - a.window : 0; // every row sees positions all_lo .. pos0; none sees what is below low
 
-        float o[NT][KS][4], m[E], l[E];
+        float o[NT][KS][4], m[E], l[E], high[E]; // high: the score that m is to be moved for
 #pragma unroll
-        for (int e = 0; e < E; e++) m[e] = -INFINITY, l[e] = 0.0f;
+        for (int e = 0; e < E; e++) m[e] = high[e] = -INFINITY, l[e] = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
             for (int mt = 0; mt < KS; mt++) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
-        for (int t = 0; t < item.tiles; t++, it++) {
-            const unsigned char *const slot = sm.ring + (it % SLOTS) * Shape::SLOT;
-            const int j0 = item.pos + t * KEYS + warp * 16;
-            if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[it % SLOTS], (it / SLOTS) & 1u))) give_up();
-            if (alive && j0 < s.length && j0 + 16 > low) {
+        for (int t = 0; t < item.tiles; t += CH) {
+            const unsigned char *slot[CH];
+            unsigned long long *empty[CH];
+            int j0[CH]; // the warp's first key of each tile; of one that is not there, past all keys
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
+                const bool there = c == 0 || t + c < item.tiles;
+                j0[c] = there ? item.pos + (t + c) * KEYS + warp * 16 : 0x7FFFFF00;
+                slot[c] = c == 0 || there ? sm.ring + slot_at * Shape::SLOT : slot[0];
+                empty[c] = &sm.empty[slot_at];
+                if (!there) break;
+                if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot_at], parity))) give_up();
+                if (++slot_at == SLOTS) slot_at = 0, parity ^= 1;
+            }
+            if (alive && j0[0] < s.length && (j0[CH - 1] + 16 > low)) {
                 // ---- scores ----
-                float z[NT][4], z_small[F32 && !PACK ? NT : 1][4];
+                constexpr int ZS = F32 && !PACK ? 2 : 1; // large and small products apart
+                float z[CH][ZS][NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) z[nt][0] = z[nt][1] = z[nt][2] = z[nt][3] = 0.0f;
-                if constexpr (F32 && !PACK) {
+                for (int c = 0; c < CH; c++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) z_small[nt][0] = z_small[nt][1] = z_small[nt][2] = z_small[nt][3] = 0.0f;
-                }
-                {
-                    unsigned code[2][K_WORDS], scale[2], shift[2];
+                    for (int k = 0; k < ZS; k++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) z[c][k][nt][0] = z[c][k][nt][1] = z[c][k][nt][2] = z[c][k][nt][3] = 0.0f;
+                unsigned k_code[CH][2][K_WORDS], k_scales[CH][2];
+#pragma unroll
+                for (int c = 0; c < CH; c++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) { // keys g and g + 8
-                        const unsigned char *at = slot + k_at + h * 8 * stride;
+                        const unsigned char *at = slot[c] + k_at + h * 8 * STRIDE;
                         if constexpr (K_WORDS == 4) {
                             const uint4 w = *reinterpret_cast<const uint4 *>(at);
-                            code[h][0] = w.x, code[h][1] = w.y, code[h][2] = w.z, code[h][3] = w.w;
+                            k_code[c][h][0] = w.x, k_code[c][h][1] = w.y, k_code[c][h][2] = w.z, k_code[c][h][3] = w.w;
                         } else {
                             const uint2 w = *reinterpret_cast<const uint2 *>(at);
-                            code[h][0] = w.x, code[h][1] = w.y;
+                            k_code[c][h][0] = w.x, k_code[c][h][1] = w.y;
                         }
-                        scale[h] = *reinterpret_cast<const unsigned short *>(slot + k_scale + h * 16 * groups);
-                        if (!k_some) scale[h] = 0;
-                        scale[h] *= 0x10001u, shift[h] = int4_shift(scale[h]);
+                        k_scales[c][h] = *reinterpret_cast<const unsigned short *>(slot[c] + k_scale + h * 16 * GROUPS);
+                        if (GROUPS % 2 && !k_some) k_scales[c][h] = 0;
+                        k_scales[c][h] *= 0x10001u;
                     }
 #pragma unroll
-                    for (int w = 0; w < K_WORDS; w++) {
+                for (int w = 0; w < K_WORDS; w++)
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
                         unsigned x[2][4];
-                        int4_pairs(x[0], code[0][w], scale[0], shift[0]), int4_pairs(x[1], code[1][w], scale[1], shift[1]);
+#pragma unroll
+                        for (int h = 0; h < 2; h++) int4_pairs(x[h], k_code[c][h][w], int4_factors(k_scales[c][h]));
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
                             const unsigned k[4] = {x[0][2 * i], x[1][2 * i], x[0][2 * i + 1], x[1][2 * i + 1]};
@@ -201,62 +225,72 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) {
                                 if constexpr (HELD) {
-                                    pg_mma(z[nt], k, held[ks].x, held[ks].y);
+                                    pg_mma(z[c][0][nt], k, held[ks].x, held[ks].y);
                                 } else {
 #pragma unroll
                                     for (int piece = QP - 1; piece >= 0; piece--) {
                                         const uint2 q = fragments[piece * (NT * KS * 32) + (nt * KS + ks) * 32 + lane];
-                                        pg_mma(F32 && piece > 0 ? z_small[F32 && !PACK ? nt : 0] : z[nt], k, q.x, q.y);
+                                        pg_mma(z[c][piece > 0 ? ZS - 1 : 0][nt], k, q.x, q.y);
                                     }
                                 }
                             }
                         }
                     }
-                }
-                float x[E][2]; // keys g and g + 8
-                if constexpr (PACK) {
+                float x[CH][E][2]; // keys g and g + 8
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        x[0][h] = z[0][2 * h];
-                        if constexpr (F32) {
-                            x[0][h] += z[0][2 * h + 1]; // two pieces here, the third beside it
-                            x[0][h] += __shfl_xor_sync(0xFFFFFFFFu, x[0][h], 1);
-                        }
-                    }
-                } else {
+                for (int c = 0; c < CH; c++)
 #pragma unroll
                     for (int e = 0; e < E; e++)
 #pragma unroll
                         for (int h = 0; h < 2; h++) {
-                            x[e][h] = z[e >> 1][2 * h + (e & 1)];
-                            if constexpr (F32) x[e][h] += z_small[e >> 1][2 * h + (e & 1)];
+                            if constexpr (PACK) {
+                                x[c][e][h] = z[c][0][0][2 * h];
+                                if constexpr (F32) {
+                                    x[c][e][h] += z[c][0][0][2 * h + 1]; // two pieces here, the third beside it
+                                    x[c][e][h] += __shfl_xor_sync(0xFFFFFFFFu, x[c][e][h], 1);
+                                }
+                            } else {
+                                x[c][e][h] = z[c][0][e >> 1][2 * h + (e & 1)];
+                                if constexpr (F32) x[c][e][h] += z[c][ZS - 1][e >> 1][2 * h + (e & 1)];
+                            }
+                        }
+                if (a.softcap > 0.0f) {
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+#pragma unroll
+                        for (int e = 0; e < E; e++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) x[c][e][h] = tanhf(x[c][e][h] * a.scale * a.cap_part); // (scale / softcap may leave 32 bits)
+                }
+                const bool edge = j0[CH - 1] + 16 > s.pos0 + 1 || j0[0] < all_lo; // (the last tile is the furthest)
+                if (edge) {
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int j = j0[c] + g + h * 8;
+#pragma unroll
+                            for (int e = 0; e < E; e++)
+                                if (j >= hi[e] || j < lo[e]) x[c][e][h] = -INFINITY;
                         }
                 }
-                const bool edge = j0 + 16 > s.pos0 + 1 || j0 < all_lo;
                 bool more = false;
 #pragma unroll
                 for (int e = 0; e < E; e++)
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float y = x[e][h];
-                        y = unit * (a.softcap > 0.0f ? tanhf(y * a.scale * a.cap_part) : y); // (scale / softcap may leave 32 bits)
-                        if (edge) {
-                            const int j = j0 + g + h * 8;
-                            if (j >= hi[e] || j < lo[e]) y = -INFINITY;
-                        }
-                        more |= y > m[e] + 8.0f;
-                        x[e][h] = y;
-                    }
+                    for (int c = 0; c < CH; c++) more |= x[c][e][0] > high[e] || x[c][e][1] > high[e];
                 if (__any_sync(0xFFFFFFFFu, more)) {
                     float keep[E];
 #pragma unroll
                     for (int e = 0; e < E; e++) {
-                        float top = fmaxf(x[e][0], x[e][1]);
+                        float top = fmaxf(x[0][e][0], x[0][e][1]);
+#pragma unroll
+                        for (int c = 1; c < CH; c++) top = fmaxf(top, fmaxf(x[c][e][0], x[c][e][1]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                        top = fmaxf(m[e], top);
+                        top = fmaxf(m[e], top * unit);
                         keep[e] = m[e] == -INFINITY ? 0.0f : paged_exp2(m[e] - top);
-                        m[e] = top, l[e] *= keep[e];
+                        m[e] = top, l[e] *= keep[e], high[e] = (top + 8.0f) * part_of_unit;
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
@@ -266,85 +300,100 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
                             for (int i = 0; i < 4; i++) o[nt][mt][i] *= keep[PACK ? 0 : 2 * nt + (i & 1)];
                 }
                 // ---- weights, as pieces and turned: keys down ----
-                unsigned w[NT][PACK ? 1 : WP][2];
+                unsigned w[CH][NT][PACK ? 1 : WP][2];
                 float base[E];
 #pragma unroll
-                for (int e = 0; e < E; e++) base[e] = m[e] == -INFINITY ? 0.0f : m[e];
+                for (int e = 0; e < E; e++) base[e] = m[e] == -INFINITY ? 0.0f : -m[e];
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float y[E];
+                for (int c = 0; c < CH; c++)
 #pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        y[e] = paged_exp2(x[e][h] - base[e]);
-                        l[e] += y[e];
-                    }
-                    if constexpr (PACK) {
-                        const float rest = y[0] - __uint_as_float(pg_pack(y[0], 0.0f) << 16);
-                        unsigned two = pg_pack(y[0], rest);
-                        if constexpr (F32) {
-                            const float last = rest - __uint_as_float(two & 0xFFFF0000u);
-                            if (t4 & 1) two = pg_pack(last, 0.0f);
+                    for (int h = 0; h < 2; h++) {
+                        float y[E];
+#pragma unroll
+                        for (int e = 0; e < E; e++) {
+                            y[e] = paged_exp2(fmaf(x[c][e][h], unit, base[e]));
+                            l[e] += y[e];
                         }
-                        w[0][0][h] = pg_transpose(two);
-                    } else {
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
-                            unsigned piece[WP];
-                            pg_split<WP>(piece, y[2 * nt], y[2 * nt + 1]);
-#pragma unroll
-                            for (int k = 0; k < WP; k++) w[nt][k][h] = pg_transpose(piece[k]);
-                        }
-                    }
-                }
-                // ---- values ----
-                unsigned code[4][V_WORDS], scale[4];
-#pragma unroll
-                for (int k = 0; k < 4; k++) { // keys 2 t4, 2 t4 + 1, and eight further on
-                    const int key = (k & 1) + (k >> 1) * 8;
-                    const unsigned char *at = slot + v_at + key * stride;
-                    if constexpr (V_WORDS == 2) {
-                        const uint2 c = *reinterpret_cast<const uint2 *>(at);
-                        code[k][0] = c.x, code[k][1] = c.y;
-                    } else {
-                        code[k][0] = *reinterpret_cast<const unsigned *>(at);
-                    }
-                    scale[k] = *reinterpret_cast<const unsigned short *>(slot + v_scale + key * groups * 2);
-                    if (!v_some) scale[k] = 0;
-                    if (edge) { // what stands in positions that no row sees, or of no sequence, counts as zero
-                        const int j = j0 + 2 * t4 + key;
-                        if (j >= s.length || j < low) scale[k] = 0;
-                    }
-                }
-                const unsigned scale0 = scale[0] | scale[1] << 16, scale1 = scale[2] | scale[3] << 16, shift0 = int4_shift(scale0), shift1 = int4_shift(scale1);
-#pragma unroll
-                for (int v = 0; v < V_WORDS; v++) {
-                    unsigned even0[4], odd0[4], even1[4], odd1[4]; // columns 2 i and 2 i + 1, of two keys each
-                    int4_pairs(even0, __byte_perm(code[0][v], code[1][v], 0x5410), scale0, shift0);
-                    int4_pairs(odd0, __byte_perm(code[0][v], code[1][v], 0x7632), scale0, shift0);
-                    int4_pairs(even1, __byte_perm(code[2][v], code[3][v], 0x5410), scale1, shift1);
-                    int4_pairs(odd1, __byte_perm(code[2][v], code[3][v], 0x7632), scale1, shift1);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const unsigned x4[4] = {even0[i], odd0[i], even1[i], odd1[i]};
-                        const int mt = 4 * v + i;
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) {
+                        if constexpr (PACK) {
+                            const float rest = y[0] - __uint_as_float(pg_pack(y[0], 0.0f) << 16);
+                            unsigned two = pg_pack(y[0], rest);
                             if constexpr (F32) {
-                                float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                const float last = rest - __uint_as_float(two & 0xFFFF0000u);
+                                if (t4 & 1) two = pg_pack(last, 0.0f);
+                            }
+                            w[c][0][0][h] = pg_transpose(two);
+                        } else {
 #pragma unroll
-                                for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(d, x4, w[nt][k][0], w[nt][k][1]);
+                            for (int nt = 0; nt < NT; nt++) {
+                                unsigned piece[WP];
+                                pg_split<WP>(piece, y[2 * nt], y[2 * nt + 1]);
 #pragma unroll
-                                for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
-                            } else {
-#pragma unroll
-                                for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[nt][k][0], w[nt][k][1]);
+                                for (int k = 0; k < WP; k++) w[c][nt][k][h] = pg_transpose(piece[k]);
                             }
                         }
                     }
+                // ---- values ----
+                unsigned code[CH][4][V_WORDS], scales[CH][2];
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+                    unsigned scale[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) { // keys 2 t4, 2 t4 + 1, and eight further on
+                        const int key = (k & 1) + (k >> 1) * 8;
+                        const unsigned char *at = slot[c] + v_at + key * STRIDE;
+                        if constexpr (V_WORDS == 2) {
+                            const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                            code[c][k][0] = v.x, code[c][k][1] = v.y;
+                        } else {
+                            code[c][k][0] = *reinterpret_cast<const unsigned *>(at);
+                        }
+                        scale[k] = *reinterpret_cast<const unsigned short *>(slot[c] + v_scale + key * GROUPS * 2);
+                    }
+                    scales[c][0] = scale[0] | scale[1] << 16, scales[c][1] = scale[2] | scale[3] << 16;
+                    if (GROUPS % 2 && !v_some) scales[c][0] = scales[c][1] = 0;
                 }
+                if (edge) { // what stands in positions that no row sees, or of no sequence, counts as zero
+#pragma unroll
+                    for (int c = 0; c < CH; c++)
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            const int j = j0[c] + 2 * t4 + (k & 1) + (k >> 1) * 8;
+                            if (j >= s.length || j < low) scales[c][k >> 1] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+                        }
+                }
+#pragma unroll
+                for (int v = 0; v < V_WORDS; v++)
+#pragma unroll
+                    for (int c = 0; c < CH; c++) {
+                        unsigned even[2][4], odd[2][4]; // columns 2 i and 2 i + 1, of two keys each
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const Int4Factors factors = int4_factors(scales[c][h]);
+                            int4_pairs(even[h], __byte_perm(code[c][2 * h][v], code[c][2 * h + 1][v], 0x5410), factors);
+                            int4_pairs(odd[h], __byte_perm(code[c][2 * h][v], code[c][2 * h + 1][v], 0x7632), factors);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const unsigned x4[4] = {even[0][i], odd[0][i], even[1][i], odd[1][i]};
+                            const int mt = 4 * v + i;
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                if constexpr (F32) {
+                                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                    for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(d, x4, w[c][nt][k][0], w[c][nt][k][1]);
+#pragma unroll
+                                    for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
+                                } else {
+#pragma unroll
+                                    for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[c][nt][k][0], w[c][nt][k][1]);
+                                }
+                            }
+                        }
+                    }
             }
             __syncwarp();
-            if (lane == 0 && alive) pg_bar_arrive(&sm.empty[it % SLOTS]); // (what it has not waited for is not given back)
+            if (lane < CH && t + lane < item.tiles && alive) pg_bar_arrive(lane == 0 ? empty[0] : empty[CH - 1]); // (what it has not waited for is not given back)
         }
 
         // ---- the item's (or its part's) end: the warps' results meet, [four warps][row][column], four of them adding to the others' ----
@@ -439,12 +488,12 @@ inline FewPlan few4_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int
     return p;
 }
 
-template <typename RT, int HDP, int NT, bool PACK>
+template <typename RT, int GROUPS, int NT, bool PACK>
 cudaError_t launch_few4_as(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
-    using Shape = Few4Shape<RT, HDP, NT, PACK>;
+    using Shape = Few4Shape<RT, GROUPS, NT, PACK>;
     FewCall f;
     f.a = a, f.whole = p.whole, f.part = static_cast<float *>(ws), f.head = p.whole ? nullptr : reinterpret_cast<int *>(static_cast<float *>(ws) + p.part_floats);
-    const auto kernel = attend_few_int4_kernel<RT, HDP, NT, PACK>;
+    const auto kernel = attend_few_int4_kernel<RT, GROUPS, NT, PACK>;
     static std::atomic<bool> known[64];
     if (device >= 64 || !known[device].load()) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
@@ -455,18 +504,23 @@ cudaError_t launch_few4_as(const AttendCall &a, const FewPlan &p, void *ws, int 
     *launches += 1;
     if (!p.whole) {
         *launches += 1;
-        return launch_following<FewCall>(attend_join_kernel<RT, Int4, HDP, Shape::ROWS>, dim3(p.blocks, p.most), 256, st, f);
+        return launch_following<FewCall>(attend_join_kernel<RT, Int4, Shape::HDP, Shape::ROWS>, dim3(p.blocks, p.most), 256, st, f);
     }
     return cudaGetLastError();
 }
-template <typename RT, int HDP>
+template <typename RT, int GROUPS>
 cudaError_t launch_few4_rows(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
-    if (p.rows < 8) return launch_few4_as<RT, HDP, 1, true>(a, p, ws, device, st, launches);
-    return p.rows == 8 ? launch_few4_as<RT, HDP, 1, false>(a, p, ws, device, st, launches) : launch_few4_as<RT, HDP, 2, false>(a, p, ws, device, st, launches);
+    if (p.rows < 8) return launch_few4_as<RT, GROUPS, 1, true>(a, p, ws, device, st, launches);
+    return p.rows == 8 ? launch_few4_as<RT, GROUPS, 1, false>(a, p, ws, device, st, launches) : launch_few4_as<RT, GROUPS, 2, false>(a, p, ws, device, st, launches);
 }
 template <typename RT>
-cudaError_t launch_few4(const AttendCall &a, const FewPlan &p, int hdp, void *ws, int device, cudaStream_t st, int *launches) {
-    return hdp == 64 ? launch_few4_rows<RT, 64>(a, p, ws, device, st, launches) : launch_few4_rows<RT, 128>(a, p, ws, device, st, launches);
+cudaError_t launch_few4(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
+    switch (int4_groups(a.c.hd)) {
+    case 1: return launch_few4_rows<RT, 1>(a, p, ws, device, st, launches);
+    case 2: return launch_few4_rows<RT, 2>(a, p, ws, device, st, launches);
+    case 3: return launch_few4_rows<RT, 3>(a, p, ws, device, st, launches);
+    default: return launch_few4_rows<RT, 4>(a, p, ws, device, st, launches);
+    }
 }
 
 } // namespace b200i

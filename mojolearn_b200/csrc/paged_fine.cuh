@@ -210,33 +210,35 @@ __global__ void __launch_bounds__(FINE_THREADS, 1) attend_fine_kernel(const __gr
                 w.next(a);
             }
         } else if constexpr (std::is_same_v<CT, Int4>) { // the codes, written as bfloat16 words
-            using Tile = Int4Tile<HDP, FINE_KEYS, 4>;
+            using Tile = Int4Tile<HDP, FINE_KEYS, 4, 1>;
             const Tile mine(warp - 4, lane);
             while (w.left > 0) {
                 const ManyItem item = w.item(a, paged_seq(a.c, w.b));
                 const int tiles = w.tiles(item), begin = (item.t0 + w.first(item)) * FINE_KEYS;
-                int id[Tile::N];
+                int id[Tile::N], next_pos;
                 typename Tile::Codes next;
                 bool next_v;
-                int next_pos = begin + load_of(0, tiles, &next_v) * FINE_KEYS;
-                mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                const auto look = [&](int p) { // the pages of part p of the item's loads
+                    next_pos = begin + load_of(p / Tile::PARTS, tiles, &next_v) * FINE_KEYS + p % Tile::PARTS * (FINE_KEYS / Tile::PARTS);
+                    mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
+                };
+                look(0);
                 mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
-                next_pos = begin + load_of(1, tiles, &next_v) * FINE_KEYS;
-                mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
-                for (int u = 0; u < 2 * tiles; u++, ld++) {
-                    const int slot = (int)(ld % SLOTS);
+                look(1);
+                const int all = 2 * tiles * Tile::PARTS;
+                for (int p = 0; p < all; p++) {
+                    const int slot = (int)(ld % SLOTS), part = p % Tile::PARTS;
                     const typename Tile::Codes codes = next;
-                    if (u + 1 < 2 * tiles) mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
-                    if (u + 2 < 2 * tiles) {
-                        next_pos = begin + load_of(u + 2, tiles, &next_v) * FINE_KEYS;
-                        mine.pages(id, a.c, w.b, next_pos, item.low, item.high);
-                    }
-                    if (alive && !pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u)) {
+                    if (p + 1 < all) mine.ask(next, id, a.c, w.kvh, next_v ? a.v : a.k, next_pos, item.low, item.high);
+                    if (p + 2 < all) look(p + 2);
+                    if (part == 0 && alive && !pg_bar_wait(&empty[slot], ((ld / SLOTS) & 1u) ^ 1u)) {
                         atomicExch(a.c.status, PAGED_WAIT);
                         alive = false; // it goes on without waiting and without writing
                     }
+                    if (alive) mine.put(ring + slot * SLOT, part, codes);
+                    if (part < Tile::PARTS - 1) continue;
+                    ld++;
                     if (!alive) continue;
-                    mine.put(ring + slot * SLOT, codes);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     pg_bar_arrive(&full[slot]);
                 }

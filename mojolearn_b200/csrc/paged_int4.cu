@@ -10,8 +10,8 @@ namespace b200i {
 FewPlan int4_few_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     return few4_plan(sms, f32_rows, batch, kv, hdp, rows, max_new, max_length, window);
 }
-cudaError_t int4_few(const AttendCall &a, bool f32_rows, const FewPlan &p, int hdp, void *ws, int device, cudaStream_t st, int *launches) {
-    return f32_rows ? launch_few4<float>(a, p, hdp, ws, device, st, launches) : launch_few4<__nv_bfloat16>(a, p, hdp, ws, device, st, launches);
+cudaError_t int4_few(const AttendCall &a, bool f32_rows, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
+    return f32_rows ? launch_few4<float>(a, p, ws, device, st, launches) : launch_few4<__nv_bfloat16>(a, p, ws, device, st, launches);
 }
 cudaError_t int4_many(const AttendCall &a, bool f32_rows, const ManyPlan &p, int hdp, void *ws, int device, cudaStream_t st, int *launches) {
     if (f32_rows) return hdp == 64 ? launch_fine_as<Int4, 64>(a, p, ws, device, st, launches) : launch_fine_as<Int4, 128>(a, p, ws, device, st, launches);

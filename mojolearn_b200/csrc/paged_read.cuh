@@ -1,7 +1,8 @@
 // Rows of a paged cache read back: keys and values of each sequence's rows as one array each.
 //
-// Bound: HBM, what is held read once and what it stands for written once. A block takes READ_ROWS rows: its warps look up where they are, one each, and its
-// threads take units of eight columns of them, keys and values alike, so that neighbours write neighbouring bytes.
+// Bound: HBM, what is held read once and what it stands for written once. A block takes up to 32 rows: the lanes of one warp look up where they are, and a thread
+// has a unit of eight columns of a head and takes it of several rows, keys and values alike, whose words are all asked for before the first is stored;
+// neighbours write neighbouring bytes.
 #pragma once
 #include <algorithm>
 
@@ -15,56 +16,81 @@ struct ReadCall {
     void *k_out, *v_out;
 };
 
-constexpr int READ_ROWS = 8;
+constexpr int READ_ROWS = 32, READ_THREADS = 256;
 
-template <typename OT> struct ReadStore;
-template <> struct ReadStore<float> {
-    static __device__ __forceinline__ void eight(float *p, const float4 &x, const float4 &y) { *reinterpret_cast<float4 *>(p) = x, *reinterpret_cast<float4 *>(p + 4) = y; }
-};
-template <> struct ReadStore<__nv_bfloat16> {
-    static __device__ __forceinline__ void eight(__nv_bfloat16 *p, const float4 &x, const float4 &y) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pg_pack(x.x, x.y), pg_pack(x.z, x.w), pg_pack(y.x, y.y), pg_pack(y.z, y.w));
-    }
-};
+// Eight columns as they are written: what is not float32 is bfloat16 words already, or codes that become them.
+__device__ __forceinline__ void read_store(float *p, const PagedWords<float>::Eight &x) { *reinterpret_cast<float4 *>(p) = x.lo, *reinterpret_cast<float4 *>(p + 4) = x.hi; }
+__device__ __forceinline__ void read_store(__nv_bfloat16 *p, const uint4 &x) { *reinterpret_cast<uint4 *>(p) = x; }
+__device__ __forceinline__ void read_store(float *p, const uint4 &x) {
+    using W = PagedWords<__nv_bfloat16>;
+    *reinterpret_cast<float4 *>(p) = W::lower(x), *reinterpret_cast<float4 *>(p + 4) = W::upper(x);
+}
+template <typename OT> __device__ __forceinline__ void read_store(OT *p, const PagedRows<Int4>::Eight &x) {
+    unsigned v[4];
+    const unsigned s = __float_as_uint(x.scale);
+    int4_pairs(v, x.word, int4_factors(s | s >> 16)); // (a bfloat16 word above zeros)
+    read_store(p, make_uint4(v[0], v[1], v[2], v[3]));
+}
 
 template <typename CT, typename OT>
-__global__ void __launch_bounds__(32 * READ_ROWS) read_kernel(const ReadCall a) {
+__global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadCall a, int rows) {
+    constexpr int ASK = 4; // rows that a thread asks for at once
     __shared__ int at[READ_ROWS]; // a row's place in the caches, of key head 0; -1: there is none, and it is zeros; -2: it belongs to no sequence
     const PagedCall &c = a.c;
-    const int warp = threadIdx.x >> 5;
-    const long long t0 = (long long)blockIdx.x * READ_ROWS, t = t0 + warp;
-    int row = -2;
-    if (t < c.rows) {
-        const int b = paged_row_seq(c, t);
-        if (b >= 0) {
-            const PagedSeq s = paged_seq_checked(c, b);
-            const int pos = s.pos0 + (int)(t - s.first);
-            if (s.n > 0) row = pos < 0 ? -1 : paged_cache_row(c, b, 0, pos);
+    const long long t0 = (long long)blockIdx.x * rows;
+    if (threadIdx.x < 32) {
+        const long long t = t0 + threadIdx.x;
+        int b = paged_row_seq(c, t0), row = -2;
+        if (b >= 0) { // the others' sequences are the first row's, or follow it
+            while (b < c.batch && t >= c.cu[b + 1]) b++;
+        } else {
+            for (int r = 1; r < rows; r++) {
+                const int of = paged_row_seq(c, t0 + r);
+                if ((int)threadIdx.x == r) b = of;
+            }
         }
+        if (b >= 0 && b < c.batch && (int)threadIdx.x < rows && t < c.rows) {
+            if (t >= c.cu[b]) {
+                const PagedSeq s = paged_seq_checked(c, b);
+                const int pos = s.pos0 + (int)(t - s.first);
+                if (s.n > 0) row = pos < 0 ? -1 : paged_cache_row(c, b, 0, pos);
+            }
+        }
+        at[threadIdx.x] = row;
     }
-    if ((threadIdx.x & 31) == 0) at[warp] = row;
     __syncthreads();
-    const int units = c.kv * c.hd / 8; // of a row
+    const int units = c.kv * c.hd / 8, span = min(units, READ_THREADS), step = READ_THREADS / span, r0 = threadIdx.x / span; // units of a row; a thread's rows are step apart
+    if (r0 >= step) return;
     const PagedRows<CT> keys(a.k_cache, c), values(a.v_cache, c);
-    for (int i = blockIdx.y * blockDim.x + threadIdx.x; i < READ_ROWS * units; i += gridDim.y * blockDim.x) {
-        const int r = i / units, u = i - r * units, head = u * 8 / c.hd, col = u * 8 - head * c.hd, place = at[r];
-        if (place == -2) continue;
-        typename PagedRows<CT>::Eight k = {}, v = {};
-        if (place >= 0) {
-            const int of = place + (head << c.page_shift);
-            k = keys.eight(of, col), v = values.eight(of, col);
+    for (int u = threadIdx.x - r0 * span; u < units; u += span) {
+        const int head = u * 8 / c.hd, col = u * 8 - head * c.hd;
+        for (int first = r0; first < rows; first += ASK * step) {
+            typename PagedRows<CT>::Eight k[ASK], v[ASK];
+            int place[ASK];
+#pragma unroll
+            for (int i = 0; i < ASK; i++) {
+                const int r = first + i * step;
+                place[i] = r < rows ? at[r] : -2;
+                k[i] = {}, v[i] = {};
+                if (place[i] < 0) continue;
+                const int of = place[i] + (head << c.page_shift);
+                k[i] = keys.eight(of, col), v[i] = values.eight(of, col);
+            }
+#pragma unroll
+            for (int i = 0; i < ASK; i++) {
+                if (place[i] == -2) continue;
+                const long long to = ((t0 + first + i * step) * c.kv + head) * c.hd + col;
+                read_store(static_cast<OT *>(a.k_out) + to, k[i]);
+                read_store(static_cast<OT *>(a.v_out) + to, v[i]);
+            }
         }
-        const long long to = ((t0 + r) * c.kv + head) * c.hd + col;
-        ReadStore<OT>::eight(static_cast<OT *>(a.k_out) + to, PagedRows<CT>::lower(k), PagedRows<CT>::upper(k));
-        ReadStore<OT>::eight(static_cast<OT *>(a.v_out) + to, PagedRows<CT>::lower(v), PagedRows<CT>::upper(v));
     }
 }
 
 template <typename CT, typename OT>
 cudaError_t launch_read(const ReadCall &a, int sms, cudaStream_t st) {
-    const long long blocks = (a.c.rows + READ_ROWS - 1) / READ_ROWS, each = ((long long)READ_ROWS * a.c.kv * a.c.hd / 8 + 32 * READ_ROWS - 1) / (32 * READ_ROWS);
-    const int y = (int)std::max<long long>(1, std::min<long long>(each, 8LL * sms / blocks)); // with a few rows a thread takes one unit
-    read_kernel<CT, OT><<<dim3((unsigned)blocks, (unsigned)y), 32 * READ_ROWS, 0, st>>>(a);
+    const int rows = (int)std::max<long long>(1, std::min<long long>(READ_ROWS, a.c.rows / (4 * sms))); // with a few rows a block takes fewer
+    read_kernel<CT, OT><<<(unsigned)((a.c.rows + rows - 1) / rows), READ_THREADS, 0, st>>>(a, rows);
     return cudaGetLastError();
 }
 
