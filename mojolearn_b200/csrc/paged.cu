@@ -11,6 +11,7 @@
 #include "paged_int4.h"
 #include "paged_many.cuh"
 #include "paged_read.cuh"
+#include "paged_unpack.cuh"
 
 using namespace b200i;
 using b200i_library::refuse;
@@ -66,8 +67,15 @@ struct AttendPlan {
     int hdp;      // head_dim as it is laid out in shared memory
     FewPlan cut;
     ManyPlan cut_many; // where they are many
-    int64_t bytes() const { return few ? cut.bytes : cut_many.bytes; }
+    int64_t unpacked;  // positions of a sequence for which there is room in bfloat16 words (0: a cache in 4 bits is read as it is), and its bytes behind the parts
+    int64_t unpacked_bytes;
+    int64_t bytes() const { return few ? cut.bytes : (unpacked ? unpacked_at() + unpacked_bytes : cut_many.bytes); }
+    int64_t unpacked_at() const { return (cut_many.bytes + 15) / 16 * 16; }
 };
+
+// A cache in 4 bits is made one of words first where a sequence's rows are more than UNPACK_BLOCKS blocks of rows, each of which would make the words for itself, and where that
+// takes at most UNPACK_MOST bytes.
+constexpr int64_t UNPACK_BLOCKS = 2, UNPACK_MOST = 256 << 20;
 
 AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
     AttendPlan p = {};
@@ -84,6 +92,11 @@ AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t
         const bool wide = row_type == B200I_T_BF16;
         p.cut_many = many_plan(b200i_library::device_sms(device), wide ? ManyShape<128>::BLOCK_ROWS : FINE_ROWS, p.hdp, wide ? MANY_KEYS : FINE_KEYS, rows, batch, n_kv, group, max_new,
                                std::min(max_length, MOST));
+        if (cache_type == B200I_T_INT4 && wide && std::min(max_new, rows) * group > UNPACK_BLOCKS * ManyShape<128>::BLOCK_ROWS && max_length <= MOST) {
+            p.unpacked = (max_length + 255) / 256 * 256;
+            if (batch * n_kv * p.unpacked <= UNPACK_MOST) p.unpacked_bytes = unpack_bytes(batch, p.unpacked, n_kv, head_dim);
+            if (p.unpacked_bytes == 0 || p.unpacked_bytes > UNPACK_MOST) p.unpacked = p.unpacked_bytes = 0;
+        }
     }
     return p;
 }
@@ -204,7 +217,11 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const AttendPlan p = attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
     if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
-    if (cache_type == B200I_T_INT4) {
+    if (cache_type == B200I_T_INT4 && max_pages * page <= p.unpacked) { // (a table of more positions than max_length says may hold longer sequences)
+        LIBRARY_CUDA_TRY(launch_unpack(&a, static_cast<unsigned char *>(ws) + p.unpacked_at(), st));
+        launches++;
+        LIBRARY_CUDA_TRY((p.hdp == 64 ? launch_many_as<__nv_bfloat16, 64>(a, p.cut_many, ws, dev, st, &launches) : launch_many_as<__nv_bfloat16, 128>(a, p.cut_many, ws, dev, st, &launches)));
+    } else if (cache_type == B200I_T_INT4) {
         LIBRARY_CUDA_TRY(p.few ? int4_few(a, row_type == B200I_T_F32, p.cut, ws, dev, st, &launches) : int4_many(a, row_type == B200I_T_F32, p.cut_many, p.hdp, ws, dev, st, &launches));
     } else if (p.few) {
         if (row_type == B200I_T_BF16)

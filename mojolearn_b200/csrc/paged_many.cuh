@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
     __shared__ unsigned tmem_slot;
     __shared__ int dead;
     const AttendCall &a = f.a;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // Where codes become words, that group is the first: the others have the scheduler's favour else, and wait for it.
+    const int tid = FOUR ? (threadIdx.x + 512) % 640 : threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < 8; i++) pg_bar_init(&pair_bars[i], 64);
         for (int s = 0; s < SLOTS; s++) {
