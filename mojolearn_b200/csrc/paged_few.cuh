@@ -36,7 +36,7 @@ template <typename CT, int HDP> struct FewKeys { static constexpr int N = FEW_SL
 // Shared memory of a block: the ring, `meet` bytes for the warps' results, the queries, barriers. Two blocks on an SM (113 KB each) where
 // that leaves two slots.
 template <int HDP, int MEET_BYTES, int QUERY_BYTES> struct FewShape {
-    static constexpr int WARPS = FEW_WARPS, COPIERS = 1, SLOT = FEW_SLOT, MEET = MEET_BYTES, QUERY = QUERY_BYTES;
+    static constexpr int WARPS = FEW_WARPS, SLOT = FEW_SLOT, MEET = MEET_BYTES, QUERY = QUERY_BYTES;
     static constexpr int REST = 1024 + 512 + MEET + FEW_ITEMS * QUERY;
     static constexpr int BLOCKS = (110 * 1024 - REST) / SLOT >= 2 ? 2 : 1;
     static constexpr int ROOM = ((BLOCKS == 2 ? 112 : 220) * 1024 - REST) / SLOT;
@@ -150,8 +150,7 @@ template <typename Shape> struct FewMemory {
 
 // The copying warp. `items`: FEW_ITEMS of them in shared memory. `bring(to, full, pos, there, low, kvh, page_of)`, all lanes, asks for the `there` pieces (of
 // min(page, KEYS) positions) of a tile that begins at pos, as bytes that `full` counts: page_of(piece) is a piece's page, and positions below low are seen by no row.
-// With two copying warps the one that LEADs tells of the items, and each brings its part of a tile.
-template <typename RT, int KEYS, bool LEAD = true, typename Shape, typename F>
+template <typename RT, int KEYS, typename Shape, typename F>
 __device__ __forceinline__ void few_copies(const FewCall &f, const FewMemory<Shape> &sm, FewItem *items, const LinePlace &p, F bring) {
     constexpr int SLOTS = Shape::SLOTS;
     const AttendCall &a = f.a;
@@ -182,9 +181,8 @@ __device__ __forceinline__ void few_copies(const FewCall &f, const FewMemory<Sha
         s = paged_seq(a.c, b), count = few_tiles(a, s, KEYS, &t0);
     for (; alive; number++) {
         const int at = number % FEW_ITEMS;
-        if (LEAD && !wait(&sm.item_empty[at], ((number / FEW_ITEMS) & 1u) ^ 1u)) break; // a fresh barrier counts as released
+        if (!wait(&sm.item_empty[at], ((number / FEW_ITEMS) & 1u) ^ 1u)) break; // a fresh barrier counts as released
         if (left <= 0) { // the others are told that there is no more
-            if (!LEAD) break;
             if (lane == 0) {
                 items[at].more = 0;
                 pg_bar_arrive(&sm.item_full[at]);
@@ -193,21 +191,19 @@ __device__ __forceinline__ void few_copies(const FewCall &f, const FewMemory<Sha
             break;
         }
         const int tiles = f.whole ? count : (int)min((long long)(count - before), left), n = min(s.n, a.max_new);
-        if constexpr (LEAD) {
-            const unsigned row_bytes = (unsigned)(a.c.group * a.c.hd * (int)sizeof(RT)); // of a token's rows, which stand side by side
-            if (lane == 0) {
-                items[at] = FewItem{kvh, b, s, n, (t0 + before) * KEYS, tiles, before, count, line, (int)p.per, 1};
-                if (s.n > a.max_new) atomicExch(a.c.status, PAGED_BAD_BOUND);
-                pg_bar_expect(&sm.item_full[at], row_bytes * (unsigned)n);
-            }
-            sent++;
-            __syncwarp();
-            if (lane < n) {
-                const RT *src = static_cast<const RT *>(a.q) + (long long)(s.first + lane) * a.ldq + (long long)kvh * a.c.group * a.c.hd;
-                asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(sm.query + at * Shape::QUERY) + lane * row_bytes), "l"(src),
-                             "r"(row_bytes), "r"(pg_smem(&sm.item_full[at]))
-                             : "memory");
-            }
+        const unsigned row_bytes = (unsigned)(a.c.group * a.c.hd * (int)sizeof(RT)); // of a token's rows, which stand side by side
+        if (lane == 0) {
+            items[at] = FewItem{kvh, b, s, n, (t0 + before) * KEYS, tiles, before, count, line, (int)p.per, 1};
+            if (s.n > a.max_new) atomicExch(a.c.status, PAGED_BAD_BOUND);
+            pg_bar_expect(&sm.item_full[at], row_bytes * (unsigned)n);
+        }
+        sent++;
+        __syncwarp();
+        for (int i = lane; i < n; i += 32) {
+            const RT *src = static_cast<const RT *>(a.q) + (long long)(s.first + i) * a.ldq + (long long)kvh * a.c.group * a.c.hd;
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(pg_smem(sm.query + at * Shape::QUERY) + i * row_bytes), "l"(src),
+                         "r"(row_bytes), "r"(pg_smem(&sm.item_full[at]))
+                         : "memory");
         }
         const int last_page = (s.length - 1) >> a.c.page_shift, low = a.window ? max(0, s.pos0 + 1 - a.window) : 0; // no row sees what is below
         const int *ids = a.c.table + (long long)b * a.c.max_pages;
@@ -275,11 +271,11 @@ __device__ __forceinline__ auto few_boxes(const CUtensorMap *map_k, const CUtens
 }
 
 // The beginning of a block: barriers, and its place on the line.
-template <int KEYS, typename Shape>
-__device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory<Shape> &sm, long long *place, unsigned *bad_rows, int *dead) {
+template <int KEYS, typename Shape, typename Bits>
+__device__ __forceinline__ LinePlace few_begin(const FewCall &f, const FewMemory<Shape> &sm, long long *place, Bits *bad_rows, int *dead) {
     if (threadIdx.x == 0) {
         for (int s = 0; s < Shape::SLOTS; s++) {
-            pg_bar_init(&sm.full[s], Shape::COPIERS);
+            pg_bar_init(&sm.full[s], 1);
             pg_bar_init(&sm.empty[s], Shape::WARPS);
         }
         for (int i = 0; i < FEW_ITEMS; i++) {
@@ -320,9 +316,9 @@ template <int WARPS = FEW_WARPS> __device__ __forceinline__ bool few_vote(bool y
     return some != 0;
 }
 // Rows that did not come out finite, done again: a masked key's zero weight met a value that is not finite.
-template <typename RT, typename CT, int WARPS = FEW_WARPS>
-__device__ __forceinline__ void few_again(const AttendCall &a, const FewItem &i, unsigned *bad_rows, int rows) {
-    const unsigned rest = *bad_rows;
+template <typename RT, typename CT, int WARPS = FEW_WARPS, typename Bits>
+__device__ __forceinline__ void few_again(const AttendCall &a, const FewItem &i, Bits *bad_rows, int rows) {
+    const Bits rest = *bad_rows;
     few_meet<WARPS>();
     if (threadIdx.x == 0) *bad_rows = 0;
     for (int r = threadIdx.x >> 5; r < rows; r += WARPS)

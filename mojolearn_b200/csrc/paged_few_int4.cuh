@@ -13,37 +13,39 @@
 #pragma once
 #include <type_traits>
 
-#include "paged_few.cuh"
 #include "paged_int4.cuh"
+#include "paged_many.cuh"
 
 namespace b200i {
 
-constexpr int FEW4_WARPS = 8, FEW4_THREADS = 32 * (FEW4_WARPS + 2), FEW4_KEYS = 16 * FEW4_WARPS; // two warps copy, keys and values
+constexpr int FEW4_WARPS = 8, FEW4_THREADS = 32 * (FEW4_WARPS + 1), FEW4_KEYS = 16 * FEW4_WARPS;
 
 template <typename RT, int GROUPS, int NT, bool PACK> struct Few4Shape {
     static constexpr bool F32 = std::is_same_v<RT, float>;
     static constexpr int HDP = GROUPS <= 2 ? 64 : 128; // head_dim as it is laid out for the products: a lane's quarter (eighth) of it lies in one group
-    static constexpr int WARPS = FEW4_WARPS, COPIERS = 2, ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
+    static constexpr int WARPS = FEW4_WARPS, ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
+    static constexpr int BLOCKS = NT > 1 ? 1 : 2;                        // on an SM
+    static constexpr int SPLIT = NT > 2 && HDP == 128 ? 2 : 1;           // warps that share keys, each for its part of the values' columns
+    static constexpr int SLICES = WARPS / SPLIT, CHUNKS = SPLIT;         // a tile's keys go to so many warps, by so many times 16
     static constexpr int HALF = FEW4_KEYS * GROUPS * INT4_BYTES, SLOT = 2 * HALF; // keys, then values
-    static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : 2;
+    static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : (NT > 2 ? 1 : 2);
     static constexpr bool HELD = PACK || (!F32 && NT == 1); // the queries stay in registers; else they lie as fragments where the warps' results meet
-    static constexpr int TOGETHER = 1;
     static constexpr int PITCH = HDP + 8;                   // floats of a row of those
-    static constexpr int MEET = FEW4_WARPS / 2 * ROWS * PITCH * 4, QUERY = ROWS * HDP * (int)sizeof(RT);
+    static constexpr int MEET = 4 * ROWS * PITCH * 4, QUERY = ROWS * HDP * (int)sizeof(RT);
     static constexpr int REST = 1024 + 512 + MEET + FEW_ITEMS * QUERY;
-    static constexpr int ROOM = (112 * 1024 - REST) / SLOT, SLOTS = ROOM > 8 ? 8 : ROOM;
+    static constexpr int ROOM = ((BLOCKS == 2 ? 112 : 220) * 1024 - REST) / SLOT, SLOTS = ROOM > 8 ? 8 : ROOM;
     static constexpr int SMEM = REST + SLOTS * SLOT;
-    static_assert(SLOTS > TOGETHER && (HELD || Q_PIECES * NT * HDP / 16 * 256 <= MEET), "shared memory");
+    static_assert(SLOTS >= 2 && (HELD || Q_PIECES * NT * HDP / 16 * 256 <= MEET), "shared memory");
 };
 
-// What brings a tile's keys (or values): a lane a piece, whose codes and scales follow one another in the cache as in the slot. Of a page larger than a tile they do
-// not, and two lanes bring them.
+// What brings a tile: two lanes a piece, its keys and its values, whose codes and scales follow one another in the cache as in the slot. Of a page larger than a tile
+// they do not, and four lanes bring them.
 template <typename Shape>
-__device__ __forceinline__ auto few4_runs(const AttendCall &a, bool values) {
-    return [&a, values](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
+__device__ __forceinline__ auto few4_runs(const AttendCall &a) {
+    return [&a](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
         const PagedCall &c = a.c;
         const int lane = threadIdx.x & 31, page = 1 << c.page_shift, rows = min(page, FEW4_KEYS), groups = int4_groups(c.hd), split = page > FEW4_KEYS;
-        const int piece = lane >> split, scales = lane & split; // this lane's
+        const int values = lane & 1, scales = (lane >> 1) & split, piece = lane >> (1 + split); // this lane's
         const int id = page_of(piece), first = piece * rows;
         const bool want = piece < there && low - pos < first + rows; // a page that nobody sees any more may be anyone's
         const bool some = want && (unsigned)id < (unsigned)c.pages;
@@ -65,41 +67,46 @@ __device__ __forceinline__ auto few4_runs(const AttendCall &a, bool values) {
 }
 
 template <typename RT, int GROUPS, int NT, bool PACK>
-__global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
+__global__ void __launch_bounds__(FEW4_THREADS, Few4Shape<RT, GROUPS, NT, PACK>::BLOCKS) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
     using Shape = Few4Shape<RT, GROUPS, NT, PACK>;
     constexpr bool F32 = Shape::F32, HELD = Shape::HELD;
-    constexpr int HDP = Shape::HDP, KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = FEW4_WARPS, QP = Shape::Q_PIECES, WP = Shape::W_PIECES, CH = Shape::TOGETHER;
-    constexpr int E = PACK ? 1 : 2 * NT;                   // rows of a lane's scores
-    constexpr int K_WORDS = HDP / 32, V_WORDS = HDP / 64;  // of codes, of a key: a quarter of its columns, an eighth
-    constexpr int STRIDE = 16 * GROUPS;                    // bytes of a key's codes
+    constexpr int HDP = Shape::HDP, KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = FEW4_WARPS, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
+    constexpr int SPLIT = Shape::SPLIT, SLICES = Shape::SLICES, CHUNKS = Shape::CHUNKS, MT = KS / SPLIT; // MT: pieces of 16 columns of the output that a warp has
+    constexpr int E = PACK ? 1 : 2 * NT;                          // rows of a lane's scores
+    constexpr int K_WORDS = HDP / 32, V_WORDS = HDP / 64 / SPLIT; // of codes, of a key: a quarter of its columns, an eighth (of the warp's)
+    constexpr int STRIDE = 16 * GROUPS;                           // bytes of a key's codes
     extern __shared__ __align__(128) unsigned char smem[];
     const FewMemory<Shape> sm(smem);
-    __shared__ float ml[WARPS][2][ROWS], joined[2][ROWS];
+    __shared__ float ml[SLICES][2][ROWS], joined[2][ROWS];
     __shared__ long long place[32];
     __shared__ FewItem items[FEW_ITEMS];
-    __shared__ unsigned bad_rows;
+    __shared__ unsigned long long bad_rows;
     __shared__ int dead;
     const AttendCall &a = f.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     const LinePlace p = few_begin<KEYS>(f, sm, place, &bad_rows, &dead);
-    if (warp >= WARPS) {
-        if (warp == WARPS)
-            few_copies<RT, KEYS, true>(f, sm, items, p, few4_runs<Shape>(a, false));
-        else
-            few_copies<RT, KEYS, false>(f, sm, items, p, few4_runs<Shape>(a, true));
+    if (warp == WARPS) {
+        few_copies<RT, KEYS>(f, sm, items, p, few4_runs<Shape>(a));
         return;
     }
 
     // of the lane's columns: of a key's quarters and of its eighths, those that are in no group of the head's count as zeros
+    const int slice = warp / SPLIT, side = warp % SPLIT, key0 = slice * 16 * CHUNKS; // the warp's keys of a tile
     const int k_group = t4 * (HDP / 4) / INT4_GROUP, v_group = g * (HDP / 8) / INT4_GROUP;
     const bool k_some = k_group < GROUPS, v_some = v_group < GROUPS;
-    // in a slot, of the warp's 16 keys: the lane's codes and scales of keys g (and g + 8), and of values 2 t4 (and 1, 8 and 9 further on)
-    const int box_rows = min(1 << a.c.page_shift, KEYS), in = (warp * 16) & (box_rows - 1), piece = (warp * 16 - in) * (GROUPS * INT4_BYTES); // the piece they lie in
-    const int k_at = piece + (in + g) * STRIDE + (k_some ? t4 * (HDP / 8) : 0), k_scale = piece + box_rows * STRIDE + (in + g) * (2 * GROUPS) + (k_some ? 2 * k_group : 0);
-    const int v_at = Shape::HALF + piece + (in + 2 * t4) * STRIDE + (v_some ? g * (HDP / 16) : 0);
-    const int v_scale = Shape::HALF + piece + box_rows * STRIDE + (in + 2 * t4) * (2 * GROUPS) + (v_some ? 2 * v_group : 0);
-    const float unit = a.softcap > 0.0f ? a.softcap * PAGED_LOG2E : a.scale * PAGED_LOG2E, part_of_unit = 1.0f / unit;
+    // in a slot, of 16 of its keys: the lane's codes and scales of keys g (and g + 8), and of values 2 t4 (and 1, 8 and 9 further on)
+    const int box_rows = min(1 << a.c.page_shift, KEYS); // of the piece that they lie in
+    int k_at[CHUNKS], k_scale[CHUNKS], v_at[CHUNKS], v_scale[CHUNKS];
+#pragma unroll
+    for (int c = 0; c < CHUNKS; c++) {
+        const int key = key0 + 16 * c, in = key & (box_rows - 1), piece = (key - in) * (GROUPS * INT4_BYTES), scales = piece + box_rows * STRIDE;
+        k_at[c] = piece + (in + g) * STRIDE + (k_some ? t4 * (HDP / 8) : 0), k_scale[c] = scales + (in + g) * (2 * GROUPS) + (k_some ? 2 * k_group : 0);
+        v_at[c] = Shape::HALF + piece + (in + 2 * t4) * STRIDE + (v_some ? g * (HDP / 16) + side * (V_WORDS * 4) : 0);
+        v_scale[c] = Shape::HALF + scales + (in + 2 * t4) * (2 * GROUPS) + (v_some ? 2 * v_group : 0);
+    }
+    const float unit = a.scale * PAGED_LOG2E, part_of_unit = 1.0f / unit; // (capped scores are still to be scaled: paged_many.cuh)
     const auto row_of = [&](int e) { return PACK ? (F32 ? t4 >> 1 : t4) : (e >> 1) * 8 + 2 * t4 + (e & 1); };
+    const auto token_of = [&](int r) { return a.c.group == 1 ? r : (int)__umulhi((unsigned)r, a.c.group_part); };
     uint2 *const fragments = reinterpret_cast<uint2 *>(sm.meet);
     unsigned slot_at = 0, parity = 0; // of the next tile
     bool alive = true, first_part = true;
@@ -111,13 +118,13 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
         const int which = number % FEW_ITEMS;
         if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.item_full[which], (number / FEW_ITEMS) & 1u))) give_up();
         if (few_vote<WARPS>(!alive)) break; // nobody goes on where one has given up: what the item is would not be known
-        const FewItem item = items[which];
+        const FewItem &item = items[which]; // what the loop over the tiles does not need is read again after it
         if (!item.more) break;
-        const PagedSeq s = item.s;
-        const int rows = min(item.n * a.c.group, ROWS);
+        const int length = item.s.length, pos0 = item.s.pos0, tiles = item.tiles, begin = item.pos + key0;
+        const auto rows_of = [&] { return min(item.n * a.c.group, ROWS); };
 
         // The rows as fragments: column n of row `row`, words col .. col + 3 of it, piece by piece.
-        const auto words = [&](uint2 (&q)[QP], int row, int col) {
+        const auto words = [&, rows = rows_of()](uint2 (&q)[QP], int row, int col) {
 #pragma unroll
             for (int k = 0; k < QP; k++) q[k] = make_uint2(0, 0);
             if (row >= rows || col >= a.c.hd) return;
@@ -155,270 +162,240 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
             }
             few_meet<WARPS>();
         }
-        int hi[E], lo[E]; // what a row sees: positions lo .. hi - 1
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            hi[e] = row_of(e) < rows ? s.pos0 + row_of(e) / a.c.group + 1 : 0;
-            lo[e] = a.window ? hi[e] - a.window : 0;
-        }
-        const int all_lo = a.window ? s.pos0 + item.n - a.window : 0, low = a.window ? s.pos0 + 1 - a.window : 0; // every row sees positions all_lo .. pos0; none sees what is below low
+        // every row sees positions all_lo .. pos0; none sees what is below low
+        const int all_lo = a.window ? pos0 + item.n - a.window : 0, low = a.window ? pos0 + 1 - a.window : 0;
 
-        float o[NT][KS][4], m[E], l[E], high[E]; // high: the score that m is to be moved for
+        float o[NT][MT][4], m[E], l[E], high[E]; // high: the score that m is to be moved for
 #pragma unroll
         for (int e = 0; e < E; e++) m[e] = high[e] = -INFINITY, l[e] = 0.0f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int mt = 0; mt < KS; mt++) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
-        for (int t = 0; t < item.tiles; t += CH) {
-            const unsigned char *slot[CH];
-            unsigned long long *empty[CH];
-            int j0[CH]; // the warp's first key of each tile; of one that is not there, past all keys
+            for (int mt = 0; mt < MT; mt++) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
+        // Scores of 16 keys of a tile, the warp's chunk c of them.
+        constexpr int ZS = F32 && !PACK ? 2 : 1; // large and small products apart
+        float z[ZS][NT][4];
+        const auto scores = [&](const unsigned char *slot, int c) {
+            unsigned code[2][K_WORDS];
+            Int4Factors factors[2];
 #pragma unroll
-            for (int c = 0; c < CH; c++) {
-                const bool there = c == 0 || t + c < item.tiles;
-                j0[c] = there ? item.pos + (t + c) * KEYS + warp * 16 : 0x7FFFFF00;
-                slot[c] = c == 0 || there ? sm.ring + slot_at * Shape::SLOT : slot[0];
-                empty[c] = &sm.empty[slot_at];
-                if (!there) break;
-                if (alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot_at], parity))) give_up();
-                if (++slot_at == SLOTS) slot_at = 0, parity ^= 1;
+            for (int h = 0; h < 2; h++) { // keys g and g + 8
+                const unsigned char *at = slot + k_at[c] + h * 8 * STRIDE;
+                if constexpr (K_WORDS == 4) {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(at);
+                    code[h][0] = w.x, code[h][1] = w.y, code[h][2] = w.z, code[h][3] = w.w;
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2 *>(at);
+                    code[h][0] = w.x, code[h][1] = w.y;
+                }
+                unsigned scale = *reinterpret_cast<const unsigned short *>(slot + k_scale[c] + h * 16 * GROUPS);
+                if (GROUPS % 2 && !k_some) scale = 0;
+                factors[h] = int4_factors(scale * 0x10001u);
             }
-            if (alive && j0[0] < s.length && (j0[CH - 1] + 16 > low)) {
-                // ---- scores ----
-                constexpr int ZS = F32 && !PACK ? 2 : 1; // large and small products apart
-                float z[CH][ZS][NT][4];
 #pragma unroll
-                for (int c = 0; c < CH; c++)
+            for (int w = 0; w < K_WORDS; w++) {
+                unsigned x[2][4];
 #pragma unroll
-                    for (int k = 0; k < ZS; k++)
+                for (int h = 0; h < 2; h++) int4_pairs(x[h], code[h][w], factors[h]);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) z[c][k][nt][0] = z[c][k][nt][1] = z[c][k][nt][2] = z[c][k][nt][3] = 0.0f;
-                unsigned k_code[CH][2][K_WORDS], k_scales[CH][2];
+                for (int i = 0; i < 2; i++) {
+                    const unsigned k[4] = {x[0][2 * i], x[1][2 * i], x[0][2 * i + 1], x[1][2 * i + 1]};
+                    const int ks = 2 * w + i;
 #pragma unroll
-                for (int c = 0; c < CH; c++)
+                    for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) { // keys g and g + 8
-                        const unsigned char *at = slot[c] + k_at + h * 8 * STRIDE;
-                        if constexpr (K_WORDS == 4) {
-                            const uint4 w = *reinterpret_cast<const uint4 *>(at);
-                            k_code[c][h][0] = w.x, k_code[c][h][1] = w.y, k_code[c][h][2] = w.z, k_code[c][h][3] = w.w;
-                        } else {
-                            const uint2 w = *reinterpret_cast<const uint2 *>(at);
-                            k_code[c][h][0] = w.x, k_code[c][h][1] = w.y;
-                        }
-                        k_scales[c][h] = *reinterpret_cast<const unsigned short *>(slot[c] + k_scale + h * 16 * GROUPS);
-                        if (GROUPS % 2 && !k_some) k_scales[c][h] = 0;
-                        k_scales[c][h] *= 0x10001u;
-                    }
-#pragma unroll
-                for (int w = 0; w < K_WORDS; w++)
-#pragma unroll
-                    for (int c = 0; c < CH; c++) {
-                        unsigned x[2][4];
-#pragma unroll
-                        for (int h = 0; h < 2; h++) int4_pairs(x[h], k_code[c][h][w], int4_factors(k_scales[c][h]));
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            const unsigned k[4] = {x[0][2 * i], x[1][2 * i], x[0][2 * i + 1], x[1][2 * i + 1]};
-                            const int ks = 2 * w + i;
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                if constexpr (HELD) {
-                                    pg_mma(z[c][0][nt], k, held[ks].x, held[ks].y);
-                                } else {
-#pragma unroll
-                                    for (int piece = QP - 1; piece >= 0; piece--) {
-                                        const uint2 q = fragments[piece * (NT * KS * 32) + (nt * KS + ks) * 32 + lane];
-                                        pg_mma(z[c][piece > 0 ? ZS - 1 : 0][nt], k, q.x, q.y);
-                                    }
-                                }
-                            }
+                        for (int piece = HELD ? 0 : QP - 1; piece >= 0; piece--) {
+                            const uint2 q = HELD ? held[HELD ? ks : 0] : fragments[piece * (NT * KS * 32) + (nt * KS + ks) * 32 + lane];
+                            float(&sum)[4] = z[!HELD && piece > 0 ? ZS - 1 : 0][nt];
+                            if (ks == 0 && (piece == 0 || piece == QP - 1))
+                                pg_mma_first(sum, k, q.x, q.y);
+                            else
+                                pg_mma(sum, k, q.x, q.y);
                         }
                     }
-                float x[CH][E][2]; // keys g and g + 8
-#pragma unroll
-                for (int c = 0; c < CH; c++)
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            if constexpr (PACK) {
-                                x[c][e][h] = z[c][0][0][2 * h];
-                                if constexpr (F32) {
-                                    x[c][e][h] += z[c][0][0][2 * h + 1]; // two pieces here, the third beside it
-                                    x[c][e][h] += __shfl_xor_sync(0xFFFFFFFFu, x[c][e][h], 1);
-                                }
-                            } else {
-                                x[c][e][h] = z[c][0][e >> 1][2 * h + (e & 1)];
-                                if constexpr (F32) x[c][e][h] += z[c][ZS - 1][e >> 1][2 * h + (e & 1)];
-                            }
-                        }
-                if (a.softcap > 0.0f) {
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-#pragma unroll
-                        for (int e = 0; e < E; e++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) x[c][e][h] = tanhf(x[c][e][h] * a.scale * a.cap_part); // (scale / softcap may leave 32 bits)
                 }
-                const bool edge = j0[CH - 1] + 16 > s.pos0 + 1 || j0[0] < all_lo; // (the last tile is the furthest)
-                if (edge) {
+            }
+        };
+        for (int i = 0; i < tiles * CHUNKS; i++) {
+            const int c = CHUNKS == 1 ? 0 : i % CHUNKS, j0 = begin + i / CHUNKS * KEYS + 16 * c;
+            const unsigned char *const slot = sm.ring + slot_at * Shape::SLOT;
+            if (c == 0 && alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot_at], parity))) give_up();
+            const auto leave = [&] {
+                if (c < CHUNKS - 1) return;
+                __syncwarp();
+                if (lane == 0 && alive) pg_bar_arrive(&sm.empty[slot_at]); // (what it has not waited for is not given back)
+                if (++slot_at == SLOTS) slot_at = 0, parity ^= 1;
+            };
+            if (!alive || j0 >= length || j0 + 16 <= low) {
+                leave();
+                continue;
+            }
+            scores(slot, c);
+            float x[E][2]; // keys g and g + 8
 #pragma unroll
-                    for (int c = 0; c < CH; c++)
+            for (int e = 0; e < E; e++)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int j = j0[c] + g + h * 8;
-#pragma unroll
-                            for (int e = 0; e < E; e++)
-                                if (j >= hi[e] || j < lo[e]) x[c][e][h] = -INFINITY;
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (PACK) {
+                        x[e][h] = z[0][0][2 * h];
+                        if constexpr (F32) {
+                            x[e][h] += z[0][0][2 * h + 1]; // two pieces here, the third beside it
+                            x[e][h] += __shfl_xor_sync(0xFFFFFFFFu, x[e][h], 1);
                         }
-                }
-                bool more = false;
-#pragma unroll
-                for (int e = 0; e < E; e++)
-#pragma unroll
-                    for (int c = 0; c < CH; c++) more |= x[c][e][0] > high[e] || x[c][e][1] > high[e];
-                if (__any_sync(0xFFFFFFFFu, more)) {
-                    float keep[E];
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        float top = fmaxf(x[0][e][0], x[0][e][1]);
-#pragma unroll
-                        for (int c = 1; c < CH; c++) top = fmaxf(top, fmaxf(x[c][e][0], x[c][e][1]));
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
-                        top = fmaxf(m[e], top * unit);
-                        keep[e] = m[e] == -INFINITY ? 0.0f : paged_exp2(m[e] - top);
-                        m[e] = top, l[e] *= keep[e], high[e] = (top + 8.0f) * part_of_unit;
+                    } else {
+                        x[e][h] = z[0][e >> 1][2 * h + (e & 1)];
+                        if constexpr (F32) x[e][h] += z[ZS - 1][e >> 1][2 * h + (e & 1)];
                     }
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int mt = 0; mt < KS; mt++)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[nt][mt][i] *= keep[PACK ? 0 : 2 * nt + (i & 1)];
                 }
-                // ---- weights, as pieces and turned: keys down ----
-                unsigned w[CH][NT][PACK ? 1 : WP][2];
-                float base[E];
+            if (a.softcap > 0.0f) { // (what is not seen may be anything, and goes after this)
+                if constexpr (F32)
+                    pg_cap_fine<2 * E>(&x[0][0], a);
+                else if (a.cap_far)
+                    pg_cap<2 * E, true>(&x[0][0], a);
+                else
+                    pg_cap<2 * E, false>(&x[0][0], a);
+            }
+            const bool edge = j0 + 16 > pos0 + 1 || j0 < all_lo;
+            unsigned counts[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}; // the scales of values
+            if (edge) { // a row sees positions up to its own, and with a window the last so many of them
 #pragma unroll
-                for (int e = 0; e < E; e++) base[e] = m[e] == -INFINITY ? 0.0f : -m[e];
-#pragma unroll
-                for (int c = 0; c < CH; c++)
+                for (int e = 0; e < E; e++) {
+                    const int r = row_of(e), hi = r < rows_of() ? pos0 + token_of(r) + 1 : 0, lo = a.window ? hi - a.window : 0;
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        float y[E];
-#pragma unroll
-                        for (int e = 0; e < E; e++) {
-                            y[e] = paged_exp2(fmaf(x[c][e][h], unit, base[e]));
-                            l[e] += y[e];
-                        }
-                        if constexpr (PACK) {
-                            const float rest = y[0] - __uint_as_float(pg_pack(y[0], 0.0f) << 16);
-                            unsigned two = pg_pack(y[0], rest);
-                            if constexpr (F32) {
-                                const float last = rest - __uint_as_float(two & 0xFFFF0000u);
-                                if (t4 & 1) two = pg_pack(last, 0.0f);
-                            }
-                            w[c][0][0][h] = pg_transpose(two);
-                        } else {
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                unsigned piece[WP];
-                                pg_split<WP>(piece, y[2 * nt], y[2 * nt + 1]);
-#pragma unroll
-                                for (int k = 0; k < WP; k++) w[c][nt][k][h] = pg_transpose(piece[k]);
-                            }
-                        }
+                        const int j = j0 + g + h * 8;
+                        if (j >= hi || j < lo) x[e][h] = -INFINITY;
                     }
-                // ---- values ----
-                unsigned code[CH][4][V_WORDS], scales[CH][2];
-#pragma unroll
-                for (int c = 0; c < CH; c++) {
-                    unsigned scale[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) { // keys 2 t4, 2 t4 + 1, and eight further on
-                        const int key = (k & 1) + (k >> 1) * 8;
-                        const unsigned char *at = slot[c] + v_at + key * STRIDE;
-                        if constexpr (V_WORDS == 2) {
-                            const uint2 v = *reinterpret_cast<const uint2 *>(at);
-                            code[c][k][0] = v.x, code[c][k][1] = v.y;
-                        } else {
-                            code[c][k][0] = *reinterpret_cast<const unsigned *>(at);
-                        }
-                        scale[k] = *reinterpret_cast<const unsigned short *>(slot[c] + v_scale + key * GROUPS * 2);
-                    }
-                    scales[c][0] = scale[0] | scale[1] << 16, scales[c][1] = scale[2] | scale[3] << 16;
-                    if (GROUPS % 2 && !v_some) scales[c][0] = scales[c][1] = 0;
-                }
-                if (edge) { // what stands in positions that no row sees, or of no sequence, counts as zero
-#pragma unroll
-                    for (int c = 0; c < CH; c++)
-#pragma unroll
-                        for (int k = 0; k < 4; k++) {
-                            const int j = j0[c] + 2 * t4 + (k & 1) + (k >> 1) * 8;
-                            if (j >= s.length || j < low) scales[c][k >> 1] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
-                        }
                 }
 #pragma unroll
-                for (int v = 0; v < V_WORDS; v++)
-#pragma unroll
-                    for (int c = 0; c < CH; c++) {
-                        unsigned even[2][4], odd[2][4]; // columns 2 i and 2 i + 1, of two keys each
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const Int4Factors factors = int4_factors(scales[c][h]);
-                            int4_pairs(even[h], __byte_perm(code[c][2 * h][v], code[c][2 * h + 1][v], 0x5410), factors);
-                            int4_pairs(odd[h], __byte_perm(code[c][2 * h][v], code[c][2 * h + 1][v], 0x7632), factors);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const unsigned x4[4] = {even[0][i], odd[0][i], even[1][i], odd[1][i]};
-                            const int mt = 4 * v + i;
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                if constexpr (F32) {
-                                    float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                                    for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(d, x4, w[c][nt][k][0], w[c][nt][k][1]);
-#pragma unroll
-                                    for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
-                                } else {
-#pragma unroll
-                                    for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[c][nt][k][0], w[c][nt][k][1]);
-                                }
-                            }
-                        }
-                    }
+                for (int k = 0; k < 4; k++) { // what stands in positions that no row sees, or of no sequence, counts as zero
+                    const int j = j0 + 2 * t4 + (k & 1) + (k >> 1) * 8;
+                    if (j >= length || j < low) counts[k >> 1] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+                }
             }
-            __syncwarp();
-            if (lane < CH && t + lane < item.tiles && alive) pg_bar_arrive(lane == 0 ? empty[0] : empty[CH - 1]); // (what it has not waited for is not given back)
+            bool more = false;
+#pragma unroll
+            for (int e = 0; e < E; e++) more |= x[e][0] > high[e] || x[e][1] > high[e];
+            if (__any_sync(0xFFFFFFFFu, more)) {
+                float keep[E];
+#pragma unroll
+                for (int e = 0; e < E; e++) {
+                    float top = fmaxf(x[e][0], x[e][1]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
+                    top = fmaxf(m[e], top * unit);
+                    keep[e] = m[e] == -INFINITY ? 0.0f : paged_exp2(m[e] - top);
+                    m[e] = top, l[e] *= keep[e], high[e] = (top + 8.0f) * part_of_unit;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) o[nt][mt][i] *= keep[PACK ? 0 : 2 * nt + (i & 1)];
+            }
+            // ---- weights ----
+            unsigned w[NT][PACK ? 1 : WP][2]; // as pieces and turned, keys down
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                const float base = m[e] == -INFINITY ? 0.0f : -m[e];
+#pragma unroll
+                for (int h = 0; h < 2; h++) x[e][h] = paged_exp2(fmaf(x[e][h], unit, base)), l[e] += x[e][h];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if constexpr (PACK) {
+                    const float rest = x[0][h] - __uint_as_float(pg_pack(x[0][h], 0.0f) << 16);
+                    unsigned two = pg_pack(x[0][h], rest);
+                    if constexpr (F32) {
+                        const float last = rest - __uint_as_float(two & 0xFFFF0000u);
+                        if (t4 & 1) two = pg_pack(last, 0.0f);
+                    }
+                    w[0][0][h] = pg_transpose(two);
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        unsigned piece[WP];
+                        pg_split<WP>(piece, x[2 * nt][h], x[2 * nt + 1][h]);
+#pragma unroll
+                        for (int k = 0; k < WP; k++) w[nt][k][h] = pg_transpose(piece[k]);
+                    }
+                }
+            }
+            // ---- values ----
+            unsigned code[4][V_WORDS], scales[2];
+            {
+                unsigned scale[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) { // keys 2 t4, 2 t4 + 1, and eight further on
+                    const int key = (k & 1) + (k >> 1) * 8;
+                    const unsigned char *at = slot + v_at[c] + key * STRIDE;
+                    if constexpr (V_WORDS == 2) {
+                        const uint2 v = *reinterpret_cast<const uint2 *>(at);
+                        code[k][0] = v.x, code[k][1] = v.y;
+                    } else {
+                        code[k][0] = *reinterpret_cast<const unsigned *>(at);
+                    }
+                    scale[k] = *reinterpret_cast<const unsigned short *>(slot + v_scale[c] + key * GROUPS * 2);
+                }
+                scales[0] = (scale[0] | scale[1] << 16) & counts[0], scales[1] = (scale[2] | scale[3] << 16) & counts[1];
+                if (GROUPS % 2 && !v_some) scales[0] = scales[1] = 0;
+            }
+            const Int4Factors factors[2] = {int4_factors(scales[0]), int4_factors(scales[1])};
+#pragma unroll
+            for (int v = 0; v < V_WORDS; v++) {
+                unsigned even[2][4], odd[2][4]; // columns 2 i and 2 i + 1, of two keys each
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    int4_pairs(even[h], __byte_perm(code[2 * h][v], code[2 * h + 1][v], 0x5410), factors[h]);
+                    int4_pairs(odd[h], __byte_perm(code[2 * h][v], code[2 * h + 1][v], 0x7632), factors[h]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const unsigned x4[4] = {even[0][i], odd[0][i], even[1][i], odd[1][i]};
+                    const int mt = 4 * v + i;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if constexpr (F32) {
+                            constexpr int LAST = (PACK ? 1 : WP) - 1;
+                            float d[4];
+                            pg_mma_first(d, x4, w[nt][LAST][0], w[nt][LAST][1]);
+#pragma unroll
+                            for (int k = LAST - 1; k >= 0; k--) pg_mma(d, x4, w[nt][k][0], w[nt][k][1]);
+#pragma unroll
+                            for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
+                        } else {
+#pragma unroll
+                            for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[nt][k][0], w[nt][k][1]);
+                        }
+                    }
+                }
+            }
+            leave();
         }
 
-        // ---- the item's (or its part's) end: the warps' results meet, [four warps][row][column], four of them adding to the others' ----
+        // ---- the item's (or its part's) end: the warps' results meet, [four places][row][column] ----
 #pragma unroll
         for (int e = 0; e < E; e++) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[e] += __shfl_xor_sync(0xFFFFFFFFu, l[e], d);
-            if (g == 0 && !(PACK && F32 && (t4 & 1))) ml[warp][0][row_of(e)] = m[e], ml[warp][1][row_of(e)] = l[e];
+            if (side == 0 && g == 0 && !(PACK && F32 && (t4 & 1))) ml[slice][0][row_of(e)] = m[e], ml[slice][1][row_of(e)] = l[e];
         }
         few_meet<WARPS>();
-        if (lane == 0 && alive) pg_bar_arrive(&sm.item_empty[which]);
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const int r = row_of(e);
             float top = ml[0][0][r], sum = 0.0f;
 #pragma unroll
-            for (int k = 1; k < WARPS; k++) top = fmaxf(top, ml[k][0][r]);
+            for (int k = 1; k < SLICES; k++) top = fmaxf(top, ml[k][0][r]);
             if (warp == 0) { // alike in all lanes that have the row
 #pragma unroll
-                for (int k = 0; k < WARPS; k++) sum = fmaf(ml[k][1][r], ml[k][0][r] == -INFINITY ? 0.0f : paged_exp2(ml[k][0][r] - top), sum);
+                for (int k = 0; k < SLICES; k++) sum = fmaf(ml[k][1][r], ml[k][0][r] == -INFINITY ? 0.0f : paged_exp2(ml[k][0][r] - top), sum);
                 joined[0][r] = top, joined[1][r] = sum;
             }
             const float keep = m[e] == -INFINITY ? 0.0f : paged_exp2(m[e] - top);
 #pragma unroll
-            for (int mt = 0; mt < KS; mt++)
+            for (int mt = 0; mt < MT; mt++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     if (PACK || (i & 1) == (e & 1)) o[PACK ? 0 : e >> 1][mt][i] *= keep;
@@ -427,7 +404,7 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
 #pragma unroll
             for (int e = 0; e < E; e++)
 #pragma unroll
-                for (int mt = 0; mt < KS; mt += 2) {
+                for (int mt = 0; mt < MT; mt += 2) {
                     float4 y;
                     const float(&u)[4] = o[PACK ? 0 : e >> 1][mt], (&v)[4] = o[PACK ? 0 : e >> 1][mt + 1];
                     if constexpr (PACK) {
@@ -440,7 +417,7 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
                     } else {
                         y = make_float4(u[e & 1], u[2 + (e & 1)], v[e & 1], v[2 + (e & 1)]);
                     }
-                    float4 *const at = reinterpret_cast<float4 *>(sm.meet + (to * ROWS + row_of(e)) * Shape::PITCH + g * (HDP / 8) + 2 * mt);
+                    float4 *const at = reinterpret_cast<float4 *>(sm.meet + (to * ROWS + row_of(e)) * Shape::PITCH + g * (HDP / 8) + 2 * (side * MT + mt));
                     if (add) {
                         const float4 x4 = *at;
                         y.x += x4.x, y.y += x4.y, y.z += x4.z, y.w += x4.w;
@@ -448,22 +425,28 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
                     *at = y;
                 }
         };
-        if (warp >= WARPS / 2) share_out(warp - WARPS / 2, false);
-        few_meet<WARPS>();
-        if (warp < WARPS / 2) share_out(warp, true);
+        if constexpr (SLICES == 4) {
+            share_out(slice, false);
+        } else { // four of the eight add to the others'
+            if (slice >= 4) share_out(slice - 4, false);
+            few_meet<WARPS>();
+            if (slice < 4) share_out(slice, true);
+        }
         few_meet<WARPS>();
         const bool is_whole = item.before == 0 && item.tiles == item.count;
         const long long part_slot = (long long)blockIdx.x * 2 + (first_part && item.before > 0 ? 0 : 1);
-        unsigned wrong = 0;
+        const PagedSeq s = item.s;
+        const int rows = rows_of();
+        unsigned long long wrong = 0;
 #pragma unroll 1
         for (int r = tid / HDP; r < rows && !dead; r += 32 * WARPS / HDP) {
-            const int col = tid % HDP, token = r / a.c.group;
+            const int col = tid % HDP, token = token_of(r);
             const float *at = sm.meet + r * Shape::PITCH + col;
             float y = (at[0] + at[ROWS * Shape::PITCH]) + (at[2 * ROWS * Shape::PITCH] + at[3 * ROWS * Shape::PITCH]);
             if (is_whole) {
                 y *= paged_share(joined[1][r], s.pos0 + token);
                 if (col < a.c.hd) paged_write(static_cast<RT *>(a.out) + ((long long)(s.first + token) * a.c.heads + item.kvh * a.c.group + r - token * a.c.group) * a.c.hd + col, y);
-                if (col < a.c.hd && !(y * 0.0f == 0.0f)) wrong |= 1u << r;
+                if (col < a.c.hd && !(y * 0.0f == 0.0f)) wrong |= 1ull << r;
             } else {
                 f.part[(part_slot * ROWS + r) * HDP + col] = y;
                 if (col == 0) {
@@ -476,15 +459,18 @@ __global__ void __launch_bounds__(FEW4_THREADS, 2) attend_few_int4_kernel(const 
         if (wrong) atomicOr(&bad_rows, wrong);
         few_meet<WARPS>(); // what met is read, `bad_rows` is whole
         if (bad_rows) few_again<RT, Int4, WARPS>(a, item, &bad_rows, rows);
+        if (lane == 0 && alive) pg_bar_arrive(&sm.item_empty[which]); // each warp for itself: it has read the item
         first_part = false;
     }
 }
 
 // ---- host side ----
+constexpr int FEW4_MOST = 24; // bfloat16 rows of an item; of float32, whose products are three for each, FEW_MOST
+
 inline FewPlan few4_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     FewPlan p;
-    p.most = rows, p.rows = rows <= (f32_rows ? 2 : 4) ? (f32_rows ? 2 : 4) : (rows <= 8 ? 8 : 16);
-    few_cut(&p, 2 * sms, FEW4_KEYS, batch, kv, hdp, max_new, max_length, window);
+    p.most = rows, p.rows = rows <= (f32_rows ? 2 : 4) ? (f32_rows ? 2 : 4) : (rows <= 8 ? 8 : (rows <= 16 ? 16 : FEW4_MOST));
+    few_cut(&p, (p.rows > 8 ? 1 : 2) * sms, FEW4_KEYS, batch, kv, hdp, max_new, max_length, window);
     return p;
 }
 
@@ -511,6 +497,9 @@ cudaError_t launch_few4_as(const AttendCall &a, const FewPlan &p, void *ws, int 
 template <typename RT, int GROUPS>
 cudaError_t launch_few4_rows(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
     if (p.rows < 8) return launch_few4_as<RT, GROUPS, 1, true>(a, p, ws, device, st, launches);
+    if constexpr (std::is_same_v<RT, __nv_bfloat16>) {
+        if (p.rows == FEW4_MOST) return launch_few4_as<RT, GROUPS, 3, false>(a, p, ws, device, st, launches);
+    }
     return p.rows == 8 ? launch_few4_as<RT, GROUPS, 1, false>(a, p, ws, device, st, launches) : launch_few4_as<RT, GROUPS, 2, false>(a, p, ws, device, st, launches);
 }
 template <typename RT>

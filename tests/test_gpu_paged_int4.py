@@ -189,10 +189,21 @@ def test_chunks(rows, heads, kv, hd):
 
 @pytest.mark.parametrize("rows", ROWS)
 @pytest.mark.parametrize("heads,kv", [(1, 1), (2, 1), (3, 1), (4, 2), (5, 1), (8, 1), (16, 1)])
-@pytest.mark.parametrize("new", [1, 2, 3, 4, 5, 8, 16])
+@pytest.mark.parametrize("new", [1, 2, 3, 4, 5, 8, 16, 24, 33, 40, 41])
 def test_a_few_rows(rows, heads, kv, new):
     """Every number of rows of a key head that has a layout of its own, and those next to it."""
     held_to_64_bits(Case4([new, 1, new], [1500, 130, 0], heads, kv, 128, 32, rows, seed=new))
+
+
+@pytest.mark.parametrize("new,heads,kv", [(3, 7, 1), (5, 28, 4), (20, 2, 1), (40, 2, 2)])
+@pytest.mark.parametrize("hd", [8, 64, 80, 96, 128])
+@pytest.mark.parametrize("page", [16, 64, 256])
+def test_rows_of_drafted_tokens(new, heads, kv, hd, page):
+    """17 to 40 rows: the columns of the values shared by two warps where a head is wide, parts of long sequences and whole short ones, a window, caps."""
+    c = Case4([new, 1, new, 2], [3000, 200, 0, 700], heads, kv, hd, page, BF16, seed=hd)
+    held_to_64_bits(c)
+    held_to_64_bits(c, window=300, softcap=20.0)
+    held_to_64_bits(Case4([new] * 2, [90, 33], heads, kv, hd, page, BF16, seed=hd), max_length=200)
 
 
 @pytest.mark.parametrize("rows", ROWS)
@@ -253,7 +264,7 @@ def test_what_is_not_seen_has_no_influence(rows, new, hd):
 
 
 @pytest.mark.parametrize("rows", ROWS)
-@pytest.mark.parametrize("new", [1, 2, 4, 6, 60, 300])
+@pytest.mark.parametrize("new", [1, 2, 4, 6, 9, 60, 300])
 def test_a_group_that_is_not_finite_reaches_only_rows_that_see_it(rows, new):
     c = Case4([new, new], [40, 500], 8, 2, 64, 16, rows, seed=new)
     codes, scale = parts(c.v_cache)
@@ -515,3 +526,23 @@ def test_refusals():
         get(k=words, v=words, hd=32)
     with pytest.raises(TypeError):
         paged.PagedCache(4, 2, 64, dtype="int8")
+
+
+# ---- caps and scales far from one ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("new", [1, 3, 5, 9, 90, 300])
+@pytest.mark.parametrize("cap", [0.01, 1.0, 60.0, 257.0, 1e5, 1e30])
+def test_caps_of_any_size(rows, new, cap):
+    """A score that is small beside its cap is almost as it was; one that is large is the cap."""
+    held_to_64_bits(Case4([new] * 3, [0, 65, 400], 8, 2, 128, 32, rows, seed=new), softcap=cap)
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("new", [1, 6, 90])
+@pytest.mark.parametrize("cap", [3.0, 1e8])
+@pytest.mark.parametrize("size", [2.0 ** -66, 2.0 ** 50])
+def test_caps_with_keys_of_any_size(rows, new, cap, size):
+    c = Case4([new] * 3, [0, 65, 400], 8, 2, 64, 32, rows)
+    c.hold(size * values(c.k_cache, 64), values(c.v_cache, 64))
+    held_to_64_bits(c, softcap=cap, scale=0.25 / size)
