@@ -1,9 +1,9 @@
 // Fresh q | k | v rows into their places in a cache of 4 bits (paged_int4.cuh): norms, rotation and the queries as in paged_append.cuh, keys and values as codes.
 //
-// A code is what the definition says of the 64-bit value of its key. The kernel's 32-bit value is off by less than 2^-20 of the two words that the rotation makes
-// it of (the norm's sum, root and products: 2^-21.4; the rotation's: 2^-23), so where the largest magnitude of a group, or a word, is nearer than that to a border between
-// two scales or codes (about one group in 5000), the warp's keys are done again in 64 bits. Values, and keys without norm and rotation, have no such error: what a
-// code leaves is computed exactly.
+// A code is what the definition says of the 64-bit value of its key. The kernel's 32-bit value is off by less than 2^-20 of itself where it is normed (the squares' sum by
+// 14 roundings of 2^-24, halved by the root, the root by 2 of 2^-23, three products), and a rotated one by less than 2^-19 of the larger of the two words that it is made of, 2^-22 where
+// they were not normed (three roundings). Where the largest magnitude of a group, or a word, is nearer than that to a border between two scales or codes (one head of 128 in 250, or 2000),
+// the head is done again in 64 bits, by the whole warp. Values, and keys without norm and rotation, have no such error.
 // Bound: HBM, and latency for a few rows. A lane takes the unit pairs of paged_append.cuh; the units of a group are in neighbouring lanes where half a rotation is
 // whole groups, and looked up else. What is not a warp's units goes by a warp a head, a column of each group a lane, in 64 bits: rotations whose halves are not whole
 // units, tables that are not on 16-byte boundaries, and the keys that are done again.
@@ -78,18 +78,38 @@ __device__ __noinline__ void append4_head(const Append4Call &f, long long t, int
     }
 }
 
+// The largest of three magnitudes; NaN where one is.
+__device__ __forceinline__ float append4_most(float x, float y, float z) {
+    float r;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+    return r;
+}
+template <int N> __device__ __forceinline__ float append4_largest(const unsigned long long (&x)[N]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float lo, hi;
+        pg_one(x[i], lo, hi);
+        m = append4_most(m, lo, hi);
+    }
+    return m;
+}
+
 // The codes of a unit's columns, as their four bits in two halves of 16: those of even columns and of odd ones. *nearest: how near the nearest word is to a
-// border between two codes.
-template <int N>
-__device__ __forceinline__ uint2 append4_codes(const float (&y)[N], float s, float inverse, float *nearest) {
+// border between two codes, where LOOK asks for that.
+template <bool LOOK, int N>
+__device__ __forceinline__ uint2 append4_codes(const unsigned long long (&x)[N / 2], float s, float inverse, float *nearest) {
     float q[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
+        float two[2];
+        pg_one(x[i / 2], two[0], two[1]);
+        const float y = two[i & 1];
         // the quotient to nearest, so that one of eight bits by five is a tie if and only if it is one
-        float p = y[i] * inverse;
-        p = fmaf(fmaf(-p, s, y[i]), inverse, p);
+        float p = y * inverse;
+        p = fmaf(fmaf(-p, s, y), inverse, p);
         q[i] = (p + 12582912.0f) - 12582912.0f;
-        *nearest = fminf(*nearest, fabsf(fabsf(fmaf(-q[i], s, y[i])) - 0.5f * s));
+        if (LOOK) *nearest = fminf(*nearest, fabsf(fabsf(fmaf(-q[i], s, y)) - 0.5f * s));
     }
     float half[2]; // 8388608 and the codes (each eight more than q) as digits of sixteen
 #pragma unroll
@@ -140,6 +160,7 @@ __global__ void __launch_bounds__(128) append_int4_kernel(const __grid_constant_
     unsigned long long c[N / 2], sn[N / 2];
     const bool turns = turned && a.cosv != nullptr;
     float turn_off = 0.0f; // of a rotated word, in units of the largest one that it is made of
+    bool still = true;     // the rotation leaves the lane's words as they are, ties too: position 0
     if (turns) {
         const long long row = (long long)max(pos, 0) * half + at0;
         append_words<N>(c, a.cosv + row);
@@ -149,8 +170,9 @@ __global__ void __launch_bounds__(128) append_int4_kernel(const __grid_constant_
             float u[4];
             pg_one(c[i], u[0], u[1]), pg_one(sn[i], u[2], u[3]);
             turn_off = fmaxf(turn_off, fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))));
+            still &= u[0] == 1.0f && u[1] == 1.0f && u[2] == 0.0f && u[3] == 0.0f;
         }
-        turn_off *= 0x1p-19f;
+        turn_off *= a.k_norm ? 0x1p-19f : (still ? 0.0f : 0x1p-22f);
     }
     for (; set < sets; set += step) {
         const int head = (set << (5 - lanes_log2)) + in_set, part = head < a.c.heads ? 0 : (head < a.c.heads + a.c.kv ? 1 : 2); // q, k, v
@@ -185,13 +207,11 @@ __global__ void __launch_bounds__(128) append_int4_kernel(const __grid_constant_
         const bool held = __any_sync(0xFFFFFFFFu, part > 0); // keys or values among the warp's heads
         // How far a word may be from its 64-bit value: by the largest words that it is made of. Of float32 values, and keys as they came, only what the quotient
         // is off by; of bfloat16 ones that is nothing.
-        const bool moved = part == 1 && (w || turns);
+        const bool moved = part == 1 && (w || (turns && turn_off != 0.0f));
         float off = -1.0f;
         if (held && (N == 4 || moved)) {
-            unsigned most = 0;
-#pragma unroll
-            for (int i = 0; i < N / 2; i++) most = max(max(most, (unsigned)(x0[i] >> 32) & 0x7FFFFFFFu), max((unsigned)x0[i] & 0x7FFFFFFFu, max((unsigned)(x1[i] >> 32) & 0x7FFFFFFFu, (unsigned)x1[i] & 0x7FFFFFFFu)));
-            off = __uint_as_float(most) * (moved ? (turns ? turn_off : 0x1p-20f) : 0x1p-22f);
+            const float most = append4_most(append4_largest(x0), append4_largest(x1), 0.0f);
+            off = most * (moved ? (turns ? turn_off : 0x1p-20f) : 0x1p-22f);
         }
         if (turns && part < 2) {
             const unsigned long long minus = pg_two(-1.0f, -1.0f);
@@ -209,47 +229,39 @@ __global__ void __launch_bounds__(128) append_int4_kernel(const __grid_constant_
         }
         if (!held) continue;
         // ---- the codes ----
-        float y0[N], y1[N], far0 = off, far1 = off;
-        unsigned most0 = 0, most1 = 0; // (a NaN's bits are larger than an infinity's)
-#pragma unroll
-        for (int i = 0; i < N / 2; i++) pg_one(x0[i], y0[2 * i], y0[2 * i + 1]), pg_one(x1[i], y1[2 * i], y1[2 * i + 1]);
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            most0 = max(most0, __float_as_uint(y0[i]) & 0x7FFFFFFFu), most1 = max(most1, __float_as_uint(y1[i]) & 0x7FFFFFFFu);
-        }
+        float most0 = append4_largest(x0), most1 = append4_largest(x1), far0 = off, far1 = off;
         if (straight) {
 #pragma unroll
             for (int o = 1; o < OF; o <<= 1) {
-                most0 = max(most0, __shfl_xor_sync(0xFFFFFFFFu, most0, o)), most1 = max(most1, __shfl_xor_sync(0xFFFFFFFFu, most1, o));
+                most0 = append4_most(most0, __shfl_xor_sync(0xFFFFFFFFu, most0, o), 0.0f), most1 = append4_most(most1, __shfl_xor_sync(0xFFFFFFFFu, most1, o), 0.0f);
                 far0 = fmaxf(far0, __shfl_xor_sync(0xFFFFFFFFu, far0, o));
             }
             far1 = far0;
         } else { // unit u of a head is lane u's first, lane u - pairs' second, or one of two neighbours behind the rotation
-            unsigned m0 = 0, m1 = 0;
-            float f0 = off, f1 = off;
+            float m0 = 0.0f, m1 = 0.0f, f0 = off, f1 = off;
 #pragma unroll 1
             for (int i = 0; i < 2 * OF; i++) {
                 const int u = (i < OF ? at0 : at1) / N / OF * OF + i % OF, r = u - 2 * pairs;
                 const int from = (all - lane) + (r < 0 ? (u < pairs ? u : u - pairs) : pairs + r / 2);
                 const bool second = r < 0 ? u >= pairs : (r & 1) != 0, there = u * N < a.c.hd;
-                const unsigned p0 = __shfl_sync(0xFFFFFFFFu, most0, from), p1 = __shfl_sync(0xFFFFFFFFu, most1, from);
+                const float p0 = __shfl_sync(0xFFFFFFFFu, most0, from), p1 = __shfl_sync(0xFFFFFFFFu, most1, from);
                 const float g = __shfl_sync(0xFFFFFFFFu, off, from);
-                if (there && i < OF) m0 = max(m0, second ? p1 : p0), f0 = fmaxf(f0, g);
-                if (there && i >= OF) m1 = max(m1, second ? p1 : p0), f1 = fmaxf(f1, g);
+                if (there && i < OF) m0 = append4_most(m0, second ? p1 : p0, 0.0f), f0 = fmaxf(f0, g);
+                if (there && i >= OF) m1 = append4_most(m1, second ? p1 : p0, 0.0f), f1 = fmaxf(f1, g);
             }
             most0 = m0, most1 = m1, far0 = f0, far1 = f1;
         }
         bool near = false;
+        const bool look = __any_sync(0xFFFFFFFFu, off >= 0.0f);
         float scale[2];
         uint2 code[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const unsigned most = h ? most1 : most0;
-            const float top = __uint_as_float(most), s5 = int4_scale(top), before = __uint_as_float(__float_as_uint(s5) - 0x80000u), far = h ? far1 : far0;
+            const float top = h ? most1 : most0, s5 = int4_scale(top), before = __uint_as_float(__float_as_uint(s5) - 0x80000u), far = h ? far1 : far0;
             float inverse, nearest = INFINITY;
             asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(s5));
             scale[h] = s5;
-            code[h] = append4_codes(h ? y1 : y0, s5, inverse, &nearest);
+            code[h] = look ? append4_codes<true, N>(h ? x1 : x0, s5, inverse, &nearest) : append4_codes<false, N>(h ? x1 : x0, s5, inverse, &nearest);
             near |= nearest <= off;
             if (moved) near |= 7.0f * s5 - top <= far || (s5 > 0x1p-100f && top - 7.0f * before <= far);
             if (!(top <= 7.0f * s5)) near = true; // words that are cut, or not finite
