@@ -81,7 +81,7 @@ AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t
     AttendPlan p = {};
     p.hdp = head_dim <= 64 ? 64 : 128;
     const int64_t group = n_heads / n_kv;
-    const int64_t most = cache_type == B200I_T_INT4 ? int4_few_most(row_type == B200I_T_F32) : FEW_MOST;
+    const int64_t most = cache_type == B200I_T_INT4 ? int4_few_most() : FEW_MOST;
     if (max_new <= most && max_new * group <= most) {
         p.few = (int)(max_new * group);
         if (cache_type == B200I_T_INT4)

@@ -497,9 +497,7 @@ cudaError_t launch_few4_as(const AttendCall &a, const FewPlan &p, void *ws, int 
 template <typename RT, int GROUPS>
 cudaError_t launch_few4_rows(const AttendCall &a, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches) {
     if (p.rows < 8) return launch_few4_as<RT, GROUPS, 1, true>(a, p, ws, device, st, launches);
-    if constexpr (std::is_same_v<RT, __nv_bfloat16>) {
-        if (p.rows == FEW4_MOST) return launch_few4_as<RT, GROUPS, 3, false>(a, p, ws, device, st, launches);
-    }
+    if (p.rows == FEW4_MOST) return launch_few4_as<RT, GROUPS, 3, false>(a, p, ws, device, st, launches);
     return p.rows == 8 ? launch_few4_as<RT, GROUPS, 1, false>(a, p, ws, device, st, launches) : launch_few4_as<RT, GROUPS, 2, false>(a, p, ws, device, st, launches);
 }
 template <typename RT>

@@ -7,7 +7,7 @@
 
 namespace b200i {
 
-int int4_few_most(bool f32_rows) { return f32_rows ? FEW_MOST : FEW4_MOST; }
+int int4_few_most() { return FEW4_MOST; }
 FewPlan int4_few_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     return few4_plan(sms, f32_rows, batch, kv, hdp, rows, max_new, max_length, window);
 }

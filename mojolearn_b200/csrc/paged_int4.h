@@ -7,7 +7,7 @@
 namespace b200i {
 
 // The most rows of a sequence and key head that int4_few takes.
-int int4_few_most(bool f32_rows);
+int int4_few_most();
 FewPlan int4_few_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window);
 cudaError_t int4_few(const AttendCall &a, bool f32_rows, const FewPlan &p, void *ws, int device, cudaStream_t st, int *launches);
 cudaError_t int4_many(const AttendCall &a, bool f32_rows, const ManyPlan &p, int hdp, void *ws, int device, cudaStream_t st, int *launches);
