@@ -105,10 +105,14 @@ __device__ __forceinline__ uint2 append4_codes(const unsigned long long (&x)[N /
         float two[2];
         pg_one(x[i / 2], two[0], two[1]);
         const float y = two[i & 1];
-        // the quotient to nearest, so that one of eight bits by five is a tie if and only if it is one
+        // the quotient to nearest: one of eight bits by five is a tie if and only if it says so, and one of 24 that says so is one where it leaves nothing
         float p = y * inverse;
         p = fmaf(fmaf(-p, s, y), inverse, p);
         q[i] = (p + 12582912.0f) - 12582912.0f;
+        if (N == 4) {
+            const float left = fmaf(-p, s, y);
+            if (fabsf(p - q[i]) == 0.5f && left != 0.0f) q[i] = p + copysignf(0.5f, left);
+        }
         if (LOOK) *nearest = fminf(*nearest, fabsf(fabsf(fmaf(-q[i], s, y)) - 0.5f * s));
     }
     float half[2]; // 8388608 and the codes (each eight more than q) as digits of sixteen
@@ -205,13 +209,12 @@ __global__ void __launch_bounds__(128) append_int4_kernel(const __grid_constant_
             }
         }
         const bool held = __any_sync(0xFFFFFFFFu, part > 0); // keys or values among the warp's heads
-        // How far a word may be from its 64-bit value: by the largest words that it is made of. Of float32 values, and keys as they came, only what the quotient
-        // is off by; of bfloat16 ones that is nothing.
+        // How far a word may be from its 64-bit value: by the largest words that it is made of; negative where it is that value.
         const bool moved = part == 1 && (w || (turns && turn_off != 0.0f));
         float off = -1.0f;
-        if (held && (N == 4 || moved)) {
+        if (held && moved) {
             const float most = append4_most(append4_largest(x0), append4_largest(x1), 0.0f);
-            off = most * (moved ? (turns ? turn_off : 0x1p-20f) : 0x1p-22f);
+            off = most * (turns ? turn_off : 0x1p-20f);
         }
         if (turns && part < 2) {
             const unsigned long long minus = pg_two(-1.0f, -1.0f);
