@@ -18,15 +18,16 @@
 
 namespace b200i {
 
-constexpr int FEW4_WARPS = 8, FEW4_THREADS = 32 * (FEW4_WARPS + 1), FEW4_KEYS = 16 * FEW4_WARPS;
+constexpr int FEW4_KEYS = 128;
 
 template <typename RT, int GROUPS, int NT, bool PACK> struct Few4Shape {
     static constexpr bool F32 = std::is_same_v<RT, float>;
     static constexpr int HDP = GROUPS <= 2 ? 64 : 128; // head_dim as it is laid out for the products: a lane's quarter (eighth) of it lies in one group
-    static constexpr int WARPS = FEW4_WARPS, ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
+    static constexpr int WARPS = NT == 1 ? 4 : 8, THREADS = 32 * (WARPS + 1), ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
     static constexpr int BLOCKS = NT > 1 ? 1 : 2;                        // on an SM
     static constexpr int SPLIT = NT > 2 && HDP == 128 ? 2 : 1;           // warps that share keys, each for its part of the values' columns
-    static constexpr int SLICES = WARPS / SPLIT, CHUNKS = SPLIT;         // a tile's keys go to so many warps, by so many times 16
+    static constexpr int SLICES = WARPS / SPLIT, CHUNKS = 8 / SLICES;    // a tile's keys go to so many warps, by so many times 16
+    static constexpr int CH = NT == 1 ? 2 : 1;                           // of which it works on so many at once
     static constexpr int HALF = FEW4_KEYS * GROUPS * INT4_BYTES, SLOT = 2 * HALF; // keys, then values
     static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : (NT > 2 ? 1 : 2);
     static constexpr bool HELD = PACK || (!F32 && NT == 1); // the queries stay in registers; else they lie as fragments where the warps' results meet
@@ -67,10 +68,10 @@ __device__ __forceinline__ auto few4_runs(const AttendCall &a) {
 }
 
 template <typename RT, int GROUPS, int NT, bool PACK>
-__global__ void __launch_bounds__(FEW4_THREADS, Few4Shape<RT, GROUPS, NT, PACK>::BLOCKS) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
+__global__ void __launch_bounds__(Few4Shape<RT, GROUPS, NT, PACK>::THREADS, Few4Shape<RT, GROUPS, NT, PACK>::BLOCKS) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
     using Shape = Few4Shape<RT, GROUPS, NT, PACK>;
     constexpr bool F32 = Shape::F32, HELD = Shape::HELD;
-    constexpr int HDP = Shape::HDP, KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = FEW4_WARPS, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
+    constexpr int HDP = Shape::HDP, KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = Shape::WARPS, CH = Shape::CH, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
     constexpr int SPLIT = Shape::SPLIT, SLICES = Shape::SLICES, CHUNKS = Shape::CHUNKS, MT = KS / SPLIT; // MT: pieces of 16 columns of the output that a warp has
     constexpr int E = PACK ? 1 : 2 * NT;                          // rows of a lane's scores
     constexpr int K_WORDS = HDP / 32, V_WORDS = HDP / 64 / SPLIT; // of codes, of a key: a quarter of its columns, an eighth (of the warp's)
@@ -174,8 +175,8 @@ __global__ void __launch_bounds__(FEW4_THREADS, Few4Shape<RT, GROUPS, NT, PACK>:
             for (int mt = 0; mt < MT; mt++) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
         // Scores of 16 keys of a tile, the warp's chunk c of them.
         constexpr int ZS = F32 && !PACK ? 2 : 1; // large and small products apart
-        float z[ZS][NT][4];
-        const auto scores = [&](const unsigned char *slot, int c) {
+        float z[CH][ZS][NT][4];
+        const auto scores = [&](const unsigned char *slot, int c, float (&z)[ZS][NT][4]) {
             unsigned code[2][K_WORDS];
             Int4Factors factors[2];
 #pragma unroll
@@ -216,71 +217,83 @@ __global__ void __launch_bounds__(FEW4_THREADS, Few4Shape<RT, GROUPS, NT, PACK>:
                 }
             }
         };
-        for (int i = 0; i < tiles * CHUNKS; i++) {
-            const int c = CHUNKS == 1 ? 0 : i % CHUNKS, j0 = begin + i / CHUNKS * KEYS + 16 * c;
+        for (int i = 0; i < tiles * (CHUNKS / CH); i++) {
+            const int c0 = CHUNKS == CH ? 0 : i % CHUNKS, j0 = begin + i / (CHUNKS / CH) * KEYS + 16 * c0; // the step's first key: it has 16 CH
             const unsigned char *const slot = sm.ring + slot_at * Shape::SLOT;
-            if (c == 0 && alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot_at], parity))) give_up();
+            if (c0 == 0 && alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot_at], parity))) give_up();
             const auto leave = [&] {
-                if (c < CHUNKS - 1) return;
+                if (c0 + CH < CHUNKS) return;
                 __syncwarp();
                 if (lane == 0 && alive) pg_bar_arrive(&sm.empty[slot_at]); // (what it has not waited for is not given back)
                 if (++slot_at == SLOTS) slot_at = 0, parity ^= 1;
             };
-            if (!alive || j0 >= length || j0 + 16 <= low) {
+            if (!alive || j0 >= length || j0 + 16 * CH <= low) {
                 leave();
                 continue;
             }
-            scores(slot, c);
-            float x[E][2]; // keys g and g + 8
 #pragma unroll
-            for (int e = 0; e < E; e++)
+            for (int c = 0; c < CH; c++) scores(slot, c0 + c, z[c]);
+            float x[CH][E][2]; // keys g and g + 8
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if constexpr (PACK) {
-                        x[e][h] = z[0][0][2 * h];
-                        if constexpr (F32) {
-                            x[e][h] += z[0][0][2 * h + 1]; // two pieces here, the third beside it
-                            x[e][h] += __shfl_xor_sync(0xFFFFFFFFu, x[e][h], 1);
-                        }
-                    } else {
-                        x[e][h] = z[0][e >> 1][2 * h + (e & 1)];
-                        if constexpr (F32) x[e][h] += z[ZS - 1][e >> 1][2 * h + (e & 1)];
-                    }
-                }
-            if (a.softcap > 0.0f) { // (what is not seen may be anything, and goes after this)
-                if constexpr (F32)
-                    pg_cap_fine<2 * E>(&x[0][0], a);
-                else if (a.cap_far)
-                    pg_cap<2 * E, true>(&x[0][0], a);
-                else
-                    pg_cap<2 * E, false>(&x[0][0], a);
-            }
-            const bool edge = j0 + 16 > pos0 + 1 || j0 < all_lo;
-            unsigned counts[2] = {0xFFFFFFFFu, 0xFFFFFFFFu}; // the scales of values
-            if (edge) { // a row sees positions up to its own, and with a window the last so many of them
+            for (int c = 0; c < CH; c++)
 #pragma unroll
-                for (int e = 0; e < E; e++) {
-                    const int r = row_of(e), hi = r < rows_of() ? pos0 + token_of(r) + 1 : 0, lo = a.window ? hi - a.window : 0;
+                for (int e = 0; e < E; e++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        const int j = j0 + g + h * 8;
-                        if (j >= hi || j < lo) x[e][h] = -INFINITY;
+                        if constexpr (PACK) {
+                            x[c][e][h] = z[c][0][0][2 * h];
+                            if constexpr (F32) {
+                                x[c][e][h] += z[c][0][0][2 * h + 1]; // two pieces here, the third beside it
+                                x[c][e][h] += __shfl_xor_sync(0xFFFFFFFFu, x[c][e][h], 1);
+                            }
+                        } else {
+                            x[c][e][h] = z[c][0][e >> 1][2 * h + (e & 1)];
+                            if constexpr (F32) x[c][e][h] += z[c][ZS - 1][e >> 1][2 * h + (e & 1)];
+                        }
                     }
-                }
+            if (a.softcap > 0.0f) { // (what is not seen may be anything, and goes after this)
+                if constexpr (F32)
+                    pg_cap_fine<2 * E * CH>(&x[0][0][0], a);
+                else if (a.cap_far)
+                    pg_cap<2 * E * CH, true>(&x[0][0][0], a);
+                else
+                    pg_cap<2 * E * CH, false>(&x[0][0][0], a);
+            }
+            const bool edge = j0 + 16 * CH > pos0 + 1 || j0 < all_lo;
+            unsigned counts[CH][2]; // the scales of values
 #pragma unroll
-                for (int k = 0; k < 4; k++) { // what stands in positions that no row sees, or of no sequence, counts as zero
-                    const int j = j0 + 2 * t4 + (k & 1) + (k >> 1) * 8;
-                    if (j >= length || j < low) counts[k >> 1] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+            for (int c = 0; c < CH; c++) counts[c][0] = counts[c][1] = 0xFFFFFFFFu;
+            if (edge) { // a row sees positions up to its own, and with a window the last so many of them
+#pragma unroll
+                for (int c = 0; c < CH; c++) {
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        const int r = row_of(e), hi = r < rows_of() ? pos0 + token_of(r) + 1 : 0, lo = a.window ? hi - a.window : 0;
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int j = j0 + 16 * c + g + h * 8;
+                            if (j >= hi || j < lo) x[c][e][h] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; k++) { // what stands in positions that no row sees, or of no sequence, counts as zero
+                        const int j = j0 + 16 * c + 2 * t4 + (k & 1) + (k >> 1) * 8;
+                        if (j >= length || j < low) counts[c][k >> 1] &= k & 1 ? 0xFFFFu : 0xFFFF0000u;
+                    }
                 }
             }
             bool more = false;
 #pragma unroll
-            for (int e = 0; e < E; e++) more |= x[e][0] > high[e] || x[e][1] > high[e];
+            for (int c = 0; c < CH; c++)
+#pragma unroll
+                for (int e = 0; e < E; e++) more |= x[c][e][0] > high[e] || x[c][e][1] > high[e];
             if (__any_sync(0xFFFFFFFFu, more)) {
                 float keep[E];
 #pragma unroll
                 for (int e = 0; e < E; e++) {
-                    float top = fmaxf(x[e][0], x[e][1]);
+                    float top = fmaxf(x[0][e][0], x[0][e][1]);
+#pragma unroll
+                    for (int c = 1; c < CH; c++) top = pg_max3(top, x[c][e][0], x[c][e][1]);
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, d));
                     top = fmaxf(m[e], top * unit);
@@ -295,82 +308,89 @@ __global__ void __launch_bounds__(FEW4_THREADS, Few4Shape<RT, GROUPS, NT, PACK>:
                         for (int i = 0; i < 4; i++) o[nt][mt][i] *= keep[PACK ? 0 : 2 * nt + (i & 1)];
             }
             // ---- weights ----
-            unsigned w[NT][PACK ? 1 : WP][2]; // as pieces and turned, keys down
+            unsigned w[CH][NT][PACK ? 1 : WP][2]; // as pieces and turned, keys down
 #pragma unroll
             for (int e = 0; e < E; e++) {
                 const float base = m[e] == -INFINITY ? 0.0f : -m[e];
 #pragma unroll
-                for (int h = 0; h < 2; h++) x[e][h] = paged_exp2(fmaf(x[e][h], unit, base)), l[e] += x[e][h];
+                for (int c = 0; c < CH; c++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) x[c][e][h] = paged_exp2(fmaf(x[c][e][h], unit, base)), l[e] += x[c][e][h];
             }
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                if constexpr (PACK) {
-                    const float rest = x[0][h] - __uint_as_float(pg_pack(x[0][h], 0.0f) << 16);
-                    unsigned two = pg_pack(x[0][h], rest);
-                    if constexpr (F32) {
-                        const float last = rest - __uint_as_float(two & 0xFFFF0000u);
-                        if (t4 & 1) two = pg_pack(last, 0.0f);
-                    }
-                    w[0][0][h] = pg_transpose(two);
-                } else {
+            for (int c = 0; c < CH; c++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        unsigned piece[WP];
-                        pg_split<WP>(piece, x[2 * nt][h], x[2 * nt + 1][h]);
+                for (int h = 0; h < 2; h++) {
+                    if constexpr (PACK) {
+                        const float rest = x[c][0][h] - __uint_as_float(pg_pack(x[c][0][h], 0.0f) << 16);
+                        unsigned two = pg_pack(x[c][0][h], rest);
+                        if constexpr (F32) {
+                            const float last = rest - __uint_as_float(two & 0xFFFF0000u);
+                            if (t4 & 1) two = pg_pack(last, 0.0f);
+                        }
+                        w[c][0][0][h] = pg_transpose(two);
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < WP; k++) w[nt][k][h] = pg_transpose(piece[k]);
+                        for (int nt = 0; nt < NT; nt++) {
+                            unsigned piece[WP];
+                            pg_split<WP>(piece, x[c][2 * nt][h], x[c][2 * nt + 1][h]);
+#pragma unroll
+                            for (int k = 0; k < WP; k++) w[c][nt][k][h] = pg_transpose(piece[k]);
+                        }
                     }
                 }
-            }
             // ---- values ----
-            unsigned code[4][V_WORDS], scales[2];
-            {
+            unsigned code[CH][4][V_WORDS];
+            Int4Factors factors[CH][2];
+#pragma unroll
+            for (int c = 0; c < CH; c++) {
                 unsigned scale[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) { // keys 2 t4, 2 t4 + 1, and eight further on
                     const int key = (k & 1) + (k >> 1) * 8;
-                    const unsigned char *at = slot + v_at[c] + key * STRIDE;
+                    const unsigned char *at = slot + v_at[c0 + c] + key * STRIDE;
                     if constexpr (V_WORDS == 2) {
                         const uint2 v = *reinterpret_cast<const uint2 *>(at);
-                        code[k][0] = v.x, code[k][1] = v.y;
+                        code[c][k][0] = v.x, code[c][k][1] = v.y;
                     } else {
-                        code[k][0] = *reinterpret_cast<const unsigned *>(at);
+                        code[c][k][0] = *reinterpret_cast<const unsigned *>(at);
                     }
-                    scale[k] = *reinterpret_cast<const unsigned short *>(slot + v_scale[c] + key * GROUPS * 2);
+                    scale[k] = *reinterpret_cast<const unsigned short *>(slot + v_scale[c0 + c] + key * GROUPS * 2);
                 }
-                scales[0] = (scale[0] | scale[1] << 16) & counts[0], scales[1] = (scale[2] | scale[3] << 16) & counts[1];
-                if (GROUPS % 2 && !v_some) scales[0] = scales[1] = 0;
+#pragma unroll
+                for (int h = 0; h < 2; h++) factors[c][h] = int4_factors(GROUPS % 2 && !v_some ? 0u : (scale[2 * h] | scale[2 * h + 1] << 16) & counts[c][h]);
             }
-            const Int4Factors factors[2] = {int4_factors(scales[0]), int4_factors(scales[1])};
 #pragma unroll
-            for (int v = 0; v < V_WORDS; v++) {
-                unsigned even[2][4], odd[2][4]; // columns 2 i and 2 i + 1, of two keys each
+            for (int v = 0; v < V_WORDS; v++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    int4_pairs(even[h], __byte_perm(code[2 * h][v], code[2 * h + 1][v], 0x5410), factors[h]);
-                    int4_pairs(odd[h], __byte_perm(code[2 * h][v], code[2 * h + 1][v], 0x7632), factors[h]);
-                }
+                for (int c = 0; c < CH; c++) {
+                    unsigned even[2][4], odd[2][4]; // columns 2 i and 2 i + 1, of two keys each
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const unsigned x4[4] = {even[0][i], odd[0][i], even[1][i], odd[1][i]};
-                    const int mt = 4 * v + i;
+                    for (int h = 0; h < 2; h++) {
+                        int4_pairs(even[h], __byte_perm(code[c][2 * h][v], code[c][2 * h + 1][v], 0x5410), factors[c][h]);
+                        int4_pairs(odd[h], __byte_perm(code[c][2 * h][v], code[c][2 * h + 1][v], 0x7632), factors[c][h]);
+                    }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if constexpr (F32) {
-                            constexpr int LAST = (PACK ? 1 : WP) - 1;
-                            float d[4];
-                            pg_mma_first(d, x4, w[nt][LAST][0], w[nt][LAST][1]);
+                    for (int i = 0; i < 4; i++) {
+                        const unsigned x4[4] = {even[0][i], odd[0][i], even[1][i], odd[1][i]};
+                        const int mt = 4 * v + i;
 #pragma unroll
-                            for (int k = LAST - 1; k >= 0; k--) pg_mma(d, x4, w[nt][k][0], w[nt][k][1]);
+                        for (int nt = 0; nt < NT; nt++) {
+                            if constexpr (F32) {
+                                constexpr int LAST = (PACK ? 1 : WP) - 1;
+                                float d[4];
+                                pg_mma_first(d, x4, w[c][nt][LAST][0], w[c][nt][LAST][1]);
 #pragma unroll
-                            for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
-                        } else {
+                                for (int k = LAST - 1; k >= 0; k--) pg_mma(d, x4, w[c][nt][k][0], w[c][nt][k][1]);
 #pragma unroll
-                            for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[nt][k][0], w[nt][k][1]);
+                                for (int k = 0; k < 4; k++) o[nt][mt][k] += d[k];
+                            } else {
+#pragma unroll
+                                for (int k = (PACK ? 1 : WP) - 1; k >= 0; k--) pg_mma(o[nt][mt], x4, w[c][nt][k][0], w[c][nt][k][1]);
+                            }
                         }
                     }
                 }
-            }
             leave();
         }
 
@@ -486,7 +506,7 @@ cudaError_t launch_few4_as(const AttendCall &a, const FewPlan &p, void *ws, int 
         if (e != cudaSuccess) return e;
         if (device < 64) known[device].store(true);
     }
-    kernel<<<p.blocks, FEW4_THREADS, Shape::SMEM, st>>>(f);
+    kernel<<<p.blocks, Shape::THREADS, Shape::SMEM, st>>>(f);
     *launches += 1;
     if (!p.whole) {
         *launches += 1;
