@@ -218,7 +218,7 @@ __device__ __forceinline__ void few_copies(const FewCall &f, const FewMemory<Sha
             if (!wait(&sm.empty[slot], ((it / SLOTS) & 1u) ^ 1u)) break;
             const int there = min(pieces, max(0, (s.length - pos + box_rows - 1) / box_rows)); // pieces that hold positions of the sequence
             const int first = pos >> a.c.page_shift;
-            if (first + pieces - 1 >= base + 32 && there > 0) { // a tile's pages (at most eight) lie in one set of 32: sets begin at its own
+            if (first + pieces - 1 >= base + 32 && there > 0) { // a tile's pages (at most sixteen) lie in one set of 32: sets begin at its own
                 base += 32;
                 id = ahead;
                 ahead = base + 32 + lane <= last_page ? ids[base + 32 + lane] : 0;
@@ -921,12 +921,12 @@ constexpr int FEW_MOST = 16;  // rows of an item
 
 template <bool F32, typename CT, int HDP, int R> constexpr int few_blocks_per_sm() { return F32 ? FewFmaShape<CT, HDP, R>::BLOCKS : FewMmaShape<HDP, R <= 8 ? 1 : 2>::BLOCKS; }
 
-// Of at most `room` blocks at a time and tiles of `keys` keys; p->rows is set.
-inline void few_cut(FewPlan *p, int room, int keys, int batch, int kv, int hdp, long long max_new, long long max_length, int window) {
+// Of at most `room` blocks at a time and tiles of `keys` keys, items of up to `whole` tiles uncut; p->rows is set.
+inline void few_cut(FewPlan *p, int room, int keys, int batch, int kv, int hdp, long long max_new, long long max_length, int window, int whole = FEW_WHOLE) {
     long long span = max_length;
     if (window > 0) span = std::min(span, (long long)window + max_new + keys);
     const long long items = (long long)batch * kv, tiles = (span + keys - 1) / keys;
-    p->whole = tiles <= FEW_WHOLE;
+    p->whole = tiles <= whole;
     const long long want = p->whole ? items : (items * tiles + FEW_LEAST - 1) / FEW_LEAST;
     p->blocks = (int)std::min<long long>(room, want);
     p->part_floats = p->whole ? 0 : (long long)p->blocks * 2 * p->rows * (hdp + 2);

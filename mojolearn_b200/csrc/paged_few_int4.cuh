@@ -18,17 +18,17 @@
 
 namespace b200i {
 
-constexpr int FEW4_KEYS = 128;
+constexpr int few4_keys(bool pack) { return pack ? 256 : 128; } // of a tile
 
 template <typename RT, int GROUPS, int NT, bool PACK> struct Few4Shape {
     static constexpr bool F32 = std::is_same_v<RT, float>;
     static constexpr int HDP = GROUPS <= 2 ? 64 : 128; // head_dim as it is laid out for the products: a lane's quarter (eighth) of it lies in one group
-    static constexpr int WARPS = NT == 1 ? 4 : 8, THREADS = 32 * (WARPS + 1), ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
-    static constexpr int BLOCKS = NT > 1 ? 1 : 2;                        // on an SM
+    static constexpr int WARPS = NT <= 2 ? 4 : 8, THREADS = 32 * (WARPS + 1), ROWS = PACK ? (F32 ? 2 : 4) : 8 * NT;
+    static constexpr int BLOCKS = NT > 2 ? 1 : 2;                        // on an SM
     static constexpr int SPLIT = NT > 2 && HDP == 128 ? 2 : 1;           // warps that share keys, each for its part of the values' columns
-    static constexpr int SLICES = WARPS / SPLIT, CHUNKS = 8 / SLICES;    // a tile's keys go to so many warps, by so many times 16
-    static constexpr int CH = NT == 1 ? 2 : 1;                           // of which it works on so many at once
-    static constexpr int HALF = FEW4_KEYS * GROUPS * INT4_BYTES, SLOT = 2 * HALF; // keys, then values
+    static constexpr int SLICES = WARPS / SPLIT, KEYS = few4_keys(PACK), CHUNKS = KEYS / 16 / SLICES; // a tile's keys go to so many warps, by so many times 16
+    static constexpr int CH = PACK ? 4 : (NT == 1 || (NT == 2 && !F32) ? 2 : 1);                          // of which it works on so many at once
+    static constexpr int HALF = KEYS * GROUPS * INT4_BYTES, SLOT = 2 * HALF; // keys, then values
     static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : (NT > 2 ? 1 : 2);
     static constexpr bool HELD = PACK || (!F32 && NT == 1); // the queries stay in registers; else they lie as fragments where the warps' results meet
     static constexpr int PITCH = HDP + 8;                   // floats of a row of those
@@ -45,7 +45,7 @@ template <typename Shape>
 __device__ __forceinline__ auto few4_runs(const AttendCall &a) {
     return [&a](unsigned char *dst, unsigned long long *full, int pos, int there, int low, int kvh, auto page_of) {
         const PagedCall &c = a.c;
-        const int lane = threadIdx.x & 31, page = 1 << c.page_shift, rows = min(page, FEW4_KEYS), groups = int4_groups(c.hd), split = page > FEW4_KEYS;
+        const int lane = threadIdx.x & 31, page = 1 << c.page_shift, rows = min(page, Shape::KEYS), groups = int4_groups(c.hd), split = page > Shape::KEYS;
         const int values = lane & 1, scales = (lane >> 1) & split, piece = lane >> (1 + split); // this lane's
         const int id = page_of(piece), first = piece * rows;
         const bool want = piece < there && low - pos < first + rows; // a page that nobody sees any more may be anyone's
@@ -71,7 +71,7 @@ template <typename RT, int GROUPS, int NT, bool PACK>
 __global__ void __launch_bounds__(Few4Shape<RT, GROUPS, NT, PACK>::THREADS, Few4Shape<RT, GROUPS, NT, PACK>::BLOCKS) attend_few_int4_kernel(const __grid_constant__ FewCall f) {
     using Shape = Few4Shape<RT, GROUPS, NT, PACK>;
     constexpr bool F32 = Shape::F32, HELD = Shape::HELD;
-    constexpr int HDP = Shape::HDP, KEYS = FEW4_KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = Shape::WARPS, CH = Shape::CH, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
+    constexpr int HDP = Shape::HDP, KEYS = Shape::KEYS, SLOTS = Shape::SLOTS, KS = HDP / 16, ROWS = Shape::ROWS, WARPS = Shape::WARPS, CH = Shape::CH, QP = Shape::Q_PIECES, WP = Shape::W_PIECES;
     constexpr int SPLIT = Shape::SPLIT, SLICES = Shape::SLICES, CHUNKS = Shape::CHUNKS, MT = KS / SPLIT; // MT: pieces of 16 columns of the output that a warp has
     constexpr int E = PACK ? 1 : 2 * NT;                          // rows of a lane's scores
     constexpr int K_WORDS = HDP / 32, V_WORDS = HDP / 64 / SPLIT; // of codes, of a key: a quarter of its columns, an eighth (of the warp's)
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(Few4Shape<RT, GROUPS, NT, PACK>::THREADS, Few4
             }
         };
         for (int i = 0; i < tiles * (CHUNKS / CH); i++) {
-            const int c0 = CHUNKS == CH ? 0 : i % CHUNKS, j0 = begin + i / (CHUNKS / CH) * KEYS + 16 * c0; // the step's first key: it has 16 CH
+            const int c0 = CHUNKS == CH ? 0 : i % (CHUNKS / CH) * CH, j0 = begin + i / (CHUNKS / CH) * KEYS + 16 * c0; // the step's first key: it has 16 CH
             const unsigned char *const slot = sm.ring + slot_at * Shape::SLOT;
             if (c0 == 0 && alive && !__all_sync(0xFFFFFFFFu, pg_bar_wait(&sm.full[slot_at], parity))) give_up();
             const auto leave = [&] {
@@ -490,7 +490,10 @@ constexpr int FEW4_MOST = 24; // bfloat16 rows of an item; of float32, whose pro
 inline FewPlan few4_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     FewPlan p;
     p.most = rows, p.rows = rows <= (f32_rows ? 2 : 4) ? (f32_rows ? 2 : 4) : (rows <= 8 ? 8 : (rows <= 16 ? 16 : FEW4_MOST));
-    few_cut(&p, (p.rows > 8 ? 1 : 2) * sms, FEW4_KEYS, batch, kv, hdp, max_new, max_length, window);
+    // Wide tiles: items of up to eight are not cut where there are as many as blocks (32 sequences of 1250 keys, 16 heads: 35 us), of up to four where there are fewer.
+    const int room = (p.rows > 16 ? 1 : 2) * sms;
+    const bool pack = p.rows < 8;
+    few_cut(&p, room, few4_keys(pack), batch, kv, hdp, max_new, max_length, window, pack && (long long)batch * kv < room ? FEW_WHOLE / 2 : FEW_WHOLE);
     return p;
 }
 

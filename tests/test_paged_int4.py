@@ -73,10 +73,21 @@ def test_the_definition():
     assert quantised(tie)[0][0, :6].sub(8).tolist() == [7, 0, 2, 2, 0, -2]
 
 
-@pytest.mark.parametrize("row_type,rows,laid", [(0, 1, 2), (0, 2, 2), (0, 3, 8), (0, 9, 16), (1, 4, 4), (1, 5, 8), (1, 16, 16)])
-def test_the_workspace_of_a_few_rows(row_type, rows, laid):
-    """Two parts of as many rows as are laid out a block, and a block at most for every four tiles of 128 keys; none where a sequence's keys are not cut."""
+@pytest.mark.parametrize("row_type,rows,laid,keys", [(0, 1, 2, 256), (0, 2, 2, 256), (0, 3, 8, 128), (0, 9, 16, 128), (0, 17, 24, 128), (1, 4, 4, 256), (1, 5, 8, 128), (1, 16, 16, 128), (1, 24, 24, 128)])
+def test_the_workspace_of_a_few_rows(row_type, rows, laid, keys):
+    """Two parts of as many rows as are laid out a block, and a block at most for every four tiles; none where a sequence's keys are not cut."""
     need = lambda length: _native.lib().b200i_paged_attention_workspace_bytes(-1, row_type, 2, rows, 1, 8, 8, 128, rows, length, 0)  # noqa: E731
     assert need(8 * 128) == 0
-    blocks = min(2 * 148, -(-8 * 40 // 4))
-    assert need(40 * 128) == blocks * (2 * laid * 130 * 4 + 32)
+    blocks = min((1 if rows > 16 else 2) * 148, -(-8 * (5120 // keys) // 4))
+    assert need(5120) == blocks * (2 * laid * 130 * 4 + 32)
+
+
+def test_the_workspace_of_many_rows_has_room_for_words():
+    """More than 512 bfloat16 rows a sequence and key head: pages of words for as many positions as are named, up to 256 MB of them; extents that overflow nothing."""
+    need = lambda batch, new, length, row_type=1, cache=2: _native.lib().b200i_paged_attention_workspace_bytes(-1, row_type, cache, batch * new, batch, 8, 8, 128, new, length, 0)  # noqa: E731
+    words = lambda batch, length: -(-length // 256) * 256 * batch * 8 * 128 * 4  # noqa: E731
+    for batch, new, length in ((1, 513, 16384), (1, 2048, 1000), (4, 600, 8192)):
+        more = need(batch, new, length) - need(batch, new, length, cache=1)
+        assert words(batch, length) <= more <= words(batch, length) * 1.01 + 4096
+    for call in ((1, 512, 16384), (1, 600, 16384, 0), (2, 600, 40000), (1 << 20, 1024, 1 << 30), (1 << 29, 1024, (1 << 31) - 1)):
+        assert need(*call) == need(*call, *([1] if len(call) == 3 else []), cache=1)
