@@ -1,15 +1,21 @@
-// Attention of few rows over a paged cache in 4 bits: a decode step's single tokens (and up to 16 rows a sequence and key head).
+// Attention of few rows over a paged cache in 4 bits: a decode step's single tokens (and up to 24 rows a sequence and key head).
 //
 // The sums, the line of tiles, the copying warp and the join are those of paged_few.cuh. Bound: HBM, 4.5 bits a word of keys and values; next to that the
-// instructions that make bfloat16 words of codes (paged_int4.cuh), one and a half a word, of which an SM has 42 words a clock to do at the HBM rate. So eight warps
-// compute, two blocks on an SM, each on 16 keys of a 128-key tile, and a word is made once and meets all rows of its key head in one instruction:
-// m16n8k16 with the KEYS as rows, S^T = K Q^T and O^T = V^T P^T, the eight columns being rows. What a word's place is in an instruction is free where both factors agree on
-// it: of a key a lane takes a quarter of its columns, which is one group and one 16-byte load; of the values an eighth of the columns of four keys, whose codes become pairs along the
-// keys by one byte permutation for eight words.
+// instructions that make bfloat16 words of codes (paged_int4.cuh), one and a half a word, of which an SM has 42 words a clock to do at the HBM rate. So a word is made once
+// and meets all rows of its key head in one instruction: m16n8k16 with the KEYS as rows, S^T = K Q^T and O^T = V^T P^T, the eight columns being rows. What a word's place is in an
+// instruction is free where both factors agree on it: of a key a lane takes a quarter of its columns, which is one group and one 16-byte load; of the values an eighth of the columns
+// of four keys, whose codes become pairs along the keys by one byte permutation for eight words.
 // PACK: up to four bfloat16 rows or two of float32 leave columns of the eight free. A weight is then two pieces of 8 bits in neighbouring columns (three in four
 // columns; and so are float32 queries), and one product serves where the others need one for each piece.
 // A tensor core cuts its 32-bit sums off where it adds to a large one: with float32 rows each 16 keys begin at zero and are added to the output to nearest.
 // Weights are taken from the largest score so far as it was when one last exceeded it by 2^8: larger ones are as exact, and the usual tile needs one vote.
+//
+// Warps. Up to 16 rows, two blocks of four computing warps and one that copies: the registers of eight warps (96 a thread) spill, those of four (168) hold the sums and
+// several chains of 16 keys, each of which hides the others' latency: four chains and tiles of 256 keys with PACK, two else (one for 16 float32 rows). More rows: one block of eight
+// warps, two of which share keys and halve the columns. Measured, 64 sequences of 2000 to 8000 keys, 32 heads on 8 of 128: eight warps 106 us, four of two chains 98, of four 95
+// (2.8 TB/s of 4.5-bit words; 167 us on a cache of bfloat16 words). One of 131000 keys with pages of 64: 47.5 us (3.2 TB/s; with pages of 16, 53; of words 94).
+// 32 float32 tokens, 16 heads, up to 1250 keys a sequence: 35 us (of words 62; eight warps 47). One token at 200 keys: 8 us. Three blocks an SM (72 registers) spill: 144 us
+// for the first. Scores worked out one step ahead of the weights gained nothing.
 #pragma once
 #include <type_traits>
 
@@ -57,6 +63,7 @@ __device__ __forceinline__ auto few4_runs(const AttendCall &a) {
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         const unsigned all = __ballot_sync(0xFFFFFFFFu, some);
+        __syncwarp(); // the zeros are there before lane 0 arrives for all
         if (lane == 0) pg_bar_expect(full, (unsigned)((__popc(all) >> split) * rows * groups * INT4_BYTES));
         __syncwarp();
         if (!some) return;
@@ -485,7 +492,9 @@ __global__ void __launch_bounds__(Few4Shape<RT, GROUPS, NT, PACK>::THREADS, Few4
 }
 
 // ---- host side ----
-constexpr int FEW4_MOST = 24; // bfloat16 rows of an item; of float32, whose products are three for each, FEW_MOST
+// Rows of an item. 21 bfloat16 rows of 32 sequences of 5000 keys: 72 us here, 89 by the kernel for many; 17 to 24 of float32: 170 and 226. For 25 to 40 rows, with two more
+// products each, this kernel took 117 to 122 us and the one for many 90.
+constexpr int FEW4_MOST = 24;
 
 inline FewPlan few4_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {
     FewPlan p;
