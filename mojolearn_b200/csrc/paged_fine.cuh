@@ -17,6 +17,7 @@
 // Measured, with what follows it: 4 prompts of 1024 tokens, 16 heads of 128: 142 us on a bfloat16 cache, 223 on a float32 one (32 and 64 at the tensor rate
 // of their products):
 // the issuing thread waits, three barriers between two products, and a product of 64 columns takes 45 cycles, not 32.
+// Of a cache in 4 bits the four warps write the codes' words, which are one piece as bfloat16 ones are: 12 chunks of up to 509 tokens behind up to 4000, 429 us (391 on words).
 #pragma once
 #include "paged_many.cuh"
 

@@ -17,6 +17,10 @@
 // Work is cut as in paged_few.cuh: all items' steps on one line, an equal piece a block, parts joined by attend_join_rows_kernel.
 // Measured, with what follows it: 2048 tokens behind 14336, 32 heads on 8 of 128, 588 us (876 TFLOP/s of 1627, at 990 of 1000 W); each stream's score,
 // softmax and sum follow one another, and two streams fill the tensor pipe to 0.54. 12 chunks of up to 509 tokens, window 1024, capped, 194 us.
+// A cache in 4 bits: three warps of the fifth group read codes and write their bfloat16 words into the ring where the copies would (paged_int4.cuh). They are
+// the block's first warps, which the scheduler favours: as the last ones they starved beside the softmax (2048 tokens behind 14336: 976 us, 861 so; such calls unpack the cache
+// first). Five drafted tokens of 24 sequences, 28 heads on 4, window 4096, capped: 90 us (80 on bfloat16 words). Seven such warps in blocks of 768 threads spill (1430 us for the
+// first), and copies of codes far ahead into shared memory were slower too (975, and 98 for the drafted ones).
 #pragma once
 #include <type_traits>
 
