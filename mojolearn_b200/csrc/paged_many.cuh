@@ -643,11 +643,6 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const __gr
                 s_count++;
                 pg_fence_after();
                 if (!alive) continue;
-                if (!__any_sync(0xFFFFFFFFu, valid)) { // the warp has no row of the item: what comes of whatever its weights are is not stored
-                    if (half) pg_bar_arrive(&p_full[2 * stream]);
-                    pg_bar_arrive(&p_full[2 * stream + half]);
-                    continue;
-                }
                 const bool edge = __any_sync(0xFFFFFFFFu, valid && (hi < 64 || lo > 0));
                 // The largest score of the tiles before this one, of both halves, is what a row's weights are taken from, so that the scores are read
                 // once and nobody waits: a tile's own may exceed it, which costs range and no exactness. Rows that have seen nothing yet have none:
