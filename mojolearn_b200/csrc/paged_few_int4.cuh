@@ -35,7 +35,7 @@ template <typename RT, int GROUPS, int NT, bool PACK> struct Few4Shape {
     static constexpr int SLICES = WARPS / SPLIT, KEYS = few4_keys(PACK), CHUNKS = KEYS / 16 / SLICES; // a tile's keys go to so many warps, by so many times 16
     static constexpr int CH = PACK ? 4 : (NT == 1 || (NT == 2 && !F32) ? 2 : 1);                          // of which it works on so many at once
     static constexpr int HALF = KEYS * GROUPS * INT4_BYTES, SLOT = 2 * HALF; // keys, then values
-    static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : (NT > 2 ? 1 : 2);
+    static constexpr int Q_PIECES = F32 ? 3 : 1, W_PIECES = F32 ? 3 : 2; // of 8 bits: what two leave of a weight, 2^-16, is far below a bfloat16 output's own rounding
     static constexpr bool HELD = PACK || (!F32 && NT == 1); // the queries stay in registers; else they lie as fragments where the warps' results meet
     static constexpr int PITCH = HDP + 8;                   // floats of a row of those
     static constexpr int MEET = 4 * ROWS * PITCH * 4, QUERY = ROWS * HDP * (int)sizeof(RT);
@@ -492,8 +492,8 @@ __global__ void __launch_bounds__(Few4Shape<RT, GROUPS, NT, PACK>::THREADS, Few4
 }
 
 // ---- host side ----
-// Rows of an item. 21 bfloat16 rows of 32 sequences of 5000 keys: 72 us here, 89 by the kernel for many; 17 to 24 of float32: 170 and 226. For 25 to 40 rows, with two more
-// products each, this kernel took 117 to 122 us and the one for many 90.
+// Rows of an item. 32 sequences of 5000 keys, 28 heads on 4, 3 tokens (21 rows): 97 us here, 157 by the kernel for many; of float32 146 and 190. 32 heads on 8, 6 tokens (24 rows): 172
+// and 285, of float32 270 and 347. Five drafted tokens of 24 sequences (35 rows, window 4096, capped) took 117 to 122 us in this kernel and 90 in the one for many.
 constexpr int FEW4_MOST = 24;
 
 inline FewPlan few4_plan(int sms, bool f32_rows, int batch, int kv, int hdp, int rows, long long max_new, long long max_length, int window) {

@@ -14,6 +14,8 @@
 // by more than 2^8: larger weights are as exact (up to 2^100, from where the row is done again), the scores are read once, and nothing is
 // exchanged between their reading and P. S of the next tile is signalled after the products before it are done, and this tile's products begin
 // when the first half of P has been stored AND both halves of O have been multiplied, so O stands still while it is.
+// P's one rounding, to 8 bits: an output's terms are off independently of one another, and its norm by 2.2e-3 to 2.4e-3 where its own rounding alone makes 1.7e-3. A second
+// piece would be half as many products again, and the products are what bounds long calls. (Weights' sums are taken before the rounding, in 32 bits.)
 // Work is cut as in paged_few.cuh: all items' steps on one line, an equal piece a block, parts joined by attend_join_rows_kernel.
 // Measured, with what follows it: 2048 tokens behind 14336, 32 heads on 8 of 128, 588 us (876 TFLOP/s of 1627, at 990 of 1000 W); each stream's score,
 // softmax and sum follow one another, and two streams fill the tensor pipe to 0.54. 12 chunks of up to 509 tokens, window 1024, capped, 194 us.

@@ -176,7 +176,11 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
 
     `max_new` and `max_length` are what the caller knows of the most new tokens of a sequence and of the longest cache (by default
     all rows and the whole table): the call is cut by them, and a sequence with more than `max_new` rows is reported by
-    `torch_ops.check_status`. `scale` is 1 / sqrt(head_dim) by default. Rows past cu[-1] are not written."""
+    `torch_ops.check_status`. `scale` is 1 / sqrt(head_dim) by default. Rows past cu[-1] are not written.
+
+    Scores, statistics and sums are of 32 bits. Weights keep 16 bits or more (float32 rows, and bfloat16 rows of sequences with up to 16 of them
+    for a key head, 24 on a cache in 4 bits), so that bfloat16 outputs are off by their own rounding (1.7e-3 of the norm); of more bfloat16 rows a
+    weight is one bfloat16 word (2.2e-3 to 2.4e-3 in all)."""
     if out is None and max_new is not None and max_length is not None and _plain_attention is not None and isinstance(q, torch.Tensor):
         done = _plain_attention(q, k_cache, v_cache, page_table, cu, lengths, max_new, max_length, _scale(q.shape[-1] if q.dim() else 1) if scale is None else scale, window, softcap)
         if done is not None:
