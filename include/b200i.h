@@ -468,7 +468,9 @@ int64_t b200i_paged_read(int64_t device, void *stream, void *k_out, void *v_out,
  * positions that a row does not see, or past a sequence's length, has no influence on it. max_new and max_length bound the
  * sequences' new tokens and lengths as the host knows them (max_new is held to: a sequence with more rows sets the status word to
  * 12 and its further rows are not written; max_length only chooses how the work is cut). A device-side wait that ran out sets the
- * status word to 13. `ws`: the scratch that b200i_paged_attention_workspace_bytes asks for, on a 16-byte boundary. */
+ * status word to 13. `ws`: the scratch that b200i_paged_attention_table_workspace_bytes asks for, on a 16-byte boundary; `positions` is max_pages * page, or 0.
+ * More than 512 bfloat16 rows of a sequence and key head over a cache in 4 bits are attended to faster with room for its words, up to 256 MB for all positions of the page
+ * tables; with less, but as much as is asked for with positions 0, the codes are read as they are. b200i_paged_attention_workspace_bytes is the same for tables of max_length positions. */
 int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache,
                               const void *v_cache, int64_t row_type, int64_t cache_type, const int32_t *page_table,
                               const int32_t *cu, const int32_t *lengths, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv,
@@ -478,6 +480,9 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
 int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch,
                                               int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length,
                                               int64_t window);
+int64_t b200i_paged_attention_table_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch,
+                                                    int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new,
+                                                    int64_t max_length, int64_t window, int64_t positions);
 
 #ifdef __cplusplus
 }

@@ -102,6 +102,7 @@ SIGNATURES = {
     "b200i_paged_read": [I64] + [VP] * 5 + [I64, I64, VP, VP, VP] + [I64] * 7 + [VP, I64],
     "b200i_paged_attention": [I64, VP, VP, VP, I64, VP, VP, I64, I64, VP, VP, VP] + [I64] * 10 + [F64, I64, F64, VP, I64, VP, I64],
     "b200i_paged_attention_workspace_bytes": [I64] * 11,
+    "b200i_paged_attention_table_workspace_bytes": [I64] * 12,
     "b200i_ffma_probe": [I64, VP, VP, I64, I64, I64, VP, I64],
     "b200i_comm_create": [I64, I64, I64, I64, VP, VP, I64],
     "b200i_comm_export": [VP, VP, I64, VP, I64],

@@ -39,10 +39,10 @@ using AppendFn = int64_t (*)(int64_t, void *, void *, void *, void *, const void
                              int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, char *, int64_t);
 using AttendFn = int64_t (*)(int64_t, void *, void *, const void *, int64_t, const void *, const void *, int64_t, int64_t, const int32_t *, const int32_t *, const int32_t *, int64_t,
                              int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, double, int64_t, double, void *, int64_t, char *, int64_t);
-using AttendNeedFn = int64_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
+using AttendNeedFn = int64_t (*)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
 AppendFn g_append = nullptr;            // b200i_paged_append
 AttendFn g_attend = nullptr;            // b200i_paged_attention
-AttendNeedFn g_attend_need = nullptr;   // b200i_paged_attention_workspace_bytes
+AttendNeedFn g_attend_need = nullptr;   // b200i_paged_attention_table_workspace_bytes
 using ReadFn = int64_t (*)(int64_t, void *, void *, void *, const void *, const void *, int64_t, int64_t, const int32_t *, const int32_t *, const int32_t *, int64_t, int64_t, int64_t,
                            int64_t, int64_t, int64_t, int64_t, char *, int64_t);
 ReadFn g_read = nullptr;                // b200i_paged_read
@@ -244,7 +244,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     const int64_t rows = q.size(0), type = q.scalar_type() == at::kBFloat16;
     if (type > c.type || !rows_of(args[0], q, &heads, c.hd, rows, &ldq) || rows == 0) Py_RETURN_NONE;
     if (!integer(args[6], &max_new) || !integer(args[7], &max_length) || !real(args[8], &scale) || !integer(args[9], &window) || !real(args[10], &softcap)) Py_RETURN_NONE;
-    const int64_t need = g_attend_need(dev.index(), type, c.type, rows, c.batch, heads, c.kv, c.hd, max_new, max_length, window);
+    const int64_t need = g_attend_need(dev.index(), type, c.type, rows, c.batch, heads, c.kv, c.hd, max_new, max_length, window, c.table.size(1) * c.page);
     at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false).memory_format(at::MemoryFormat::Contiguous)), ws;
     if (need > 0) ws = at::empty({need}, q.options().requires_grad(false).dtype(at::kByte));
     char message[ERR_CAP] = "";

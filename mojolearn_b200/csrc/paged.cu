@@ -67,17 +67,21 @@ struct AttendPlan {
     int hdp;      // head_dim as it is laid out in shared memory
     FewPlan cut;
     ManyPlan cut_many; // where they are many
-    int64_t unpacked;  // positions of a sequence for which there is room in bfloat16 words (0: a cache in 4 bits is read as it is), and its bytes behind the parts
-    int64_t unpacked_bytes;
-    int64_t bytes() const { return few ? cut.bytes : (unpacked ? unpacked_at() + unpacked_bytes : cut_many.bytes); }
+    int64_t unpacked_bytes; // behind the parts, for a cache in 4 bits as bfloat16 words; 0: it is read as it is
+    int64_t bytes() const { return few ? cut.bytes : (unpacked_bytes ? unpacked_at() + unpacked_bytes : cut_many.bytes); }
     int64_t unpacked_at() const { return (cut_many.bytes + 15) / 16 * 16; }
 };
 
-// A cache in 4 bits is made one of words first where a sequence's rows are more than UNPACK_BLOCKS blocks of rows, each of which would make the words for itself, and where that
-// takes at most UNPACK_MOST bytes of words. Measured, 16384 keys, 8 heads: 500 rows a key head 89 us without and 100 with it, 600 rows 141 and 109, 800 rows 191 and 134.
+// A cache in 4 bits is made one of words first where a sequence's rows are more than UNPACK_BLOCKS blocks of rows, each of which would make the words for itself, and where the
+// words of all positions that the page table has room for take at most UNPACK_MOST bytes. Measured, 16384 keys, 8 heads: 500 rows a key head 89 us without and 100 with it, 600 rows
+// 141 and 109, 800 rows 191 and 134. It is done for the whole call: of a mixed one the single tokens' sequences are unpacked too, which still gains (a chunk of 1024 tokens behind 3000
+// beside 12 single ones at 4000, 32 heads on 8: 218 us, 288 without; 512 tokens 170 and 200; 150 behind 7000 beside 6 at 7000: 152 and 151) or takes the call past UNPACK_MOST. Short
+// calls lose 3 to 6 us, up to some 2000 positions: 1024 tokens behind nothing 62 us and 57 without, behind 300 68 and 69.
 constexpr int64_t UNPACK_BLOCKS = 2, UNPACK_MOST = 256 << 20;
 
-AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window) {
+// `positions`: of the page table, max_pages * page. What a call does and what room it asks for go by the same plan.
+AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_new, int64_t max_length, int64_t window,
+                       int64_t positions) {
     AttendPlan p = {};
     p.hdp = head_dim <= 64 ? 64 : 128;
     const int64_t group = n_heads / n_kv;
@@ -93,12 +97,9 @@ AttendPlan attend_plan(int device, int64_t row_type, int64_t cache_type, int64_t
         const bool wide = row_type == B200I_T_BF16;
         p.cut_many = many_plan(b200i_library::device_sms(device), wide ? ManyShape<128>::BLOCK_ROWS : FINE_ROWS, p.hdp, wide ? MANY_KEYS : FINE_KEYS, rows, batch, n_kv, group, max_new,
                                std::min(max_length, MOST));
-        if (cache_type == B200I_T_INT4 && wide && std::min(max_new, rows) * group > UNPACK_BLOCKS * ManyShape<128>::BLOCK_ROWS && max_length <= MOST) {
-            p.unpacked = (max_length + 255) / 256 * 256;
-            const bool fits = 4.0 * (double)batch * (double)n_kv * (double)head_dim * (double)p.unpacked <= (double)UNPACK_MOST;
-            if (fits) p.unpacked_bytes = unpack_bytes(batch, p.unpacked, n_kv, head_dim); // (and the table, a thousandth of it)
-            if (!fits) p.unpacked = 0;
-        }
+        if (cache_type == B200I_T_INT4 && wide && std::min(max_new, rows) * group > UNPACK_BLOCKS * ManyShape<128>::BLOCK_ROWS && positions > 0 &&
+            4.0 * (double)batch * (double)n_kv * (double)head_dim * (double)positions <= (double)UNPACK_MOST)
+            p.unpacked_bytes = unpack_bytes(batch, positions, n_kv, head_dim); // (and the table, a thousandth of it)
     }
     return p;
 }
@@ -178,12 +179,18 @@ int64_t b200i_paged_read(int64_t device, void *stream, void *k_out, void *v_out,
     return 0;
 }
 
-int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
-                                              int64_t max_new, int64_t max_length, int64_t window) {
+int64_t b200i_paged_attention_table_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                                                    int64_t max_new, int64_t max_length, int64_t window, int64_t positions) {
     if (rows <= 0 || batch <= 0 || n_kv <= 0 || n_heads < n_kv || head_dim <= 0 || max_new <= 0 || max_length <= 0 || window < 0) return 0;
     int dev = (int)device;
     if (device < 0 && cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); dev = -1; }
-    return attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window).bytes();
+    return attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window, positions).bytes();
+}
+
+int64_t b200i_paged_attention_workspace_bytes(int64_t device, int64_t row_type, int64_t cache_type, int64_t rows, int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim,
+                                              int64_t max_new, int64_t max_length, int64_t window) {
+    const int64_t positions = max_length <= MOST ? (max_length + 255) / 256 * 256 : 0; // of whole pages of any size
+    return b200i_paged_attention_table_workspace_bytes(device, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window, positions);
 }
 
 int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const void *q, int64_t ldq, const void *k_cache, const void *v_cache, int64_t row_type, int64_t cache_type,
@@ -217,10 +224,11 @@ int64_t b200i_paged_attention(int64_t device, void *stream, void *out, const voi
     int dev, launches = 0;
     if (enter(&a.c, "paged_attention", device, &dev, err, err_cap)) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const AttendPlan p = attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window);
+    AttendPlan p = attend_plan(dev, row_type, cache_type, rows, batch, n_heads, n_kv, head_dim, max_new, max_length, window, max_pages * page);
+    if (ws_bytes < p.bytes()) p.unpacked_bytes = 0; // there is no room for words
     if (ws_bytes < p.bytes()) return refuse(err, err_cap, "paged_attention: the workspace holds %lld bytes of %lld", (long long)ws_bytes, (long long)p.bytes());
-    if (cache_type == B200I_T_INT4 && max_pages * page <= p.unpacked) { // (a table of more positions than max_length says may hold longer sequences)
-        LIBRARY_CUDA_TRY(launch_unpack(&a, static_cast<unsigned char *>(ws) + p.unpacked_at(), st));
+    if (p.unpacked_bytes) {
+        LIBRARY_CUDA_TRY(launch_unpack(&a, static_cast<unsigned char *>(ws) + p.unpacked_at(), max_length, st));
         launches++;
         LIBRARY_CUDA_TRY((p.hdp == 64 ? launch_many_as<__nv_bfloat16, 64>(a, p.cut_many, ws, dev, st, &launches) : launch_many_as<__nv_bfloat16, 128>(a, p.cut_many, ws, dev, st, &launches)));
     } else if (cache_type == B200I_T_INT4) {

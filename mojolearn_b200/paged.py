@@ -180,7 +180,10 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
 
     Scores, statistics and sums are of 32 bits. Weights keep 16 bits or more (float32 rows, and bfloat16 rows of sequences with up to 16 of them
     for a key head, 24 on a cache in 4 bits), so that bfloat16 outputs are off by their own rounding (1.7e-3 of the norm); of more bfloat16 rows a
-    weight is one bfloat16 word (2.2e-3 to 2.4e-3 in all)."""
+    weight is one bfloat16 word (2.2e-3 to 2.4e-3 in all).
+
+    More than 512 bfloat16 rows of a sequence and key head over a cache in 4 bits take scratch for its words, of all positions that the page table has
+    room for, where that is at most 256 MB; a wider table's codes are read as they are, which is slower."""
     if out is None and max_new is not None and max_length is not None and _plain_attention is not None and isinstance(q, torch.Tensor):
         done = _plain_attention(q, k_cache, v_cache, page_table, cu, lengths, max_new, max_length, _scale(q.shape[-1] if q.dim() else 1) if scale is None else scale, window, softcap)
         if done is not None:
@@ -197,7 +200,8 @@ def attention(q, k_cache, v_cache, page_table, cu, lengths, *, max_new=None, max
         return out
     with _on(q.device):
         types = _TYPES[q.dtype], _CACHES[k_cache.dtype]
-        need = int(_native.lib().b200i_paged_attention_workspace_bytes(q.device.index, *types, rows, batch, n_heads, n_kv, hd, max_new, max_length, int(window)))
+        need = int(_native.lib().b200i_paged_attention_table_workspace_bytes(q.device.index, *types, rows, batch, n_heads, n_kv, hd, max_new, max_length, int(window),
+                                                                               max_pages * page))
         ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
         _native.call("b200i_paged_attention", q.device.index, _stream(q.device), _vp(out), _vp(q), ldq, _vp(k_cache), _vp(v_cache), *types, _vp(page_table), _vp(cu),
                      _vp(lengths), rows, batch, n_heads, n_kv, hd, pages, page, max_pages, max_new, max_length, _scale(hd) if scale is None else float(scale),

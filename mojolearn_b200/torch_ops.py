@@ -118,7 +118,7 @@ def _bind_host_call():
     except _native.NativeError:
         return False
     _host_call.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (lib.b200i_gemm_w_plan, lib.b200i_product_workspace_bytes, lib.b200i_plan_workspace_bytes,
-                                                                      lib.b200i_paged_append, lib.b200i_paged_attention, lib.b200i_paged_attention_workspace_bytes,
+                                                                      lib.b200i_paged_append, lib.b200i_paged_attention, lib.b200i_paged_attention_table_workspace_bytes,
                                                                       lib.b200i_paged_read)),
                     _native.NativeError)
     return True
