@@ -42,18 +42,20 @@ __device__ __forceinline__ PagedSeq paged_seq_checked(const PagedCall &c, int b)
     return paged_place(lo, hi, length, (int)c.rows, capacity);
 }
 
-// The sequence of row t, or -1: a warp looks at 32 entries of cu at a time. All lanes call it with one t.
-__device__ __forceinline__ int paged_row_seq(const PagedCall &c, long long t) {
+// The first sequence that ends behind row t, or c.batch: a warp looks at 32 entries of cu at a time. All lanes call it with one t.
+__device__ __forceinline__ int paged_seq_after(const PagedCall &c, long long t) {
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < c.batch; b0 += 32) {
         const int b = b0 + lane;
         const unsigned here = __ballot_sync(0xFFFFFFFFu, b < c.batch && t < (long long)c.cu[b + 1]);
-        if (here) {
-            const int found = b0 + __ffs(here) - 1;
-            return t >= (long long)c.cu[found] ? found : -1;
-        }
+        if (here) return b0 + __ffs(here) - 1;
     }
-    return -1;
+    return c.batch;
+}
+// The sequence of row t, or -1.
+__device__ __forceinline__ int paged_row_seq(const PagedCall &c, long long t) {
+    const int b = paged_seq_after(c, t);
+    return b < c.batch && t >= (long long)c.cu[b] ? b : -1;
 }
 
 // The row (of head_dim) of position `pos` of sequence b and head h in a cache, or -1 (and the status word) for a bad page.

@@ -40,24 +40,29 @@ __global__ void __launch_bounds__(READ_THREADS) read_kernel(const ReadCall a, in
     const PagedCall &c = a.c;
     const long long t0 = (long long)blockIdx.x * rows;
     if (threadIdx.x < 32) {
-        const long long t = t0 + threadIdx.x;
-        int b = paged_row_seq(c, t0), row = -2;
-        if (b >= 0) { // the others' sequences are the first row's, or follow it
-            while (b < c.batch && t >= c.cu[b + 1]) b++;
-        } else {
-            for (int r = 1; r < rows; r++) {
-                const int of = paged_row_seq(c, t0 + r);
-                if ((int)threadIdx.x == r) b = of;
+        const int lane = threadIdx.x;
+        const long long t = t0 + lane;
+        const bool mine = lane < rows && t < c.rows;
+        int b0 = paged_seq_after(c, t0), row = -2;
+        int b = b0 < c.batch && t < c.cu[b0 + 1] ? b0 : c.batch; // the first sequence that ends behind the lane's row: the first row's, or one after it
+        for (; b0 < c.batch && __any_sync(0xFFFFFFFFu, mine && b == c.batch); b0 += 32) {
+            int end = b0 + lane < c.batch ? c.cu[b0 + lane + 1] : -1, before = 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) { // the largest end up to the lane's: these never fall, whatever cu says
+                const int lower = __shfl_up_sync(0xFFFFFFFFu, end, o);
+                end = max(end, lane >= o ? lower : end);
             }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) before += __shfl_sync(0xFFFFFFFFu, end, before + o - 1) <= t ? o : 0;
+            const bool found = __shfl_sync(0xFFFFFFFFu, end, before) > t;
+            if (b == c.batch && found) b = b0 + before;
         }
-        if (b >= 0 && b < c.batch && (int)threadIdx.x < rows && t < c.rows) {
-            if (t >= c.cu[b]) {
-                const PagedSeq s = paged_seq_checked(c, b);
-                const int pos = s.pos0 + (int)(t - s.first);
-                if (s.n > 0) row = pos < 0 ? -1 : paged_cache_row(c, b, 0, pos);
-            }
+        if (mine && b < c.batch && t >= c.cu[b]) {
+            const PagedSeq s = paged_seq_checked(c, b);
+            const int pos = s.pos0 + (int)(t - s.first);
+            if (s.n > 0) row = pos < 0 ? -1 : paged_cache_row(c, b, 0, pos);
         }
-        at[threadIdx.x] = row;
+        at[lane] = row;
     }
     __syncthreads();
     const int units = c.kv * c.hd / 8, span = min(units, READ_THREADS), step = READ_THREADS / span, r0 = threadIdx.x / span; // units of a row; a thread's rows are step apart
