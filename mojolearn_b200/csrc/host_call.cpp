@@ -235,7 +235,7 @@ PyObject *paged_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     if (nargs != 11 || !g_attend || !g_attend_need || modes()) Py_RETURN_NONE;
     at::Tensor q;
-    if (!plain(args[0], q, false) || q.dim() != 3 || q.dim() != 3 || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
+    if (!plain(args[0], q, false) || q.dim() != 3 || (q.scalar_type() != at::kFloat && q.scalar_type() != at::kBFloat16)) Py_RETURN_NONE;
     const c10::Device dev = q.device();
     Pages c;
     if (!c.read(args + 1, dev, q.size(2)) || c10::cuda::current_device() != dev.index()) Py_RETURN_NONE;
