@@ -4,7 +4,7 @@ import ctypes
 import pytest
 import torch
 
-from paged_int4_ref import Case4
+from paged_int4_ref import Case4, packed, parts
 from paged_ref import BF16, check
 
 pytestmark = pytest.mark.gpu
@@ -94,4 +94,92 @@ def test_without_room_for_words_the_codes_are_read():
         made.append(launches(call))
         assert torch.equal(out, want)
     assert made[0] == made[1] + 1 == made[2] + 1
+    torch_ops.check_status()
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("room", [0, 8192])
+def test_a_page_outside_the_pool_is_reported(page, room):
+    """It counts as a page of zeros, as one of scale zero does."""
+    c = Case4([150, 1], [800, 90], 8, 2, 64, page, BF16)
+    zeros = []
+    for cache in (c.k_cache, c.v_cache):
+        codes, scale = parts(cache)
+        scale[int(c.table[0, 2])] = 0.0
+        zeros.append(packed(codes, scale))
+    c.k_cache, c.v_cache = zeros
+    table = widened(c, room) if room else c.table.clone()
+    want = attend(c, table)
+    check(want, c.attention(), BF16, c.most())
+    torch_ops.check_status()
+    for wrong in (c.pages, -1, 1 << 30):
+        table[0, 2] = wrong
+        got = attend(c, table)
+        with pytest.raises(_native.NativeError, match="outside the pool"):
+            torch_ops.check_status()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("window", [0, 70])
+@pytest.mark.parametrize("page", [16, 256])
+def test_what_is_not_seen_has_no_influence(page, window):
+    """NaN past the lengths, in pages of nobody, before a window, and in the memory that the workspace takes; page numbers of pages that no row sees mean nothing."""
+    c = Case4([150, 0, 2], [500, 40, 33], 8, 2, 64, page, BF16, pad=3)
+    out = torch.full_like(c.q.contiguous(), 7.0)
+    want = attend(c, window=window, out=out)[:c.first[-1]].clone()
+    assert bool((out[c.first[-1]:] == 7.0).all())
+    check(want, c.attention(window)[:c.first[-1]], BF16, c.most())
+    seen = torch.zeros(c.pages, page, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(c.length):
+        for pos in range(max(0, n - c.new[b] + 1 - window) if window else 0, n if c.new[b] else 0):
+            seen[int(c.table[b, pos // page]), pos % page] = True
+    for name in ("k_cache", "v_cache"):
+        codes, scale = parts(getattr(c, name))
+        setattr(c, name, packed(torch.where(seen[:, None, :, None, None], codes, 15), torch.where(seen[:, None, :, None], scale, float("nan"))))
+    table = widened(c, 4096)
+    for b, n in enumerate(c.length):
+        table[b, :max(0, n - c.new[b] + 1 - window) // page if window else 0] = -5
+        if not c.new[b]:
+            table[b] = -5
+    for byte in (0xFF, 0x7F, 0x80):
+        full = torch.full((64 << 20,), byte, dtype=torch.uint8, device="cuda")
+        del full  # what the call's workspace is cut from
+        assert torch.equal(attend(c, table, window=window)[:c.first[-1]], want)
+    torch_ops.check_status()
+
+
+@pytest.mark.parametrize("room", [0, 4096])
+def test_on_another_stream_and_in_a_graph(room):
+    """Captured twice and replayed in turn with other rows, lengths and pages, each graph with a workspace of its own."""
+    c = Case4([140, 140], [100, 400], 8, 2, 64, 64, BF16, spare=6)
+    table = torch.cat([c.table, torch.full((2, 1), -1, dtype=torch.int32, device="cuda")], dim=1) if not room else widened(c, room)
+    free = sorted(set(range(c.pages)) - set(c.table.flatten().tolist()))
+    for b in range(2):
+        table[b, -(-c.length[b] // 64)] = free[b]
+    q, lengths, side = c.q.clone(), c.lengths.clone(), torch.cuda.Stream()
+
+    def step():
+        return paged.attention(q, c.k_cache, c.v_cache, table, c.cu, lengths, max_new=140, max_length=620)
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+        for graph in graphs:
+            with torch.cuda.graph(graph, stream=side):
+                outs.append(step())
+        g = torch.Generator(device="cuda").manual_seed(5)
+        for i in range(4):
+            q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+            lengths.copy_(c.lengths + 3 * i)
+            order = torch.randperm(c.pages, generator=g, device="cuda").to(torch.int32)
+            table[:, :10] = torch.where(table[:, :10] >= 0, order[table[:, :10].clamp(0, c.pages - 1)], table[:, :10])
+            graphs[0].replay(), graphs[1].replay()
+            got = [x.clone() for x in outs]
+            want = step()
+            assert torch.equal(got[0], want) and torch.equal(got[1], want)
+            c.table, c.length = table, lengths.tolist()
+            check(want, c.attention(q=q), BF16, c.most())
+    side.synchronize()
     torch_ops.check_status()
