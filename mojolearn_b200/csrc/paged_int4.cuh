@@ -5,7 +5,9 @@
 //   x = s (n - 8),   s the smallest number of five significant bits, from 2^-100 on, with 7 s >= max |x|;   n - 8 = x / s to the nearest, ties to even
 //
 // Five bits times three are eight: what a code stands for is a bfloat16 word, so that the tensor cores multiply the cached values themselves and nothing
-// is rounded a second time on any way through them. s ends at 2^90 (words beyond 7 s are cut to it), so that no sum over 2^31 keys leaves 32 bits. The scale
+// is rounded a second time on any way through them. s ends at 2^90 (words beyond 7 s are cut to it), so that with weights of at most one no sum over 2^31 keys leaves 32 bits.
+// Kernels whose weights exceed one for a while (by 2^8 with few rows, up to 2^100 with many) may overflow: such a row does not come out finite and is done again with
+// weights of at most one, like a row that met an infinity. The scale
 // of a group with a word that is not finite is NaN, as are all its words then. A page and head are one run of bytes: the codes of its positions, 16 bytes a
 // group, then their scales, 2 bytes a group. A 32-bit word of codes holds eight columns, 2 i in its i-th four bits and 2 i + 1 in the (i + 4)-th: a shift and a mask make
 // a pair of neighbouring columns as two 16-bit words.
