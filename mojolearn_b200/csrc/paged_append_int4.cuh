@@ -7,8 +7,7 @@
 // Bound: HBM, and latency for a few rows. A lane takes the unit pairs of paged_append.cuh; the units of a group are in neighbouring lanes where half a rotation is
 // whole groups, and looked up else. What is not a warp's units goes by a warp a head, a column of each group a lane, in 64 bits: rotations whose halves are not whole
 // units, tables that are not on 16-byte boundaries, and the keys that are done again.
-// 16 prompts of 33 to 1024 tokens, 32 heads on 8 of 128, norms: 69 us (44 into a cache of bfloat16 words, whose 32-bit keys need no second look), of which the heads that are done again
-// are some 9; those in a kernel of their own took 16 us or more, those of a row gathered behind its loop 72.5 in all.
+// 16 prompts of 33 to 1024 tokens, 32 heads on 8 of 128, norms: 70 us (45 into a cache of bfloat16 words), 60 without the second look and the heads that are done again for it; those in a kernel of their own took 16 us or more, those of a row gathered behind its loop 72.5 in all.
 #pragma once
 #include "paged_append.cuh"
 #include "paged_int4.cuh"

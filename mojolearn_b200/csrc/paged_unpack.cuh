@@ -2,7 +2,7 @@
 //
 // The words go to pages of a workspace, in the order of the sequences' positions: page i of sequence b is page b max_pages + i there, and the table says so. A word is the one
 // that the codes stand for, so nothing is rounded. Bound: HBM and L2, 4.5 bits read and 16 written a word; pages that no row sees are left as they are.
-// 2048 tokens behind 14336, 32 heads on 8 of 128: 556 us, some 20 of them here, and 860 with words made in the attention, where each of a key head's 32 blocks of 256
+// 2048 tokens behind 14336, 32 heads on 8 of 128: 560 to 600 us (at the power limit; by the box), some 20 of them here, and 862 with words made in the attention, where each of a key head's 32 blocks of 256
 // rows makes them for itself.
 #pragma once
 #include "paged_int4.cuh"
